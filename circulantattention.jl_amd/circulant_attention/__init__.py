@@ -19,8 +19,13 @@ Julia name              -> here
 Gradients flow through torch.autograd with the reference's rrules
 (src/rrules.jl); Zygote.accum's role is played by autograd accumulation.
 
+`tokens` holds the attention of token models, without a counterpart in the
+reference: sliding_mh_attention (causal window with sinks), paged_mh_attention
+and paged_append_ (the same over a paged cache) and axial_rotary (positions).
+
 `layers` holds downstream modules in the manner of GroupCDL (README.md:33-38):
-CircAttBlock and GroupThresholding, on channels-last feature maps.
+CircAttBlock and GroupThresholding, on channels-last feature maps, and
+SlidingAttBlock on token signals.
 """
 from . import _lib
 from .circulant import (AbstractSimilarity, Circulant, DistanceSimilarity, DotSimilarity, Otimes,
@@ -30,7 +35,8 @@ from .circulant import (AbstractSimilarity, Circulant, DistanceSimilarity, DotSi
                         circulant_similarity_, circulant_transposed_attention, otimes, scale,
                         kernel_length, softmax, softmax_, spatial_dims, spatial_size)
 
-from .layers import CircAttBlock, GroupThresholding  # noqa: E402
+from .tokens import axial_rotary, paged_append_, paged_mh_attention, sliding_mh_attention  # noqa: E402
+from .layers import CircAttBlock, GroupThresholding, SlidingAttBlock  # noqa: E402
 
 Circulant.__matmul__ = lambda A, x: otimes(A, x)
 
@@ -40,5 +46,6 @@ __all__ = [
     "circulant_mh_adjacency", "circulant_mh_attention", "circulant_mh_transposed_attention",
     "circulant_similarity", "circulant_similarity_", "circulant_transposed_attention", "otimes",
     "kernel_length", "scale", "softmax", "softmax_", "spatial_dims", "spatial_size",
-    "CircAttBlock", "GroupThresholding",
+    "axial_rotary", "paged_append_", "paged_mh_attention", "sliding_mh_attention",
+    "CircAttBlock", "GroupThresholding", "SlidingAttBlock",
 ]

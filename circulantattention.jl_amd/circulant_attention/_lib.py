@@ -30,6 +30,8 @@ DOT = 0
 DISTANCE = 1
 F32 = 0
 C32 = 1
+F16 = 2   # the token operators only
+BF16 = 3
 CHANNELS_LAST = 16  # OR-ed into dtype of the fused entry points
 
 MATH_SPLIT_F16 = 0
@@ -76,6 +78,20 @@ SIGNATURES = {
     "circatt_copy_blocks": (_int, [_p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
     "circatt_sum_middle": (_int, [_p, _p, _i64, _i64, _i64, _p]),
     "circatt_count_unequal": (_int, [_int, _i64, _p, _p, _p, _p]),
+    "circatt_sliding_fwd": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _i64,
+                                   _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p]),
+    "circatt_sliding_bwd_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "circatt_sliding_bwd": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _i64,
+                                   _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _p, _p,
+                                   _p, _p, _i64, _p]),
+    "circatt_paged_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "circatt_paged_attention": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _p,
+                                       _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _int, _p,
+                                       _i64, _p]),
+    "circatt_paged_append": (_int, [_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64,
+                                    _i64, _p, _i64, _i64, _p, _p, _p]),
+    "circatt_axial_rotary": (_int, [_int, _int, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                    _i32, _i32, _i32, _f32, _p, _i64, _p, _i64, _p, _p]),
     "circatt_malloc": (_int, [ctypes.POINTER(_p), _i64]),
     "circatt_free": (_int, [_p]),
     "circatt_memcpy": (_int, [_p, _p, _i64, _int]),

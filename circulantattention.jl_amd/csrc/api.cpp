@@ -14,6 +14,7 @@
 
 #include "circatt.h"
 #include "circatt_kernels.h"
+#include "token_kernels.h"
 
 using namespace circatt;
 
@@ -596,6 +597,334 @@ int circatt_count_unequal(int kind, int64_t n, const void *a, const void *b, int
                                            static_cast<const uint32_t *>(b), count,
                                            as_stream(stream)),
                       "circatt_count_unequal");
+}
+
+// ---------------------------------------------------------------------------
+// Token operators.
+
+namespace {
+
+int check_token_dtype(int dtype) {
+    if (dtype != CIRCATT_F32 && dtype != CIRCATT_F16 && dtype != CIRCATT_BF16)
+        return fail(CIRCATT_ERR_UNSUPPORTED, "dtype %d not supported (Float32, Float16 or BFloat16)", dtype);
+    return CIRCATT_OK;
+}
+int esize_of(int dtype) { return dtype == CIRCATT_F32 ? 4 : 2; }
+
+// Heads of one call: nheads of queries over kv_heads of keys and values.
+int check_heads(int64_t nheads, int64_t kv_heads, int64_t dh) {
+    if (nheads < 1 || kv_heads < 1 || nheads > 65536)
+        return fail(CIRCATT_ERR_INVALID, "invalid head counts %lld, %lld", (long long)nheads, (long long)kv_heads);
+    if (nheads % kv_heads != 0)
+        return fail(CIRCATT_ERR_INVALID, "nheads (%lld) must be divisible by kv_heads (%lld)", (long long)nheads,
+                    (long long)kv_heads);
+    if (dh < 1) return fail(CIRCATT_ERR_INVALID, "invalid channels per head %lld", (long long)dh);
+    if (dh > 128 || dh % 8 != 0)
+        return fail(CIRCATT_ERR_UNSUPPORTED, "channels per head (%lld) must be a multiple of 8 up to 128", (long long)dh);
+    return CIRCATT_OK;
+}
+int check_window(int64_t window, int64_t sinks, float scale) {
+    if (window < 1) return fail(CIRCATT_ERR_INVALID, "window W=%lld must be >= 1", (long long)window);
+    if (sinks < 0) return fail(CIRCATT_ERR_INVALID, "sinks=%lld must be >= 0", (long long)sinks);
+    if (!(scale > 0.f) || !std::isfinite(scale))
+        return fail(CIRCATT_ERR_INVALID, "scale=%g must be positive and finite", (double)scale);
+    return CIRCATT_OK;
+}
+// Rows of a token signal: channels adjacent, 16-byte aligned, row over row.
+int check_rows(const char *name, const void *p, int64_t row, int64_t batch, int64_t channels, int esize) {
+    if (p == nullptr) return fail(CIRCATT_ERR_INVALID, "%s is NULL", name);
+    if (row < channels || batch < 0 || row > (int64_t)1 << 24)
+        return fail(CIRCATT_ERR_INVALID, "%s: strides %lld, %lld do not fit rows of %lld channels", name,
+                    (long long)row, (long long)batch, (long long)channels);
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || row * esize % 16 != 0 || batch * esize % 16 != 0)
+        return fail(CIRCATT_ERR_INVALID, "%s must have 16-byte aligned rows", name);
+    return CIRCATT_OK;
+}
+
+int sliding_problem(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
+                    int64_t sinks, float scale, SlidingProblem &pr) {
+    CIRCATT_TRY(check_token_dtype(dtype));
+    CIRCATT_TRY(check_heads(nheads, kv_heads, dh));
+    CIRCATT_TRY(check_window(window, sinks, scale));
+    if (L < 0 || B < 0 || L > INT32_MAX / 2 || B > INT32_MAX || L * nheads > INT32_MAX / 2)
+        return fail(CIRCATT_ERR_INVALID, "invalid signal size L=%lld, B=%lld", (long long)L, (long long)B);
+    // launch dimensions: at most one workgroup for 4 rows
+    if (B > 0 && L * nheads > (int64_t)INT32_MAX / B)
+        return fail(CIRCATT_ERR_UNSUPPORTED, "B*L*nheads = %lld * %lld exceeds 2^31", (long long)B, (long long)(L * nheads));
+    pr = SlidingProblem{};
+    pr.dtype = dtype;
+    pr.B = (int)B;
+    pr.L = (int)L;
+    pr.H = (int)nheads;
+    pr.Hk = (int)kv_heads;
+    pr.G = (int)(nheads / kv_heads);
+    pr.D = (int)dh;
+    // a window that holds every token leaves no sinks outside it
+    pr.W = (int)(window < L ? window : L);
+    pr.S = window >= L ? 0 : (int)(sinks < L ? sinks : L);
+    pr.scale = scale;
+    return CIRCATT_OK;
+}
+
+int paged_table(int64_t B, int64_t npages, int64_t page_size, int64_t page_stride, int64_t row_stride, int64_t channels,
+                const int32_t *pages, int64_t pages_row, int64_t maxp, const int32_t *lengths, const void *cache_k,
+                const void *cache_v, int esize, int &log2) {
+    if (B < 1 || B > INT32_MAX / 2) return fail(CIRCATT_ERR_INVALID, "invalid sequence count %lld", (long long)B);
+    if (page_size < 1 || page_size > 65536 || (page_size & (page_size - 1)) != 0)
+        return fail(CIRCATT_ERR_UNSUPPORTED, "page size %lld must be a power of two up to 65536", (long long)page_size);
+    for (log2 = 0; (1 << log2) < page_size;) ++log2;
+    if (npages < 1 || npages > INT32_MAX / page_size)
+        return fail(CIRCATT_ERR_INVALID, "a cache of %lld pages of %lld tokens", (long long)npages, (long long)page_size);
+    if (maxp < 1 || pages_row < maxp || maxp > (int64_t)1 << (30 - log2))
+        return fail(CIRCATT_ERR_INVALID, "a page table of %lld pages, rows of %lld", (long long)maxp, (long long)pages_row);
+    CIRCATT_NONNULL(pages);
+    CIRCATT_NONNULL(lengths);
+    if (row_stride < channels || page_stride < 0 || (npages > 1 && page_stride < row_stride))
+        return fail(CIRCATT_ERR_INVALID, "cache strides %lld, %lld do not fit rows of %lld channels",
+                    (long long)page_stride, (long long)row_stride, (long long)channels);
+    for (const void *p : {cache_k, cache_v}) {
+        if (p == nullptr) return fail(CIRCATT_ERR_INVALID, "cache is NULL");
+        if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || row_stride * esize % 16 != 0 || page_stride * esize % 16 != 0)
+            return fail(CIRCATT_ERR_INVALID, "the cache must have 16-byte aligned rows");
+    }
+    return CIRCATT_OK;
+}
+
+int paged_problem(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
+                  int64_t sinks, float scale, int64_t page_size, int64_t maxp, PagedProblem &pr) {
+    CIRCATT_TRY(check_token_dtype(dtype));
+    CIRCATT_TRY(check_heads(nheads, kv_heads, dh));
+    CIRCATT_TRY(check_window(window, sinks, scale));
+    if (T < 0 || B < 1 || B > 65535 || T > INT32_MAX / 2 / nheads)
+        return fail(CIRCATT_ERR_INVALID, "invalid sizes T=%lld, B=%lld", (long long)T, (long long)B);
+    if (maxp < 1 || page_size < 1 || maxp > ((int64_t)1 << 30) / page_size)
+        return fail(CIRCATT_ERR_INVALID, "a page table of %lld pages of %lld tokens", (long long)maxp, (long long)page_size);
+    pr = PagedProblem{};
+    pr.dtype = dtype;
+    pr.T = T;
+    pr.B = (int)B;
+    pr.H = (int)nheads;
+    pr.Hk = (int)kv_heads;
+    pr.G = (int)(nheads / kv_heads);
+    pr.D = (int)dh;
+    const int64_t most = maxp * page_size;
+    pr.W = (int)(window < most ? window : most);
+    pr.S = window >= most ? 0 : (int)(sinks < most ? sinks : most);
+    pr.scale = scale;
+    pr.page = (int)page_size;
+    pr.maxp = (int)maxp;
+    return CIRCATT_OK;
+}
+
+}  // namespace
+
+int circatt_sliding_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
+                        int64_t sinks, float scale, const void *q, int64_t q_row, int64_t q_batch, const void *k,
+                        int64_t k_row, int64_t k_batch, const void *v, int64_t v_row, int64_t v_batch,
+                        const int32_t *lengths, void *y, float *lse, void *stream) {
+    SlidingProblem pr;
+    CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
+    if (L == 0 || B == 0) return ok();
+    const int es = esize_of(dtype);
+    CIRCATT_TRY(check_rows("q", q, q_row, q_batch, nheads * dh, es));
+    CIRCATT_TRY(check_rows("k", k, k_row, k_batch, kv_heads * dh, es));
+    CIRCATT_TRY(check_rows("v", v, v_row, v_batch, kv_heads * dh, es));
+    CIRCATT_TRY(check_rows("y", y, nheads * dh, 0, nheads * dh, es));
+    pr.q = q, pr.q_row = q_row, pr.q_batch = q_batch;
+    pr.k = k, pr.k_row = k_row, pr.k_batch = k_batch;
+    pr.v = v, pr.v_row = v_row, pr.v_batch = v_batch;
+    pr.lengths = lengths;
+    pr.y = y;
+    pr.lse = lse;
+    return hip_result(launch_sliding_fwd(pr, as_stream(stream)), "circatt_sliding_fwd");
+}
+
+int64_t circatt_sliding_bwd_workspace_bytes(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads,
+                                            int64_t dh, int64_t window, int64_t sinks) {
+    SlidingProblem pr;
+    if (sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, 1.f, pr) != CIRCATT_OK) return -1;
+    return L == 0 || B == 0 ? 0 : 4 * sliding_bwd_workspace_floats(pr);
+}
+
+int circatt_sliding_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
+                        int64_t sinks, float scale, const void *q, int64_t q_row, int64_t q_batch, const void *k,
+                        int64_t k_row, int64_t k_batch, const void *v, int64_t v_row, int64_t v_batch,
+                        const int32_t *lengths, const void *y, const float *lse, const void *dy, int64_t dy_row,
+                        int64_t dy_batch, void *dq, void *dk, void *dv, void *workspace, int64_t workspace_bytes,
+                        void *stream) {
+    SlidingProblem pr;
+    CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
+    if (L == 0 || B == 0) return ok();
+    const int es = esize_of(dtype);
+    CIRCATT_TRY(check_rows("q", q, q_row, q_batch, nheads * dh, es));
+    CIRCATT_TRY(check_rows("k", k, k_row, k_batch, kv_heads * dh, es));
+    CIRCATT_TRY(check_rows("v", v, v_row, v_batch, kv_heads * dh, es));
+    CIRCATT_TRY(check_rows("y", y, nheads * dh, 0, nheads * dh, es));
+    CIRCATT_TRY(check_rows("dy", dy, dy_row, dy_batch, nheads * dh, es));
+    CIRCATT_TRY(check_rows("dq", dq, nheads * dh, 0, nheads * dh, es));
+    CIRCATT_NONNULL(lse);
+    if ((dk == nullptr) != (dv == nullptr)) return fail(CIRCATT_ERR_INVALID, "dk and dv go together");
+    if (dk != nullptr) {
+        CIRCATT_TRY(check_rows("dk", dk, kv_heads * dh, 0, kv_heads * dh, es));
+        CIRCATT_TRY(check_rows("dv", dv, kv_heads * dh, 0, kv_heads * dh, es));
+    }
+    CIRCATT_NONNULL(workspace);
+    const int64_t need = 4 * sliding_bwd_workspace_floats(pr);
+    if (workspace_bytes < need)
+        return fail(CIRCATT_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(CIRCATT_ERR_INVALID, "workspace must be 16-byte aligned");
+    pr.q = q, pr.q_row = q_row, pr.q_batch = q_batch;
+    pr.k = k, pr.k_row = k_row, pr.k_batch = k_batch;
+    pr.v = v, pr.v_row = v_row, pr.v_batch = v_batch;
+    pr.lengths = lengths;
+    pr.y = const_cast<void *>(y);
+    pr.lse = const_cast<float *>(lse);
+    pr.dy = dy, pr.dy_row = dy_row, pr.dy_batch = dy_batch;
+    pr.dq = dq, pr.dk = dk, pr.dv = dv;
+    pr.work = static_cast<float *>(workspace);
+    return hip_result(launch_sliding_bwd(pr, as_stream(stream)), "circatt_sliding_bwd");
+}
+
+int64_t circatt_paged_workspace_bytes(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
+                                      int64_t window, int64_t sinks, int64_t page_size, int64_t max_pages) {
+    PagedProblem pr;
+    if (paged_problem(dtype, T, B, nheads, kv_heads, dh, window, sinks, 1.f, page_size, max_pages, pr) != CIRCATT_OK)
+        return -1;
+    return T == 0 ? 0 : 4 * paged_workspace_floats(pr);
+}
+
+int circatt_paged_attention(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
+                            int64_t window, int64_t sinks, float scale, const void *q, int64_t q_row,
+                            const void *cache_k, const void *cache_v, int64_t npages, int64_t page_size,
+                            int64_t page_stride, int64_t row_stride, const int32_t *pages, int64_t pages_row,
+                            int64_t max_pages, const int32_t *lengths, const int32_t *offsets, void *y, int zero_tail,
+                            void *workspace, int64_t workspace_bytes, void *stream) {
+    PagedProblem pr;
+    CIRCATT_TRY(paged_problem(dtype, T, B, nheads, kv_heads, dh, window, sinks, scale, page_size, max_pages, pr));
+    const int es = esize_of(dtype);
+    CIRCATT_TRY(paged_table(B, npages, page_size, page_stride, row_stride, kv_heads * dh, pages, pages_row, max_pages,
+                            lengths, cache_k, cache_v, es, pr.page_log2));
+    if (offsets == nullptr && T != B)
+        return fail(CIRCATT_ERR_INVALID, "without offsets q has one row for each sequence: %lld rows, %lld sequences",
+                    (long long)T, (long long)B);
+    if (T == 0) return ok();
+    CIRCATT_TRY(check_rows("q", q, q_row, 0, nheads * dh, es));
+    CIRCATT_TRY(check_rows("y", y, nheads * dh, 0, nheads * dh, es));
+    const int64_t need = 4 * paged_workspace_floats(pr);
+    if (need > 0) {
+        CIRCATT_NONNULL(workspace);
+        if (workspace_bytes < need)
+            return fail(CIRCATT_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                        (long long)need);
+        if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+            return fail(CIRCATT_ERR_INVALID, "workspace must be 16-byte aligned");
+    }
+    pr.q = q, pr.q_row = q_row;
+    pr.k = cache_k, pr.v = cache_v;
+    pr.npages = (int)npages;
+    pr.page_stride = page_stride, pr.row_stride = row_stride;
+    pr.pages = pages, pr.pages_row = pages_row;
+    pr.lengths = lengths, pr.offsets = offsets;
+    pr.y = y;
+    pr.zero_tail = zero_tail != 0;
+    pr.work = static_cast<float *>(workspace);
+    return hip_result(launch_paged(pr, as_stream(stream)), "circatt_paged_attention");
+}
+
+int circatt_paged_append(int dtype, int64_t T, int64_t B, int64_t channels, const void *k, int64_t k_row, const void *v,
+                         int64_t v_row, void *cache_k, void *cache_v, int64_t npages, int64_t page_size,
+                         int64_t page_stride, int64_t row_stride, const int32_t *pages, int64_t pages_row,
+                         int64_t max_pages, const int32_t *lengths, const int32_t *offsets, void *stream) {
+    AppendProblem pr{};
+    CIRCATT_TRY(check_token_dtype(dtype));
+    if (T < 0 || T > INT32_MAX / 2) return fail(CIRCATT_ERR_INVALID, "invalid token count %lld", (long long)T);
+    if (channels < 1 || channels > 1 << 24) return fail(CIRCATT_ERR_INVALID, "invalid channel count %lld", (long long)channels);
+    pr.esize = esize_of(dtype);
+    CIRCATT_TRY(paged_table(B, npages, page_size, page_stride, row_stride, channels, pages, pages_row, max_pages,
+                            lengths, cache_k, cache_v, pr.esize, pr.page_log2));
+    if (offsets == nullptr && T != B)
+        return fail(CIRCATT_ERR_INVALID, "without offsets there is one row for each sequence: %lld rows, %lld sequences",
+                    (long long)T, (long long)B);
+    if (T == 0) return ok();
+    CIRCATT_NONNULL(k);
+    CIRCATT_NONNULL(v);
+    if (k_row < 0 || v_row < 0) return fail(CIRCATT_ERR_INVALID, "negative stride");
+    pr.T = T;
+    pr.B = (int)B;
+    pr.C = channels;
+    pr.k = k, pr.k_row = k_row, pr.v = v, pr.v_row = v_row;
+    pr.cache_k = cache_k, pr.cache_v = cache_v;
+    pr.page_stride = page_stride, pr.row_stride = row_stride;
+    pr.npages = (int)npages;
+    pr.pages = pages, pr.pages_row = pages_row, pr.maxp = (int)max_pages;
+    pr.lengths = lengths, pr.offsets = offsets;
+    return hip_result(launch_append(pr, as_stream(stream)), "circatt_paged_append");
+}
+
+int circatt_axial_rotary(int dtype, int inverse, int interleaved, int naxes, int64_t n1, int64_t n2, int64_t n3,
+                         int64_t P, int64_t nb, int64_t nheads, int64_t dh, int32_t p1, int32_t p2, int32_t p3,
+                         float base, const void *x, int64_t x_row, const int32_t *positions, int64_t pos_batch,
+                         void *y, void *stream) {
+    CIRCATT_TRY(check_token_dtype(dtype));
+    if (naxes < 1 || naxes > 3) return fail(CIRCATT_ERR_INVALID, "naxes=%d must be 1, 2 or 3", naxes);
+    if (nheads < 1 || nheads > 65536 || dh < 2 || dh % 2 != 0 || dh > 65536)
+        return fail(CIRCATT_ERR_INVALID, "invalid heads: %lld of %lld channels (even)", (long long)nheads, (long long)dh);
+    RotaryProblem pr{};
+    const int32_t p[3] = {p1, naxes > 1 ? p2 : 0, naxes > 2 ? p3 : 0};
+    int64_t total = 0;
+    for (int a = 0; a < naxes; ++a) {
+        if (p[a] < 1) return fail(CIRCATT_ERR_INVALID, "axis %d has %d pairs: at least one is needed", a + 1, p[a]);
+        total += p[a];
+    }
+    if (2 * total > dh)
+        return fail(CIRCATT_ERR_INVALID, "%lld pairs do not fit heads of %lld channels", (long long)total, (long long)dh);
+    if (total > kMaxPairs)
+        return fail(CIRCATT_ERR_UNSUPPORTED, "%lld pairs: at most %d are supported", (long long)total, kMaxPairs);
+    if (!(base > 0.f) || !std::isfinite(base)) return fail(CIRCATT_ERR_INVALID, "base=%g must be positive and finite", (double)base);
+    if (P < 0 || nb < 0 || P > INT32_MAX / 2 || nb > INT32_MAX || (nb > 0 && P > (int64_t)INT32_MAX / nb))
+        return fail(CIRCATT_ERR_INVALID, "invalid sizes P=%lld, nb=%lld", (long long)P, (long long)nb);
+    if (positions == nullptr) {
+        const int64_t n[3] = {n1, naxes > 1 ? n2 : 1, naxes > 2 ? n3 : 1};
+        int64_t prod = 1;
+        for (int64_t m : n) {
+            if (m < 0 || m > INT32_MAX / 2) return fail(CIRCATT_ERR_INVALID, "invalid grid size %lld", (long long)m);
+            prod = m > 0 && prod > INT32_MAX / m ? INT32_MAX : prod * m;
+        }
+        if (prod != P) return fail(CIRCATT_ERR_INVALID, "a grid of %lld pixels for %lld tokens", (long long)prod, (long long)P);
+        pr.n1 = (int)n[0];
+        pr.n2 = (int)n[1];
+    } else {
+        if (pos_batch != 0 && pos_batch < P * naxes)
+            return fail(CIRCATT_ERR_INVALID, "positions: images %lld apart hold %lld", (long long)pos_batch, (long long)(P * naxes));
+        pr.n1 = pr.n2 = 1;
+    }
+    if (P == 0 || nb == 0) return ok();
+    CIRCATT_NONNULL(x);
+    CIRCATT_NONNULL(y);
+    if (x_row < nheads * dh)
+        return fail(CIRCATT_ERR_INVALID, "x: token stride %lld below %lld channels", (long long)x_row, (long long)(nheads * dh));
+    if (x == y) return fail(CIRCATT_ERR_INVALID, "y must not alias x");
+    pr.dtype = dtype;
+    pr.inverse = inverse != 0;
+    pr.interleaved = interleaved != 0;
+    pr.naxes = naxes;
+    pr.P = P;
+    pr.nb = nb;
+    pr.H = (int)nheads;
+    pr.D = (int)dh;
+    pr.x = x;
+    pr.x_row = x_row;
+    pr.positions = positions;
+    pr.pos_batch = pos_batch;
+    pr.y = y;
+    pr.npairs = (int)total;
+    int at = 0;
+    for (int a = 0; a < naxes; ++a) {
+        pr.pairs[a] = p[a];
+        for (int i = 0; i < p[a]; ++i)
+            pr.turns[at++] = std::pow((double)base, -(double)i / p[a]) / 6.283185307179586476925;
+    }
+    return hip_result(launch_rotary(pr, as_stream(stream)), "circatt_axial_rotary");
 }
 
 int circatt_memcpy(void *dst, const void *src, int64_t bytes, int kind) {

@@ -16,6 +16,8 @@ const CIRCATT_DOT = Cint(0)
 const CIRCATT_DISTANCE = Cint(1)
 const CIRCATT_F32 = Cint(0)
 const CIRCATT_C32 = Cint(1)
+const CIRCATT_F16 = Cint(2)
+const CIRCATT_BF16 = Cint(3)
 # OR-ed into dtype of the fused entry points: (C, spatial..., B) tensors
 const CIRCATT_CHANNELS_LAST = Cint(16)
 const CIRCATT_MATH_SPLIT_F16 = Cint(0)
@@ -154,6 +156,70 @@ circatt_count_unequal(kind, n, a, b, count, stream) =
     ccall((:circatt_count_unequal, libcircatt), Cint,
           (Cint, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Int64}, Ptr{Cvoid}),
           kind, n, a, b, count, stream)
+
+circatt_sliding_fwd(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, q_batch, k,
+                    k_row, k_batch, v, v_row, v_batch, lengths, y, lse, stream) =
+    ccall((:circatt_sliding_fwd, libcircatt), Cint,
+          (Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Cfloat, Ptr{Cvoid},
+           Int64, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Int32},
+           Ptr{Cvoid}, Ptr{Cfloat}, Ptr{Cvoid}),
+          dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, q_batch, k,
+          k_row, k_batch, v, v_row, v_batch, lengths, y, lse, stream)
+
+circatt_sliding_bwd_workspace_bytes(dtype, L, B, nheads, kv_heads, dh, window, sinks) =
+    ccall((:circatt_sliding_bwd_workspace_bytes, libcircatt), Int64,
+          (Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64),
+          dtype, L, B, nheads, kv_heads, dh, window, sinks)
+
+circatt_sliding_bwd(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, q_batch, k,
+                    k_row, k_batch, v, v_row, v_batch, lengths, y, lse, dy, dy_row, dy_batch, dq,
+                    dk, dv, workspace, workspace_bytes, stream) =
+    ccall((:circatt_sliding_bwd, libcircatt), Cint,
+          (Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Cfloat, Ptr{Cvoid},
+           Int64, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Int32},
+           Ptr{Cvoid}, Ptr{Cfloat}, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid},
+           Ptr{Cvoid}, Ptr{Cvoid}, Int64, Ptr{Cvoid}),
+          dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, q_batch, k,
+          k_row, k_batch, v, v_row, v_batch, lengths, y, lse, dy, dy_row, dy_batch, dq,
+          dk, dv, workspace, workspace_bytes, stream)
+
+circatt_paged_workspace_bytes(dtype, T, B, nheads, kv_heads, dh, window, sinks, page_size,
+                              max_pages) =
+    ccall((:circatt_paged_workspace_bytes, libcircatt), Int64,
+          (Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Int64),
+          dtype, T, B, nheads, kv_heads, dh, window, sinks, page_size, max_pages)
+
+circatt_paged_attention(dtype, T, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, cache_k,
+                        cache_v, npages, page_size, page_stride, row_stride, pages, pages_row,
+                        max_pages, lengths, offsets, y, zero_tail, workspace, workspace_bytes,
+                        stream) =
+    ccall((:circatt_paged_attention, libcircatt), Cint,
+          (Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Cfloat, Ptr{Cvoid},
+           Int64, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Int64, Ptr{Int32}, Int64,
+           Int64, Ptr{Int32}, Ptr{Int32}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Int64,
+           Ptr{Cvoid}),
+          dtype, T, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, cache_k,
+          cache_v, npages, page_size, page_stride, row_stride, pages, pages_row,
+          max_pages, lengths, offsets, y, zero_tail, workspace, workspace_bytes, stream)
+
+circatt_paged_append(dtype, T, B, channels, k, k_row, v, v_row, cache_k, cache_v, npages, page_size,
+                     page_stride, row_stride, pages, pages_row, max_pages, lengths, offsets, stream)
+                     =
+    ccall((:circatt_paged_append, libcircatt), Cint,
+          (Cint, Int64, Int64, Int64, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Int64, Ptr{Cvoid},
+           Ptr{Cvoid}, Int64, Int64, Int64, Int64, Ptr{Int32}, Int64, Int64, Ptr{Int32},
+           Ptr{Int32}, Ptr{Cvoid}),
+          dtype, T, B, channels, k, k_row, v, v_row, cache_k, cache_v, npages, page_size,
+          page_stride, row_stride, pages, pages_row, max_pages, lengths, offsets, stream)
+
+circatt_axial_rotary(dtype, inverse, interleaved, naxes, n1, n2, n3, P, nb, nheads, dh, p1, p2, p3,
+                     base, x, x_row, positions, pos_batch, y, stream) =
+    ccall((:circatt_axial_rotary, libcircatt), Cint,
+          (Cint, Cint, Cint, Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Int32,
+           Int32, Int32, Cfloat, Ptr{Cvoid}, Int64, Ptr{Int32}, Int64, Ptr{Cvoid},
+           Ptr{Cvoid}),
+          dtype, inverse, interleaved, naxes, n1, n2, n3, P, nb, nheads, dh, p1, p2, p3,
+          base, x, x_row, positions, pos_batch, y, stream)
 
 circatt_malloc(ptr, bytes) =
     ccall((:circatt_malloc, libcircatt), Cint, (Ptr{Ptr{Cvoid}}, Int64), ptr, bytes)

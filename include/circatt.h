@@ -45,6 +45,9 @@ extern "C" {
 /* Element types of signals: Float32, ComplexF32. */
 #define CIRCATT_F32 0
 #define CIRCATT_C32 1
+/* Element types of the token operators only (they take CIRCATT_F32 as well). */
+#define CIRCATT_F16 2
+#define CIRCATT_BF16 3
 
 /*
  * Layout flag, OR-ed into dtype of the fused entry points (circatt_fused_*):
@@ -294,6 +297,95 @@ int circatt_sum_middle(const float *src, float *dst, int64_t inner, int64_t nsum
                        void *stream);
 int circatt_count_unequal(int kind, int64_t n, const void *a, const void *b, int64_t *count,
                           void *stream);
+
+/*
+ * Token operators.  No counterpart in the reference: the attention of this
+ * library for models of token sequences, whose window ends at the query (a
+ * token sees no later one) and does not wrap.
+ *
+ * Signals are channels-last, Julia size (C, L, B), of CIRCATT_F32,
+ * CIRCATT_F16 or CIRCATT_BF16: channel c of head g of token i of signal b at
+ * g*dh + c + i*row + b*batch, strides in elements (row >= channels; rows
+ * 16-byte aligned), so that the three parts of one projection's output are
+ * read in place.  Outputs are contiguous.  kv_heads heads of keys and values
+ * serve nheads/kv_heads heads of queries each: head h of q reads head
+ * h / (nheads/kv_heads) of k and v.  dh is a multiple of 8 up to 128.  Sums,
+ * softmax and statistics are Float32; probabilities and score gradients are
+ * rounded to the element type where they enter a matrix product.
+ *
+ * circatt_sliding_fwd: token i of signal b, i < lengths[b] (lengths NULL: L),
+ * sees key j <= i if j > i - window or j < sinks, and
+ *   y = softmax_j(scale * <q_i, k_j>) v.
+ * Rows from lengths[b] on are zero and nothing of q, k, v behind lengths[b]
+ * has an influence, whatever it holds.  lse (nheads*L*B floats, for the
+ * backward) may be NULL.
+ *
+ * circatt_sliding_bwd: dq, dk, dv of the same (dk and dv both NULL: dq alone),
+ * from y and lse of the forward.  No atomics; gradients of a shared head are
+ * summed over its queries' heads in a fixed order.
+ */
+int circatt_sliding_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
+                        int64_t window, int64_t sinks, float scale, const void *q, int64_t q_row,
+                        int64_t q_batch, const void *k, int64_t k_row, int64_t k_batch, const void *v,
+                        int64_t v_row, int64_t v_batch, const int32_t *lengths, void *y, float *lse,
+                        void *stream);
+int64_t circatt_sliding_bwd_workspace_bytes(int dtype, int64_t L, int64_t B, int64_t nheads,
+                                            int64_t kv_heads, int64_t dh, int64_t window, int64_t sinks);
+int circatt_sliding_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
+                        int64_t window, int64_t sinks, float scale, const void *q, int64_t q_row,
+                        int64_t q_batch, const void *k, int64_t k_row, int64_t k_batch, const void *v,
+                        int64_t v_row, int64_t v_batch, const int32_t *lengths, const void *y,
+                        const float *lse, const void *dy, int64_t dy_row, int64_t dy_batch, void *dq,
+                        void *dk, void *dv, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * The same attention for serving, over a paged cache: a cache holds npages
+ * pages of page_size tokens (a power of two), token s of page p at
+ * p*page_stride + s*row_stride, and token j of sequence b lies in page
+ * pages[b*pages_row + j/page_size].  lengths[b] tokens of sequence b are in
+ * the cache, its new ones (the last) included.  The T rows of q are the new
+ * tokens of the B sequences in order: sequence b has the rows offsets[b] ..
+ * offsets[b+1] - 1 (offsets: B+1 ascending numbers from 0; NULL: one row for
+ * each sequence, T = B).  pages, lengths and offsets are device arrays that
+ * are read when the kernel runs, so a captured call follows their contents.
+ * A page number outside [0, npages) is never followed: its tokens are hidden,
+ * and a row that sees nothing is zero.  Rows of y behind the last sequence are
+ * zero with zero_tail = 1 and left as they were with 0.
+ *
+ * circatt_paged_append writes the new tokens' k and v, packed the same way,
+ * into their pages; a token whose page number is outside the cache is dropped.
+ * No two tokens may share a slot.
+ */
+int64_t circatt_paged_workspace_bytes(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads,
+                                      int64_t dh, int64_t window, int64_t sinks, int64_t page_size,
+                                      int64_t max_pages);
+int circatt_paged_attention(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads,
+                            int64_t dh, int64_t window, int64_t sinks, float scale, const void *q,
+                            int64_t q_row, const void *cache_k, const void *cache_v, int64_t npages,
+                            int64_t page_size, int64_t page_stride, int64_t row_stride,
+                            const int32_t *pages, int64_t pages_row, int64_t max_pages,
+                            const int32_t *lengths, const int32_t *offsets, void *y, int zero_tail,
+                            void *workspace, int64_t workspace_bytes, void *stream);
+int circatt_paged_append(int dtype, int64_t T, int64_t B, int64_t channels, const void *k, int64_t k_row,
+                         const void *v, int64_t v_row, void *cache_k, void *cache_v, int64_t npages,
+                         int64_t page_size, int64_t page_stride, int64_t row_stride,
+                         const int32_t *pages, int64_t pages_row, int64_t max_pages,
+                         const int32_t *lengths, const int32_t *offsets, void *stream);
+
+/*
+ * Rotary positions with naxes (1 to 3) axes on P tokens of each of nb signals
+ * (rows x_row elements apart): the first 2*p1 channels of a head belong to
+ * axis 1, the next 2*p2 to axis 2, then 2*p3; pair i of an axis (channels i
+ * and i + p of its section, or 2i and 2i + 1 when interleaved) is turned by
+ * position * base^(-i/p); the channels behind stay.  positions (Int32, naxes a
+ * token, P tokens; pos_batch apart from signal to signal, 0: shared), or NULL:
+ * token i1 + n1*(i2 + n2*i3) has the positions (i1, i2, i3).  inverse: the
+ * turn the other way, which is the gradient.
+ */
+int circatt_axial_rotary(int dtype, int inverse, int interleaved, int naxes, int64_t n1, int64_t n2,
+                         int64_t n3, int64_t P, int64_t nb, int64_t nheads, int64_t dh, int32_t p1,
+                         int32_t p2, int32_t p3, float base, const void *x, int64_t x_row,
+                         const int32_t *positions, int64_t pos_batch, void *y, void *stream);
 
 /*
  * Device memory helpers for hosts without a GPU array package (the reference
