@@ -73,7 +73,7 @@ def _rows(t):
         sr += -sr % e
     if B == 1:
         sb = 0
-    if (sc != 1 and C > 1) or sr < C or sr % e or sb % e or t.data_ptr() % 16 or sr > 1 << 24:
+    if (sc != 1 and C > 1) or sr < C or sr % e or sb % e or t.data_ptr() % 16 or sr > 1 << 22:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()

@@ -633,7 +633,7 @@ int check_window(int64_t window, int64_t sinks, float scale) {
 // Rows of a token signal: channels adjacent, 16-byte aligned, row over row.
 int check_rows(const char *name, const void *p, int64_t row, int64_t batch, int64_t channels, int esize) {
     if (p == nullptr) return fail(CIRCATT_ERR_INVALID, "%s is NULL", name);
-    if (row < channels || batch < 0 || row > (int64_t)1 << 24)
+    if (row < channels || batch < 0 || row > (int64_t)1 << 22)
         return fail(CIRCATT_ERR_INVALID, "%s: strides %lld, %lld do not fit rows of %lld channels", name,
                     (long long)row, (long long)batch, (long long)channels);
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || row * esize % 16 != 0 || batch * esize % 16 != 0)

@@ -1,0 +1,259 @@
+// Tiles of keys and values in LDS, and the matrix-core forward of 32 rows of
+// queries over one of them.
+//
+// Score tile, transposed: S' = K Q' (32 keys x 32 query rows, K the first
+// operand).  In the 32x32 result lane l holds column l % 32, one query row, and
+// the keys 8 (i / 4) + 4 (l / 32) + i % 4 in registers i = 0 .. 15: the softmax
+// runs over registers, with one exchange between the two halves of the
+// wavefront, and the probabilities are already the second operand of
+// O' = V' P' (lane l: column l % 32, eight consecutive places along k), when
+// the places of k are read in the same order of keys.  V' is the first operand
+// of that product: lane l needs one channel of eight keys, which the
+// transposing LDS read gives out of rows of channels (4 keys x 16 channels for
+// 16 lanes).  Nothing crosses lanes between the two products.  Float32 operands
+// take the same registers: place j of every lane is one 32x32x2 product.
+//
+// Rows lie in LDS as PC 16-byte units, the unit c of row r at c ^ f(r): eight
+// consecutive rows of one unit (the 16-byte reads) and four rows of two units
+// (the transposing reads) fall into different banks.  The tiles arrive by
+// 16-byte LDS-DMA, whose lanes write consecutive units, so the permutation is
+// applied to the addresses that they read.
+#pragma once
+
+#include "buffer_dma.h"
+#include "token_rows.h"
+
+namespace circatt {
+namespace tok {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+template <typename T>
+using V8 = T __attribute__((ext_vector_type(8)));
+template <typename T>
+using V4 = T __attribute__((ext_vector_type(4)));
+#define CIRCATT_LDS __attribute__((address_space(3)))
+
+__device__ __forceinline__ f16v mma(V8<__bf16> a, V8<__bf16> b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16v mma(V8<_Float16> a, V8<_Float16> b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16v mma(V8<float> a, V8<float> b, f16v c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+
+// DP: channels of a head, padded to a multiple of 32 (zeros).
+template <typename T, int DP>
+struct Tile {
+    static constexpr int UNITS = DP * (int)sizeof(T) / 16;  // read
+    static constexpr int PC = UNITS <= 4 ? 4 : UNITS <= 8 ? 8 : UNITS <= 16 ? 16 : 32;
+    static constexpr int ROW = PC * 16;  // bytes
+    __device__ static __forceinline__ int f(int r) {
+        return PC >= 16 ? ((r & 7) << 1) | ((r >> 3) & 1)
+                        : PC == 8 ? ((r & 3) << 1) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1);
+    }
+    // eight channels 8 c .. 8 c + 7 of row r
+    __device__ static __forceinline__ V8<T> row(const CIRCATT_LDS char *t, int r, int c) {
+        if constexpr (sizeof(T) == 2) {
+            return *(const CIRCATT_LDS V8<T> *)(t + r * ROW + ((c ^ f(r)) << 4));
+        } else {
+            const f4v a = *(const CIRCATT_LDS f4v *)(t + r * ROW + (((2 * c) ^ f(r)) << 4));
+            const f4v b = *(const CIRCATT_LDS f4v *)(t + r * ROW + (((2 * c + 1) ^ f(r)) << 4));
+            return V8<T>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        }
+    }
+    // channel 32 t + lane % 32 of the rows r0 + 8 (j / 4) + 4 (lane / 32) + j % 4,
+    // j = 0 .. 7; r0 a multiple of 16
+    __device__ static __forceinline__ V8<T> col(const CIRCATT_LDS char *tile, int r0, int t, int lane) {
+        if constexpr (sizeof(T) == 2) {
+            const int i = lane & 15, d = 4 * t + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+            union {
+                s4v s[2];
+                V8<T> v;
+            } u;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int r = 8 * k + 4 * (lane >> 5) + (i >> 2);
+                u.s[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (CIRCATT_LDS s4v *)(tile + (r0 + r) * ROW + ((d ^ f(r)) << 4) + ((i & 1) << 3)));
+            }
+            return u.v;
+        } else {
+            V8<T> v;
+            const int d = 32 * t + (lane & 31);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = 8 * (j >> 2) + 4 * (lane >> 5) + (j & 3);
+                v[j] = *(const CIRCATT_LDS float *)(tile + (r0 + r) * ROW + (((d >> 2) ^ f(r)) << 4) + ((d & 3) << 2));
+            }
+            return v;
+        }
+    }
+};
+
+// waits for this wavefront's DMA and LDS reads, then for the workgroup
+__device__ __forceinline__ void dma_barrier() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+// 16 bytes from every lane's own address to LDS byte m0 + 16 lane
+__device__ __forceinline__ void dma16_global(const void *p, unsigned m0) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(m0) : "memory");
+}
+__device__ __forceinline__ unsigned lds_byte(const CIRCATT_LDS char *p) { return (unsigned)(uintptr_t)p; }
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Eight channels from global memory, zero from channel D on (D a multiple of 8).
+template <typename T>
+__device__ __forceinline__ V8<T> load8(const T *p, int d, int D) {
+    V8<T> v{};
+    if (d < D) {
+        if constexpr (sizeof(T) == 2) {
+            v = *reinterpret_cast<const V8<T> *>(p + d);
+        } else {
+            const f4v a = *reinterpret_cast<const f4v *>(p + d), b = *reinterpret_cast<const f4v *>(p + d + 4);
+            v = V8<T>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        }
+    }
+    return v;
+}
+
+// What a query row sees: keys j with j <= at and j > at - W or j < S.
+struct Sight {
+    int W, S;
+    __device__ __forceinline__ bool operator()(int at, int j) const {
+        const int back = at - j;
+        return back >= 0 && (back < W || j < S);
+    }
+    // keys [k0, k0 + n): seen by none, or by all, of the rows at [lo, hi]
+    __device__ __forceinline__ bool none(int lo, int hi, int k0, int n) const {
+        return k0 > hi || (k0 + n - 1 <= lo - W && k0 >= S);
+    }
+    __device__ __forceinline__ bool all(int lo, int hi, int k0, int n) const {
+        return k0 + n - 1 <= lo && (k0 > hi - W || k0 + n <= S);
+    }
+};
+
+// The tiles of KT keys that rows at [lo, hi] see, in order: tiles of sinks, then
+// of the window.
+template <int KT>
+struct TileList {
+    int sinks, first, count;
+    __device__ TileList(int lo, int hi, int W, int S) {
+        const int w = lo - W + 1 > 0 ? (lo - W + 1) / KT : 0, s = (S + KT - 1) / KT;
+        first = w;
+        sinks = s < w ? s : w;
+        count = hi < 0 ? 0 : sinks + hi / KT + 1 - w;
+    }
+    __device__ __forceinline__ int key(int i) const { return (i < sinks ? i : first + i - sinks) * KT; }
+};
+
+// Running softmax and output of 32 rows (lane l and l + 32: row l % 32).
+// Scores count in units of log2(e) scale; the row's maximum is raised only when
+// a score passes it by more than 2^6 in the exponent, so that most tiles leave
+// the output as it is: probabilities stay below 2^6, which Float32 sums and
+// either 16-bit type hold with their full relative precision.
+template <typename T, int DP>
+struct Rows {
+    static constexpr int STEPS = DP / 16, OT = DP / 32;
+    static constexpr float RAISE = 6.f;
+    V8<T> q[STEPS];
+    f16v o[OT];
+    float m, l;  // l: this lane's keys alone
+
+    __device__ __forceinline__ void start(const T *qrow, int D, int lane) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) q[s] = load8(qrow, 16 * s + 8 * (lane >> 5), D);
+#pragma unroll
+        for (int t = 0; t < OT; ++t) o[t] = f16v{};
+        m = -INFINITY;
+        l = 0.f;
+    }
+
+    // NB blocks of 32 keys from key k0 on; masked: test every key, with bit
+    // (key - k0) of hidden set where it is not there at all
+    template <int NB, bool MASKED>
+    __device__ __forceinline__ void tile(const CIRCATT_LDS char *kt, const CIRCATT_LDS char *vt, int lane, int at,
+                                         int k0, Sight see, uint64_t hidden, float c) {
+        typedef Tile<T, DP> Tl;
+        f16v s[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            s[n] = f16v{};
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+                s[n] = mma(Tl::row(kt, 32 * n + (lane & 31), 2 * k + (lane >> 5)), q[k], s[n]);
+        }
+        if (MASKED) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int j = 32 * n + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+                    if (!see(at, k0 + j) || ((hidden >> j) & 1)) s[n][i] = -INFINITY;
+                }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+        if (__any(mx > m + RAISE || (m == -INFINITY && mx > -INFINITY))) {
+            const float mn = fmaxf(m, mx), r = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            l *= r;
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] *= r;
+            m = mn;
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+        V8<T> p[2 * NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -mu));
+                sum += e;
+                p[2 * n + (i >> 3)][i & 7] = (T)e;
+            }
+        l += sum;
+#pragma unroll
+        for (int t = 0; t < OT; ++t)
+#pragma unroll
+            for (int n = 0; n < 2 * NB; ++n) o[t] = mma(Tl::col(vt, 16 * n, t, lane), p[n], o[t]);
+    }
+
+    // sum over both halves' keys
+    __device__ __forceinline__ float total() const { return l + __shfl_xor(l, 32, 64); }
+
+    // Writes the row's channels, times f; whether one of them is not finite.
+    __device__ __forceinline__ bool store(T *y, int D, int lane, float f) const {
+        bool bad = false;
+#pragma unroll
+        for (int t = 0; t < OT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int d = 32 * t + 2 * i + 4 * (lane >> 5);
+                V4<T> v;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float x = o[t][i + j] * f;
+                    bad |= !(fabsf(x) < INFINITY) && d < D;
+                    v[j] = (T)x;
+                }
+                if (d < D) *reinterpret_cast<V4<T> *>(y + d) = v;
+            }
+        return bad;
+    }
+};
+
+}  // namespace tok
+}  // namespace circatt
