@@ -57,39 +57,56 @@ struct Tile {
         return PC >= 16 ? ((r & 7) << 1) | ((r >> 3) & 1)
                         : PC == 8 ? ((r & 3) << 1) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1);
     }
-    // eight channels 8 c .. 8 c + 7 of row r
-    __device__ static __forceinline__ V8<T> row(const CIRCATT_LDS char *t, int r, int c) {
+    // LDS bytes are 32-bit numbers here: a lane's place in a tile, and every read
+    // of it is that number with a few bits flipped (the unit's number) and a
+    // constant added (rows): one register holds all of a lane's addresses.
+    //
+    // A lane's place for row(): row lane % 32, channels 8 (lane / 32) ..
+    __device__ static __forceinline__ unsigned row_lane(int lane) {
+        const int r = lane & 31, u = (lane >> 5) * (sizeof(T) == 2 ? 1 : 2);
+        return r * ROW + ((u ^ f(r)) << 4);
+    }
+    // channels 16 k + 8 (lane / 32) .. + 7 of row m + lane % 32, m a multiple of 32
+    __device__ static __forceinline__ V8<T> row(unsigned at, int m, int k) {
         if constexpr (sizeof(T) == 2) {
-            return *(const CIRCATT_LDS V8<T> *)(t + r * ROW + ((c ^ f(r)) << 4));
+            return *(const CIRCATT_LDS V8<T> *)((at ^ (k << 5)) + m * ROW);
         } else {
-            const f4v a = *(const CIRCATT_LDS f4v *)(t + r * ROW + (((2 * c) ^ f(r)) << 4));
-            const f4v b = *(const CIRCATT_LDS f4v *)(t + r * ROW + (((2 * c + 1) ^ f(r)) << 4));
+            const f4v a = *(const CIRCATT_LDS f4v *)((at ^ (k << 6)) + m * ROW);
+            const f4v b = *(const CIRCATT_LDS f4v *)((at ^ (k << 6 | 16)) + m * ROW);
             return V8<T>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         }
     }
-    // channel 32 t + lane % 32 of the rows r0 + 8 (j / 4) + 4 (lane / 32) + j % 4,
-    // j = 0 .. 7; r0 a multiple of 16
-    __device__ static __forceinline__ V8<T> col(const CIRCATT_LDS char *tile, int r0, int t, int lane) {
+    // A lane's place for col(); 16-bit: rows 4 (lane / 32) + lane % 16 / 4, four
+    // channels of 16 (lane / 16 % 2) on; Float32: channel lane % 32.
+    __device__ static __forceinline__ unsigned col_lane(int lane) {
         if constexpr (sizeof(T) == 2) {
-            const int i = lane & 15, d = 4 * t + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+            const int i = lane & 15, r = 4 * (lane >> 5) + (i >> 2), u = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+            return r * ROW + ((u ^ f(r)) << 4) + ((i & 1) << 3);
+        } else {
+            const int r = 4 * (lane >> 5), d = lane & 31;
+            return r * ROW + (((d >> 2) ^ f(r)) << 4) + ((d & 3) << 2);
+        }
+    }
+    // channel 32 t + lane % 32 of the rows m + 8 (j / 4) + 4 (lane / 32) + j % 4,
+    // j = 0 .. 7; m a multiple of 16.  f(x + y) = f(x) ^ f(y) for the disjoint bits
+    // x = 4 (lane / 32) (and lane % 16 / 4), y = 8 (j / 4) (and j % 4).
+    __device__ static __forceinline__ V8<T> col(unsigned at, int m, int t) {
+        if constexpr (sizeof(T) == 2) {
             union {
                 s4v s[2];
                 V8<T> v;
             } u;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int r = 8 * k + 4 * (lane >> 5) + (i >> 2);
+            for (int k = 0; k < 2; ++k)
                 u.s[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (CIRCATT_LDS s4v *)(tile + (r0 + r) * ROW + ((d ^ f(r)) << 4) + ((i & 1) << 3)));
-            }
+                    (CIRCATT_LDS s4v *)((at ^ (t << 6 | f(8 * k) << 4)) + (m + 8 * k) * ROW));
             return u.v;
         } else {
             V8<T> v;
-            const int d = 32 * t + (lane & 31);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int r = 8 * (j >> 2) + 4 * (lane >> 5) + (j & 3);
-                v[j] = *(const CIRCATT_LDS float *)(tile + (r0 + r) * ROW + (((d >> 2) ^ f(r)) << 4) + ((d & 3) << 2));
+                const int r = 8 * (j >> 2) + (j & 3);
+                v[j] = *(const CIRCATT_LDS float *)((at ^ (t << 7 | f(r) << 4)) + (m + r) * ROW);
             }
             return v;
         }
@@ -175,21 +192,21 @@ struct Rows {
         l = 0.f;
     }
 
-    // NB blocks of 32 keys from key k0 on; masked: test every key, with bit
-    // (key - k0) of hidden set where it is not there at all
-    template <int NB, bool MASKED>
-    __device__ __forceinline__ void tile(const CIRCATT_LDS char *kt, const CIRCATT_LDS char *vt, int lane, int at,
-                                         int k0, Sight see, uint64_t hidden, float c) {
+    // NB blocks of 32 keys from key k0 on, at the lane's places kt (row) and vt
+    // (col); masked: test every key, with bit (key - k0) of hidden set where it is
+    // not there at all
+    template <int NB>
+    __device__ __forceinline__ void tile(unsigned kt, unsigned vt, int lane, int at, int k0, Sight see, bool masked,
+                                         uint64_t hidden, float c) {
         typedef Tile<T, DP> Tl;
         f16v s[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             s[n] = f16v{};
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-                s[n] = mma(Tl::row(kt, 32 * n + (lane & 31), 2 * k + (lane >> 5)), q[k], s[n]);
+            for (int k = 0; k < STEPS; ++k) s[n] = mma(Tl::row(kt, 32 * n, k), q[k], s[n]);
         }
-        if (MASKED) {
+        if (masked) {
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -228,32 +245,37 @@ struct Rows {
 #pragma unroll
         for (int t = 0; t < OT; ++t)
 #pragma unroll
-            for (int n = 0; n < 2 * NB; ++n) o[t] = mma(Tl::col(vt, 16 * n, t, lane), p[n], o[t]);
+            for (int n = 0; n < 2 * NB; ++n) o[t] = mma(Tl::col(vt, 16 * n, t), p[n], o[t]);
     }
 
     // sum over both halves' keys
     __device__ __forceinline__ float total() const { return l + __shfl_xor(l, 32, 64); }
-
-    // Writes the row's channels, times f; whether one of them is not finite.
-    __device__ __forceinline__ bool store(T *y, int D, int lane, float f) const {
-        bool bad = false;
-#pragma unroll
-        for (int t = 0; t < OT; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int d = 32 * t + 2 * i + 4 * (lane >> 5);
-                V4<T> v;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float x = o[t][i + j] * f;
-                    bad |= !(fabsf(x) < INFINITY) && d < D;
-                    v[j] = (T)x;
-                }
-                if (d < D) *reinterpret_cast<V4<T> *>(y + d) = v;
-            }
-        return bad;
-    }
 };
+
+// Writes a row's channels (one lane and its other half), times f; whether one of
+// them is not finite in the row's type.
+template <typename T, int OT>
+__device__ __forceinline__ bool store_channels(const f16v (&o)[OT], T *y, int D, int lane, float f) {
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = 32 * t + 2 * i + 4 * (lane >> 5);
+            V4<T> v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = (T)(o[t][i + j] * f);
+                bad |= !(fabsf((float)v[j]) < INFINITY) && d < D;
+            }
+            if (d < D) *reinterpret_cast<V4<T> *>(y + d) = v;
+        }
+    return bad;
+}
+template <typename T>
+__device__ __forceinline__ void zero_channels(T *y, int D, int lane) {
+    for (int d = 4 * (lane >> 5); d < D; d += 8) *reinterpret_cast<V4<T> *>(y + d) = V4<T>{};
+}
 
 }  // namespace tok
 }  // namespace circatt
