@@ -613,7 +613,7 @@ int esize_of(int dtype) { return dtype == CIRCATT_F32 ? 4 : 2; }
 
 // Heads of one call: nheads of queries over kv_heads of keys and values.
 int check_heads(int64_t nheads, int64_t kv_heads, int64_t dh) {
-    if (nheads < 1 || kv_heads < 1 || nheads > 65536)
+    if (nheads < 1 || kv_heads < 1 || nheads > 32768)
         return fail(CIRCATT_ERR_INVALID, "invalid head counts %lld, %lld", (long long)nheads, (long long)kv_heads);
     if (nheads % kv_heads != 0)
         return fail(CIRCATT_ERR_INVALID, "nheads (%lld) must be divisible by kv_heads (%lld)", (long long)nheads,
