@@ -22,23 +22,16 @@ _CODES = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
 _EVERY = 1 << 30  # a window that holds every token
 
 
-def _on(device):
-    """The device of the tensors made current for the call where it is not."""
+def _call(device, fn, *args):
+    """fn(*args, stream) on the device's current stream, the device made current
+    where it is not."""
     if device.index == torch.cuda.current_device():
-        return None
-    return torch.cuda.device(device)
-
-
-def _call(device, name, *args):
-    fn = getattr(L.lib, name)
-    guard = _on(device)
-    if guard is None:
         rc = fn(*args, stream_ptr(device))
     else:
-        with guard:
+        with torch.cuda.device(device):
             rc = fn(*args, stream_ptr(device))
     if rc != L.OK:
-        L.check(rc, name)
+        L.check(rc)
 
 
 def _require(t, name, like=None, dtypes=_CODES):
@@ -98,7 +91,7 @@ class SlidingAttentionFn(torch.autograd.Function):
         train = any(ctx.needs_input_grad[:3])
         lse = torch.empty((B, H * n), dtype=torch.float32, device=q.device) if train else None
         code = _CODES[q.dtype]
-        _call(q.device, "circatt_sliding_fwd", code, n, B, H, Hk, C // H, W, S, scale, q.data_ptr(), qr, qb,
+        _call(q.device, L.lib.circatt_sliding_fwd, code, n, B, H, Hk, C // H, W, S, scale, q.data_ptr(), qr, qb,
               k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), ptr(lse))
         if train:
             ctx.save_for_backward(q, k, v, y, lse, lengths)
@@ -119,7 +112,7 @@ class SlidingAttentionFn(torch.autograd.Function):
             dv = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         wbytes = L.lib.circatt_sliding_bwd_workspace_bytes(code, n, B, H, Hk, C // H, W, S)
         work = torch.empty((max(wbytes, 4) // 4,), dtype=torch.float32, device=q.device)
-        _call(q.device, "circatt_sliding_bwd", code, n, B, H, Hk, C // H, W, S, scale, q.data_ptr(), qr, qb,
+        _call(q.device, L.lib.circatt_sliding_bwd, code, n, B, H, Hk, C // H, W, S, scale, q.data_ptr(), qr, qb,
               k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), lse.data_ptr(), dy.data_ptr(),
               dr, db, dq.data_ptr(), ptr(dk), ptr(dv), work.data_ptr(), wbytes)
         return dq, dk, dv, None, None, None, None, None, None
@@ -235,7 +228,7 @@ def paged_mh_attention(q, cache_k, cache_v, pages, lengths, W, nheads: int, *, k
     code = _CODES[q.dtype]
     wbytes = L.lib.circatt_paged_workspace_bytes(code, T, B, nheads, kv_heads, dh, W, sinks, page, pages.shape[1])
     work = torch.empty((wbytes // 4,), dtype=torch.float32, device=q.device) if wbytes > 0 else None
-    _call(q.device, "circatt_paged_attention", code, T, B, nheads, kv_heads, dh, W, sinks, scale, q.data_ptr(), q_row,
+    _call(q.device, L.lib.circatt_paged_attention, code, T, B, nheads, kv_heads, dh, W, sinks, scale, q.data_ptr(), q_row,
           cache_k.data_ptr(), cache_v.data_ptr(), npages, page, page_stride, row_stride, pages.data_ptr(),
           pages.stride(0), pages.shape[1], lengths.data_ptr(), ptr(offsets), y.data_ptr(), 1 if out is None else 0,
           ptr(work), wbytes)
@@ -254,7 +247,7 @@ def paged_append_(cache_k, cache_v, k, v, pages, lengths, *, offsets: torch.Tens
         raise AssertionError(f"k and v must be (T, {C}), got {tuple(k.shape)} and {tuple(v.shape)}")
     pages, B, lengths, offsets = _table(pages, lengths, offsets, k)
     k, v = (t.detach() if t.stride(1) == 1 or C == 1 else t.detach().contiguous() for t in (k, v))
-    _call(k.device, "circatt_paged_append", _CODES[k.dtype], k.shape[0], B, C, k.data_ptr(), k.stride(0), v.data_ptr(),
+    _call(k.device, L.lib.circatt_paged_append, _CODES[k.dtype], k.shape[0], B, C, k.data_ptr(), k.stride(0), v.data_ptr(),
           v.stride(0), cache_k.data_ptr(), cache_v.data_ptr(), npages, page, page_stride, row_stride, pages.data_ptr(),
           pages.stride(0), pages.shape[1], lengths.data_ptr(), ptr(offsets))
 
@@ -262,6 +255,8 @@ def paged_append_(cache_k, cache_v, k, v, pages, lengths, *, offsets: torch.Tens
 def _token_stride(x):
     """(x, elements from token to token): one distance over all leading dims."""
     C = x.shape[-1]
+    if x.is_contiguous():
+        return x, C
     row = None
     if x.stride(-1) == 1 or C == 1:
         step = None
@@ -300,12 +295,13 @@ class AxialRotaryFn(torch.autograd.Function):
 
 def _turn(x, inverse, grid, pairs, H, base, per_image, interleaved, positions):
     x, row = _token_stride(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    C = x.shape[-1]
-    nb, P = (x.shape[0], math.prod(x.shape[1:-1])) if x.dim() > 2 else (1, x.shape[0])
+    shape = x.shape
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    C = shape[-1]
+    nb, P = (shape[0], math.prod(shape[1:-1])) if len(shape) > 2 else (1, shape[0])
     n1, n2, n3 = grid
     p1, p2, p3 = (*pairs, 0, 0)[:3]
-    _call(x.device, "circatt_axial_rotary", _CODES[x.dtype], inverse, 1 if interleaved else 0, len(pairs), n1, n2, n3,
+    _call(x.device, L.lib.circatt_axial_rotary, _CODES[x.dtype], inverse, 1 if interleaved else 0, len(pairs), n1, n2, n3,
           P, nb, H, C // H, p1, p2, p3, base, x.data_ptr(), row, ptr(positions),
           P * len(pairs) if per_image else 0, y.data_ptr())
     return y

@@ -17,16 +17,9 @@ struct alignas(sizeof(T) * V == 16 ? 16 : sizeof(T)) Vec {
     T e[V];
 };
 
-// TB tokens a workgroup; V channels a unit (V divides D, every section and
-// every row); a thread turns the unit that holds a pair's first member, and the
-// unit of its second where the two lie apart.
-template <typename T, int V, bool INTERLEAVED>
-__global__ __launch_bounds__(256) void rotary_kernel(RotaryProblem pr, int TB, FastDiv d1, FastDiv d2, FastDiv dtoken,
-                                                     FastDiv dunits, FastDiv dpairs) {
-    extern __shared__ float2 table[];  // (TB, npairs): cos, sin
-    const int64_t blocks = (pr.P + TB - 1) / TB;
-    const int64_t img = blockIdx.x / blocks, t0 = (blockIdx.x - img * blocks) * TB;
-    const int nt = pr.P - t0 < TB ? (int)(pr.P - t0) : TB;
+// The (nt, npairs) cosines and sines of tokens t0 .. t0 + nt of image img.
+__device__ __forceinline__ void form_angles(const RotaryProblem &pr, float2 *table, int64_t img, int64_t t0, int nt,
+                                            FastDiv d1, FastDiv d2, FastDiv dpairs) {
     for (int e = threadIdx.x; e < nt * pr.npairs; e += 256) {
         const int t = fdiv(e, dpairs), i = e - t * pr.npairs;
         const int axis = i < pr.pairs[0] ? 0 : i < pr.pairs[0] + pr.pairs[1] ? 1 : 2;
@@ -41,6 +34,93 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryProblem pr, int TB, F
         const float f = (float)(turns - __builtin_rint(turns)), sn = __builtin_amdgcn_sinf(f);
         table[e] = make_float2(__builtin_amdgcn_cosf(f), pr.inverse ? -sn : sn);
     }
+}
+
+// The section of channel c of a head: its first channel and pair, and its pairs
+// (0: the channel stays).  Sections of 2 p channels follow axis by axis.
+struct Section {
+    int at, pair, p;
+    __device__ __forceinline__ Section(const RotaryProblem &pr, int c) : at(0), pair(0), p(0) {
+        for (int a = 0; a < pr.naxes; ++a) {
+            p = pr.pairs[a];
+            if (c < at + 2 * p) return;
+            at += 2 * p;
+            pair += p;
+        }
+        p = 0;
+    }
+};
+
+// Heads of 16-byte units whose sections may end within one: TB tokens
+// go to LDS, and every channel reads its partner and its angle there, at places
+// that a thread, which has the same unit of a head for every token and head,
+// knows from the start.
+template <typename T>
+__global__ __launch_bounds__(256) void rotary_any_kernel(RotaryProblem pr, int TB, FastDiv d1, FastDiv d2, FastDiv dheads,
+                                                         FastDiv dpairs) {
+    constexpr int V = 16 / sizeof(T);
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    extern __shared__ char mem[];
+    const int row = pr.H * pr.D, uph = pr.D / V, upt = pr.H * uph;
+    T *xs = reinterpret_cast<T *>(mem);                            // (TB, row)
+    float2 *table = reinterpret_cast<float2 *>(xs + TB * row);     // (TB, npairs)
+    const int64_t blocks = (pr.P + TB - 1) / TB;
+    const int64_t img = blockIdx.x / blocks, t0 = (blockIdx.x - img * blocks) * TB;
+    const int nt = pr.P - t0 < TB ? (int)(pr.P - t0) : TB;
+    const T *x = static_cast<const T *>(pr.x) + (img * pr.P + t0) * pr.x_row;
+    T *y = static_cast<T *>(pr.y) + (img * pr.P + t0) * (int64_t)row;
+    // whole heads: the threads behind the last one are idle
+    const int step = 256 / uph, h0 = threadIdx.x / uph, u = threadIdx.x - h0 * uph;
+    if (h0 < step)
+        for (int n = h0; n < nt * pr.H; n += step) {
+            const int t = fdiv(n, dheads);
+            reinterpret_cast<u4 *>(xs)[n * uph + u] =
+                reinterpret_cast<const u4 *>(x + t * pr.x_row)[(n - t * pr.H) * uph + u];
+        }
+    form_angles(pr, table, img, t0, nt, d1, d2, dpairs);
+    __syncthreads();
+    if (h0 >= step) return;
+    int partner[V], pair[V];
+    bool second[V];
+    for (int e = 0; e < V; ++e) {
+        const int c = u * V + e;
+        const Section sec(pr, c);
+        const int k = c - sec.at;
+        second[e] = sec.p > 0 && (pr.interleaved ? k & 1 : k >= sec.p);
+        partner[e] = sec.p == 0 ? 0 : pr.interleaved ? (k & 1 ? -1 : 1) : k < sec.p ? sec.p : -sec.p;
+        pair[e] = sec.p == 0 ? -1 : sec.pair + (pr.interleaved ? k / 2 : k < sec.p ? k : k - sec.p);
+    }
+    for (int n = h0; n < nt * pr.H; n += step) {
+        const int t = fdiv(n, dheads);
+        const T *xr = xs + n * pr.D + u * V;
+        const float2 *cs = table + t * pr.npairs;
+        union {
+            u4 u;
+            T e[V];
+        } v;
+        v.u = *reinterpret_cast<const u4 *>(xr);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            if (pair[e] < 0) continue;
+            const float2 w = cs[pair[e]];
+            const float m = (float)xr[e + partner[e]] * w.y;
+            v.e[e] = (T)fmaf((float)v.e[e], w.x, second[e] ? m : -m);
+        }
+        reinterpret_cast<u4 *>(y)[n * uph + u] = v.u;
+    }
+}
+
+// TB tokens a workgroup; V channels a unit (V divides D, every section and
+// every row); a thread turns the unit that holds a pair's first member, and the
+// unit of its second where the two lie apart.
+template <typename T, int V, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryProblem pr, int TB, FastDiv d1, FastDiv d2, FastDiv dtoken,
+                                                     FastDiv dunits, FastDiv dpairs) {
+    extern __shared__ float2 table[];  // (TB, npairs): cos, sin
+    const int64_t blocks = (pr.P + TB - 1) / TB;
+    const int64_t img = blockIdx.x / blocks, t0 = (blockIdx.x - img * blocks) * TB;
+    const int nt = pr.P - t0 < TB ? (int)(pr.P - t0) : TB;
+    form_angles(pr, table, img, t0, nt, d1, d2, dpairs);
     __syncthreads();
     const T *x = static_cast<const T *>(pr.x) + (img * pr.P + t0) * pr.x_row;
     T *y = static_cast<T *>(pr.y) + (img * pr.P + t0) * ((int64_t)pr.H * pr.D);
@@ -52,35 +132,28 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryProblem pr, int TB, F
         const int c = (u - fdiv(u, dunits) * uph) * V;  // channel in the head
         const U *xp = reinterpret_cast<const U *>(x + t * pr.x_row) + u;
         U *yp = reinterpret_cast<U *>(y) + n;
-        // the section of the channel: sections of 2 p channels, axis by axis
-        int at = 0, pair = 0, p = 0;
-        for (int a = 0; a < pr.naxes; ++a) {
-            p = pr.pairs[a];
-            if (c < at + 2 * p) break;
-            at += 2 * p;
-            pair += p;
-            p = 0;
-        }
+        const Section sec(pr, c);
+        const int p = sec.p;
         if (p == 0) {
             *yp = *xp;
         } else if (INTERLEAVED) {
             U v = *xp;
-            const int i = pair + (c - at) / 2;
+            const int i = sec.pair + (c - sec.at) / 2;
             for (int e = 0; e < V / 2; ++e) {
                 const float2 w = cs[i + e];
                 const float a = (float)v.e[2 * e], b = (float)v.e[2 * e + 1];
                 v.e[2 * e] = (T)fmaf(a, w.x, -(b * w.y));
-                v.e[2 * e + 1] = (T)fmaf(a, w.y, b * w.x);
+                v.e[2 * e + 1] = (T)fmaf(b, w.x, a * w.y);
             }
             *yp = v;
-        } else if (c < at + p) {
-            const int i = pair + c - at, far = p / V;
+        } else if (c < sec.at + p) {
+            const int i = sec.pair + c - sec.at, far = p / V;
             U va = *xp, vb = xp[far];
             for (int e = 0; e < V; ++e) {
                 const float2 w = cs[i + e];
                 const float a = (float)va.e[e], b = (float)vb.e[e];
                 va.e[e] = (T)fmaf(a, w.x, -(b * w.y));
-                vb.e[e] = (T)fmaf(a, w.y, b * w.x);
+                vb.e[e] = (T)fmaf(b, w.x, a * w.y);
             }
             *yp = va;
             yp[far] = vb;
@@ -104,19 +177,32 @@ void launch(const RotaryProblem &pr, hipStream_t s) {
         rotary_kernel<T, V, false><<<blocks, 256, lds, s>>>(pr, TB, d1, d2, dt, du, dp);
 }
 
-// Units of 16 bytes, or of one pair (interleaved) or one channel, by what
-// divides the head, its sections, the token stride and both addresses.
+template <typename T>
+bool launch_any(const RotaryProblem &pr, hipStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const int row = pr.H * pr.D, units = row / V, most = 4096 / pr.npairs;
+    int TB = (1024 + units - 1) / units;
+    TB = TB < most ? TB : most;
+    const size_t lds = (size_t)TB * (row * sizeof(T) + pr.npairs * 8);
+    if (pr.D / V > 256 || lds > 64 * 1024) return false;
+    rotary_any_kernel<T><<<(unsigned)(pr.nb * ((pr.P + TB - 1) / TB)), 256, lds, s>>>(
+        pr, TB, make_fastdiv(pr.n1), make_fastdiv(pr.n2), make_fastdiv(pr.H), make_fastdiv(pr.npairs));
+    return true;
+}
+
+// Units of 16 bytes where they divide the head, its sections, the token stride
+// and both addresses; by way of LDS where they divide all but the sections; else
+// single pairs (interleaved) or channels.
 template <typename T>
 void route(const RotaryProblem &pr, hipStream_t s) {
     const int per = pr.interleaved ? 2 : 1;
     int sections = pr.D;
     for (int a = 0; a < pr.naxes; ++a) sections |= pr.pairs[a] * per;
-    auto fits = [&](int v) {
-        const uint64_t addr = reinterpret_cast<uint64_t>(pr.x) | reinterpret_cast<uint64_t>(pr.y);
-        return sections % v == 0 && pr.x_row % v == 0 && addr % (v * sizeof(T)) == 0;
-    };
     constexpr int W = 16 / sizeof(T);
-    if (fits(W)) launch<T, W>(pr, s);
+    const uint64_t addr = reinterpret_cast<uint64_t>(pr.x) | reinterpret_cast<uint64_t>(pr.y);
+    const bool rows = pr.D % W == 0 && pr.x_row % W == 0 && addr % 16 == 0;
+    if (rows && sections % W == 0) launch<T, W>(pr, s);
+    else if (rows && launch_any<T>(pr, s)) return;
     else if (pr.interleaved) launch<T, 2>(pr, s);
     else launch<T, 1>(pr, s);
 }
