@@ -60,9 +60,9 @@ __device__ __forceinline__ void fetch_rows(const T *p, int64_t row, int k0, int 
 
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void sliding_fwd(SlidingProblem pr, int blocks) {
-    typedef FwdShape<T, DP> Sh;
-    constexpr int KT = Sh::KT, NB = KT / 32;
-    __shared__ char lds_mem[4 * Sh::TILE];
+    typedef Ring<T, DP> Rg;
+    constexpr int KT = Rg::KT, NB = Rg::NB;
+    __shared__ char lds_mem[Rg::BYTES];
     const CIRCATT_LDS char *lds = (const CIRCATT_LDS char *)lds_mem;
     const BlockOrder w(pr.B * pr.Hk, blocks);
     if (w.unit < 0) return;
@@ -84,22 +84,82 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
         const Sight see{pr.W, pr.S};
         const TileList<KT> tiles(r0 / pr.G, last / pr.G, pr.W, pr.S);
         const float c = pr.scale * kLog2e;
-        auto fetch = [&](int i) {
-            const int k0 = tiles.key(i);
-            fetch_rows<T, DP, KT, 256>(kh, pr.k_row, k0, n, pr.D, lds + (i & 1) * 2 * Sh::TILE);
-            fetch_rows<T, DP, KT, 256>(vh, pr.v_row, k0, n, pr.D, lds + (i & 1) * 2 * Sh::TILE + Sh::TILE);
+        const Feed<T, DP> fk(kh, pr.k_row, n, pr.D), fv(vh, pr.v_row, n, pr.D);
+        const unsigned ring = lds_byte(lds);
+        const int count = uniform(tiles.count);
+        // places of K tile i + 1 (and i + 3, i) and V tile i (i + 1: the other)
+        int kp = 0, vp = 1;
+        auto round = [&](int i) {
+            Rg::wait(i + 2 < count);
+            if (i + 1 < count) fv.fetch(tiles.key(i + 1), ring + Rg::V + (vp ^ 1) * Rg::TILE);
+            if (i + 3 < count) fk.fetch(tiles.key(i + 3), ring + (kp == 0 ? 2 : kp - 1) * Rg::TILE);
         };
-        const unsigned row_at = Tile<T, DP>::row_lane(lane), col_at = Tile<T, DP>::col_lane(lane);
+        auto next = [&] {
+            kp = kp == 2 ? 0 : kp + 1;
+            vp ^= 1;
+        };
+        fk.fetch(tiles.key(0), ring);
+        if (count > 1) fk.fetch(tiles.key(1), ring + Rg::TILE);
         Rows<T, DP> x;
-        fetch(0);
         x.start(qh + at * pr.q_row + (int64_t)g * pr.D, pr.D, lane);
-        for (int i = 0; i < tiles.count; ++i) {
-            dma_barrier();
-            if (i + 1 < tiles.count) fetch(i + 1);
+        // the tiles that this wavefront's rows see: from `first` to `end`, but for
+        // those that the list leaves out
+        int first = 0, end = live ? count - 1 : -1;
+        while (first < end && see.none(lo, hi, tiles.key(first), KT)) ++first;
+        while (end > first && see.none(lo, hi, tiles.key(end), KT)) --end;
+        const unsigned row_at = Tile<T, DP>::row_lane(lane) + ring, col_at = Tile<T, DP>::col_lane(lane) + ring + Rg::V;
+        float mx = 0.f;
+        auto look = [&](f16v (&s)[NB], int i) {  // hide keys of tile i, largest score
             const int k0 = tiles.key(i);
-            const unsigned to = lds_byte(lds) + (i & 1) * 2 * Sh::TILE;
-            if (!live || see.none(lo, hi, k0, KT)) continue;
-            x.template tile<NB>(row_at + to, col_at + to + Sh::TILE, lane, at, k0, see, !see.all(lo, hi, k0, KT), 0, c);
+            if (!see.all(lo, hi, k0, KT)) {
+                asm volatile("");  // a branch: few tiles need it
+#pragma unroll
+                for (int m = 0; m < NB; ++m) {
+                    const int b0 = at + 1 - k0 - 32 * m, s0 = pr.S - k0 - 32 * m;
+                    const uint32_t half = (bits_between(b0 - pr.W, b0) | bits_between(0, b0 < s0 ? b0 : s0)) >> (4 * (lane >> 5));
+#pragma unroll
+                    for (int y = 0; y < 16; ++y)
+                        if (!(half & place_bit(y))) s[m][y] = -INFINITY;
+                }
+            }
+            mx = x.largest(s) * c;
+        };
+        auto step = [&](const f16v (&s)[NB], f16v (&t)[NB], int i) {
+            round(i);
+            V8<T> p[2 * NB];
+            x.raise(mx);
+            x.scores(row_at + kp * Rg::TILE, t);
+            x.weigh(s, p, c);
+            x.template add<NB>(col_at + vp * Rg::TILE, p);
+            next();
+            look(t, i + 1);
+        };
+        f16v a[NB], b[NB];
+        int i = -1;
+        for (; i < (live ? first - 1 : count); ++i, next()) round(i);
+        if (live) {
+            round(i);
+            x.scores(row_at + kp * Rg::TILE, a);
+            look(a, first);
+            next();
+            ++i;
+            for (; i + 1 < end; i += 2) {
+                step(a, b, i);
+                step(b, a, i + 1);
+            }
+            if (i < end) {
+                step(a, b, i);
+#pragma unroll
+                for (int m = 0; m < NB; ++m) a[m] = b[m];
+                ++i;
+            }
+            round(i);
+            V8<T> p[2 * NB];
+            x.raise(mx);
+            x.weigh(a, p, c);
+            x.template add<NB>(col_at + vp * Rg::TILE, p);
+            next();
+            for (++i; i < count; ++i, next()) round(i);
         }
         if (live) {
             const float l = x.total(), inv = l == 0.f ? 0.f : 1.f / l;

@@ -125,6 +125,13 @@ __device__ __forceinline__ void dma16_global(const void *p, unsigned m0) {
 __device__ __forceinline__ unsigned lds_byte(const CIRCATT_LDS char *p) { return (unsigned)(uintptr_t)p; }
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// the other half's value of the same query row
+__device__ __forceinline__ float other_half(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x),
+                                                    false, false);
+    return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+
 // Eight channels from global memory, zero from channel D on (D a multiple of 8).
 template <typename T>
 __device__ __forceinline__ V8<T> load8(const T *p, int d, int D) {
@@ -156,6 +163,15 @@ struct Sight {
     }
 };
 
+// Bits x of [lo, hi) among 0 .. 31.
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
+    const uint32_t below = hi <= 0 ? 0u : hi >= 32 ? ~0u : (1u << hi) - 1u;
+    return lo <= 0 ? below : lo >= 32 ? 0u : below & (~0u << lo);
+}
+// The place of a 32x32 result's register i in a word of 32 places that is shifted
+// down by 4 for the lanes of the second half.
+__device__ __forceinline__ constexpr uint32_t place_bit(int i) { return 1u << (8 * (i >> 2) + (i & 3)); }
+
 // The tiles of KT keys that rows at [lo, hi] see, in order: tiles of sinks, then
 // of the window.
 template <int KT>
@@ -168,6 +184,68 @@ struct TileList {
         count = hi < 0 ? 0 : sinks + hi / KT + 1 - w;
     }
     __device__ __forceinline__ int key(int i) const { return (i < sinks ? i : first + i - sinks) * KT; }
+};
+
+// A workgroup's tiles of KT keys in LDS, three places for K and two for V.  Round
+// i forms the scores of tile i + 1 from its K tile while it adds the values of tile
+// i; then V tile i + 1 and K tile i + 3 set out for the places that round i - 1
+// left.
+template <typename T, int DP>
+struct Ring {
+    typedef Tile<T, DP> Tl;
+    // Float32 rows are twice as long: half the keys fill the same LDS
+    static constexpr int NB = sizeof(T) == 2 ? 2 : 1, KT = 32 * NB;
+    static constexpr int TILE = KT * Tl::ROW, BYTES = 5 * TILE, V = 3 * TILE;
+    static constexpr int EACH = KT * Tl::PC / 256;  // a thread's DMA for one tile
+    static_assert(EACH >= 1, "");
+    // the workgroup's DMA but for the last tile's, or all of it, is done, and every
+    // wavefront is past the round before
+    __device__ static __forceinline__ void wait(bool but_one) {
+        if (but_one) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(EACH) : "memory");
+        else dma_barrier();
+    }
+};
+
+// One tensor's n rows on the way into a ring: byte offsets of this thread's units
+// of a tile, which are the same for every tile, and the buffer.  A tensor whose
+// rows span less than 2 GiB is one buffer, and a tile an offset in it; else every
+// tile is a buffer of its own.
+template <typename T, int DP>
+struct Feed {
+    typedef Tile<T, DP> Tl;
+    static constexpr int KT = Ring<T, DP>::KT, EACH = Ring<T, DP>::EACH;
+    const T *p;
+    int64_t row;
+    int n, rb, last;  // bytes from row to row, and of a row's channels
+    bool one;
+    dma::i4v all;
+    int off[EACH];
+    __device__ __forceinline__ Feed(const T *p, int64_t row, int n, int D) : p(p), row(row), n(n) {
+        rb = (int)(row * (int)sizeof(T));
+        last = D * (int)sizeof(T);
+        const int64_t bytes = (int64_t)(n - 1) * rb + last;
+        one = bytes + KT * (int64_t)rb < dma::kMaxBytes;
+        all = dma::dma_rsrc(reinterpret_cast<const float *>(p), one ? (int)bytes : 0);
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            const int slot = threadIdx.x + k * 256, r = slot / Tl::PC, u = (slot % Tl::PC) ^ Tl::f(r);
+            off[k] = u * 16 < last ? r * rb + u * 16 : dma::kOut;
+        }
+    }
+    // rows [k0, k0 + KT), k0 < n, to LDS byte `to`; rows from n on are zeros
+    __device__ __forceinline__ void fetch(int k0, unsigned to) const {
+        const unsigned m0 = to + uniform(threadIdx.x >> 6) * 1024;
+        if (__builtin_expect(one, 1)) {
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) dma::dma16(all, m0 + k * 4096, off[k], k0 * rb);
+        } else {
+            const int64_t bytes = (int64_t)(n - 1 - k0) * rb + last;
+            const dma::i4v rs = dma::dma_rsrc(reinterpret_cast<const float *>(p + k0 * row),
+                                              (int)(bytes < dma::kMaxBytes ? bytes : dma::kMaxBytes));
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) dma::dma16(rs, m0 + k * 4096, off[k], 0);
+        }
+    }
 };
 
 // Running softmax and output of 32 rows (lane l and l + 32: row l % 32).
@@ -246,6 +324,59 @@ struct Rows {
         for (int t = 0; t < OT; ++t)
 #pragma unroll
             for (int n = 0; n < 2 * NB; ++n) o[t] = mma(Tl::col(vt, 16 * n, t), p[n], o[t]);
+    }
+
+    // The same in steps, for NB blocks of 32 keys a round.
+    template <int NB>
+    __device__ __forceinline__ void scores(unsigned kt, f16v (&s)[NB]) const {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) s[n] = f16v{};
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) s[n] = mma(Tile<T, DP>::row(kt, 32 * n, k), q[k], s[n]);
+    }
+    // the row's largest score, over both halves
+    template <int NB>
+    __device__ __forceinline__ static float largest(const f16v (&s)[NB]) {
+        float mx = s[0][0];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
+        return fmaxf(mx, other_half(mx));
+    }
+    __device__ __forceinline__ void raise(float mx) {
+        if (__any(mx > m + RAISE || (m == -INFINITY && mx > -INFINITY))) {
+            const float mn = fmaxf(m, mx), r = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            l *= r;
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] *= r;
+            m = mn;
+        }
+    }
+    template <int NB>
+    __device__ __forceinline__ void weigh(const f16v (&s)[NB], V8<T> (&p)[2 * NB], float c) {
+        const float mu = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -mu));
+                sum += e;
+                p[2 * n + (i >> 3)][i & 7] = (T)e;
+            }
+        l += sum;
+    }
+    template <int NB>
+    __device__ __forceinline__ void add(unsigned vt, const V8<T> (&p)[2 * NB]) {
+#pragma unroll
+        for (int n = 0; n < 2 * NB; ++n)
+#pragma unroll
+            for (int t = 0; t < OT; ++t) o[t] = mma(Tile<T, DP>::col(vt, 16 * n, t), p[n], o[t]);
     }
 
     // sum over both halves' keys
