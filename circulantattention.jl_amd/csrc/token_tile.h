@@ -13,9 +13,9 @@
 // 16 lanes).  Nothing crosses lanes between the two products.  Float32 operands
 // take the same registers: place j of every lane is one 32x32x2 product.
 //
-// Rows lie in LDS as PC 16-byte units, the unit c of row r at c ^ f(r): eight
-// consecutive rows of one unit (the 16-byte reads) and four rows of two units
-// (the transposing reads) fall into different banks.  The tiles arrive by
+// Rows lie in LDS as PC 16-byte units, the unit c of row r at c ^ f(r): 16 rows of
+// one unit (the 16-byte reads) and four rows of four units (the transposing reads
+// of 32 lanes) each fill the 64 banks once.  The tiles arrive by
 // 16-byte LDS-DMA, whose lanes write consecutive units, so the permutation is
 // applied to the addresses that they read.
 #pragma once
@@ -53,9 +53,9 @@ struct Tile {
     static constexpr int UNITS = DP * (int)sizeof(T) / 16;  // read
     static constexpr int PC = UNITS <= 4 ? 4 : UNITS <= 8 ? 8 : UNITS <= 16 ? 16 : 32;
     static constexpr int ROW = PC * 16;  // bytes
-    __device__ static __forceinline__ int f(int r) {
-        return PC >= 16 ? ((r & 7) << 1) | ((r >> 3) & 1)
-                        : PC == 8 ? ((r & 3) << 1) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1);
+    __device__ static __forceinline__ constexpr int f(int r) {
+        return PC >= 16 ? ((r & 3) << 2) | ((r >> 2) & 3)
+                        : PC == 8 ? ((r & 2) << 1) | ((r >> 2) & 3) : (r >> 2) & 3;
     }
     // LDS bytes are 32-bit numbers here: a lane's place in a tile, and every read
     // of it is that number with a few bits flipped (the unit's number) and a
@@ -99,14 +99,14 @@ struct Tile {
 #pragma unroll
             for (int k = 0; k < 2; ++k)
                 u.s[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (CIRCATT_LDS s4v *)((at ^ (t << 6 | f(8 * k) << 4)) + (m + 8 * k) * ROW));
+                    (CIRCATT_LDS s4v *)((at ^ (t << 6) ^ (f(8 * k) << 4)) + (m + 8 * k) * ROW));
             return u.v;
         } else {
             V8<T> v;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int r = 8 * (j >> 2) + (j & 3);
-                v[j] = *(const CIRCATT_LDS float *)((at ^ (t << 7 | f(r) << 4)) + (m + r) * ROW);
+                v[j] = *(const CIRCATT_LDS float *)((at ^ (t << 7) ^ (f(r) << 4)) + (m + r) * ROW);
             }
             return v;
         }
