@@ -167,7 +167,7 @@ void paged_kernel(PagedProblem pr, PagedGrid gr) {
     typedef PagedShape<T, DP, ONE> Sh;
     typedef Tile<T, DP> Tl;
     constexpr int KT = Sh::KT, NB = KT / 32, R = Sh::R, NW = Sh::NW, OT = DP / 32;
-    __shared__ char lds_mem[Sh::LDS];
+    __shared__ __attribute__((aligned(1024))) char lds_mem[Sh::LDS];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const CIRCATT_LDS char *lds = (const CIRCATT_LDS char *)lds_mem + (ONE ? wave * 4 * Sh::TILE : 0);
     const int hk = blockIdx.y, split = blockIdx.z;
@@ -215,6 +215,7 @@ void paged_kernel(PagedProblem pr, PagedGrid gr) {
         int now = key_row(i0), next = i0 + 1 < i1 ? key_row(i0 + 1) : -1;
         fetch_pages<T, DP, KT, ONE ? 64 : 256>(pg, now, pr.D, lds);
         x.start(qr, pr.D, lane);
+        loads_here();
         for (int i = i0; i < i1; ++i) {
             if (ONE) dma_wait();
             else dma_barrier();

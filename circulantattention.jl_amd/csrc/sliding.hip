@@ -62,7 +62,7 @@ template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void sliding_fwd(SlidingProblem pr, int blocks) {
     typedef Ring<T, DP> Rg;
     constexpr int KT = Rg::KT, NB = Rg::NB;
-    __shared__ char lds_mem[Rg::BYTES];
+    __shared__ __attribute__((aligned(1024))) char lds_mem[Rg::BYTES];
     const CIRCATT_LDS char *lds = (const CIRCATT_LDS char *)lds_mem;
     const BlockOrder w(pr.B * pr.Hk, blocks);
     if (w.unit < 0) return;
@@ -115,8 +115,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
                 asm volatile("");  // a branch: few tiles need it
 #pragma unroll
                 for (int m = 0; m < NB; ++m) {
-                    const int b0 = at + 1 - k0 - 32 * m, s0 = pr.S - k0 - 32 * m;
-                    const uint32_t half = (bits_between(b0 - pr.W, b0) | bits_between(0, b0 < s0 ? b0 : s0)) >> (4 * (lane >> 5));
+                    const uint32_t half = see.bits(at, k0 + 32 * m) >> (4 * (lane >> 5));
 #pragma unroll
                     for (int y = 0; y < 16; ++y)
                         if (!(half & place_bit(y))) s[m][y] = -INFINITY;
@@ -201,7 +200,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
     typedef FwdShape<T, DP> Sh;
     typedef Tile<T, DP> Tl;
     constexpr int KT = Sh::KT, STEPS = DP / 16, OT = DP / 32;
-    __shared__ char lds_mem[4 * Sh::TILE];
+    __shared__ __attribute__((aligned(1024))) char lds_mem[4 * Sh::TILE];
     const CIRCATT_LDS char *lds = (const CIRCATT_LDS char *)lds_mem;
     const BlockOrder w(pr.B * pr.Hk, blocks);
     if (w.unit < 0) return;
@@ -250,6 +249,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
 #pragma unroll
         for (int t = 0; t < OT; ++t) o[t] = f16v{};
         const unsigned row_at = Tl::row_lane(lane), col_at = Tl::col_lane(lane);
+        loads_here();
         for (int i = 0; i < tiles.count; ++i) {
             dma_barrier();
             if (i + 1 < tiles.count) fetch(i + 1);
@@ -260,25 +260,25 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
                 const unsigned to = lds_byte(lds) + (i & 1) * 2 * Sh::TILE + m * Tl::ROW;
                 const unsigned kr = row_at + to, vr = kr + Sh::TILE, kc = col_at + to;
                 f16v s = f16v{}, dp = f16v{};
-#pragma unroll
-                for (int k = 0; k < STEPS; ++k) {
-                    s = mma(Tl::row(kr, 0, k), q[k], s);
-                    dp = mma(Tl::row(vr, 0, k), dy[k], dp);
-                }
+                products<T, 2 * STEPS, 4>([&](int i) { return Tl::row(i & 1 ? vr : kr, 0, i >> 1); },
+                                          [&](int i, V8<T> a) {
+                                              if (i & 1) dp = mma(a, dy[i >> 1], dp);
+                                              else s = mma(a, q[i >> 1], s);
+                                          });
 #pragma unroll
                 for (int x = 0; x < 16; ++x) s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -lse)) * (dp[x] - d);
                 if (!see.all(lo, hi, k0, 32)) {
+                    asm volatile("");  // a branch: few tiles need it
+                    const uint32_t half = see.bits(at, k0) >> (4 * (lane >> 5));
 #pragma unroll
                     for (int x = 0; x < 16; ++x)
-                        if (!see(at, k0 + 8 * (x >> 2) + 4 * (lane >> 5) + (x & 3))) s[x] = 0.f;
+                        if (!(half & place_bit(x))) s[x] = 0.f;
                 }
                 V8<T> ds[2];
 #pragma unroll
                 for (int x = 0; x < 16; ++x) ds[x >> 3][x & 7] = (T)s[x];
-#pragma unroll
-                for (int t = 0; t < OT; ++t)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) o[t] = mma(Tl::col(kc, 16 * h, t), ds[h], o[t]);
+                products<T, 2 * OT, 4>([&](int i) { return Tl::col(kc, 16 * (i & 1), i >> 1); },
+                                       [&](int i, V8<T> a) { o[i >> 1] = mma(a, ds[i & 1], o[i >> 1]); });
             }
         }
         if (live) {
@@ -301,281 +301,442 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
 }
 
 // ---------------------------------------------------------------------------
-// Backward, keys: a workgroup has 128 keys of one head, 32 a wavefront, whose k
-// and v it keeps as second operands, and walks the query rows that see them in
-// tiles of QT rows of q and dy in LDS: S = Q K', dP = dY V' (lane: one key;
-// registers: query rows), P and dS = P (dP - d) as second operands of
+// Backward, keys: a wavefront keeps k and v of 32 keys as second operands and
+// walks the query rows that see them, 32 at a time: S = Q K', dP = dY V' (lane:
+// one key; registers: query rows), P and dS = P (dP - d) as second operands of
 // dV' += dY' P and dK' += Q' dS with dY' and Q' by the transposing reads.
 //
-// Blocks whose walk is long (sinks are seen to the signal's end; a causal
-// window without end; few signals and heads) are split over workgroups by the
-// tiles of the walk: each leaves Float32 partial sums, added up in order by
-// sliding_dkdv_join.
+// A workgroup has 128 keys of one head and NG groups of four wavefronts, which
+// take turns at tiles of QT rows of q and dy in LDS (two buffers each) and add up
+// at the end: one workgroup fills a compute unit's registers, and a block of keys
+// needs no second workgroup for it.  Where blocks are still few, their walks are
+// split over `parts` workgroups, whose Float32 sums sliding_dkdv_join adds up in
+// order.
+//
+// The rows that see a sink from behind its block's window are another walk,
+// sliding_dkdv_far's, for 32 keys and with a wavefront for every tile: a few
+// sinks would leave most of a workgroup of 128 keys idle.
 template <typename T, int DP>
 struct BwdShape {
     static constexpr int QT = sizeof(T) == 2 ? 64 : 32;
     static constexpr int TILE = QT * Tile<T, DP>::ROW;
-    static constexpr int PART = 128 * DP * 2;  // floats of one partial pair
+    // Float32 operands and sums of wide heads take more than half the registers
+    static constexpr int NG = sizeof(T) == 2 || DP <= 32 ? 2 : 1;
+    static constexpr int PART = 128 * DP * 2;  // floats of one pair of partial sums
+    static constexpr int FAR_PART = 32 * DP * 2;
+    static constexpr int FAR_TILE = 32 * Tile<T, DP>::ROW;
 };
 
-// How the walk is split: blocks of keys below `far` see the signal's end.
 struct WalkSplit {
-    int blocks, far, parts_far, parts;  // of 128 keys; workgroups a block of each kind
-    FastDiv heads;                      // G
-    int64_t units, far_units;           // workgroups for one signal and head of keys
+    int blocks, parts;   // of 128 keys; workgroups a block
+    int far, far_parts;  // groups of 32 sinks that rows behind their window see; workgroups each
+    FastDiv heads;       // G
+    int64_t far_at, part_at;  // floats before the far sums and the parts' in the workspace
 };
 
-struct Walk {
-    int first, count;  // packed query rows from first on, tiles
-    __device__ Walk(const SlidingProblem &pr, int kb, int n, int QT) {
-        const int k0 = kb * 128, kn = k0 + 127 < n - 1 ? k0 + 127 : n - 1;
-        int end = n;
-        if (k0 >= pr.S && n - kn > pr.W) end = kn + pr.W;
-        first = k0 * pr.G;
-        count = k0 < n ? ((end - k0) * pr.G + QT - 1) / QT : 0;
+// Tokens [begin, end) behind the window of the block of keys that key k0 is in.
+struct FarRows {
+    int first, count;  // packed query rows, and those behind them
+    __device__ FarRows(const SlidingProblem &pr, int k0, int n) {
+        const int last = k0 / 128 * 128 + 127;
+        const int begin = n - pr.W > last ? last + pr.W : n;
+        first = begin * pr.G;
+        count = (n - begin) * pr.G;
     }
 };
 
-// Packed query rows [r0, r0 + QT) of a head group: row r is head r % G of token
-// r / G; rows behind token n - 1 are zeros.
-template <typename T, int DP, int QT>
-__device__ __forceinline__ void fetch_packed(const T *p, int64_t row, int r0, int G, FastDiv dg, int n, int D,
-                                             const CIRCATT_LDS char *to) {
+// Packed query rows [r0, r0 + ROWS) of a head group by THREADS threads, this one
+// the tid-th: row r is head r % G of token r / G; rows behind token n - 1 are zeros.
+template <typename T, int DP, int ROWS, int THREADS>
+__device__ __forceinline__ void fetch_packed(const T *p, int64_t row, int r0, int G, FastDiv dg, int n, int D, int tid,
+                                             unsigned to) {
     typedef Tile<T, DP> Tl;
-    const int rb = (int)(row * (int)sizeof(T)), units = D * (int)sizeof(T) / 16;
+    const int rb = (int)(row * (int)sizeof(T)), hb = D * (int)sizeof(T);
     const int t0 = uniform(fdiv(r0, dg));
-    const int64_t bytes = n > t0 ? (int64_t)(n - 1 - t0) * rb + G * units * 16 : 0;
+    const int64_t bytes = n > t0 ? (int64_t)(n - 1 - t0) * rb + G * hb : 0;
     const dma::i4v rs = dma::dma_rsrc(reinterpret_cast<const float *>(p + t0 * row),
                                       (int)(bytes < dma::kMaxBytes ? bytes : dma::kMaxBytes));
-    const int tid = threadIdx.x;
-    const unsigned m0 = lds_byte(to) + uniform(tid >> 6) * 1024;
+    const unsigned m0 = to + uniform(tid >> 6) * 1024;
 #pragma unroll
-    for (int k = 0; k < QT * Tl::PC / 256; ++k) {
-        const int slot = tid + k * 256, rl = slot / Tl::PC, u = (slot % Tl::PC) ^ Tl::f(rl);
+    for (int k = 0; k < ROWS * Tl::PC / THREADS; ++k) {
+        const int slot = tid + k * THREADS, rl = slot / Tl::PC, u = ((slot % Tl::PC) ^ Tl::f(rl)) * 16;
         const int t = fdiv(r0 + rl, dg), g = r0 + rl - t * G;
-        dma::dma16(rs, m0 + k * 4096, u < units ? (t - t0) * rb + (g * units + u) * 16 : dma::kOut, 0);
+        // units from D on stay out of the buffer whatever is added
+        dma::dma16(rs, m0 + k * THREADS * 16, (t - t0) * rb + g * hb + (u < hb ? u : dma::kOut), 0);
     }
 }
-// QT floats from p on into LDS by the calling wavefront, zeros behind p[rows - 1]
-template <int QT>
-__device__ __forceinline__ void fetch_stats(const float *p, int r0, int rows, const CIRCATT_LDS char *to) {
-    const dma::i4v rs = dma::dma_rsrc(p + r0, rows > r0 ? (rows - r0 < QT ? rows - r0 : QT) * 4 : 0);
+// COUNT floats from p + r0 on into LDS by the calling wavefront, zeros behind p[rows - 1]
+template <int COUNT>
+__device__ __forceinline__ void fetch_stats(const float *p, int r0, int rows, unsigned to) {
+    const dma::i4v rs = dma::dma_rsrc(p + r0, rows > r0 ? (rows - r0 < COUNT ? rows - r0 : COUNT) * 4 : 0);
     const int lane = threadIdx.x & 63;
-    const unsigned m0 = lds_byte(to);
-    if (lane < QT)
-        asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" : : "v"(lane * 4), "s"(rs), "{m0}"(m0) : "memory");
+    if (lane < COUNT)
+        asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" : : "v"(lane * 4), "s"(rs), "{m0}"(to) : "memory");
 }
 
-// the partial sums behind rowsum(dy y), at a multiple of 16 bytes
-__device__ __forceinline__ float *partials(const SlidingProblem &pr) {
-    return pr.work + (((int64_t)pr.B * pr.Hk * pr.L * pr.G + 3) & ~(int64_t)3);
-}
-
+// One wavefront's 32 keys: operands, sums, and 32 query rows' share of them.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void sliding_dkdv(SlidingProblem pr, WalkSplit sp) {
-    typedef BwdShape<T, DP> Sh;
+struct KeySums {
     typedef Tile<T, DP> Tl;
-    constexpr int QT = Sh::QT, STEPS = DP / 16, OT = DP / 32;
-    __shared__ char lds_mem[4 * Sh::TILE + 4 * QT * 4];
-    const CIRCATT_LDS char *lds = (const CIRCATT_LDS char *)lds_mem;
-    // workgroup numbers of one unit: far blocks part by part, then the others
-    const int64_t id = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-    const int64_t unit = id / sp.units;
-    if (unit >= (int64_t)pr.B * pr.Hk) return;
-    const int in = (int)(id - unit * sp.units);
-    const bool is_far = in < sp.far_units;
-    const int parts = is_far ? sp.parts_far : sp.parts;
-    const int kb = is_far ? in / parts : sp.far + (in - (int)sp.far_units) / parts;
-    const int part = (is_far ? in : in - (int)sp.far_units) % parts;
-    const int b = (int)(unit / pr.Hk), hk = (int)(unit - (int64_t)b * pr.Hk), n = uniform(signal_length(pr, b));
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    const Walk walk(pr, kb, n, QT);
-    const int i0 = (int)((int64_t)walk.count * part / parts), i1 = (int)((int64_t)walk.count * (part + 1) / parts);
-    const int j0 = kb * 128 + 32 * wave, j = j0 + (lane & 31), jj = j < n ? j : n - 1;
-    const int rows = n * pr.G;
-    const bool live = j0 < n;
-    const T *kh = static_cast<const T *>(pr.k) + b * pr.k_batch + (int64_t)hk * pr.D;
-    const T *vh = static_cast<const T *>(pr.v) + b * pr.v_batch + (int64_t)hk * pr.D;
-    const T *qh = static_cast<const T *>(pr.q) + b * pr.q_batch + (int64_t)hk * pr.G * pr.D;
-    const T *gh = static_cast<const T *>(pr.dy) + b * pr.dy_batch + (int64_t)hk * pr.G * pr.D;
-    const int64_t stat = ((int64_t)b * pr.Hk + hk) * pr.L * pr.G;
-    const float *lse = pr.lse + stat, *dsum = pr.work + stat;
-    const Sight see{pr.W, pr.S};
-    const float c = pr.scale * kLog2e;
+    static constexpr int STEPS = DP / 16, OT = DP / 32, AHEAD = 4;
+    V8<T> k[STEPS], v[STEPS];
     f16v dk[OT], dv[OT];
-#pragma unroll
-    for (int t = 0; t < OT; ++t) dk[t] = dv[t] = f16v{};
-    if (i0 < i1) {
-        const CIRCATT_LDS char *stats = lds + 4 * Sh::TILE;
-        auto fetch = [&](int i) {
-            const int r0 = walk.first + i * QT;
-            const CIRCATT_LDS char *to = lds + (i & 1) * 2 * Sh::TILE;
-            fetch_packed<T, DP, QT>(qh, pr.q_row, r0, pr.G, sp.heads, n, pr.D, to);
-            fetch_packed<T, DP, QT>(gh, pr.dy_row, r0, pr.G, sp.heads, n, pr.D, to + Sh::TILE);
-            if (wave == 0) fetch_stats<QT>(lse, r0, rows, stats + (i & 1) * QT * 8);
-            if (wave == 1) fetch_stats<QT>(dsum, r0, rows, stats + (i & 1) * QT * 8 + QT * 4);
-        };
-        fetch(i0);
-        V8<T> k[STEPS], v[STEPS];
+
+    __device__ __forceinline__ void start(const T *kr, const T *vr, int D, int lane) {
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            k[s] = load8(kh + jj * pr.k_row, 16 * s + 8 * (lane >> 5), pr.D);
-            v[s] = load8(vh + jj * pr.v_row, 16 * s + 8 * (lane >> 5), pr.D);
+            k[s] = load8(kr, 16 * s + 8 * (lane >> 5), D);
+            v[s] = load8(vr, 16 * s + 8 * (lane >> 5), D);
         }
-        const unsigned row_at = Tl::row_lane(lane), col_at = Tl::col_lane(lane);
-        for (int i = i0; i < i1; ++i) {
-            dma_barrier();
-            if (i + 1 < i1) fetch(i + 1);
-            if (!live) continue;
-            for (int m = 0; m < QT; m += 32) {
-                const int r0 = walk.first + i * QT + m;
-                // tokens of the 32 rows
-                const int t0 = uniform(fdiv(r0, sp.heads)), t1 = uniform(fdiv(r0 + 31, sp.heads));
-                if (t0 >= n || j0 > t1 || (j0 + 31 <= t0 - pr.W && j0 >= pr.S)) continue;
-                const unsigned to = lds_byte(lds) + (i & 1) * 2 * Sh::TILE + m * Tl::ROW;
-                const unsigned qr = row_at + to, gr = qr + Sh::TILE, qc = col_at + to, gc = qc + Sh::TILE;
-                const CIRCATT_LDS char *st = stats + (i & 1) * QT * 8 + (m + 4 * (lane >> 5)) * 4;
-                f16v s = f16v{}, dp = f16v{};
+        clear();
+        loads_here();
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-                for (int x = 0; x < STEPS; ++x) {
-                    s = mma(Tl::row(qr, 0, x), k[x], s);
-                    dp = mma(Tl::row(gr, 0, x), v[x], dp);
-                }
+        for (int t = 0; t < OT; ++t) dk[t] = dv[t] = f16v{};
+    }
+    // rows of q and dy at the lane's places qr, gr (row) and qc, gc (col); lse and d
+    // of the rows at LDS bytes st and st + stride; half: the rows that see the key, a
+    // bit each, or all where every() holds
+    __device__ __forceinline__ void add(unsigned qr, unsigned gr, unsigned qc, unsigned gc, unsigned st, int stride,
+                                        bool every, uint32_t half, float c) {
+        f16v s = f16v{}, dp = f16v{};
+        products<T, 2 * STEPS, AHEAD>([&](int i) { return Tl::row(i & 1 ? gr : qr, 0, i >> 1); },
+                                      [&](int i, V8<T> a) {
+                                          if (i & 1) dp = mma(a, v[i >> 1], dp);
+                                          else s = mma(a, k[i >> 1], s);
+                                      });
 #pragma unroll
-                for (int x = 0; x < 16; x += 4) {
-                    const f4v ls = *(const CIRCATT_LDS f4v *)(st + 8 * x);
-                    const f4v dd = *(const CIRCATT_LDS f4v *)(st + QT * 4 + 8 * x);
+        for (int x = 0; x < 16; x += 4) {
+            const f4v ls = *(const CIRCATT_LDS f4v *)(st + 8 * x);
+            const f4v dd = *(const CIRCATT_LDS f4v *)(st + stride + 8 * x);
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        s[x + y] = __builtin_amdgcn_exp2f(fmaf(s[x + y], c, -ls[y]));
-                        dp[x + y] = s[x + y] * (dp[x + y] - dd[y]);
-                    }
-                }
-                if (!(j0 + 31 <= t0 && (j0 > t1 - pr.W || j0 + 32 <= pr.S))) {
-#pragma unroll
-                    for (int x = 0; x < 16; ++x)
-                        if (!see(fdiv(r0 + 8 * (x >> 2) + 4 * (lane >> 5) + (x & 3), sp.heads), j)) s[x] = dp[x] = 0.f;
-                }
-                V8<T> p[2], ds[2];
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    p[x >> 3][x & 7] = (T)s[x];
-                    ds[x >> 3][x & 7] = (T)dp[x];
-                }
-#pragma unroll
-                for (int t = 0; t < OT; ++t)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        dv[t] = mma(Tl::col(gc, 16 * h, t), p[h], dv[t]);
-                        dk[t] = mma(Tl::col(qc, 16 * h, t), ds[h], dk[t]);
-                    }
+            for (int y = 0; y < 4; ++y) {
+                s[x + y] = __builtin_amdgcn_exp2f(fmaf(s[x + y], c, -ls[y]));
+                dp[x + y] = s[x + y] * (dp[x + y] - dd[y]);
             }
         }
+        if (!every) {
+            asm volatile("");  // a branch: few rows need it
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+                if (!(half & place_bit(x))) s[x] = dp[x] = 0.f;
+        }
+        V8<T> p[2], ds[2];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            p[x >> 3][x & 7] = (T)s[x];
+            ds[x >> 3][x & 7] = (T)dp[x];
+        }
+        products<T, 4 * OT, AHEAD>([&](int i) { return Tl::col(i & 1 ? qc : gc, 16 * ((i >> 1) & 1), i >> 2); },
+                                   [&](int i, V8<T> a) {
+                                       if (i & 1) dk[i >> 2] = mma(a, ds[(i >> 1) & 1], dk[i >> 2]);
+                                       else dv[i >> 2] = mma(a, p[(i >> 1) & 1], dv[i >> 2]);
+                                   });
     }
-    if (parts > 1) {
-        const int64_t slot = is_far ? unit * sp.far_units + in
-                                    : (sp.parts_far > 1 ? (int64_t)pr.B * pr.Hk * sp.far_units : 0) +
-                                          unit * (sp.units - sp.far_units) + (in - sp.far_units);
-        float *w = partials(pr) + slot * Sh::PART + (32 * wave + (lane & 31)) * DP;
+    // through LDS or a workspace, one float for every register and lane
+    template <typename P>
+    __device__ __forceinline__ void put(P to, int lane) const {
+#pragma unroll
+        for (int t = 0; t < OT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                to[(16 * t + i) * 64 + lane] = dk[t][i];
+                to[(16 * (OT + t) + i) * 64 + lane] = dv[t][i];
+            }
+    }
+    __device__ __forceinline__ void take(const CIRCATT_LDS float *from, int lane) {
+#pragma unroll
+        for (int t = 0; t < OT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                dk[t][i] += from[(16 * t + i) * 64 + lane];
+                dv[t][i] += from[(16 * (OT + t) + i) * 64 + lane];
+            }
+    }
+    // Float32 sums to a workspace: the lane's key's channels, dv `apart` floats
+    // behind dk
+    __device__ __forceinline__ void write(float *w, int apart, int lane) const {
 #pragma unroll
         for (int t = 0; t < OT; ++t)
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const int d = 32 * t + 2 * i + 4 * (lane >> 5);
                 *reinterpret_cast<f4v *>(w + d) = f4v{dk[t][i], dk[t][i + 1], dk[t][i + 2], dk[t][i + 3]};
-                *reinterpret_cast<f4v *>(w + 128 * DP + d) = f4v{dv[t][i], dv[t][i + 1], dv[t][i + 2], dv[t][i + 3]};
+                *reinterpret_cast<f4v *>(w + apart + d) = f4v{dv[t][i], dv[t][i + 1], dv[t][i + 2], dv[t][i + 3]};
             }
+    }
+};
+
+// A head of keys and its group of queries' heads.
+template <typename T>
+struct HeadGroup {
+    int b, hk, n, rows;
+    const T *k, *v, *q, *dy;
+    const float *lse, *dsum;
+    __device__ HeadGroup(const SlidingProblem &pr, int64_t unit) {
+        b = (int)(unit / pr.Hk);
+        hk = (int)(unit - (int64_t)b * pr.Hk);
+        n = uniform(signal_length(pr, b));
+        rows = n * pr.G;
+        const int64_t head = (int64_t)hk * pr.D;
+        k = static_cast<const T *>(pr.k) + b * pr.k_batch + head;
+        v = static_cast<const T *>(pr.v) + b * pr.v_batch + head;
+        q = static_cast<const T *>(pr.q) + b * pr.q_batch + head * pr.G;
+        dy = static_cast<const T *>(pr.dy) + b * pr.dy_batch + head * pr.G;
+        const int64_t stat = unit * pr.L * pr.G;
+        lse = pr.lse + stat;
+        dsum = pr.work + stat;
+    }
+    // dk, dv of key j from its rows alone
+    __device__ void again(const SlidingProblem &pr, int j) const {
+        const int64_t out = ((int64_t)b * pr.L + j) * pr.Hk * pr.D + (int64_t)hk * pr.D;
+        dkdv_row(k + j * pr.k_row, v + j * pr.v_row, q, pr.q_row, dy, pr.dy_row, lse, dsum, static_cast<T *>(pr.dk) + out,
+                 static_cast<T *>(pr.dv) + out, j, n, pr.W, pr.S, pr.G, pr.D, pr.scale * kLog2e, pr.scale);
+    }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void sliding_dkdv_far(SlidingProblem pr, WalkSplit sp) {
+    typedef BwdShape<T, DP> Sh;
+    typedef Tile<T, DP> Tl;
+    // two buffers for each wavefront, but for tiles that are too long for that
+    constexpr int BUFS = 16 * Sh::FAR_TILE <= 128 * 1024 ? 2 : 1, STATS = 8 * BUFS * Sh::FAR_TILE;
+    constexpr int SUMS = 32 * DP * 2 * 4;
+    __shared__ __attribute__((aligned(1024))) char lds_mem[STATS + BUFS * 1024 > SUMS ? STATS + BUFS * 1024 : SUMS];
+    const int64_t unit = blockIdx.x / (sp.far * sp.far_parts);
+    const int in = (int)(blockIdx.x - unit * (sp.far * sp.far_parts)), k0 = in / sp.far_parts * 32, part = in % sp.far_parts;
+    const HeadGroup<T> hg(pr, unit);
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), j = k0 + (lane & 31);
+    const unsigned lds = lds_byte((const CIRCATT_LDS char *)lds_mem) + wave * (2 * BUFS * Sh::FAR_TILE);
+    const unsigned st = lds_byte((const CIRCATT_LDS char *)lds_mem) + STATS + wave * BUFS * 256;
+    KeySums<T, DP> x;
+    // a block of keys in which none is seen from behind its window adds nothing
+    const FarRows far(pr, k0, hg.n);
+    const int tiles = (far.count + 31) / 32, parts = 4 * sp.far_parts, w = 4 * part + wave;
+    const int i0 = (int)((int64_t)tiles * w / parts), i1 = (int)((int64_t)tiles * (w + 1) / parts);
+    if (i0 < i1) {
+        const int jj = j < hg.n ? j : hg.n - 1;
+        x.start(hg.k + jj * pr.k_row, hg.v + jj * pr.v_row, pr.D, lane);
+        const unsigned row_at = Tl::row_lane(lane) + lds, col_at = Tl::col_lane(lane) + lds;
+        auto fetch = [&](int i) {
+            const int r0 = far.first + 32 * i, y = BUFS == 2 ? i & 1 : 0;
+            const unsigned to = lds + y * 2 * Sh::FAR_TILE;
+            fetch_packed<T, DP, 32, 64>(hg.q, pr.q_row, r0, pr.G, sp.heads, hg.n, pr.D, lane, to);
+            fetch_packed<T, DP, 32, 64>(hg.dy, pr.dy_row, r0, pr.G, sp.heads, hg.n, pr.D, lane, to + Sh::FAR_TILE);
+            fetch_stats<32>(hg.lse, r0, hg.rows, st + y * 256);
+            fetch_stats<32>(hg.dsum, r0, hg.rows, st + y * 256 + 128);
+        };
+        if (BUFS == 2) fetch(i0);
+        for (int i = i0; i < i1; ++i) {
+            const int y = BUFS == 2 ? i & 1 : 0;
+            dma_wait();  // the tile's DMA, and the reads of the one before
+            if (BUFS == 1) {
+                fetch(i);
+                dma_wait();
+            } else if (i + 1 < i1) {
+                fetch(i + 1);
+            }
+            const unsigned to = y * 2 * Sh::FAR_TILE;
+            x.add(row_at + to, row_at + to + Sh::FAR_TILE, col_at + to, col_at + to + Sh::FAR_TILE,
+                  st + y * 256 + 16 * (lane >> 5), 128, k0 + 32 <= pr.S, j < pr.S ? ~0u : 0u, pr.scale * kLog2e);
+        }
+    } else {
+        x.clear();
+    }
+    // one after another into the first wavefront's
+    CIRCATT_LDS float *buf = (CIRCATT_LDS float *)lds_mem;
+    for (int y = 1; y < 4; ++y) {
+        __syncthreads();
+        if (wave == y) x.put(buf, lane);
+        __syncthreads();
+        if (wave == 0) x.take(buf, lane);
+    }
+    if (wave == 0) x.put(pr.work + sp.far_at + (int64_t)blockIdx.x * Sh::FAR_PART, lane);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__((256 * BwdShape<T, DP>::NG), (sizeof(T) == 2 && DP <= 64 ? 2 : 1))
+void sliding_dkdv(SlidingProblem pr, WalkSplit sp) {
+    typedef BwdShape<T, DP> Sh;
+    typedef Tile<T, DP> Tl;
+    constexpr int QT = Sh::QT, NG = Sh::NG;
+    __shared__ __attribute__((aligned(1024))) char lds_mem[NG * (4 * Sh::TILE + 16 * QT)];
+    // workgroups of one unit: its blocks, part by part, on one XCD
+    const int64_t id = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    const int64_t unit = id / (sp.blocks * sp.parts);
+    if (unit >= (int64_t)pr.B * pr.Hk) return;
+    const int in = (int)(id - unit * (sp.blocks * sp.parts)), kb = in / sp.parts, part = in - kb * sp.parts;
+    const HeadGroup<T> hg(pr, unit);
+    const int n = hg.n, lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6) & 3, group = uniform(threadIdx.x >> 8);
+    const int tid = threadIdx.x & 255;
+    // packed query rows of the walk: the block's tokens and W - 1 behind
+    const int k0 = kb * 128, kn = k0 + 127 < n - 1 ? k0 + 127 : n - 1, end = n - kn > pr.W ? kn + pr.W : n;
+    const int tiles = k0 < n ? ((end - k0) * pr.G + QT - 1) / QT : 0;
+    const int i0 = (int)((int64_t)tiles * part / sp.parts), i1 = (int)((int64_t)tiles * (part + 1) / sp.parts);
+    const int j0 = k0 + 32 * wave, j = j0 + (lane & 31), jj = j < n ? j : n - 1;
+    const unsigned lds = lds_byte((const CIRCATT_LDS char *)lds_mem) + group * 4 * Sh::TILE;
+    const unsigned stats = lds_byte((const CIRCATT_LDS char *)lds_mem) + NG * 4 * Sh::TILE + group * 16 * QT;
+    const float c = pr.scale * kLog2e;
+    KeySums<T, DP> x;
+    if (i0 < i1) {
+        // a group's turn i: tile i0 + NG i + group
+        const int mine = (i1 - i0 - group + NG - 1) / NG, turns = (i1 - i0 + NG - 1) / NG;
+        auto first_row = [&](int i) { return k0 * pr.G + (i0 + NG * i + group) * QT; };
+        auto fetch = [&](int i) {
+            const int r0 = first_row(i);
+            const unsigned to = lds + (i & 1) * 2 * Sh::TILE, st = stats + (i & 1) * 8 * QT;
+            fetch_packed<T, DP, QT, 256>(hg.q, pr.q_row, r0, pr.G, sp.heads, n, pr.D, tid, to);
+            fetch_packed<T, DP, QT, 256>(hg.dy, pr.dy_row, r0, pr.G, sp.heads, n, pr.D, tid, to + Sh::TILE);
+            if (wave == 0) fetch_stats<QT>(hg.lse, r0, hg.rows, st);
+            if (wave == 1) fetch_stats<QT>(hg.dsum, r0, hg.rows, st + 4 * QT);
+        };
+        if (mine > 0) fetch(0);
+        x.start(hg.k + jj * pr.k_row, hg.v + jj * pr.v_row, pr.D, lane);
+        const unsigned row_at = Tl::row_lane(lane) + lds, col_at = Tl::col_lane(lane) + lds;
+        // the rows that see key j: from its token on, to its window's end or, of a sink,
+        // the walk's (rows behind it in the last tile belong to sliding_dkdv_far)
+        const int see0 = j * pr.G, see1 = j < pr.S || end - j < pr.W ? end * pr.G : (j + pr.W) * pr.G;
+        // and those that see all of the wavefront's keys, or any
+        const int all0 = (j0 + 31) * pr.G, all1 = j0 + 31 < pr.S || end - j0 < pr.W ? end * pr.G : (j0 + pr.W) * pr.G;
+        const int any1 = j0 < pr.S || end - (j0 + 31) < pr.W ? end * pr.G : (j0 + 31 + pr.W) * pr.G;
+        for (int i = 0; i < turns; ++i) {
+            dma_barrier();
+            if (i + 1 < mine) fetch(i + 1);
+            if (i >= mine || j0 >= n) continue;
+            for (int m = 0; m < QT; m += 32) {
+                const int r0 = first_row(i) + m;
+                if (r0 + 32 <= j0 * pr.G || r0 >= any1) continue;
+                const unsigned to = (i & 1) * 2 * Sh::TILE + m * Tl::ROW;
+                x.add(row_at + to, row_at + to + Sh::TILE, col_at + to, col_at + to + Sh::TILE,
+                      stats + (i & 1) * 8 * QT + m * 4 + 16 * (lane >> 5), 4 * QT, r0 >= all0 && r0 + 32 <= all1,
+                      bits_between(see0 - r0, see1 - r0) >> (4 * (lane >> 5)), c);
+            }
+        }
+    } else {
+        x.clear();
+    }
+    CIRCATT_LDS float *buf = (CIRCATT_LDS float *)lds_mem;
+    if (NG == 2) {
+        __syncthreads();
+        if (group == 1) x.put(buf + wave * 64 * DP, lane);
+        __syncthreads();
+        if (group == 0) x.take(buf + wave * 64 * DP, lane);
+    }
+    if (sp.parts == 1 && kb * 4 < sp.far) {
+        // the far sums of the block's keys, by everybody
+        const int groups = sp.far - kb * 4 < 4 ? sp.far - kb * 4 : 4;
+        const float *w = pr.work + sp.far_at + (unit * sp.far + kb * 4) * sp.far_parts * Sh::FAR_PART;
+        __syncthreads();
+        for (int e = 4 * threadIdx.x; e < groups * Sh::FAR_PART; e += 1024 * NG) {
+            const float *we = w + (int64_t)(e / Sh::FAR_PART) * sp.far_parts * Sh::FAR_PART + e % Sh::FAR_PART;
+            f4v sum = f4v{};
+#pragma unroll 8
+            for (int y = 0; y < sp.far_parts; ++y) sum += *reinterpret_cast<const f4v *>(we + (int64_t)y * Sh::FAR_PART);
+            *(CIRCATT_LDS f4v *)(buf + e) = sum;
+        }
+        __syncthreads();
+        if (group == 0 && wave < groups) x.take(buf + wave * 64 * DP, lane);
+    }
+    if (group == 1) return;
+    if (sp.parts > 1) {
+        x.write(pr.work + sp.part_at + (unit * sp.blocks * sp.parts + in) * Sh::PART + (32 * wave + (lane & 31)) * DP,
+                128 * DP, lane);
         return;
     }
-    const int64_t out = ((int64_t)b * pr.L + j) * pr.Hk * pr.D + (int64_t)hk * pr.D;
+    const int64_t out = ((int64_t)hg.b * pr.L + j) * pr.Hk * pr.D + (int64_t)hg.hk * pr.D;
     T *kd = static_cast<T *>(pr.dk) + out, *vd = static_cast<T *>(pr.dv) + out;
     bool bad = false;
     if (j < n) {
-        bad = store_channels(dk, kd, pr.D, lane, pr.scale);
-        bad |= store_channels(dv, vd, pr.D, lane, 1.f);
+        bad = store_channels(x.dk, kd, pr.D, lane, pr.scale);
+        bad |= store_channels(x.dv, vd, pr.D, lane, 1.f);
     } else if (j < pr.L) {
         zero_channels(kd, pr.D, lane);
         zero_channels(vd, pr.D, lane);
     }
     uint64_t again = __ballot(bad);
     again = (again | again >> 32) & 0xffffffffu;
-    for (; again; again &= again - 1) {
-        const int x = j0 + __builtin_ctzll(again);
-        const int64_t ox = ((int64_t)b * pr.L + x) * pr.Hk * pr.D + (int64_t)hk * pr.D;
-        dkdv_row(kh + x * pr.k_row, vh + x * pr.v_row, qh, pr.q_row, gh, pr.dy_row, lse, dsum,
-                 static_cast<T *>(pr.dk) + ox, static_cast<T *>(pr.dv) + ox, x, n, pr.W, pr.S, pr.G, pr.D, c, pr.scale);
-    }
+    for (; again; again &= again - 1) hg.again(pr, j0 + __builtin_ctzll(again));
 }
 
-// The partial sums of split blocks, in the order of their parts: a wavefront a
-// key.
+// The partial sums of a key, the far ones first, in the order of their parts: a
+// wavefront a key.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void sliding_dkdv_join(SlidingProblem pr, WalkSplit sp) {
-    constexpr int PART = BwdShape<T, DP>::PART;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int first = sp.parts_far > 1 ? 0 : sp.far, last = sp.parts > 1 ? sp.blocks : sp.far;
-    const int64_t id = (int64_t)blockIdx.x * 4 + wave, keys = (int64_t)(last - first) * 128;
-    const int64_t unit = id / keys;
+    typedef BwdShape<T, DP> Sh;
+    const int lane = threadIdx.x & 63;
+    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), unit = id / pr.L;
     if (unit >= (int64_t)pr.B * pr.Hk) return;
-    const int j = first * 128 + (int)(id - unit * keys), kb = j >> 7;
-    if (j >= pr.L) return;
-    const bool is_far = kb < sp.far;
-    const int parts = is_far ? sp.parts_far : sp.parts;
-    const int64_t slot = is_far ? unit * sp.far_units + (int64_t)kb * parts
-                                : (sp.parts_far > 1 ? (int64_t)pr.B * pr.Hk * sp.far_units : 0) +
-                                      unit * (sp.units - sp.far_units) + (int64_t)(kb - sp.far) * parts;
-    const float *w = partials(pr) + slot * PART + (j & 127) * DP;
+    const int j = (int)(id - unit * pr.L);
     Pair k{0.f, 0.f}, v{0.f, 0.f};
-    for (int i = 0; i < parts; ++i, w += PART) {
-        const Pair a = load_row(w, lane, DP), c = load_row(w + 128 * DP, lane, DP);
-        k.a += a.a;
-        k.b += a.b;
-        v.a += c.a;
-        v.b += c.b;
+    auto sum = [&](const float *w, int parts, int size) {
+        for (int i = 0; i < parts; ++i, w += size) {
+            const Pair a = load_row(w, lane, DP), c = load_row(w + size / 2, lane, DP);
+            k.a += a.a;
+            k.b += a.b;
+            v.a += c.a;
+            v.b += c.b;
+        }
+    };
+    if (j / 32 < sp.far) {
+        // channel d of the key, as a wavefront's registers hold it
+        auto place = [&](int d) { return (16 * (d >> 5) + 4 * ((d >> 3) & 3) + (d & 3)) * 64 + (j & 31) + 8 * (d & 4); };
+        const float *w = pr.work + sp.far_at + (unit * sp.far + j / 32) * sp.far_parts * Sh::FAR_PART;
+        for (int i = 0; i < sp.far_parts; ++i, w += Sh::FAR_PART) {
+            if (lane < DP) k.a += w[place(lane)], v.a += w[Sh::FAR_PART / 2 + place(lane)];
+            if (lane + 64 < DP) k.b += w[place(lane + 64)], v.b += w[Sh::FAR_PART / 2 + place(lane + 64)];
+        }
     }
-    const int b = (int)(unit / pr.Hk), hk = (int)(unit - (int64_t)b * pr.Hk), n = signal_length(pr, b);
-    const int64_t head = (int64_t)hk * pr.D, out = ((int64_t)b * pr.L + j) * pr.Hk * pr.D + head;
-    T *kd = static_cast<T *>(pr.dk) + out, *vd = static_cast<T *>(pr.dv) + out;
+    sum(pr.work + sp.part_at + (unit * sp.blocks + (j >> 7)) * sp.parts * Sh::PART + (j & 127) * DP, sp.parts, Sh::PART);
+    const HeadGroup<T> hg(pr, unit);
+    const int64_t out = ((int64_t)hg.b * pr.L + j) * pr.Hk * pr.D + (int64_t)hg.hk * pr.D;
     k.a *= pr.scale;
     k.b *= pr.scale;
-    store_row(kd, lane, pr.D, k);
-    store_row(vd, lane, pr.D, v);
+    store_row(static_cast<T *>(pr.dk) + out, lane, pr.D, k);
+    store_row(static_cast<T *>(pr.dv) + out, lane, pr.D, v);
     // as in sliding_dkdv: not finite, or not in the type's range
-    const float sum = fabsf((float)(T)k.a) + fabsf((float)(T)k.b) + fabsf((float)(T)v.a) + fabsf((float)(T)v.b);
-    if (__any(!(sum < INFINITY)) && j < n) {
-        const int64_t stat = ((int64_t)b * pr.Hk + hk) * pr.L * pr.G;
-        dkdv_row(static_cast<const T *>(pr.k) + b * pr.k_batch + j * pr.k_row + head,
-                 static_cast<const T *>(pr.v) + b * pr.v_batch + j * pr.v_row + head,
-                 static_cast<const T *>(pr.q) + b * pr.q_batch + head * pr.G, pr.q_row,
-                 static_cast<const T *>(pr.dy) + b * pr.dy_batch + head * pr.G, pr.dy_row, pr.lse + stat, pr.work + stat,
-                 kd, vd, j, n, pr.W, pr.S, pr.G, pr.D, pr.scale * kLog2e, pr.scale);
-    }
+    const float size = fabsf((float)(T)k.a) + fabsf((float)(T)k.b) + fabsf((float)(T)v.a) + fabsf((float)(T)v.b);
+    if (__any(!(size < INFINITY)) && j < hg.n) hg.again(pr, j);
 }
 
-// Tiles of the longest walk of blocks kb0 .. (all of one kind).
-int64_t walk_tiles(const SlidingProblem &pr, int64_t k0, bool far, int QT) {
-    const int64_t tokens = far || pr.L - k0 < 128 + (int64_t)pr.W - 1 ? pr.L - k0 : 128 + (int64_t)pr.W - 1;
-    return (tokens * pr.G + QT - 1) / QT;
-}
-
-// Parts of about 1/768 of all tiles, three rounds of the chip's 256 compute
-// units, and not below 16 tiles: writing and adding up a partial pair takes as
-// long as some 4 tiles.
+// Parts: the estimate counts rounds of the chip's 256 compute units at the mean
+// walk, or the longest walk alone, and three tiles' time for a workgroup's start
+// and end, six where it leaves partial sums.  (The lengths of a padded batch are
+// not known here: all signals count as full.)
 WalkSplit walk_split(const SlidingProblem &pr) {
-    const int QT = pr.dtype == CIRCATT_F32 ? 32 : 64;
+    const bool wide = pr.dtype == CIRCATT_F32;
+    const int QT = wide ? 32 : 64, DP = (pr.D + 31) / 32 * 32;
     WalkSplit sp;
-    sp.blocks = (pr.L + 127) / 128;
-    sp.far = (pr.S + 127) / 128 < sp.blocks ? (pr.S + 127) / 128 : sp.blocks;
-    int64_t all = 0;
-    for (int kb = 0; kb < sp.blocks; ++kb) all += walk_tiles(pr, (int64_t)kb * 128, kb < sp.far, QT);
-    all *= (int64_t)pr.B * pr.Hk;
-    const int64_t part = all / 768 > 16 ? all / 768 : 16;
-    auto parts = [&](int kb, bool far) { return (int)((walk_tiles(pr, (int64_t)kb * 128, far, QT) + part - 1) / part); };
-    sp.parts_far = sp.far > 0 ? parts(0, true) : 1;
-    sp.parts = sp.far < sp.blocks ? parts(sp.far, false) : 1;
     sp.heads = make_fastdiv(pr.G);
-    sp.far_units = (int64_t)sp.far * sp.parts_far;
-    sp.units = sp.far_units + (int64_t)(sp.blocks - sp.far) * sp.parts;
+    sp.blocks = (pr.L + 127) / 128;
+    const int64_t units = (int64_t)pr.B * pr.Hk, n = units * sp.blocks;
+    auto walk = [&](int64_t k0) {
+        const int64_t tokens = pr.L - k0 < 127 + (int64_t)pr.W ? pr.L - k0 : 127 + (int64_t)pr.W;
+        return (double)tokens * pr.G / QT;
+    };
+    double all = 0;
+    for (int kb = 0; kb < sp.blocks; ++kb) all += walk(kb * 128);
+    const double mean = all / sp.blocks, longest = walk(0);
+    double best = 1e300;
+    for (int p = 1; p <= 8; ++p) {
+        const double rounds = (double)((n * p + 255) / 256), a = rounds * (mean / p), b = longest / p;
+        const double cost = (a > b ? a : b) + rounds * (p > 1 ? 6 : 3);
+        if (cost < best) best = cost, sp.parts = p;
+    }
+    // sinks that are seen from behind the window of their block; 4 tiles of 32 rows
+    // for each of four wavefronts
+    sp.far = 0;
+    sp.far_parts = 1;
+    const int64_t behind = (int64_t)pr.L - 127 - pr.W;
+    if (pr.S > 0 && behind > 0) {
+        const int64_t seen = pr.S < behind + 127 ? pr.S : behind + 127;
+        sp.far = (int)((seen + 31) / 32);
+        // and no more workgroups than fill the chip four times
+        const int64_t parts = (behind * pr.G + 511) / 512, most = 2048 / (units * sp.far);
+        sp.far_parts = (int)(parts < most ? parts : most < 1 ? 1 : most);
+    }
+    sp.far_at = ((int64_t)pr.B * pr.L * pr.H + 3) & ~(int64_t)3;
+    sp.part_at = sp.far_at + units * sp.far * sp.far_parts * 32 * DP * 2;
     return sp;
 }
 
@@ -597,9 +758,10 @@ hipError_t backward(const SlidingProblem &pr, hipStream_t s) {
     sliding_dq<T, DP><<<grid8((int64_t)pr.B * pr.Hk * blocks), 256, 0, s>>>(pr, blocks);
     if (pr.dk != nullptr) {
         const WalkSplit sp = walk_split(pr);
-        sliding_dkdv<T, DP><<<grid8((int64_t)pr.B * pr.Hk * sp.units), 256, 0, s>>>(pr, sp);
-        const int64_t split = (sp.parts_far > 1 ? sp.far : 0) + (sp.parts > 1 ? sp.blocks - sp.far : 0);
-        if (split > 0) sliding_dkdv_join<T, DP><<<(unsigned)(pr.B * pr.Hk * split * 32), 256, 0, s>>>(pr, sp);
+        const int64_t units = (int64_t)pr.B * pr.Hk;
+        if (sp.far > 0) sliding_dkdv_far<T, DP><<<(unsigned)(units * sp.far * sp.far_parts), 256, 0, s>>>(pr, sp);
+        sliding_dkdv<T, DP><<<grid8(units * sp.blocks * sp.parts), 256 * BwdShape<T, DP>::NG, 0, s>>>(pr, sp);
+        if (sp.parts > 1) sliding_dkdv_join<T, DP><<<(unsigned)((units * pr.L + 3) / 4), 256, 0, s>>>(pr, sp);
     }
     return hipGetLastError();
 }
@@ -614,10 +776,8 @@ hipError_t backward(const SlidingProblem &pr, hipStream_t s) {
 
 int64_t sliding_bwd_workspace_floats(const SlidingProblem &pr) {
     const WalkSplit sp = walk_split(pr);
-    const int64_t slots = (sp.parts_far > 1 ? sp.far_units : 0) + (sp.parts > 1 ? sp.units - sp.far_units : 0);
     const int DP = (pr.D + 31) / 32 * 32;
-    // the partial sums start at a multiple of 16 bytes
-    return (int64_t)pr.B * pr.Hk * pr.L * pr.G + 4 + pr.B * (int64_t)pr.Hk * slots * 128 * DP * 2;
+    return sp.part_at + (sp.parts > 1 ? (int64_t)pr.B * pr.Hk * sp.blocks * sp.parts * 128 * DP * 2 : 0);
 }
 
 hipError_t launch_sliding_fwd(const SlidingProblem &pr, hipStream_t s) {

@@ -118,6 +118,10 @@ __device__ __forceinline__ void dma_barrier() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+// All loads of this wavefront are here, said so that the compiler knows it too: a
+// load that is first used inside a loop makes it wait there in every round, and for
+// the DMA of the next tile with it.
+__device__ __forceinline__ void loads_here() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 // 16 bytes from every lane's own address to LDS byte m0 + 16 lane
 __device__ __forceinline__ void dma16_global(const void *p, unsigned m0) {
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(m0) : "memory");
@@ -147,21 +151,27 @@ __device__ __forceinline__ V8<T> load8(const T *p, int d, int D) {
     return v;
 }
 
-// What a query row sees: keys j with j <= at and j > at - W or j < S.
-struct Sight {
-    int W, S;
-    __device__ __forceinline__ bool operator()(int at, int j) const {
-        const int back = at - j;
-        return back >= 0 && (back < W || j < S);
+// N products whose first operands are read from LDS, read(i) AHEAD products before
+// use(i, operand): a read takes several products' time to arrive, and the
+// compiler's own order asks for most of them one product ahead.
+template <typename T, int N, int AHEAD, typename Read, typename Use>
+__device__ __forceinline__ void products(Read read, Use use) {
+    if constexpr (sizeof(T) == 2) {
+        V8<T> a[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD && i < N; ++i) a[i] = read(i);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            __builtin_amdgcn_sched_barrier(0x0006);  // arithmetic may pass
+            use(i, a[i % AHEAD]);
+            if (i + AHEAD < N) a[i % AHEAD] = read(i + AHEAD);
+        }
+        __builtin_amdgcn_sched_barrier(0x0006);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) use(i, read(i));
     }
-    // keys [k0, k0 + n): seen by none, or by all, of the rows at [lo, hi]
-    __device__ __forceinline__ bool none(int lo, int hi, int k0, int n) const {
-        return k0 > hi || (k0 + n - 1 <= lo - W && k0 >= S);
-    }
-    __device__ __forceinline__ bool all(int lo, int hi, int k0, int n) const {
-        return k0 + n - 1 <= lo && (k0 > hi - W || k0 + n <= S);
-    }
-};
+}
 
 // Bits x of [lo, hi) among 0 .. 31.
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
@@ -171,6 +181,27 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
 // The place of a 32x32 result's register i in a word of 32 places that is shifted
 // down by 4 for the lanes of the second half.
 __device__ __forceinline__ constexpr uint32_t place_bit(int i) { return 1u << (8 * (i >> 2) + (i & 3)); }
+
+// What a query row sees: keys j with j <= at and j > at - W or j < S.
+struct Sight {
+    int W, S;
+    __device__ __forceinline__ bool operator()(int at, int j) const {
+        const int back = at - j;
+        return back >= 0 && (back < W || j < S);
+    }
+    // of the keys k0 .. k0 + 31, a bit each
+    __device__ __forceinline__ uint32_t bits(int at, int k0) const {
+        const int end = at + 1 - k0, sinks = S - k0;
+        return bits_between(end - W, end) | bits_between(0, end < sinks ? end : sinks);
+    }
+    // keys [k0, k0 + n): seen by none, or by all, of the rows at [lo, hi]
+    __device__ __forceinline__ bool none(int lo, int hi, int k0, int n) const {
+        return k0 > hi || (k0 + n - 1 <= lo - W && k0 >= S);
+    }
+    __device__ __forceinline__ bool all(int lo, int hi, int k0, int n) const {
+        return k0 + n - 1 <= lo && (k0 > hi - W || k0 + n <= S);
+    }
+};
 
 // The tiles of KT keys that rows at [lo, hi] see, in order: tiles of sinks, then
 // of the window.
