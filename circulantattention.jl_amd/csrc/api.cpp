@@ -682,6 +682,10 @@ int paged_table(int64_t B, int64_t npages, int64_t page_size, int64_t page_strid
     if (row_stride < channels || page_stride < 0 || (npages > 1 && page_stride < row_stride))
         return fail(CIRCATT_ERR_INVALID, "cache strides %lld, %lld do not fit rows of %lld channels",
                     (long long)page_stride, (long long)row_stride, (long long)channels);
+    // rows are addressed in units of 16 bytes, in 32 bits
+    if (row_stride > (int64_t)1 << 24 || page_stride > (int64_t)1 << 36 ||
+        ((npages - 1) * (double)page_stride + (page_size - 1) * (double)row_stride + channels) * esize > 6.8e10)
+        return fail(CIRCATT_ERR_UNSUPPORTED, "a cache of more than 63 GiB from end to end");
     for (const void *p : {cache_k, cache_v}) {
         if (p == nullptr) return fail(CIRCATT_ERR_INVALID, "cache is NULL");
         if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || row_stride * esize % 16 != 0 || page_stride * esize % 16 != 0)

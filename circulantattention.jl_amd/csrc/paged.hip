@@ -28,18 +28,19 @@ __device__ __forceinline__ NewToken new_token(const int32_t *offsets, const int3
 
 // ---------------------------------------------------------------------------
 // Attention.  Rows are packed as in sliding.hip: row r of a sequence and a head
-// of keys is head r % G of its new token r / G.  A block is R of them:
-//   R = 128, a tile of keys for four wavefronts of 32 rows each (chunks);
-//   R = 32, tiles of 32 keys for each of NW wavefronts, which share the rows and
-//   join their sums at the end (single tokens: bound by reading the cache).
-// Blocks of sequence b are numbered from offsets[b] G / R + b on, so that a block
-// finds its sequence from the offsets on the device.  Where blocks are few, each
-// is split along its tiles over `splits` workgroups, whose partial sums
-// paged_join adds up.
+// of keys is head r % G of its new token r / G.  A block is R of them.
+//   paged_few (R = 32): tiles of 32 keys for each of NW wavefronts, which share the
+//   rows and join their sums at the end; bound by reading the cache.
+//   paged_chunk (R = 128): four wavefronts of 32 rows share the tiles, as in
+//   sliding_fwd, and NG such groups share the block's keys; bound by the products.
+// Where blocks are few, each is split along its tiles over `splits` workgroups,
+// whose partial sums paged_join adds up.
+enum Which { kAll, kShort, kLong };  // sequences: all, those of up to 32 rows, the others
 struct PagedGrid {
-    int blocks;   // numbers of blocks of one head of keys
+    int which;
+    int blocks;        // numbers of blocks of one head of keys
     int splits;
-    int64_t rows;  // of partial sums
+    int64_t at, rows;  // of partial sums: floats before them, rows
 };
 
 // Sequence b with its block's first row, rows and positions; b < 0: none.
@@ -47,8 +48,11 @@ struct Block {
     int b, r0, rows, first, len;
     int64_t q0;  // row of q of its first new token
 };
+// Blocks of sequence b are numbered from offsets[b] G / R + b on (from b without
+// offsets or among short sequences, which have one), so that a block finds its
+// sequence from the offsets on the device.
 template <int R>
-__device__ __forceinline__ Block find_block(const PagedProblem &pr, int id) {
+__device__ __forceinline__ Block find_block(const PagedProblem &pr, int which, int id) {
     Block x;
     if (pr.offsets == nullptr) {
         const int per = (pr.G + R - 1) / R;
@@ -56,25 +60,32 @@ __device__ __forceinline__ Block find_block(const PagedProblem &pr, int id) {
         x.r0 = (id - x.b * per) * R;
         x.rows = pr.G;
         x.q0 = x.b;
+        if (x.b >= pr.B) x.b = -1;
     } else {
-        // the last b whose number is not past id: ascending, so a count
-        const int lane = threadIdx.x & 63;
-        int count = 0;
-        for (int b0 = 0; b0 < pr.B; b0 += 64) {
-            const int b = b0 + lane;
-            const bool in = b < pr.B && (int64_t)pr.offsets[b] * pr.G / R + b <= id;
-            const int got = __popcll(__ballot(in));
-            count += got;
-            if (got < 64) break;
+        if (which == kShort) {
+            x.b = id < pr.B ? id : -1;
+        } else {
+            // the last b whose number is not past id: ascending, so a count
+            const int lane = threadIdx.x & 63;
+            int count = 0;
+            for (int b0 = 0; b0 < pr.B; b0 += 64) {
+                const int b = b0 + lane;
+                const bool in = b < pr.B && (int64_t)pr.offsets[b] * pr.G / R + b <= id;
+                const int got = __popcll(__ballot(in));
+                count += got;
+                if (got < 64) break;
+            }
+            x.b = uniform(count - 1);
         }
-        x.b = uniform(count - 1);
         if (x.b < 0) return x;
         const int o = uniform(pr.offsets[x.b]), m = uniform(pr.offsets[x.b + 1]) - o;
-        x.r0 = (id - (int)((int64_t)o * pr.G / R + x.b)) * R;
+        x.r0 = which == kShort ? 0 : (id - (int)((int64_t)o * pr.G / R + x.b)) * R;
         x.rows = m * pr.G;
         x.q0 = o;
         if (o < 0 || m < 0 || (int64_t)o + m > pr.T) x.rows = 0;
+        if (which != kAll && (x.rows <= 32) != (which == kShort)) x.rows = 0;
     }
+    if (x.b < 0) return x;
     x.len = uniform(pr.lengths[x.b]);
     x.len = x.len > 0 ? x.len : 0;
     x.first = x.len - x.rows / pr.G;
@@ -82,43 +93,69 @@ __device__ __forceinline__ Block find_block(const PagedProblem &pr, int id) {
     return x;
 }
 
-// What a block's rows may read of the cache: keys [0, S) and [low, len) below
-// the table's end.
+// One row of a block as its lane sees it, and what the block's rows see together.
+// at: its position, -1 where it sees nothing (before the first token, or behind the
+// table's end); blo, bhi: the block's first and last position that see something.
+struct RowSight {
+    int tok, g, at, blo, bhi;
+    template <int R>
+    __device__ static __forceinline__ RowSight of(const PagedProblem &pr, const Block &w, int r) {
+        RowSight x;
+        const int rr = r < w.rows ? r : w.rows - 1, last = w.r0 + R - 1 < w.rows ? w.r0 + R - 1 : w.rows - 1;
+        const int64_t held = (int64_t)pr.maxp << pr.page_log2;
+        x.tok = rr / pr.G;
+        x.g = rr - x.tok * pr.G;
+        const int pos = w.first + x.tok;
+        x.at = pos >= held ? -1 : pos;
+        x.blo = w.first + w.r0 / pr.G;
+        x.bhi = w.first + last / pr.G;
+        if (x.bhi >= held) x.bhi = (int)held - 1;
+        if (x.blo < 0) x.blo = 0;
+        if (x.blo > x.bhi) x.bhi = -1;  // nothing: no tiles
+        return x;
+    }
+};
+
+// What a block's rows may read of the cache: keys [0, S) and [low, len).
 template <typename T>
 struct Pages {
     const T *k, *v;
     const int32_t *table;
-    int64_t page_stride, row_stride;
+    uint32_t page_units, row_units;  // strides in 16 bytes
     int npages, log2, low, S, len;
-    // the cache row of key j, -1 if it is not there
-    __device__ __forceinline__ int row(int j) const {
-        if (j >= len || (j < low && j >= S)) return -1;
-        const int pg = table[j >> log2];
-        return (unsigned)pg < (unsigned)npages ? (pg << log2) | (j & ((1 << log2) - 1)) : -1;
-    }
-    __device__ __forceinline__ int64_t at(int row) const {
-        return (row >> log2) * page_stride + (row & ((1 << log2) - 1)) * row_stride;
+    __device__ __forceinline__ Pages(const PagedProblem &pr, const Block &w, const RowSight &x, int hk)
+        : k(static_cast<const T *>(pr.k) + (int64_t)hk * pr.D), v(static_cast<const T *>(pr.v) + (int64_t)hk * pr.D),
+          table(pr.pages + w.b * pr.pages_row), page_units((uint32_t)(pr.page_stride * (int)sizeof(T) / 16)),
+          row_units((uint32_t)(pr.row_stride * (int)sizeof(T) / 16)), npages(pr.npages), log2(pr.page_log2),
+          low(x.blo - pr.W + 1), S(pr.S), len(x.bhi + 1) {}
+    // key j's row in units of 16 bytes from the cache's start, kNone if not there
+    // from its page's number.  The number is loaded a round before the row is
+    // formed: a load that is used in its own round would make the wavefront wait for
+    // the DMA that it issued since.
+    static constexpr uint32_t kNone = ~0u;
+    __device__ __forceinline__ int page(int j) const { return table[(j < len ? j : len - 1) >> log2]; }
+    __device__ __forceinline__ uint32_t row(int j, int pg) const {
+        if (j >= len || (j < low && j >= S) || (unsigned)pg >= (unsigned)npages) return kNone;
+        return pg * page_units + (j & ((1 << log2) - 1)) * row_units;
     }
 };
 
 __device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
 
-// KT keys and values, lane l of the calling wavefronts holding the cache row of
-// the tile's key l, into LDS by THREADS threads; rows that are not there and
-// units from D on are zeros.
+// KT keys (or values) from p into LDS by THREADS threads, this one the tid-th;
+// lane l of each of their wavefronts holds the row of the tile's key l.  Rows that
+// are not there and units from D on are zeros.
 template <typename T, int DP, int KT, int THREADS>
-__device__ __forceinline__ void fetch_pages(const Pages<T> &pg, int row, int D, const CIRCATT_LDS char *kt) {
+__device__ __forceinline__ void fetch_paged(const T *p, uint32_t row, int D, int tid, unsigned to) {
     typedef Tile<T, DP> Tl;
-    const int tid = threadIdx.x & (THREADS - 1), units = D * (int)sizeof(T) / 16;
-    const unsigned m0 = lds_byte(kt) + uniform(tid >> 6) * 1024;
+    const int units = D * (int)sizeof(T) / 16;
+    const unsigned m0 = to + uniform(tid >> 6) * 1024;
 #pragma unroll
     for (int k = 0; k < KT * Tl::PC / THREADS; ++k) {
         const int slot = tid + k * THREADS, r = slot / Tl::PC, u = (slot % Tl::PC) ^ Tl::f(r);
-        const int cr = __shfl(row, r, 64);
-        const bool there = cr >= 0 && u < units;
-        const int64_t at = there ? pg.at(cr) + u * (16 / (int)sizeof(T)) : 0;
-        dma16_global(there ? (const void *)(pg.k + at) : (const void *)kZeros, m0 + k * THREADS * 16);
-        dma16_global(there ? (const void *)(pg.v + at) : (const void *)kZeros, m0 + KT * Tl::ROW + k * THREADS * 16);
+        const uint32_t cr = __shfl(row, r, 64);
+        const char *at = reinterpret_cast<const char *>(p) + u * 16 + ((uint64_t)cr << 4);
+        dma16_global(cr != Pages<T>::kNone && u < units ? (const void *)at : (const void *)kZeros, m0 + k * THREADS * 16);
     }
 }
 
@@ -126,7 +163,7 @@ __device__ __forceinline__ void fetch_pages(const Pages<T> &pg, int row, int D, 
 struct Partial {
     float *o, *ml;
     __device__ Partial(const PagedProblem &pr, const PagedGrid &gr, int64_t row)
-        : o(pr.work + row * pr.D), ml(pr.work + gr.rows * pr.D + row * 2) {}
+        : o(pr.work + gr.at + row * pr.D), ml(pr.work + gr.at + gr.rows * pr.D + row * 2) {}
 };
 template <int OT>
 __device__ __forceinline__ void store_partial(const f16v (&o)[OT], Partial p, float m, float l, int D, int lane) {
@@ -150,228 +187,362 @@ __device__ __forceinline__ PagedKV<T> paged_rows_of(const PagedProblem &pr, int 
                       pr.row_stride, pr.pages + b * pr.pages_row, pr.npages, pr.page_log2};
 }
 
-// One workgroup: a block, a head of keys and a part of the block's tiles.
-// ONE: R = 32 and the wavefronts share the rows.
-template <typename T, int DP, bool ONE>
-struct PagedShape {
-    static constexpr int NW = ONE && sizeof(T) == 4 && DP > 64 ? 2 : 4;
-    static constexpr int R = ONE ? 32 : 128;
-    static constexpr int KT = ONE || sizeof(T) == 4 ? 32 : 64;
-    static constexpr int TILE = KT * Tile<T, DP>::ROW;
-    static constexpr int LDS = (ONE ? NW : 1) * 4 * TILE;
-};
+// Rows of y behind the last sequence: zeros, by the workgroups behind the blocks.
+template <typename T>
+__device__ __forceinline__ void zero_rows(const PagedProblem &pr, int blocks) {
+    if (blockIdx.y != 0 || blockIdx.z != 0) return;
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    const int end = pr.offsets[pr.B];
+    const int64_t per = (int64_t)pr.H * pr.D / (16 / (int)sizeof(T)), from = (int64_t)(end < 0 ? 0 : end) * per;
+    const int64_t step = (int64_t)(gridDim.x - blocks) * blockDim.x;
+    for (int64_t i = from + (int64_t)(blockIdx.x - blocks) * blockDim.x + threadIdx.x; i < pr.T * per; i += step)
+        static_cast<u4 *>(pr.y)[i] = u4{};
+}
 
-template <typename T, int DP, bool ONE>
-__global__ __launch_bounds__((64 * PagedShape<T, DP, ONE>::NW), ((sizeof(T) == 4 && DP > 64) || ONE ? 1 : 2))
-void paged_kernel(PagedProblem pr, PagedGrid gr) {
-    typedef PagedShape<T, DP, ONE> Sh;
-    typedef Tile<T, DP> Tl;
-    constexpr int KT = Sh::KT, NB = KT / 32, R = Sh::R, NW = Sh::NW, OT = DP / 32;
-    __shared__ __attribute__((aligned(1024))) char lds_mem[Sh::LDS];
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    const CIRCATT_LDS char *lds = (const CIRCATT_LDS char *)lds_mem + (ONE ? wave * 4 * Sh::TILE : 0);
-    const int hk = blockIdx.y, split = blockIdx.z;
-    if ((int)blockIdx.x >= gr.blocks) {
-        // rows behind the last sequence
-        if (hk != 0 || split != 0) return;
-        const int end = pr.offsets[pr.B];
-        const int64_t per = (int64_t)pr.H * pr.D / (16 / (int)sizeof(T)), from = (int64_t)(end < 0 ? 0 : end) * per;
-        const int64_t step = (int64_t)(gridDim.x - gr.blocks) * blockDim.x;
-        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-        for (int64_t i = from + (int64_t)(blockIdx.x - gr.blocks) * blockDim.x + threadIdx.x; i < pr.T * per; i += step)
-            static_cast<u4 *>(pr.y)[i] = u4{};
-        return;
-    }
-    const Block w = find_block<R>(pr, blockIdx.x);
-    if (w.b < 0) return;
-    const int r0 = w.r0 + (ONE ? 0 : 32 * wave), r = r0 + (lane & 31);
-    const int rr = r < w.rows ? r : w.rows - 1, tok = rr / pr.G, g = rr - tok * pr.G;
-    const int64_t held = (int64_t)pr.maxp << pr.page_log2;
-    // a position before the first token or behind the table: the row sees nothing
-    const int pos = w.first + tok, at = pos >= held ? -1 : pos;
-    const bool live = r0 < w.rows;
-    // the block's positions, and this wavefront's
-    const int b_last = w.r0 + R - 1 < w.rows ? w.r0 + R - 1 : w.rows - 1;
-    int blo = w.first + w.r0 / pr.G, bhi = w.first + b_last / pr.G;
-    if (bhi >= held) bhi = (int)held - 1;
-    if (blo < 0) blo = 0;
-    const int lo = uniform(at), hi = __builtin_amdgcn_readlane(at, 31);
-    const bool plain = lo >= 0 && hi >= lo;  // ascending: no row without sight
-    const Sight see{pr.W, pr.S};
-    const TileList<KT> tiles(blo, blo > bhi ? -1 : bhi, pr.W, pr.S);
+// A wavefront's 32 rows (lane: row r of the block's sequence): their outputs, or
+// their partial sums.  Outputs that a value which is not finite reached are formed
+// again from the keys that the row sees alone.
+template <typename T, int DP, int R>
+__device__ __forceinline__ void finish_rows(const PagedProblem &pr, const PagedGrid &gr, const Block &w, const RowSight &rs,
+                                            int r, int lane, const f16v (&o)[DP / 32], float m, float l) {
+    const int hk = blockIdx.y;
     const int64_t head = (int64_t)hk * pr.D;
-    const Pages<T> pg{static_cast<const T *>(pr.k) + head, static_cast<const T *>(pr.v) + head,
-                      pr.pages + w.b * pr.pages_row, pr.page_stride, pr.row_stride, pr.npages, pr.page_log2,
-                      blo - pr.W + 1, pr.S, bhi + 1};
-    const int parts = gr.splits * (ONE ? NW : 1), part = split * (ONE ? NW : 1) + (ONE ? wave : 0);
-    const int i0 = (int)((int64_t)tiles.count * part / parts), i1 = (int)((int64_t)tiles.count * (part + 1) / parts);
-    const float c = pr.scale * kLog2e;
-    Rows<T, DP> x;
-    const T *qr = static_cast<const T *>(pr.q) + (w.q0 + tok) * pr.q_row + (head * pr.G + (int64_t)g * pr.D);
-    if (i0 < i1) {
-        const unsigned row_at = Tl::row_lane(lane), col_at = Tl::col_lane(lane);
-        auto key_row = [&](int i) { return lane < KT ? pg.row(tiles.key(i) + lane) : -1; };
-        // the rows of the tile in work, of the next one, and of the one after
-        int now = key_row(i0), next = i0 + 1 < i1 ? key_row(i0 + 1) : -1;
-        fetch_pages<T, DP, KT, ONE ? 64 : 256>(pg, now, pr.D, lds);
-        x.start(qr, pr.D, lane);
-        loads_here();
-        for (int i = i0; i < i1; ++i) {
-            if (ONE) dma_wait();
-            else dma_barrier();
-            int after = -1;
-            if (i + 1 < i1) {
-                fetch_pages<T, DP, KT, ONE ? 64 : 256>(pg, next, pr.D, lds + ((i + 1 - i0) & 1) * 2 * Sh::TILE);
-                if (i + 2 < i1) after = key_row(i + 2);
-            }
-            const int k0 = tiles.key(i);
-            const uint64_t hidden = ~__ballot(now >= 0) & (KT == 64 ? ~0ull : 0xffffffffull);
-            now = next;
-            next = after;
-            if (!live || (plain && see.none(lo, hi, k0, KT))) continue;
-            const unsigned to = lds_byte(lds) + ((i - i0) & 1) * 2 * Sh::TILE;
-            x.template tile<NB>(row_at + to, col_at + to + Sh::TILE, lane, at, k0, see,
-                                !(plain && see.all(lo, hi, k0, KT)) || hidden != 0, hidden, c);
-        }
-    } else {
-        x.start(qr, 0, lane);
-    }
-    float l = x.total(), m = x.m;
-    if (ONE) {
-        // join the wavefronts' sums in LDS: each one's maximum and sum, then the
-        // outputs, 32 channels at a time, in the order of the wavefronts
-        __syncthreads();
-        float *ml = reinterpret_cast<float *>(lds_mem), *buf = ml + NW * 64;
-        if (lane < 32) {
-            ml[wave * 64 + lane] = m;
-            ml[wave * 64 + 32 + lane] = l;
-        }
-        __syncthreads();
-        float mm = -INFINITY, ll = 0.f;
-        for (int v = 0; v < NW; ++v) mm = fmaxf(mm, ml[v * 64 + (lane & 31)]);
-        for (int v = 0; v < NW; ++v) {
-            const float mv = ml[v * 64 + (lane & 31)];
-            ll += mv == -INFINITY ? ml[v * 64 + 32 + (lane & 31)] : ml[v * 64 + 32 + (lane & 31)] * __builtin_amdgcn_exp2f(mv - mm);
-        }
-        const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mm);
-#pragma unroll
-        for (int t = 0; t < OT; ++t) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) buf[(wave * 16 + i) * 64 + lane] = x.o[t][i] * f;
-            __syncthreads();
-            if (wave == 0)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float sum = 0.f;
-                    for (int v = 0; v < NW; ++v) sum += buf[(v * 16 + i) * 64 + lane];
-                    x.o[t][i] = sum;
-                }
-            __syncthreads();
-        }
-        m = mm;
-        l = ll;
-        if (wave != 0) return;
-    }
-    if (!live) return;
     if (gr.splits > 1) {
         if (r < w.rows)
-            store_partial(x.o, Partial(pr, gr, (((int64_t)blockIdx.x * pr.Hk + hk) * gr.splits + split) * R + r - w.r0), m, l,
-                          pr.D, lane);
+            store_partial(o, Partial(pr, gr, (((int64_t)blockIdx.x * pr.Hk + hk) * gr.splits + blockIdx.z) * R + r - w.r0), m,
+                          l, pr.D, lane);
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T *y = static_cast<T *>(pr.y) + w.q0 * pr.H * pr.D + head * pr.G;
-    uint64_t again = __ballot(r < w.rows && store_channels(x.o, y + ((int64_t)tok * pr.H + g) * pr.D, pr.D, lane, inv));
+    uint64_t again = __ballot(r < w.rows && store_channels(o, y + ((int64_t)rs.tok * pr.H + rs.g) * pr.D, pr.D, lane, inv));
     again = (again | again >> 32) & 0xffffffffu;
     const PagedKV<T> kv = paged_rows_of<T>(pr, w.b, head);
     for (; again; again &= again - 1) {
         const int j = __builtin_ctzll(again);
-        const int tj = __builtin_amdgcn_readlane(tok, j), gj = __builtin_amdgcn_readlane(g, j);
+        const int tj = __builtin_amdgcn_readlane(rs.tok, j), gj = __builtin_amdgcn_readlane(rs.g, j);
         forward_row(static_cast<const T *>(pr.q) + (w.q0 + tj) * pr.q_row + (head * pr.G + (int64_t)gj * pr.D),
-                    y + ((int64_t)tj * pr.H + gj) * pr.D, (float *)nullptr, kv, __builtin_amdgcn_readlane(at, j), pr.W, pr.S,
-                    pr.D, c);
+                    y + ((int64_t)tj * pr.H + gj) * pr.D, (float *)nullptr, kv, __builtin_amdgcn_readlane(rs.at, j), pr.W, pr.S,
+                    pr.D, pr.scale * kLog2e);
     }
 }
 
-// Adds up a row's partial sums in the order of the splits: a wavefront a row.
+template <typename T, int DP>
+struct FewShape {
+    static constexpr int NW = sizeof(T) == 4 && DP > 64 ? 2 : 4, TILE = 32 * Tile<T, DP>::ROW, LDS = NW * 4 * TILE;
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__((64 * FewShape<T, DP>::NW), 1) void paged_few(PagedProblem pr, PagedGrid gr) {
+    typedef FewShape<T, DP> Sh;
+    typedef Tile<T, DP> Tl;
+    constexpr int NW = Sh::NW, OT = DP / 32;
+    __shared__ __attribute__((aligned(1024))) char lds_mem[Sh::LDS];
+    if ((int)blockIdx.x >= gr.blocks) return zero_rows<T>(pr, gr.blocks);
+    const Block w = find_block<32>(pr, gr.which, blockIdx.x);
+    if (w.b < 0) return;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), hk = blockIdx.y;
+    const unsigned lds = lds_byte((const CIRCATT_LDS char *)lds_mem) + wave * 4 * Sh::TILE;
+    const int r = w.r0 + (lane & 31);
+    const RowSight rs = RowSight::of<32>(pr, w, r);
+    const Sight see{pr.W, pr.S};
+    const TileList<32> tiles(rs.blo, rs.bhi, pr.W, pr.S);
+    const Pages<T> pg(pr, w, rs, hk);
+    const int parts = gr.splits * NW, part = blockIdx.z * NW + wave;
+    const int i0 = (int)((int64_t)tiles.count * part / parts), i1 = (int)((int64_t)tiles.count * (part + 1) / parts);
+    Rows<T, DP> x;
+    const T *qr = static_cast<const T *>(pr.q) + (w.q0 + rs.tok) * pr.q_row + ((int64_t)(hk * pr.G + rs.g) * pr.D);
+    if (i0 < i1) {
+        const unsigned row_at = Tl::row_lane(lane) + lds, col_at = Tl::col_lane(lane) + lds + Sh::TILE;
+        const int lo = uniform(rs.at), hi = __builtin_amdgcn_readlane(rs.at, 31);
+        const bool plain = lo >= 0 && hi >= lo;  // ascending: no row without sight
+        auto fetch = [&](uint32_t row, int i) {
+            const unsigned to = lds + ((i - i0) & 1) * 2 * Sh::TILE;
+            fetch_paged<T, DP, 32, 64>(pg.k, row, pr.D, lane, to);
+            fetch_paged<T, DP, 32, 64>(pg.v, row, pr.D, lane, to + Sh::TILE);
+        };
+        auto key = [&](int i) { return tiles.key(i < i1 ? i : i1 - 1) + (lane & 31); };
+        // the rows of the tile in work, and the page numbers of the next one
+        uint32_t now = pg.row(key(i0), pg.page(key(i0)));
+        fetch(now, i0);
+        x.start(qr, pr.D, lane);
+        int raw = pg.page(key(i0 + 1));
+        loads_here();
+        for (int i = i0; i < i1; ++i) {
+            dma_wait();
+            const uint32_t next = pg.row(key(i + 1), raw);
+            if (i + 1 < i1) fetch(next, i + 1);
+            raw = pg.page(key(i + 2));
+            const int k0 = tiles.key(i);
+            const uint32_t there = (uint32_t)__ballot(now != Pages<T>::kNone);
+            now = next;
+            const unsigned to = ((i - i0) & 1) * 2 * Sh::TILE;
+            f16v s[1];
+            V8<T> p[2];
+            x.scores(row_at + to, s);
+            if (there != ~0u || !(plain && see.all(lo, hi, k0, 32))) hide_keys(s[0], see.bits(rs.at, k0) & there, lane);
+            x.raise(x.largest(s) * (pr.scale * kLog2e));
+            x.weigh(s, p, pr.scale * kLog2e);
+            x.template add<1>(col_at + to, p);
+        }
+    } else {
+        x.start(qr, 0, lane);
+    }
+    // join the wavefronts' sums in LDS: each one's maximum and sum, then the outputs,
+    // 32 channels at a time, in the order of the wavefronts
+    float m = x.m, l = x.total();
+    __syncthreads();
+    float *ml = reinterpret_cast<float *>(lds_mem), *buf = ml + NW * 64;
+    if (lane < 32) {
+        ml[wave * 64 + lane] = m;
+        ml[wave * 64 + 32 + lane] = l;
+    }
+    __syncthreads();
+    float mm = -INFINITY, ll = 0.f;
+    for (int v = 0; v < NW; ++v) mm = fmaxf(mm, ml[v * 64 + (lane & 31)]);
+    for (int v = 0; v < NW; ++v) {
+        const float mv = ml[v * 64 + (lane & 31)], lv = ml[v * 64 + 32 + (lane & 31)];
+        ll += mv == -INFINITY ? lv : lv * __builtin_amdgcn_exp2f(mv - mm);
+    }
+    const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mm);
+#pragma unroll
+    for (int t = 0; t < OT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) buf[(wave * 16 + i) * 64 + lane] = x.o[t][i] * f;
+        __syncthreads();
+        if (wave == 0)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float sum = 0.f;
+                for (int v = 0; v < NW; ++v) sum += buf[(v * 16 + i) * 64 + lane];
+                x.o[t][i] = sum;
+            }
+        __syncthreads();
+    }
+    if (wave == 0) finish_rows<T, DP, 32>(pr, gr, w, rs, r, lane, x.o, mm, ll);
+}
+
+template <typename T, int DP>
+struct ChunkShape {
+    static constexpr int NB = sizeof(T) == 2 ? 2 : 1, KT = 32 * NB, TILE = KT * Tile<T, DP>::ROW;
+    // Float32 operands of wide heads take more than half the registers
+    static constexpr int NG = sizeof(T) == 2 || DP <= 64 ? 2 : 1;
+    static constexpr int LDS = NG * 4 * TILE;
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__((256 * ChunkShape<T, DP>::NG), 1) void paged_chunk(PagedProblem pr, PagedGrid gr) {
+    typedef ChunkShape<T, DP> Sh;
+    typedef Tile<T, DP> Tl;
+    constexpr int KT = Sh::KT, NB = Sh::NB, NG = Sh::NG, OT = DP / 32;
+    __shared__ __attribute__((aligned(1024))) char lds_mem[Sh::LDS];
+    if ((int)blockIdx.x >= gr.blocks) return zero_rows<T>(pr, gr.blocks);
+    const Block w = find_block<128>(pr, gr.which, blockIdx.x);
+    if (w.b < 0) return;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6) & 3, group = uniform(threadIdx.x >> 8);
+    const int tid = threadIdx.x & 255, hk = blockIdx.y;
+    const unsigned lds = lds_byte((const CIRCATT_LDS char *)lds_mem) + group * 4 * Sh::TILE;
+    const int r0 = w.r0 + 32 * wave, r = r0 + (lane & 31);
+    const RowSight rs = RowSight::of<128>(pr, w, r);
+    const bool live = r0 < w.rows;
+    const Sight see{pr.W, pr.S};
+    const TileList<KT> tiles(rs.blo, rs.bhi, pr.W, pr.S);
+    const Pages<T> pg(pr, w, rs, hk);
+    const int parts = gr.splits * NG;
+    auto bound = [&](int part) { return (int)((int64_t)tiles.count * part / parts); };
+    const int part = blockIdx.z * NG + group, i0 = bound(part), i1 = bound(part + 1);
+    int rounds = 0;  // of the longest group: they share their barriers
+    for (int g = 0; g < NG; ++g) {
+        const int n = bound(blockIdx.z * NG + g + 1) - bound(blockIdx.z * NG + g);
+        rounds = n > rounds ? n : rounds;
+    }
+    const float c = pr.scale * kLog2e;
+    Rows<T, DP> x;
+    const T *qr = static_cast<const T *>(pr.q) + (w.q0 + rs.tok) * pr.q_row + ((int64_t)(hk * pr.G + rs.g) * pr.D);
+    x.start(qr, i0 < i1 ? pr.D : 0, lane);
+    if (rounds > 0) {
+        const unsigned row_at = Tl::row_lane(lane) + lds, col_at = Tl::col_lane(lane) + lds + Sh::TILE;
+        const int lo = uniform(rs.at), hi = __builtin_amdgcn_readlane(rs.at, 31);
+        const bool plain = lo >= 0 && hi >= lo;
+        auto key = [&](int i) { return tiles.key(i < i1 ? i : i1 > 0 ? i1 - 1 : 0) + (lane & (KT - 1)); };
+        auto fetch = [&](uint32_t row, int i) {
+            if (i >= i1) return;
+            const unsigned to = lds + ((i - i0) & 1) * 2 * Sh::TILE;
+            fetch_paged<T, DP, KT, 256>(pg.k, row, pr.D, tid, to);
+            fetch_paged<T, DP, KT, 256>(pg.v, row, pr.D, tid, to + Sh::TILE);
+        };
+        uint32_t now = pg.row(key(i0), pg.page(key(i0)));
+        fetch(now, i0);
+        int raw = pg.page(key(i0 + 1));
+        loads_here();
+        // The two groups are half a round apart: one's score products run beside the
+        // other's exponentials and value products.
+        if (group == 1) __builtin_amdgcn_s_barrier();
+        for (int i = i0; i < i0 + rounds; ++i) {
+            dma_barrier();
+            const uint32_t next = pg.row(key(i + 1), raw);
+            fetch(next, i + 1);
+            raw = pg.page(key(i + 2));
+            const uint64_t there = __ballot(now != Pages<T>::kNone);
+            now = next;
+            const bool mine = live && i < i1;
+            const int k0 = tiles.key(i);
+            const unsigned to = ((i - i0) & 1) * 2 * Sh::TILE;
+            constexpr uint64_t kFull = KT == 64 ? ~0ull : 0xffffffffull;
+            f16v s[NB];
+            V8<T> p[2 * NB];
+            if (mine) x.scores(row_at + to, s);
+            if (NG == 2) __builtin_amdgcn_s_barrier();
+            if (!mine) continue;
+            if ((there & kFull) != kFull || !(plain && see.all(lo, hi, k0, KT))) {
+#pragma unroll
+                for (int m = 0; m < NB; ++m)
+                    hide_keys(s[m], see.bits(rs.at, k0 + 32 * m) & (uint32_t)(there >> (32 * m)), lane);
+            }
+            x.raise(x.largest(s) * c);
+            x.weigh(s, p, c);
+            x.template add<NB>(col_at + to, p);
+        }
+        if (NG == 2 && group == 0) __builtin_amdgcn_s_barrier();
+    }
+    float m = x.m, l = x.total();
+    if (NG == 2) {
+        // the second group's sums through LDS
+        CIRCATT_LDS float *buf = (CIRCATT_LDS float *)lds_mem + wave * (16 * OT + 2) * 64;
+        __syncthreads();
+        if (group == 1) {
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) buf[(16 * t + i) * 64 + lane] = x.o[t][i];
+            buf[16 * OT * 64 + lane] = m;
+            buf[(16 * OT + 1) * 64 + lane] = l;
+        }
+        __syncthreads();
+        if (group == 1) return;
+        const float m1 = buf[16 * OT * 64 + lane], l1 = buf[(16 * OT + 1) * 64 + lane], mm = fmaxf(m, m1);
+        const float f0 = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mm);
+        const float f1 = m1 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m1 - mm);
+        l = l * f0 + l1 * f1;
+        m = mm;
+#pragma unroll
+        for (int t = 0; t < OT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x.o[t][i] = x.o[t][i] * f0 + buf[(16 * t + i) * 64 + lane] * f1;
+    }
+    if (live) finish_rows<T, DP, 128>(pr, gr, w, rs, r, lane, x.o, m, l);
+}
+
+// Adds up the partial sums of a block's rows in the order of the splits: half a
+// wavefront a row, four channels a lane.
 template <typename T, int R>
 __global__ __launch_bounds__(256) void paged_join(PagedProblem pr, PagedGrid gr) {
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    const int64_t t = id / pr.H;
-    if (t >= pr.T) return;
-    const int h = (int)(id - t * pr.H), hk = h / pr.G, g = h - hk * pr.G;
-    const NewToken w = new_token(pr.offsets, pr.lengths, pr.B, t);
-    if (w.b >= pr.B) return;
-    int64_t block, row;
-    if (pr.offsets == nullptr) {
-        block = t * ((pr.G + R - 1) / R) + g / R;
-        row = g % R;
-    } else {
-        const int64_t o = pr.offsets[w.b], r = (t - o) * pr.G + g;
-        block = o * pr.G / R + w.b + r / R;
-        row = r % R;
-    }
-    const int64_t slot = ((block * pr.Hk + hk) * gr.splits) * R + row;
-    float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < gr.splits; ++s) m = fmaxf(m, Partial(pr, gr, slot + s * R).ml[0]);
-    Pair o{0.f, 0.f};
-    for (int s = 0; s < gr.splits; ++s) {
-        const Partial p(pr, gr, slot + s * R);
-        const float ls = p.ml[1];
-        if (ls == 0.f) continue;  // saw nothing, and wrote no outputs
-        const float f = __builtin_amdgcn_exp2f(p.ml[0] - m);
-        const Pair x = load_row(p.o, lane, pr.D);
-        l += ls * f;
-        o.a += x.a * f;
-        o.b += x.b * f;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    o.a *= inv;
-    o.b *= inv;
-    T *y = static_cast<T *>(pr.y) + (t * pr.H + h) * pr.D;
-    store_row(y, lane, pr.D, o);
-    if (__any(!(fabsf(o.a) + fabsf(o.b) < INFINITY))) {
-        const int64_t held = (int64_t)pr.maxp << pr.page_log2;
-        forward_row(static_cast<const T *>(pr.q) + t * pr.q_row + (int64_t)h * pr.D, y, (float *)nullptr,
-                    paged_rows_of<T>(pr, w.b, (int64_t)hk * pr.D), w.pos >= held ? -1 : w.pos, pr.W, pr.S, pr.D,
-                    pr.scale * kLog2e);
+    const Block w = find_block<R>(pr, gr.which, blockIdx.x);
+    if (w.b < 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hk = blockIdx.y, d = 4 * (lane & 31);
+    const int64_t slot = ((int64_t)blockIdx.x * pr.Hk + hk) * gr.splits * R, head = (int64_t)hk * pr.D;
+    const int rows = w.rows - w.r0 < R ? w.rows - w.r0 : R;
+    for (int i0 = 2 * wave; i0 < rows; i0 += 8) {
+        const int i = i0 + (lane >> 5), ii = i < rows ? i : rows - 1;
+        float m = -INFINITY, l = 0.f;
+        for (int s = 0; s < gr.splits; ++s) m = fmaxf(m, Partial(pr, gr, slot + s * R + ii).ml[0]);
+        f4v o = f4v{};
+        for (int s = 0; s < gr.splits; ++s) {
+            const Partial p(pr, gr, slot + s * R + ii);
+            const float ls = p.ml[1];
+            if (ls == 0.f) continue;  // saw nothing, and wrote no outputs
+            const float f = __builtin_amdgcn_exp2f(p.ml[0] - m);
+            l += ls * f;
+            if (d < pr.D) o += *reinterpret_cast<const f4v *>(p.o + d) * f;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int tok = (w.r0 + ii) / pr.G, g = w.r0 + ii - tok * pr.G;
+        T *y = static_cast<T *>(pr.y) + (w.q0 + tok) * pr.H * pr.D + head * pr.G + (int64_t)g * pr.D;
+        V4<T> v;
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = (T)(o[e] * inv);
+            bad |= !(fabsf((float)v[e]) < INFINITY);
+        }
+        if (i < rows && d < pr.D) *reinterpret_cast<V4<T> *>(y + d) = v;
+        const uint64_t again = __ballot(bad && i < rows && d < pr.D);
+        for (int h = 0; h < 2; ++h) {
+            if (!(uint32_t)(again >> (32 * h))) continue;
+            const int rj = w.r0 + i0 + h, tj = rj / pr.G, gj = rj - tj * pr.G;
+            const int64_t held = (int64_t)pr.maxp << pr.page_log2;
+            const int pos = w.first + tj;
+            forward_row(static_cast<const T *>(pr.q) + (w.q0 + tj) * pr.q_row + (head * pr.G + (int64_t)gj * pr.D),
+                        static_cast<T *>(pr.y) + (w.q0 + tj) * pr.H * pr.D + head * pr.G + (int64_t)gj * pr.D, (float *)nullptr,
+                        paged_rows_of<T>(pr, w.b, head), pos >= held ? -1 : pos, pr.W, pr.S, pr.D, pr.scale * kLog2e);
+        }
     }
 }
 
-// Rows of 32 for each sequence and head of keys where there is no more than
-// that on average, else of 128.
-bool rows_of_32(const PagedProblem &pr) { return pr.T * pr.G <= (int64_t)pr.B * 32; }
+// The kernels of a call: blocks of 32 rows where a sequence has one token, or no more
+// rows than that on average; else blocks of 128, and blocks of 32 for the sequences of a
+// batch that have no more.
+struct PagedPlan {
+    bool few, chunk;
+    PagedGrid few_grid, chunk_grid;
+    int64_t floats;
+};
 
-PagedGrid paged_grid(const PagedProblem &pr) {
-    const bool one = rows_of_32(pr);
-    const int R = one ? 32 : 128;
+// Splits: the estimate counts rounds of the chip's 256 compute units at a
+// workgroup's rounds of tiles, three tiles' time for its start and end, and eight
+// for another kernel that adds up.  blocks: about as many as will have rows.
+int count_splits(double blocks, double tiles) {
+    int best = 1;
+    double least = 1e300;
+    for (int p = 1; p <= 64 && p <= tiles; ++p) {
+        const double rounds = (double)(int64_t)((blocks * p + 255) / 256);
+        const double cost = rounds * (tiles / p + 3) + (p > 1 ? 8 : 0);
+        if (cost < least) least = cost, best = p;
+    }
+    return best;
+}
+
+PagedPlan paged_plan(const PagedProblem &pr) {
+    PagedPlan pl;
+    const int64_t rows = pr.T * pr.G;
+    pl.chunk = pr.T != pr.B && rows > (int64_t)pr.B * 32;
+    pl.few = !pl.chunk || pr.B > 1;
     const bool wide = pr.dtype == CIRCATT_F32;
-    const int KT = one || wide ? 32 : 64, NW = !one ? 1 : wide && pr.D > 64 ? 2 : 4;
-    PagedGrid gr;
-    gr.blocks = (int)(pr.T * pr.G / R) + pr.B;
-    // two workgroups a compute unit, four tiles for each wavefront at least
-    const int64_t span = (int64_t)pr.maxp * pr.page, most = (int64_t)pr.W + pr.S + R / pr.G + KT;
-    const int64_t tiles = ((span < most ? span : most) + KT - 1) / KT;
-    int64_t splits = 512 / ((int64_t)gr.blocks * pr.Hk), limit = tiles / (4 * NW);
-    splits = splits < limit ? splits : limit;
-    gr.splits = (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
-    gr.rows = gr.splits > 1 ? (int64_t)gr.blocks * pr.Hk * gr.splits * R : 0;
-    return gr;
+    const int64_t held = (int64_t)pr.maxp * pr.page, window = (int64_t)pr.W + pr.S;
+    auto grid = [&](int R, int KT, int waves, int which) {
+        PagedGrid gr;
+        gr.which = which;
+        gr.blocks = which == kShort ? pr.B : (int)(rows / R) + pr.B;
+        const int64_t seen = window + R / pr.G < held ? window + R / pr.G : held;
+        const double blocks = which == kLong ? (double)rows / R + 1 : gr.blocks;
+        gr.splits = count_splits(blocks * pr.Hk, (double)((seen + KT - 1) / KT) / waves);
+        gr.rows = gr.splits > 1 ? (int64_t)gr.blocks * pr.Hk * gr.splits * R : 0;
+        return gr;
+    };
+    pl.few_grid = grid(32, 32, wide && pr.D > 64 ? 2 : 4, pl.chunk ? kShort : kAll);
+    pl.chunk_grid = grid(128, wide ? 32 : 64, wide && pr.D > 64 ? 1 : 2, pl.few ? kLong : kAll);
+    pl.few_grid.at = 0;
+    pl.chunk_grid.at = pl.few ? (pl.few_grid.rows * (pr.D + 2) + 3) & ~(int64_t)3 : 0;
+    pl.floats = pl.chunk ? pl.chunk_grid.at + pl.chunk_grid.rows * (pr.D + 2) : pl.few_grid.rows * (pr.D + 2);
+    return pl;
 }
 
 template <typename T, int DP>
 void launch(const PagedProblem &pr, hipStream_t s) {
-    const PagedGrid gr = paged_grid(pr);
-    const bool tail = pr.zero_tail && pr.offsets != nullptr;
-    const int R = rows_of_32(pr) ? 32 : 128;
-    const dim3 grid(pr.offsets == nullptr ? pr.B * ((pr.G + R - 1) / R) : gr.blocks + (tail ? 8 : 0), pr.Hk, gr.splits);
-    if (rows_of_32(pr)) paged_kernel<T, DP, true><<<grid, 64 * PagedShape<T, DP, true>::NW, 0, s>>>(pr, gr);
-    else paged_kernel<T, DP, false><<<grid, 256, 0, s>>>(pr, gr);
-    if (gr.splits > 1) {
-        const unsigned rows = (unsigned)((pr.T * pr.H + 3) / 4);
-        if (rows_of_32(pr)) paged_join<T, 32><<<rows, 256, 0, s>>>(pr, gr);
-        else paged_join<T, 128><<<rows, 256, 0, s>>>(pr, gr);
+    const PagedPlan pl = paged_plan(pr);
+    int tail = pr.zero_tail && pr.offsets != nullptr ? 8 : 0;
+    if (pl.few) {
+        const PagedGrid &gr = pl.few_grid;
+        // without offsets the numbers of blocks end at the last sequence's
+        const unsigned blocks = pr.offsets == nullptr ? pr.B * ((pr.G + 31) / 32) : gr.blocks;
+        paged_few<T, DP><<<dim3(blocks + tail, pr.Hk, gr.splits), 64 * FewShape<T, DP>::NW, 0, s>>>(pr, gr);
+        if (gr.splits > 1) paged_join<T, 32><<<dim3(blocks, pr.Hk), 256, 0, s>>>(pr, gr);
+        tail = 0;
+    }
+    if (pl.chunk) {
+        const PagedGrid &gr = pl.chunk_grid;
+        paged_chunk<T, DP><<<dim3(gr.blocks + tail, pr.Hk, gr.splits), 256 * ChunkShape<T, DP>::NG, 0, s>>>(pr, gr);
+        if (gr.splits > 1) paged_join<T, 128><<<dim3(gr.blocks, pr.Hk), 256, 0, s>>>(pr, gr);
     }
 }
 template <int DT>
@@ -410,7 +581,7 @@ __global__ __launch_bounds__(256) void append_rows(AppendProblem pr) {
 
 }  // namespace
 
-int64_t paged_workspace_floats(const PagedProblem &pr) { return paged_grid(pr).rows * (pr.D + 2); }
+int64_t paged_workspace_floats(const PagedProblem &pr) { return paged_plan(pr).floats; }
 
 hipError_t launch_paged(const PagedProblem &pr, hipStream_t s) {
     if (pr.dtype == CIRCATT_F32) launch<0>(pr, s);

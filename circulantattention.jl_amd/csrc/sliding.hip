@@ -112,14 +112,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
         auto look = [&](f16v (&s)[NB], int i) {  // hide keys of tile i, largest score
             const int k0 = tiles.key(i);
             if (!see.all(lo, hi, k0, KT)) {
-                asm volatile("");  // a branch: few tiles need it
 #pragma unroll
-                for (int m = 0; m < NB; ++m) {
-                    const uint32_t half = see.bits(at, k0 + 32 * m) >> (4 * (lane >> 5));
-#pragma unroll
-                    for (int y = 0; y < 16; ++y)
-                        if (!(half & place_bit(y))) s[m][y] = -INFINITY;
-                }
+                for (int m = 0; m < NB; ++m) hide_keys(s[m], see.bits(at, k0 + 32 * m), lane);
             }
             mx = x.largest(s) * c;
         };

@@ -279,6 +279,15 @@ struct Feed {
     }
 };
 
+// Hides the keys of a 32x32 block of scores whose bits are not set.
+__device__ __forceinline__ void hide_keys(f16v &s, uint32_t seen, int lane) {
+    asm volatile("");  // a branch to here: few tiles need it
+    const uint32_t half = seen >> (4 * (lane >> 5));
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (!(half & place_bit(i))) s[i] = -INFINITY;
+}
+
 // Running softmax and output of 32 rows (lane l and l + 32: row l % 32).
 // Scores count in units of log2(e) scale; the row's maximum is raised only when
 // a score passes it by more than 2^6 in the exponent, so that most tiles leave
@@ -301,63 +310,7 @@ struct Rows {
         l = 0.f;
     }
 
-    // NB blocks of 32 keys from key k0 on, at the lane's places kt (row) and vt
-    // (col); masked: test every key, with bit (key - k0) of hidden set where it is
-    // not there at all
-    template <int NB>
-    __device__ __forceinline__ void tile(unsigned kt, unsigned vt, int lane, int at, int k0, Sight see, bool masked,
-                                         uint64_t hidden, float c) {
-        typedef Tile<T, DP> Tl;
-        f16v s[NB];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            s[n] = f16v{};
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k) s[n] = mma(Tl::row(kt, 32 * n, k), q[k], s[n]);
-        }
-        if (masked) {
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = 32 * n + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-                    if (!see(at, k0 + j) || ((hidden >> j) & 1)) s[n][i] = -INFINITY;
-                }
-        }
-        float mx = s[0][0];
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
-        if (__any(mx > m + RAISE || (m == -INFINITY && mx > -INFINITY))) {
-            const float mn = fmaxf(m, mx), r = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-            l *= r;
-#pragma unroll
-            for (int t = 0; t < OT; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[t][i] *= r;
-            m = mn;
-        }
-        const float mu = m == -INFINITY ? 0.f : m;
-        float sum = 0.f;
-        V8<T> p[2 * NB];
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -mu));
-                sum += e;
-                p[2 * n + (i >> 3)][i & 7] = (T)e;
-            }
-        l += sum;
-#pragma unroll
-        for (int t = 0; t < OT; ++t)
-#pragma unroll
-            for (int n = 0; n < 2 * NB; ++n) o[t] = mma(Tl::col(vt, 16 * n, t), p[n], o[t]);
-    }
-
-    // The same in steps, for NB blocks of 32 keys a round.
+    // A round of NB blocks of 32 keys, in steps.
     template <int NB>
     __device__ __forceinline__ void scores(unsigned kt, f16v (&s)[NB]) const {
 #pragma unroll

@@ -90,6 +90,7 @@ def paged(L, dtype=3, T=4, B=4, H=4, Hk=2, dh=64, W=16, S=0, scale=0.125, q=P, q
     (dict(row_stride=132), -1, "16-byte"), (dict(ck=ODD), -1, "16-byte"), (dict(cv=None), -1, "cache is NULL"),
     (dict(T=5), -1, "without offsets"), (dict(q=None), -1, "q is NULL"), (dict(y=ODD), -1, "16-byte"),
     (dict(B=0), -1, "sizes"), (dict(T=-1, offsets=P), -1, "sizes"),
+    (dict(npages=1 << 24, page_stride=1 << 12), -2, "63 GiB"), (dict(npages=1, row_stride=1 << 25), -2, "63 GiB"),
 ])
 def test_paged_refusals(L, args, code, fragment):
     expect(L, paged(L, **args), code, fragment)
