@@ -29,9 +29,9 @@ __device__ __forceinline__ NewToken new_token(const int32_t *offsets, const int3
 // ---------------------------------------------------------------------------
 // Attention.  Rows are packed as in sliding.hip: row r of a sequence and a head
 // of keys is head r % G of its new token r / G.  A block is R of them.
-//   paged_few (R = 32): tiles of 32 keys for each of NW wavefronts, which share the
+//   few_rows (R = 32): tiles of 32 keys for each of NW wavefronts, which share the
 //   rows and join their sums at the end; bound by reading the cache.
-//   paged_chunk (R = 128): four wavefronts of 32 rows share the tiles, as in
+//   chunk_rows (R = 128): four wavefronts of 32 rows share the tiles, as in
 //   sliding_fwd, and NG such groups share the block's keys; bound by the products.
 // Where blocks are few, each is split along its tiles over `splits` workgroups,
 // whose partial sums paged_join adds up.
@@ -203,13 +203,13 @@ __device__ __forceinline__ void zero_rows(const PagedProblem &pr, int blocks) {
 // their partial sums.  Outputs that a value which is not finite reached are formed
 // again from the keys that the row sees alone.
 template <typename T, int DP, int R>
-__device__ __forceinline__ void finish_rows(const PagedProblem &pr, const PagedGrid &gr, const Block &w, const RowSight &rs,
-                                            int r, int lane, const f16v (&o)[DP / 32], float m, float l) {
+__device__ __forceinline__ void finish_rows(const PagedProblem &pr, const PagedGrid &gr, int id, const Block &w,
+                                            const RowSight &rs, int r, int lane, const f16v (&o)[DP / 32], float m, float l) {
     const int hk = blockIdx.y;
     const int64_t head = (int64_t)hk * pr.D;
     if (gr.splits > 1) {
         if (r < w.rows)
-            store_partial(o, Partial(pr, gr, (((int64_t)blockIdx.x * pr.Hk + hk) * gr.splits + blockIdx.z) * R + r - w.r0), m,
+            store_partial(o, Partial(pr, gr, (((int64_t)id * pr.Hk + hk) * gr.splits + blockIdx.z) * R + r - w.r0), m,
                           l, pr.D, lane);
         return;
     }
@@ -232,14 +232,14 @@ struct FewShape {
     static constexpr int NW = sizeof(T) == 4 && DP > 64 ? 2 : 4, TILE = 32 * Tile<T, DP>::ROW, LDS = NW * 4 * TILE;
 };
 
+// Block number id, by the first NW wavefronts of a workgroup.
 template <typename T, int DP>
-__global__ __launch_bounds__((64 * FewShape<T, DP>::NW), 1) void paged_few(PagedProblem pr, PagedGrid gr) {
+__device__ __forceinline__ void few_rows(const PagedProblem &pr, const PagedGrid &gr, int id, char *lds_mem) {
     typedef FewShape<T, DP> Sh;
     typedef Tile<T, DP> Tl;
     constexpr int NW = Sh::NW, OT = DP / 32;
-    __shared__ __attribute__((aligned(1024))) char lds_mem[Sh::LDS];
-    if ((int)blockIdx.x >= gr.blocks) return zero_rows<T>(pr, gr.blocks);
-    const Block w = find_block<32>(pr, gr.which, blockIdx.x);
+    if (threadIdx.x >= 64 * NW) return;
+    const Block w = find_block<32>(pr, gr.which, id);
     if (w.b < 0) return;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), hk = blockIdx.y;
     const unsigned lds = lds_byte((const CIRCATT_LDS char *)lds_mem) + wave * 4 * Sh::TILE;
@@ -319,7 +319,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP>::NW), 1) void paged_few(Paged
             }
         __syncthreads();
     }
-    if (wave == 0) finish_rows<T, DP, 32>(pr, gr, w, rs, r, lane, x.o, mm, ll);
+    if (wave == 0) finish_rows<T, DP, 32>(pr, gr, id, w, rs, r, lane, x.o, mm, ll);
 }
 
 template <typename T, int DP>
@@ -331,13 +331,11 @@ struct ChunkShape {
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__((256 * ChunkShape<T, DP>::NG), 1) void paged_chunk(PagedProblem pr, PagedGrid gr) {
+__device__ __forceinline__ void chunk_rows(const PagedProblem &pr, const PagedGrid &gr, int id, char *lds_mem) {
     typedef ChunkShape<T, DP> Sh;
     typedef Tile<T, DP> Tl;
     constexpr int KT = Sh::KT, NB = Sh::NB, NG = Sh::NG, OT = DP / 32;
-    __shared__ __attribute__((aligned(1024))) char lds_mem[Sh::LDS];
-    if ((int)blockIdx.x >= gr.blocks) return zero_rows<T>(pr, gr.blocks);
-    const Block w = find_block<128>(pr, gr.which, blockIdx.x);
+    const Block w = find_block<128>(pr, gr.which, id);
     if (w.b < 0) return;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6) & 3, group = uniform(threadIdx.x >> 8);
     const int tid = threadIdx.x & 255, hk = blockIdx.y;
@@ -430,7 +428,29 @@ __global__ __launch_bounds__((256 * ChunkShape<T, DP>::NG), 1) void paged_chunk(
 #pragma unroll
             for (int i = 0; i < 16; ++i) x.o[t][i] = x.o[t][i] * f0 + buf[(16 * t + i) * 64 + lane] * f1;
     }
-    if (live) finish_rows<T, DP, 128>(pr, gr, w, rs, r, lane, x.o, m, l);
+    if (live) finish_rows<T, DP, 128>(pr, gr, id, w, rs, r, lane, x.o, m, l);
+}
+
+// A call's blocks: those of 128 rows (which take longest) first, those of 32 behind
+// them, and workgroups for the rows behind the last sequence.
+template <typename T, int DP>
+__global__ __launch_bounds__((64 * FewShape<T, DP>::NW), 1) void paged_few(PagedProblem pr, PagedGrid gr) {
+    __shared__ __attribute__((aligned(1024))) char lds_mem[FewShape<T, DP>::LDS];
+    if ((int)blockIdx.x >= gr.blocks) return zero_rows<T>(pr, gr.blocks);
+    few_rows<T, DP>(pr, gr, blockIdx.x, lds_mem);
+}
+template <typename T, int DP>
+__global__ __launch_bounds__((256 * ChunkShape<T, DP>::NG), 1) void paged_chunk(PagedProblem pr, PagedGrid chunk, PagedGrid few) {
+    constexpr int LDS = FewShape<T, DP>::LDS > ChunkShape<T, DP>::LDS ? FewShape<T, DP>::LDS : ChunkShape<T, DP>::LDS;
+    __shared__ __attribute__((aligned(1024))) char lds_mem[LDS];
+    const int id = blockIdx.x, split = blockIdx.z;
+    if (id < chunk.blocks) {
+        if (split < chunk.splits) chunk_rows<T, DP>(pr, chunk, id, lds_mem);
+    } else if (id < chunk.blocks + few.blocks) {
+        if (split < few.splits) few_rows<T, DP>(pr, few, id - chunk.blocks, lds_mem);
+    } else {
+        zero_rows<T>(pr, chunk.blocks + few.blocks);
+    }
 }
 
 // Adds up the partial sums of a block's rows in the order of the splits: half a
@@ -530,19 +550,22 @@ PagedPlan paged_plan(const PagedProblem &pr) {
 template <typename T, int DP>
 void launch(const PagedProblem &pr, hipStream_t s) {
     const PagedPlan pl = paged_plan(pr);
-    int tail = pr.zero_tail && pr.offsets != nullptr ? 8 : 0;
-    if (pl.few) {
+    const int tail = pr.zero_tail && pr.offsets != nullptr ? 8 : 0;
+    if (pl.chunk) {
+        PagedGrid few = pl.few_grid;
+        if (!pl.few) few.blocks = 0, few.splits = 1;
+        const PagedGrid &chunk = pl.chunk_grid;
+        const int splits = chunk.splits > few.splits ? chunk.splits : few.splits;
+        paged_chunk<T, DP><<<dim3(chunk.blocks + few.blocks + tail, pr.Hk, splits), 256 * ChunkShape<T, DP>::NG, 0, s>>>(
+            pr, chunk, few);
+        if (chunk.splits > 1) paged_join<T, 128><<<dim3(chunk.blocks, pr.Hk), 256, 0, s>>>(pr, chunk);
+        if (few.splits > 1) paged_join<T, 32><<<dim3(few.blocks, pr.Hk), 256, 0, s>>>(pr, few);
+    } else {
         const PagedGrid &gr = pl.few_grid;
         // without offsets the numbers of blocks end at the last sequence's
         const unsigned blocks = pr.offsets == nullptr ? pr.B * ((pr.G + 31) / 32) : gr.blocks;
         paged_few<T, DP><<<dim3(blocks + tail, pr.Hk, gr.splits), 64 * FewShape<T, DP>::NW, 0, s>>>(pr, gr);
         if (gr.splits > 1) paged_join<T, 32><<<dim3(blocks, pr.Hk), 256, 0, s>>>(pr, gr);
-        tail = 0;
-    }
-    if (pl.chunk) {
-        const PagedGrid &gr = pl.chunk_grid;
-        paged_chunk<T, DP><<<dim3(gr.blocks + tail, pr.Hk, gr.splits), 256 * ChunkShape<T, DP>::NG, 0, s>>>(pr, gr);
-        if (gr.splits > 1) paged_join<T, 128><<<dim3(gr.blocks, pr.Hk), 256, 0, s>>>(pr, gr);
     }
 }
 template <int DT>

@@ -389,11 +389,14 @@ struct KeySums {
 #pragma unroll
         for (int t = 0; t < OT; ++t) dk[t] = dv[t] = f16v{};
     }
-    // rows of q and dy at the lane's places qr, gr (row) and qc, gc (col); lse and d
+    // rows of q and dy at the lane's places qr, gr (row), then qc, gc (col); lse and d
     // of the rows at LDS bytes st and st + stride; half: the rows that see the key, a
-    // bit each, or all where every() holds
-    __device__ __forceinline__ void add(unsigned qr, unsigned gr, unsigned qc, unsigned gc, unsigned st, int stride,
-                                        bool every, uint32_t half, float c) {
+    // bit each, unless every one does
+    struct Weights {
+        V8<T> p[2], ds[2];
+    };
+    __device__ __forceinline__ void weigh(unsigned qr, unsigned gr, unsigned st, int stride, bool every, uint32_t half,
+                                          float c, Weights &w) const {
         f16v s = f16v{}, dp = f16v{};
         products<T, 2 * STEPS, AHEAD>([&](int i) { return Tl::row(i & 1 ? gr : qr, 0, i >> 1); },
                                       [&](int i, V8<T> a) {
@@ -416,16 +419,17 @@ struct KeySums {
             for (int x = 0; x < 16; ++x)
                 if (!(half & place_bit(x))) s[x] = dp[x] = 0.f;
         }
-        V8<T> p[2], ds[2];
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-            p[x >> 3][x & 7] = (T)s[x];
-            ds[x >> 3][x & 7] = (T)dp[x];
+            w.p[x >> 3][x & 7] = (T)s[x];
+            w.ds[x >> 3][x & 7] = (T)dp[x];
         }
+    }
+    __device__ __forceinline__ void add(unsigned qc, unsigned gc, const Weights &w) {
         products<T, 4 * OT, AHEAD>([&](int i) { return Tl::col(i & 1 ? qc : gc, 16 * ((i >> 1) & 1), i >> 2); },
                                    [&](int i, V8<T> a) {
-                                       if (i & 1) dk[i >> 2] = mma(a, ds[(i >> 1) & 1], dk[i >> 2]);
-                                       else dv[i >> 2] = mma(a, p[(i >> 1) & 1], dv[i >> 2]);
+                                       if (i & 1) dk[i >> 2] = mma(a, w.ds[(i >> 1) & 1], dk[i >> 2]);
+                                       else dv[i >> 2] = mma(a, w.p[(i >> 1) & 1], dv[i >> 2]);
                                    });
     }
     // through LDS or a workspace, one float for every register and lane
@@ -532,8 +536,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
                 fetch(i + 1);
             }
             const unsigned to = y * 2 * Sh::FAR_TILE;
-            x.add(row_at + to, row_at + to + Sh::FAR_TILE, col_at + to, col_at + to + Sh::FAR_TILE,
-                  st + y * 256 + 16 * (lane >> 5), 128, k0 + 32 <= pr.S, j < pr.S ? ~0u : 0u, pr.scale * kLog2e);
+            typename KeySums<T, DP>::Weights wt;
+            x.weigh(row_at + to, row_at + to + Sh::FAR_TILE, st + y * 256 + 16 * (lane >> 5), 128, k0 + 32 <= pr.S,
+                    j < pr.S ? ~0u : 0u, pr.scale * kLog2e, wt);
+            x.add(col_at + to, col_at + to + Sh::FAR_TILE, wt);
         }
     } else {
         x.clear();
@@ -594,6 +600,8 @@ void sliding_dkdv(SlidingProblem pr, WalkSplit sp) {
         // and those that see all of the wavefront's keys, or any
         const int all0 = (j0 + 31) * pr.G, all1 = j0 + 31 < pr.S || end - j0 < pr.W ? end * pr.G : (j0 + pr.W) * pr.G;
         const int any1 = j0 < pr.S || end - (j0 + 31) < pr.W ? end * pr.G : (j0 + 31 + pr.W) * pr.G;
+        // (Groups half a block apart, one forming weights while the other adds, took 167
+        // us where this takes 112: the weights that wait at the barrier between spill.)
         for (int i = 0; i < turns; ++i) {
             dma_barrier();
             if (i + 1 < mine) fetch(i + 1);
@@ -602,9 +610,10 @@ void sliding_dkdv(SlidingProblem pr, WalkSplit sp) {
                 const int r0 = first_row(i) + m;
                 if (r0 + 32 <= j0 * pr.G || r0 >= any1) continue;
                 const unsigned to = (i & 1) * 2 * Sh::TILE + m * Tl::ROW;
-                x.add(row_at + to, row_at + to + Sh::TILE, col_at + to, col_at + to + Sh::TILE,
-                      stats + (i & 1) * 8 * QT + m * 4 + 16 * (lane >> 5), 4 * QT, r0 >= all0 && r0 + 32 <= all1,
-                      bits_between(see0 - r0, see1 - r0) >> (4 * (lane >> 5)), c);
+                typename KeySums<T, DP>::Weights w;
+                x.weigh(row_at + to, row_at + to + Sh::TILE, stats + (i & 1) * 8 * QT + m * 4 + 16 * (lane >> 5), 4 * QT,
+                        r0 >= all0 && r0 + 32 <= all1, bits_between(see0 - r0, see1 - r0) >> (4 * (lane >> 5)), c, w);
+                x.add(col_at + to, col_at + to + Sh::TILE, w);
             }
         }
     } else {
