@@ -239,7 +239,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
         }
         d += __shfl_xor(d, 32, 64);
         const float lse = pr.lse[stat + rr];
-        if (r < rows && lane < 32) pr.work[stat + r] = d;
+        float rest = 0.f;
 #pragma unroll
         for (int t = 0; t < OT; ++t) o[t] = f16v{};
         const unsigned row_at = Tl::row_lane(lane), col_at = Tl::col_lane(lane);
@@ -270,11 +270,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
                 }
                 V8<T> ds[2];
 #pragma unroll
-                for (int x = 0; x < 16; ++x) ds[x >> 3][x & 7] = (T)s[x];
+                for (int x = 0; x < 16; ++x) {
+                    rest += s[x];
+                    ds[x >> 3][x & 7] = (T)s[x];
+                }
                 products<T, 2 * OT, 4>([&](int i) { return Tl::col(kc, 16 * (i & 1), i >> 1); },
                                        [&](int i, V8<T> a) { o[i >> 1] = mma(a, ds[i & 1], o[i >> 1]); });
             }
         }
+        // <dy, y> of the exact y is sum_j p_j <dy, v_j>: d, from the rounded y, and what
+        // the score gradients, whose sum is zero, left of it
+        rest += other_half(rest);
+        if (r < rows && lane < 32) pr.work[stat + r] = d + rest;
         if (live) {
             uint64_t again = __ballot(r < rows && store_channels(o, dq + out, pr.D, lane, pr.scale));
             again = (again | again >> 32) & 0xffffffffu;
