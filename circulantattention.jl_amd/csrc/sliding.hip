@@ -562,6 +562,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
     if (wave == 0) x.put(pr.work + sp.far_at + (int64_t)blockIdx.x * Sh::FAR_PART, lane);
 }
 
+// The far sums of `groups` groups of 32 keys from w on, added up in the order of
+// their parts into LDS as they lie in memory, by all of THREADS threads.
+template <typename T, int DP, int THREADS>
+__device__ __forceinline__ void sum_far(const float *w, int groups, int parts, CIRCATT_LDS float *buf) {
+    constexpr int SIZE = BwdShape<T, DP>::FAR_PART;
+    for (int e = 4 * threadIdx.x; e < groups * SIZE; e += 4 * THREADS) {
+        const float *we = w + (int64_t)(e / SIZE) * parts * SIZE + e % SIZE;
+        f4v sum = f4v{};
+#pragma unroll 8
+        for (int y = 0; y < parts; ++y) sum += *reinterpret_cast<const f4v *>(we + (int64_t)y * SIZE);
+        *(CIRCATT_LDS f4v *)(buf + e) = sum;
+    }
+}
+
 template <typename T, int DP>
 __global__ __launch_bounds__((256 * BwdShape<T, DP>::NG), (sizeof(T) == 2 && DP <= 64 ? 2 : 1))
 void sliding_dkdv(SlidingProblem pr, WalkSplit sp) {
@@ -636,15 +650,9 @@ void sliding_dkdv(SlidingProblem pr, WalkSplit sp) {
     if (sp.parts == 1 && kb * 4 < sp.far) {
         // the far sums of the block's keys, by everybody
         const int groups = sp.far - kb * 4 < 4 ? sp.far - kb * 4 : 4;
-        const float *w = pr.work + sp.far_at + (unit * sp.far + kb * 4) * sp.far_parts * Sh::FAR_PART;
         __syncthreads();
-        for (int e = 4 * threadIdx.x; e < groups * Sh::FAR_PART; e += 1024 * NG) {
-            const float *we = w + (int64_t)(e / Sh::FAR_PART) * sp.far_parts * Sh::FAR_PART + e % Sh::FAR_PART;
-            f4v sum = f4v{};
-#pragma unroll 8
-            for (int y = 0; y < sp.far_parts; ++y) sum += *reinterpret_cast<const f4v *>(we + (int64_t)y * Sh::FAR_PART);
-            *(CIRCATT_LDS f4v *)(buf + e) = sum;
-        }
+        sum_far<T, DP, 256 * NG>(pr.work + sp.far_at + (unit * sp.far + kb * 4) * sp.far_parts * Sh::FAR_PART, groups,
+                                 sp.far_parts, buf);
         __syncthreads();
         if (group == 0 && wave < groups) x.take(buf + wave * 64 * DP, lane);
     }
@@ -669,44 +677,48 @@ void sliding_dkdv(SlidingProblem pr, WalkSplit sp) {
     for (; again; again &= again - 1) hg.again(pr, j0 + __builtin_ctzll(again));
 }
 
-// The partial sums of a key, the far ones first, in the order of their parts: a
+// The partial sums of 32 keys, the far ones first, in the order of their parts: a
 // wavefront a key.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void sliding_dkdv_join(SlidingProblem pr, WalkSplit sp) {
     typedef BwdShape<T, DP> Sh;
-    const int lane = threadIdx.x & 63;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), unit = id / pr.L;
-    if (unit >= (int64_t)pr.B * pr.Hk) return;
-    const int j = (int)(id - unit * pr.L);
-    Pair k{0.f, 0.f}, v{0.f, 0.f};
-    auto sum = [&](const float *w, int parts, int size) {
-        for (int i = 0; i < parts; ++i, w += size) {
-            const Pair a = load_row(w, lane, DP), c = load_row(w + size / 2, lane, DP);
+    __shared__ __attribute__((aligned(16))) float far_mem[Sh::FAR_PART];
+    CIRCATT_LDS float *far = (CIRCATT_LDS float *)far_mem;
+    const int lane = threadIdx.x & 63, groups = (pr.L + 31) / 32;
+    const int64_t unit = blockIdx.x / groups;
+    const int group = (int)(blockIdx.x - unit * groups);
+    if (group < sp.far) {
+        sum_far<T, DP, 256>(pr.work + sp.far_at + (unit * sp.far + group) * sp.far_parts * Sh::FAR_PART, 1, sp.far_parts, far);
+        __syncthreads();
+    }
+    const HeadGroup<T> hg(pr, unit);
+    for (int x = threadIdx.x >> 6; x < 32; x += 4) {
+        const int j = group * 32 + x;
+        if (j >= pr.L) return;
+        Pair k{0.f, 0.f}, v{0.f, 0.f};
+        if (group < sp.far) {
+            // channel d of the key, as a wavefront's registers hold it
+            auto place = [&](int d) { return (16 * (d >> 5) + 4 * ((d >> 3) & 3) + (d & 3)) * 64 + x + 8 * (d & 4); };
+            if (lane < DP) k.a = far[place(lane)], v.a = far[Sh::FAR_PART / 2 + place(lane)];
+            if (lane + 64 < DP) k.b = far[place(lane + 64)], v.b = far[Sh::FAR_PART / 2 + place(lane + 64)];
+        }
+        const float *w = pr.work + sp.part_at + (unit * sp.blocks + (j >> 7)) * sp.parts * Sh::PART + (j & 127) * DP;
+        for (int i = 0; i < sp.parts; ++i, w += Sh::PART) {
+            const Pair a = load_row(w, lane, DP), c = load_row(w + Sh::PART / 2, lane, DP);
             k.a += a.a;
             k.b += a.b;
             v.a += c.a;
             v.b += c.b;
         }
-    };
-    if (j / 32 < sp.far) {
-        // channel d of the key, as a wavefront's registers hold it
-        auto place = [&](int d) { return (16 * (d >> 5) + 4 * ((d >> 3) & 3) + (d & 3)) * 64 + (j & 31) + 8 * (d & 4); };
-        const float *w = pr.work + sp.far_at + (unit * sp.far + j / 32) * sp.far_parts * Sh::FAR_PART;
-        for (int i = 0; i < sp.far_parts; ++i, w += Sh::FAR_PART) {
-            if (lane < DP) k.a += w[place(lane)], v.a += w[Sh::FAR_PART / 2 + place(lane)];
-            if (lane + 64 < DP) k.b += w[place(lane + 64)], v.b += w[Sh::FAR_PART / 2 + place(lane + 64)];
-        }
+        const int64_t out = ((int64_t)hg.b * pr.L + j) * pr.Hk * pr.D + (int64_t)hg.hk * pr.D;
+        k.a *= pr.scale;
+        k.b *= pr.scale;
+        store_row(static_cast<T *>(pr.dk) + out, lane, pr.D, k);
+        store_row(static_cast<T *>(pr.dv) + out, lane, pr.D, v);
+        // as in sliding_dkdv: not finite, or not in the type's range
+        const float size = fabsf((float)(T)k.a) + fabsf((float)(T)k.b) + fabsf((float)(T)v.a) + fabsf((float)(T)v.b);
+        if (__any(!(size < INFINITY)) && j < hg.n) hg.again(pr, j);
     }
-    sum(pr.work + sp.part_at + (unit * sp.blocks + (j >> 7)) * sp.parts * Sh::PART + (j & 127) * DP, sp.parts, Sh::PART);
-    const HeadGroup<T> hg(pr, unit);
-    const int64_t out = ((int64_t)hg.b * pr.L + j) * pr.Hk * pr.D + (int64_t)hg.hk * pr.D;
-    k.a *= pr.scale;
-    k.b *= pr.scale;
-    store_row(static_cast<T *>(pr.dk) + out, lane, pr.D, k);
-    store_row(static_cast<T *>(pr.dv) + out, lane, pr.D, v);
-    // as in sliding_dkdv: not finite, or not in the type's range
-    const float size = fabsf((float)(T)k.a) + fabsf((float)(T)k.b) + fabsf((float)(T)v.a) + fabsf((float)(T)v.b);
-    if (__any(!(size < INFINITY)) && j < hg.n) hg.again(pr, j);
 }
 
 // Parts: the estimate counts rounds of the chip's 256 compute units at the mean
@@ -771,7 +783,7 @@ hipError_t backward(const SlidingProblem &pr, hipStream_t s) {
         const int64_t units = (int64_t)pr.B * pr.Hk;
         if (sp.far > 0) sliding_dkdv_far<T, DP><<<(unsigned)(units * sp.far * sp.far_parts), 256, 0, s>>>(pr, sp);
         sliding_dkdv<T, DP><<<grid8(units * sp.blocks * sp.parts), 256 * BwdShape<T, DP>::NG, 0, s>>>(pr, sp);
-        if (sp.parts > 1) sliding_dkdv_join<T, DP><<<(unsigned)((units * pr.L + 3) / 4), 256, 0, s>>>(pr, sp);
+        if (sp.parts > 1) sliding_dkdv_join<T, DP><<<(unsigned)(units * ((pr.L + 31) / 32)), 256, 0, s>>>(pr, sp);
     }
     return hipGetLastError();
 }
