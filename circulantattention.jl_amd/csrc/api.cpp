@@ -97,7 +97,7 @@ int check_kind(int kind) {
 
 extern "C" {
 
-int circatt_version(void) { return 10000; }
+int circatt_version(void) { return 10100; }
 
 int circatt_set_math(int mode) {
     if (mode != CIRCATT_MATH_SPLIT_F16 && mode != CIRCATT_MATH_F32)
@@ -871,7 +871,7 @@ int circatt_axial_rotary(int dtype, int inverse, int interleaved, int naxes, int
                          void *y, void *stream) {
     CIRCATT_TRY(check_token_dtype(dtype));
     if (naxes < 1 || naxes > 3) return fail(CIRCATT_ERR_INVALID, "naxes=%d must be 1, 2 or 3", naxes);
-    if (nheads < 1 || nheads > 65536 || dh < 2 || dh % 2 != 0 || dh > 65536)
+    if (nheads < 1 || nheads > 65536 || dh < 2 || dh % 2 != 0 || dh > 65536 || nheads * dh > 1 << 24)
         return fail(CIRCATT_ERR_INVALID, "invalid heads: %lld of %lld channels (even)", (long long)nheads, (long long)dh);
     RotaryProblem pr{};
     const int32_t p[3] = {p1, naxes > 1 ? p2 : 0, naxes > 2 ? p3 : 0};

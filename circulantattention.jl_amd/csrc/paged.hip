@@ -215,7 +215,8 @@ __device__ __forceinline__ void finish_rows(const PagedProblem &pr, const PagedG
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T *y = static_cast<T *>(pr.y) + w.q0 * pr.H * pr.D + head * pr.G;
-    uint64_t again = __ballot(r < w.rows && store_channels(o, y + ((int64_t)rs.tok * pr.H + rs.g) * pr.D, pr.D, lane, inv));
+    const bool bad = r < w.rows && store_channels(o, y + ((int64_t)rs.tok * pr.H + rs.g) * pr.D, pr.D, lane, inv);
+    uint64_t again = __ballot(bad && l == l);  // NaN weights: the row is NaN, whatever it sees
     again = (again | again >> 32) & 0xffffffffu;
     const PagedKV<T> kv = paged_rows_of<T>(pr, w.b, head);
     for (; again; again &= again - 1) {
@@ -280,7 +281,10 @@ __device__ __forceinline__ void few_rows(const PagedProblem &pr, const PagedGrid
             f16v s[1];
             V8<T> p[2];
             x.scores(row_at + to, s);
-            if (there != ~0u || !(plain && see.all(lo, hi, k0, 32))) hide_keys(s[0], see.bits(rs.at, k0) & there, lane);
+            if (there != ~0u || !(plain && see.all(lo, hi, k0, 32))) {
+                asm volatile("");
+                hide_keys(s[0], see.bits(rs.at, k0) & there, lane);
+            }
             x.raise(x.largest(s) * (pr.scale * kLog2e));
             x.weigh(s, p, pr.scale * kLog2e);
             x.template add<1>(col_at + to, p);
@@ -393,6 +397,7 @@ __device__ __forceinline__ void chunk_rows(const PagedProblem &pr, const PagedGr
             if (NG == 2) __builtin_amdgcn_s_barrier();
             if (!mine) continue;
             if ((there & kFull) != kFull || !(plain && see.all(lo, hi, k0, KT))) {
+                asm volatile("");
 #pragma unroll
                 for (int m = 0; m < NB; ++m)
                     hide_keys(s[m], see.bits(rs.at, k0 + 32 * m) & (uint32_t)(there >> (32 * m)), lane);
@@ -483,10 +488,10 @@ __global__ __launch_bounds__(256) void paged_join(PagedProblem pr, PagedGrid gr)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             v[e] = (T)(o[e] * inv);
-            bad |= !(fabsf((float)v[e]) < INFINITY);
+            bad |= !(fabsf(o[e] * inv) < INFINITY);
         }
         if (i < rows && d < pr.D) *reinterpret_cast<V4<T> *>(y + d) = v;
-        const uint64_t again = __ballot(bad && i < rows && d < pr.D);
+        const uint64_t again = __ballot(bad && l == l && i < rows && d < pr.D);
         for (int h = 0; h < 2; ++h) {
             if (!(uint32_t)(again >> (32 * h))) continue;
             const int rj = w.r0 + i0 + h, tj = rj / pr.G, gj = rj - tj * pr.G;

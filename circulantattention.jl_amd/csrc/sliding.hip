@@ -112,6 +112,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
         auto look = [&](f16v (&s)[NB], int i) {  // hide keys of tile i, largest score
             const int k0 = tiles.key(i);
             if (!see.all(lo, hi, k0, KT)) {
+                asm volatile("");
 #pragma unroll
                 for (int m = 0; m < NB; ++m) hide_keys(s[m], see.bits(at, k0 + 32 * m), lane);
             }
@@ -164,8 +165,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             }
             // A value that is not finite reaches, as 0 times itself, every row of
             // a wavefront whose tile holds it: such rows are formed again from
-            // the keys that they see alone.
-            uint64_t again = __ballot(bad);
+            // the keys that they see alone.  (Not where the sum of the weights is
+            // NaN: then the row is, whatever it sees.)
+            uint64_t again = __ballot(bad && l == l);
             again = (again | again >> 32) & 0xffffffffu;
             const SignalKV<T> kv{kh, vh, pr.k_row, pr.v_row};
             for (; again; again &= again - 1) {
@@ -283,7 +285,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
         rest += other_half(rest);
         if (r < rows && lane < 32) pr.work[stat + r] = d + rest;
         if (live) {
-            uint64_t again = __ballot(r < rows && store_channels(o, dq + out, pr.D, lane, pr.scale));
+            // formed again as in the forward; a row whose statistics are NaN is NaN
+            const bool bad = r < rows && store_channels(o, dq + out, pr.D, lane, pr.scale);
+            uint64_t again = __ballot(bad && lse == lse && d == d);
             again = (again | again >> 32) & 0xffffffffu;
             const SignalKV<T> kv{kh, vh, pr.k_row, pr.v_row};
             for (; again; again &= again - 1) {
@@ -363,7 +367,8 @@ __device__ __forceinline__ void fetch_packed(const T *p, int64_t row, int r0, in
         const int slot = tid + k * THREADS, rl = slot / Tl::PC, u = ((slot % Tl::PC) ^ Tl::f(rl)) * 16;
         const int t = fdiv(r0 + rl, dg), g = r0 + rl - t * G;
         // units from D on stay out of the buffer whatever is added
-        dma::dma16(rs, m0 + k * THREADS * 16, (t - t0) * rb + g * hb + (u < hb ? u : dma::kOut), 0);
+        const unsigned off = (unsigned)((t - t0) * rb + g * hb) + (unsigned)(u < hb ? u : dma::kOut);
+        dma::dma16(rs, m0 + k * THREADS * 16, (int)off, 0);
     }
 }
 // COUNT floats from p + r0 on into LDS by the calling wavefront, zeros behind p[rows - 1]
@@ -405,7 +410,7 @@ struct KeySums {
     __device__ __forceinline__ void weigh(unsigned qr, unsigned gr, unsigned st, int stride, bool every, uint32_t half,
                                           float c, Weights &w) const {
         f16v s = f16v{}, dp = f16v{};
-        products<T, 2 * STEPS, AHEAD>([&](int i) { return Tl::row(i & 1 ? gr : qr, 0, i >> 1); },
+        products<T, 2 * STEPS, AHEAD - 1>([&](int i) { return Tl::row(i & 1 ? gr : qr, 0, i >> 1); },
                                       [&](int i, V8<T> a) {
                                           if (i & 1) dp = mma(a, v[i >> 1], dp);
                                           else s = mma(a, k[i >> 1], s);
@@ -640,12 +645,13 @@ void sliding_dkdv(SlidingProblem pr, WalkSplit sp) {
     } else {
         x.clear();
     }
+    const int lane_e = lane_again(), j_e = j0 + (lane_e & 31);
     CIRCATT_LDS float *buf = (CIRCATT_LDS float *)lds_mem;
     if (NG == 2) {
         __syncthreads();
-        if (group == 1) x.put(buf + wave * 64 * DP, lane);
+        if (group == 1) x.put(buf + wave * 64 * DP, lane_e);
         __syncthreads();
-        if (group == 0) x.take(buf + wave * 64 * DP, lane);
+        if (group == 0) x.take(buf + wave * 64 * DP, lane_e);
     }
     if (sp.parts == 1 && kb * 4 < sp.far) {
         // the far sums of the block's keys, by everybody
@@ -654,24 +660,26 @@ void sliding_dkdv(SlidingProblem pr, WalkSplit sp) {
         sum_far<T, DP, 256 * NG>(pr.work + sp.far_at + (unit * sp.far + kb * 4) * sp.far_parts * Sh::FAR_PART, groups,
                                  sp.far_parts, buf);
         __syncthreads();
-        if (group == 0 && wave < groups) x.take(buf + wave * 64 * DP, lane);
+        if (group == 0 && wave < groups) x.take(buf + wave * 64 * DP, lane_e);
     }
     if (group == 1) return;
     if (sp.parts > 1) {
-        x.write(pr.work + sp.part_at + (unit * sp.blocks * sp.parts + in) * Sh::PART + (32 * wave + (lane & 31)) * DP,
-                128 * DP, lane);
+        x.write(pr.work + sp.part_at + (unit * sp.blocks * sp.parts + in) * Sh::PART + (32 * wave + (lane_e & 31)) * DP,
+                128 * DP, lane_e);
         return;
     }
-    const int64_t out = ((int64_t)hg.b * pr.L + j) * pr.Hk * pr.D + (int64_t)hg.hk * pr.D;
+    const int64_t out = ((int64_t)hg.b * pr.L + j_e) * pr.Hk * pr.D + (int64_t)hg.hk * pr.D;
     T *kd = static_cast<T *>(pr.dk) + out, *vd = static_cast<T *>(pr.dv) + out;
     bool bad = false;
-    if (j < n) {
-        bad = store_channels(x.dk, kd, pr.D, lane, pr.scale);
-        bad |= store_channels(x.dv, vd, pr.D, lane, 1.f);
-    } else if (j < pr.L) {
-        zero_channels(kd, pr.D, lane);
-        zero_channels(vd, pr.D, lane);
+    if (j_e < n) {
+        bad = store_channels(x.dk, kd, pr.D, lane_e, pr.scale);
+        bad |= store_channels(x.dv, vd, pr.D, lane_e, 1.f);
+    } else if (j_e < pr.L) {
+        zero_channels(kd, pr.D, lane_e);
+        zero_channels(vd, pr.D, lane_e);
     }
+    // formed again as in the forward; a key that holds NaN has NaN gradients
+    if (bad) bad = !any_nan(hg.k + j_e * pr.k_row, pr.D);
     uint64_t again = __ballot(bad);
     again = (again | again >> 32) & 0xffffffffu;
     for (; again; again &= again - 1) hg.again(pr, j0 + __builtin_ctzll(again));
@@ -715,9 +723,11 @@ __global__ __launch_bounds__(256) void sliding_dkdv_join(SlidingProblem pr, Walk
         k.b *= pr.scale;
         store_row(static_cast<T *>(pr.dk) + out, lane, pr.D, k);
         store_row(static_cast<T *>(pr.dv) + out, lane, pr.D, v);
-        // as in sliding_dkdv: not finite, or not in the type's range
-        const float size = fabsf((float)(T)k.a) + fabsf((float)(T)k.b) + fabsf((float)(T)v.a) + fabsf((float)(T)v.b);
-        if (__any(!(size < INFINITY)) && j < hg.n) hg.again(pr, j);
+        // as in sliding_dkdv
+        if (__any(!(fabsf(k.a) + fabsf(k.b) + fabsf(v.a) + fabsf(v.b) < INFINITY)) && j < hg.n) {
+            const Pair key = load_row(hg.k + j * pr.k_row, lane, pr.D);
+            if (!__any(key.a != key.a || key.b != key.b)) hg.again(pr, j);
+        }
     }
 }
 

@@ -136,6 +136,14 @@ __device__ __forceinline__ float other_half(float x) {
     return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// The lane's number formed anew, for what follows a loop whose registers are full: no
+// address that hangs on it is kept through the loop.
+__device__ __forceinline__ int lane_again() {
+    int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
 // Eight channels from global memory, zero from channel D on (D a multiple of 8).
 template <typename T>
 __device__ __forceinline__ V8<T> load8(const T *p, int d, int D) {
@@ -279,9 +287,9 @@ struct Feed {
     }
 };
 
-// Hides the keys of a 32x32 block of scores whose bits are not set.
+// Hides the keys of a 32x32 block of scores whose bits are not set.  (Callers keep
+// the branch to it, as few tiles need it, by an empty asm before.)
 __device__ __forceinline__ void hide_keys(f16v &s, uint32_t seen, int lane) {
-    asm volatile("");  // a branch to here: few tiles need it
     const uint32_t half = seen >> (4 * (lane >> 5));
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -367,8 +375,16 @@ struct Rows {
     __device__ __forceinline__ float total() const { return l + __shfl_xor(l, 32, 64); }
 };
 
+// Whether a row holds NaN.
+template <typename T>
+__device__ __forceinline__ bool any_nan(const T *p, int D) {
+    bool nan = false;
+    for (int d = 0; d < D; ++d) nan |= (float)p[d] != (float)p[d];
+    return nan;
+}
+
 // Writes a row's channels (one lane and its other half), times f; whether one of
-// them is not finite in the row's type.
+// them is not finite (as Float32: one that the row's type cannot hold is itself).
 template <typename T, int OT>
 __device__ __forceinline__ bool store_channels(const f16v (&o)[OT], T *y, int D, int lane, float f) {
     bool bad = false;
@@ -380,8 +396,9 @@ __device__ __forceinline__ bool store_channels(const f16v (&o)[OT], T *y, int D,
             V4<T> v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                v[j] = (T)(o[t][i + j] * f);
-                bad |= !(fabsf((float)v[j]) < INFINITY) && d < D;
+                const float x = o[t][i + j] * f;
+                bad |= !(fabsf(x) < INFINITY) && d < D;
+                v[j] = (T)x;
             }
             if (d < D) *reinterpret_cast<V4<T> *>(y + d) = v;
         }

@@ -131,6 +131,57 @@ def test_sliding_other_rows_do_not_feel_a_bad_token(ca, dtype, value, t):
             M.check(g[~touched], r[0][~touched], r[1][~touched], "untouched")
 
 
+def test_sliding_everything_nan(ca):
+    """Inputs that are NaN throughout, as of a run that diverged: NaN results, and
+    no row formed again (a second at this size if each were)."""
+    q, k, v, dy = (torch.full((1, 2048, 256), math.nan, dtype=torch.bfloat16, device="cuda") for _ in range(4))
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    e0, e1 = torch.cuda.Event(True), torch.cuda.Event(True)
+    for _ in range(2):
+        e0.record()
+        y = ca.sliding_mh_attention(*leaves, None, 2)
+        grads = torch.autograd.grad(y, leaves, dy)
+        e1.record()
+    torch.cuda.synchronize()
+    assert all(torch.isnan(t).all() for t in (y, *grads))
+    assert e0.elapsed_time(e1) < 50.0
+
+
+def test_sliding_float16_gradients_out_of_range(ca):
+    """Score gradients that Float16 cannot hold: the rows are formed again in
+    Float32; gradients that it cannot hold are infinite."""
+    L, H, D, W = 64, 1, 64, 8
+    q, k, v = (randn(25 + i, 1, L, D, dtype=torch.float16) for i in range(3))
+    dy = randn(28, 1, L, D, dtype=torch.float16) * 3000
+    k = k * 0.05
+    leaves = [gpu(t, True) for t in (q, k, v)]
+    grads = torch.autograd.grad(ca.sliding_mh_attention(*leaves, W, H), leaves, dy.cuda())
+    want = M.sliding(*(t.double() for t in (q, k, v)), W, H, H, 0, 1 / math.sqrt(D), None, torch.float16, dy.double())[1:]
+    for g, (x, bx), name in zip(grads, want, ("dq", "dk", "dv")):
+        inside = x.abs() + bx < 65504
+        assert inside.float().mean() > 0.5, name
+        g = g.detach().double().cpu()
+        assert (torch.isinf(g) | ((g - x).abs() <= bx))[x.abs() + bx >= 65504].all(), name
+        M.check(g[inside], x[inside], bx[inside], name)
+
+
+def test_sliding_rows_past_2_gib(ca):
+    """Rows so far apart that a signal spans more than 2^31 bytes."""
+    L, H, Hk, D, W, S = 1100, 2, 1, 64, 60, 3
+    wide = torch.empty((1, L, 1 << 20), dtype=torch.bfloat16, device="cuda")
+    qkv = randn(35, 1, L, (H + 2 * Hk) * D, dtype=torch.bfloat16).cuda()
+    far = wide[..., :qkv.shape[-1]]
+    far.copy_(qkv)
+    dy = wide[..., 4096:4096 + H * D]
+    dy.copy_(randn(36, 1, L, H * D, dtype=torch.bfloat16))
+    res = []
+    for x, g in ((qkv, dy.contiguous()), (far, dy)):
+        q, k, v = (t.detach().requires_grad_(True) for t in x.split([H * D, Hk * D, Hk * D], -1))
+        y = ca.sliding_mh_attention(q, k, v, W, H, kv_heads=Hk, sinks=S)
+        res.append([y, *torch.autograd.grad(y, (q, k, v), g)])
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
 def test_sliding_large_scores(ca):
     """Scores of some hundreds, where a row is one key alone, and of the lowest
     values: the running maximum keeps every row finite."""
@@ -375,6 +426,42 @@ def test_paged_bad_tables_hide_tokens(ca):
         assert torch.isfinite(y).all() and (y[0] == 0).all()
 
 
+@pytest.mark.parametrize("new", [1, 40])
+def test_paged_other_rows_do_not_feel_a_bad_token(ca, new):
+    """A value that is not finite in a token that some rows see and others do not."""
+    dt, H, Hk, D, page, W, S = torch.bfloat16, 4, 2, 64, 16, 30, 2
+    c = Case([(200, new), (333, new), (64, min(new, 40))], H, Hk, D, page, dt)
+    args = [t.cuda() for t in (c.pages, c.lengths)]
+    kw = dict(kv_heads=Hk, sinks=S, offsets=c.offsets.cuda())
+    want, bound = M.paged(c.q.double(), *(t.double() for t in c.cache), c.pages, c.lengths, c.offsets, W, H, Hk, S,
+                          1 / math.sqrt(D), dt)
+    for b, t in ((0, 185), (1, 1), (1, 305), (1, 120), (2, 63)):
+        for which in (0, 1):
+            cache = [x.clone() for x in c.cache]
+            cache[which][c.pages[b, t // page], t % page] = math.nan
+            y = ca.paged_mh_attention(c.q.cuda(), *(x.cuda() for x in cache), *args, W, H, **kw)
+            seen = torch.zeros(c.q.shape[0], dtype=torch.bool)
+            lo, hi, n = int(c.offsets[b]), int(c.offsets[b + 1]), int(c.lengths[b])
+            seen[lo:hi] = M.visible(torch.arange(n - (hi - lo), n), n, W, S)[:, t]
+            assert torch.isnan(y.cpu()[seen]).all()
+            M.check(y[~seen], want[~seen], bound[~seen], f"token {t} of {b}")
+
+
+def test_paged_many_sequences(ca):
+    """More sequences than a wavefront has lanes, some without new tokens."""
+    g = torch.Generator().manual_seed(9)
+    n = torch.randint(0, 90, (150,), generator=g).tolist()
+    seqs = [(t, min(t, int(torch.randint(0, 5, (1,), generator=g)))) for t in n]
+    seqs[77] = (260, 100)
+    for dtype in (torch.bfloat16, torch.float32):
+        c = Case(seqs, 4, 2, 32, 8, dtype, pad=2)
+        want, bound = M.paged(c.q.double(), *(t.double() for t in c.cache), c.pages, c.lengths, c.offsets, 25, 4, 2, 3,
+                              1 / math.sqrt(32), dtype)
+        y = ca.paged_mh_attention(*(t.cuda() for t in (c.q, *c.cache, c.pages, c.lengths)), 25, 4, kv_heads=2, sinks=3,
+                                  offsets=c.offsets.cuda())
+        M.check(y, want, bound, "y")
+
+
 def test_paged_views_of_one_cache(ca):
     """k and v as halves of one allocation, by page and by channel."""
     dt, H, Hk, D, page = torch.bfloat16, 4, 2, 32, 16
@@ -582,6 +669,7 @@ def test_block_trains_and_serves(ca):
     y = m(xg)
     want = plain_block(m, x)
     # Float32 projections of 64 channels around the attention: 3 * 64 products' roundings
+    want = want.detach()
     tol = 400 * 2.0 ** -24 * float(want.abs().max() + 4)
     assert float((y.detach().double().cpu() - want).abs().max()) <= tol
     w = randn(401, 2, L, C).cuda()

@@ -128,7 +128,7 @@ def rotary(L, dtype=3, naxes=2, n=(8, 8, 1), tokens=64, nb=2, H=4, dh=64, p=(16,
     (dict(base=0.0), -1, "base"), (dict(base=math.nan), -1, "base"), (dict(tokens=65), -1, "grid of 64"),
     (dict(n=(1 << 20, 1 << 20, 1)), -1, "grid"), (dict(positions=P, pos_batch=100), -1, "positions"),
     (dict(x=None), -1, "x is NULL"), (dict(x_row=128), -1, "token stride"), (dict(y=P), -1, "alias"),
-    (dict(tokens=-1, positions=P), -1, "sizes"),
+    (dict(tokens=-1, positions=P), -1, "sizes"), (dict(H=1 << 16, dh=1 << 10), -1, "heads"),
 ])
 def test_rotary_refusals(L, args, code, fragment):
     expect(L, rotary(L, **args), code, fragment)
