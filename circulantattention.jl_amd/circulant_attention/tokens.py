@@ -80,22 +80,25 @@ def _head_count(C, nheads, what):
     return C // nheads
 
 
+def _sliding(train, q, k, v, W, S, H, Hk, scale, lengths):
+    """y, and with train what the backward takes of the call."""
+    (q, qr, qb), (k, kr, kb), (v, vr, vb) = _rows(q), _rows(k), _rows(v)
+    B, n, C = q.shape
+    y = torch.empty((B, n, C), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H * n), dtype=torch.float32, device=q.device) if train else None
+    code = _CODES[q.dtype]
+    _call(q.device, L.lib.circatt_sliding_fwd, code, n, B, H, Hk, C // H, W, S, scale, q.data_ptr(), qr, qb,
+          k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), ptr(lse))
+    return y, (q, k, v, y, lse, lengths), (code, W, S, H, Hk, scale, qr, qb, kr, kb, vr, vb)
+
+
 class SlidingAttentionFn(torch.autograd.Function):
     """y of sliding_mh_attention (circatt_sliding_fwd / circatt_sliding_bwd)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, W, S, H, Hk, scale, lengths):
-        (q, qr, qb), (k, kr, kb), (v, vr, vb) = _rows(q), _rows(k), _rows(v)
-        B, n, C = q.shape
-        y = torch.empty((B, n, C), dtype=q.dtype, device=q.device)
-        train = any(ctx.needs_input_grad[:3])
-        lse = torch.empty((B, H * n), dtype=torch.float32, device=q.device) if train else None
-        code = _CODES[q.dtype]
-        _call(q.device, L.lib.circatt_sliding_fwd, code, n, B, H, Hk, C // H, W, S, scale, q.data_ptr(), qr, qb,
-              k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), ptr(lse))
-        if train:
-            ctx.save_for_backward(q, k, v, y, lse, lengths)
-            ctx.meta = (code, W, S, H, Hk, scale, qr, qb, kr, kb, vr, vb)
+    def forward(ctx, *args):
+        y, saved, ctx.meta = _sliding(True, *args)
+        ctx.save_for_backward(*saved)
         return y
 
     @staticmethod
@@ -155,7 +158,10 @@ def sliding_mh_attention(q, k, v, W, nheads: int, *, kv_heads: int = None, sinks
     W, sinks, scale = _window(W, sinks, scale, dh)
     if lengths is not None:
         lengths = _index(lengths, "lengths", q, (q.shape[0],))
-    return SlidingAttentionFn.apply(q, k, v, W, sinks, nheads, kv_heads, scale, lengths)
+    args = (q, k, v, W, sinks, nheads, kv_heads, scale, lengths)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return SlidingAttentionFn.apply(*args)
+    return _sliding(False, *args)[0]
 
 
 def _cache(cache_k, cache_v, like):
@@ -281,10 +287,10 @@ class AxialRotaryFn(torch.autograd.Function):
     the other way."""
 
     @staticmethod
-    def forward(ctx, x, grid, pairs, H, base, positions, per_image, interleaved):
-        ctx.meta = (grid, pairs, H, base, per_image, interleaved)
+    def forward(ctx, x, positions, *meta):
+        ctx.meta = meta
         ctx.save_for_backward(positions)
-        return _turn(x, 0, *ctx.meta, positions)
+        return _turn(x, 0, *meta, positions)
 
     @staticmethod
     @once_differentiable
@@ -340,7 +346,10 @@ def axial_rotary(x, pairs, nheads: int, *, base: float = 10000.0, positions: tor
         per_image = x.dim() > 2 and positions.dim() == x.dim()
         shape = x.shape[:-1] if per_image or x.dim() == 2 else x.shape[1:-1]
         positions = _index(positions, "positions", x, (*shape, len(pairs)))
-    return AxialRotaryFn.apply(x, grid, pairs, int(nheads), float(base), positions, per_image, bool(interleaved))
+    meta = (grid, pairs, int(nheads), float(base), per_image, bool(interleaved))
+    if torch.is_grad_enabled() and x.requires_grad:
+        return AxialRotaryFn.apply(x, positions, *meta)
+    return _turn(x, 0, *meta, positions)
 
 
 __all__ = ["axial_rotary", "paged_append_", "paged_mh_attention", "sliding_mh_attention"]
