@@ -30,11 +30,18 @@ __device__ __forceinline__ NewToken new_token(const int32_t *offsets, const int3
 // Attention.  Rows are packed as in sliding.hip: row r of a sequence and a head
 // of keys is head r % G of its new token r / G.  A block is R of them.
 //   few_rows (R = 32): tiles of 32 keys for each of NW wavefronts, which share the
-//   rows and join their sums at the end; bound by reading the cache.
+//   rows and join their sums at the end; bound by reading the cache.  The next
+//   token of 64 sequences of up to 8192, window 4096, 8 heads of 128 keys, bf16:
+//   182 us, 5.2 TB/s, the rate of a large copy.
 //   chunk_rows (R = 128): four wavefronts of 32 rows share the tiles, as in
-//   sliding_fwd, and NG such groups share the block's keys; bound by the products.
+//   sliding_fwd, and NG such groups share the block's keys, half a round apart (in
+//   step: 117 us at the size that follows); bound by the products.  Two chunks of
+//   512 tokens behind up to 12000, window 4096, 32 heads of 128 over 8: 86 us, 650
+//   TFLOP/s.
 // Where blocks are few, each is split along its tiles over `splits` workgroups,
-// whose partial sums paged_join adds up.
+// whose partial sums paged_join adds up.  A mixed batch has both kinds in one launch
+// (33 sequences, some of one token, some of up to 128: 59 us; in two launches 104,
+// all in blocks of 128 rows 91).
 enum Which { kAll, kShort, kLong };  // sequences: all, those of up to 32 rows, the others
 struct PagedGrid {
     int which;
@@ -586,7 +593,8 @@ void launch(const PagedProblem &pr, hipStream_t s) {
 // Append.
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// One wavefront a token: its k, then its v, in units of U.
+// One wavefront a token: its k, then its v, in units of U.  Bound by memory: chunks of
+// 4 x 4096 tokens of 1024 channels, bf16, 21.7 us with the call, 4.8 TB/s.
 template <typename U>
 __global__ __launch_bounds__(256) void append_rows(AppendProblem pr) {
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
