@@ -35,13 +35,12 @@ __device__ __forceinline__ NewToken new_token(const int32_t *offsets, const int3
 //   182 us, 5.2 TB/s, the rate of a large copy.
 //   chunk_rows (R = 128): four wavefronts of 32 rows share the tiles, as in
 //   sliding_fwd, and NG such groups share the block's keys, half a round apart (in
-//   step: 117 us at the size that follows); bound by the products.  Two chunks of
+//   step: 91 us at the size that follows); bound by the products.  Two chunks of
 //   512 tokens behind up to 12000, window 4096, 32 heads of 128 over 8: 86 us, 650
 //   TFLOP/s.
 // Where blocks are few, each is split along its tiles over `splits` workgroups,
 // whose partial sums paged_join adds up.  A mixed batch has both kinds in one launch
-// (33 sequences, some of one token, some of up to 128: 59 us; in two launches 104,
-// all in blocks of 128 rows 91).
+// (33 sequences, some of one token, some of up to 128: 59 us; in two launches 104).
 enum Which { kAll, kShort, kLong };  // sequences: all, those of up to 32 rows, the others
 struct PagedGrid {
     int which;

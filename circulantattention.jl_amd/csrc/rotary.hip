@@ -6,7 +6,10 @@
 // every head of a token reads them: the angle is formed in turns in 64 bits
 // (positions up to 2^31 keep it to 2^-24 of a turn) and reduced to half a
 // turn, which the hardware's sine and cosine, whose argument is in turns, take
-// to 1.2e-7.  Then it streams its tokens once through 16-byte units.
+// to 1.2e-7.  Then it streams its tokens once through 16-byte units: bound by
+// memory.  4 x 256 x 256 pixels of 64 Float32 channels 26 us, 5.1 TB/s; 80 x 45 x
+// 16 video tokens of 16 heads of 128, bf16, whose sections end within units, 112
+// us with the call, 4.2 TB/s (by single channels 310).
 #include "token_kernels.h"
 
 namespace circatt {

@@ -22,20 +22,20 @@ __device__ __forceinline__ int signal_length(const SlidingProblem &pr, int b) {
 // whose L2 then holds their common tiles.
 //
 // Bound by the products and the softmax between them, not by memory: a wavefront's
-// tile is 32 products of 32 cycles and some 190 other vector instructions, 32 of
-// them exponentials of 8 cycles.  8192 tokens, 32 heads of 128 over 8, window 1024,
-// 4 sinks, bf16: 166 us, 780 TFLOP/s of the pairs that are seen (some 850 of those
+// tile is 32 products of 32 cycles and, by the counters, some 270 other vector
+// instructions with starts and edges, 32 of them exponentials of 8 cycles.  8192 tokens, 32 heads of 128 over 8, window 1024,
+// 4 sinks, bf16: 166 us, 780 TFLOP/s of the pairs that are seen (870 of those
 // formed: edges of tiles); the same without a window 535 us, 1030 TFLOP/s, where a
 // large library product of this card reaches 1190.  Copies of the kernel without
-// its DMA, or with operands from registers instead of LDS, take 21 and 53 us less.
-// Two rounds in one run (the next tile's scores among this one's exponentials)
+// its DMA, or with operands from registers instead of LDS, take 21 and 32 us less
+// (both: 53).  Two rounds in one run (the next tile's scores among this one's exponentials)
 // take 166 us where one after another took 175; explicit orders of the run's
 // instructions, wavefront priorities, operands read earlier and tiles of 32 keys
 // in five places changed nothing or lost (177 us).
 //
 // Backward, queries: the same blocks with tiles in two buffers.
 template <typename T, int DP>
-struct FwdShape {
+struct DqShape {
     // Float32 rows are twice as long: half the keys fill the same LDS
     static constexpr int KT = sizeof(T) == 2 ? 64 : 32;
     static constexpr int TILE = KT * Tile<T, DP>::ROW;
@@ -204,12 +204,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
 // of its 32 rows as second operands; for 32 keys at a time it forms S' = K Q'
 // and dP' = V dY', from them dS' = P' (dP' - d) in the layout of a second
 // operand, and dQ' += K' dS' with K' by the transposing reads.  dS is rounded to
-// the element type there, as P is in the forward: its error is that of dq's own
-// rounding.  2 x 4096 tokens, 16 heads of 128 over 4, window 512, bf16: 80 us, 610
-// TFLOP/s of the pairs that are seen.
+// the element type there, as P is in the forward, and d is formed from the
+// rounded y: each term is off by up to half a step of itself, and with small
+// windows, where few terms average out, the error of dq has been up to 1.8 times
+// that of a form that rounds only its results.  2 x 4096 tokens, 16 heads of 128
+// over 4, window 512, bf16: 80 us, 610 TFLOP/s of the pairs that are seen.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void sliding_dq(SlidingProblem pr, int blocks) {
-    typedef FwdShape<T, DP> Sh;
+    typedef DqShape<T, DP> Sh;
     typedef Tile<T, DP> Tl;
     constexpr int KT = Sh::KT, STEPS = DP / 16, OT = DP / 32;
     __shared__ __attribute__((aligned(1024))) char lds_mem[4 * Sh::TILE];
@@ -334,14 +336,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
 // split over `parts` workgroups, whose Float32 sums sliding_dkdv_join adds up in
 // order.  At the size above 109 us, 600 TFLOP/s; the operands and sums of 32 keys
 // take 192 of a lane's 256 registers, and what is left bounds how far ahead
-// operands can be read (read one product ahead: 146 us).  Workgroups of one group
-// whose walks were split in three for a full chip took 187 us and 23 more to add
-// up; barriers of a group alone, by a count in LDS, changed nothing.
+// operands can be read.  An earlier form, workgroups of one group whose walks were
+// split in three for a full chip, took 187 us and 23 more to add up; barriers of a group alone, by a count in LDS, changed nothing.
 //
 // The rows that see a sink from behind its block's window are another walk,
 // sliding_dkdv_far's, for 32 keys and with a wavefront for every tile: a few
-// sinks would leave most of a workgroup of 128 keys idle (18 us at the size above,
-// latency of four tiles a wavefront).
+// sinks would leave most of a workgroup of 128 keys idle (18 us at the size above).
 template <typename T, int DP>
 struct BwdShape {
     static constexpr int QT = sizeof(T) == 2 ? 64 : 32;
