@@ -79,11 +79,11 @@ SIGNATURES = {
     "circatt_sum_middle": (_int, [_p, _p, _i64, _i64, _i64, _p]),
     "circatt_count_unequal": (_int, [_int, _i64, _p, _p, _p, _p]),
     "circatt_sliding_fwd": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _i64,
-                                   _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p]),
+                                   _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p]),
     "circatt_sliding_bwd_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "circatt_sliding_bwd": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _i64,
-                                   _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _p, _p,
-                                   _p, _p, _i64, _p]),
+                                   _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _p,
+                                   _p, _p, _p, _i64, _p]),
     "circatt_paged_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "circatt_paged_attention": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _p,
                                        _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _int, _p,

@@ -86,10 +86,11 @@ def _sliding(train, q, k, v, W, S, H, Hk, scale, lengths):
     B, n, C = q.shape
     y = torch.empty((B, n, C), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, H * n), dtype=torch.float32, device=q.device) if train else None
+    rest = torch.empty_like(y) if train and q.dtype != torch.float32 else None
     code = _CODES[q.dtype]
     _call(q.device, L.lib.circatt_sliding_fwd, code, n, B, H, Hk, C // H, W, S, scale, q.data_ptr(), qr, qb,
-          k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), ptr(lse))
-    return y, (q, k, v, y, lse, lengths), (code, W, S, H, Hk, scale, qr, qb, kr, kb, vr, vb)
+          k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), ptr(rest), ptr(lse))
+    return y, (q, k, v, y, rest, lse, lengths), (code, W, S, H, Hk, scale, qr, qb, kr, kb, vr, vb)
 
 
 class SlidingAttentionFn(torch.autograd.Function):
@@ -104,7 +105,7 @@ class SlidingAttentionFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        q, k, v, y, lse, lengths = ctx.saved_tensors
+        q, k, v, y, rest, lse, lengths = ctx.saved_tensors
         code, W, S, H, Hk, scale, qr, qb, kr, kb, vr, vb = ctx.meta
         B, n, C = q.shape
         dy, dr, db = _rows(dy)
@@ -116,8 +117,8 @@ class SlidingAttentionFn(torch.autograd.Function):
         wbytes = L.lib.circatt_sliding_bwd_workspace_bytes(code, n, B, H, Hk, C // H, W, S)
         work = torch.empty((max(wbytes, 4) // 4,), dtype=torch.float32, device=q.device)
         _call(q.device, L.lib.circatt_sliding_bwd, code, n, B, H, Hk, C // H, W, S, scale, q.data_ptr(), qr, qb,
-              k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), lse.data_ptr(), dy.data_ptr(),
-              dr, db, dq.data_ptr(), ptr(dk), ptr(dv), work.data_ptr(), wbytes)
+              k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), ptr(rest), lse.data_ptr(),
+              dy.data_ptr(), dr, db, dq.data_ptr(), ptr(dk), ptr(dv), work.data_ptr(), wbytes)
         return dq, dk, dv, None, None, None, None, None, None
 
 

@@ -720,12 +720,24 @@ int paged_problem(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_he
     return CIRCATT_OK;
 }
 
+bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y ? y - x < (uintptr_t)na : x - y < (uintptr_t)nb;
+}
+
+int check_rests(const void *rest, const void *y, int64_t bytes, int dtype) {
+    if (dtype == CIRCATT_F32) return fail(CIRCATT_ERR_INVALID, "y_rest belongs to the 16-bit types");
+    if (reinterpret_cast<uintptr_t>(rest) % 16 != 0) return fail(CIRCATT_ERR_INVALID, "y_rest must be 16-byte aligned");
+    if (overlap(rest, bytes, y, bytes)) return fail(CIRCATT_ERR_INVALID, "y_rest must not overlap y");
+    return CIRCATT_OK;
+}
+
 }  // namespace
 
 int circatt_sliding_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
                         int64_t sinks, float scale, const void *q, int64_t q_row, int64_t q_batch, const void *k,
                         int64_t k_row, int64_t k_batch, const void *v, int64_t v_row, int64_t v_batch,
-                        const int32_t *lengths, void *y, float *lse, void *stream) {
+                        const int32_t *lengths, void *y, void *y_rest, float *lse, void *stream) {
     SlidingProblem pr;
     CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
     if (L == 0 || B == 0) return ok();
@@ -738,7 +750,9 @@ int circatt_sliding_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t
     pr.k = k, pr.k_row = k_row, pr.k_batch = k_batch;
     pr.v = v, pr.v_row = v_row, pr.v_batch = v_batch;
     pr.lengths = lengths;
+    if (y_rest != nullptr) CIRCATT_TRY(check_rests(y_rest, y, L * B * nheads * dh * es, dtype));
     pr.y = y;
+    pr.y_rest = y_rest;
     pr.lse = lse;
     return hip_result(launch_sliding_fwd(pr, as_stream(stream)), "circatt_sliding_fwd");
 }
@@ -753,8 +767,8 @@ int64_t circatt_sliding_bwd_workspace_bytes(int dtype, int64_t L, int64_t B, int
 int circatt_sliding_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
                         int64_t sinks, float scale, const void *q, int64_t q_row, int64_t q_batch, const void *k,
                         int64_t k_row, int64_t k_batch, const void *v, int64_t v_row, int64_t v_batch,
-                        const int32_t *lengths, const void *y, const float *lse, const void *dy, int64_t dy_row,
-                        int64_t dy_batch, void *dq, void *dk, void *dv, void *workspace, int64_t workspace_bytes,
+                        const int32_t *lengths, const void *y, const void *y_rest, const float *lse, const void *dy,
+                        int64_t dy_row, int64_t dy_batch, void *dq, void *dk, void *dv, void *workspace, int64_t workspace_bytes,
                         void *stream) {
     SlidingProblem pr;
     CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
@@ -781,7 +795,9 @@ int circatt_sliding_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t
     pr.k = k, pr.k_row = k_row, pr.k_batch = k_batch;
     pr.v = v, pr.v_row = v_row, pr.v_batch = v_batch;
     pr.lengths = lengths;
+    if (y_rest != nullptr) CIRCATT_TRY(check_rests(y_rest, y, L * B * nheads * dh * es, dtype));
     pr.y = const_cast<void *>(y);
+    pr.y_rest = const_cast<void *>(y_rest);
     pr.lse = const_cast<float *>(lse);
     pr.dy = dy, pr.dy_row = dy_row, pr.dy_batch = dy_batch;
     pr.dq = dq, pr.dk = dk, pr.dv = dv;
@@ -823,6 +839,12 @@ int circatt_paged_attention(int dtype, int64_t T, int64_t B, int64_t nheads, int
         if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
             return fail(CIRCATT_ERR_INVALID, "workspace must be 16-byte aligned");
     }
+    // a block writes rows that others still read of the cache, and splits read q again
+    const int64_t y_bytes = T * nheads * dh * es, q_bytes = ((T - 1) * q_row + nheads * dh) * es;
+    const int64_t cache_bytes = ((npages - 1) * page_stride + (page_size - 1) * row_stride + kv_heads * dh) * es;
+    if (overlap(y, y_bytes, q, q_bytes) || overlap(y, y_bytes, cache_k, cache_bytes) ||
+        overlap(y, y_bytes, cache_v, cache_bytes))
+        return fail(CIRCATT_ERR_INVALID, "y must not overlap q or the caches");
     pr.q = q, pr.q_row = q_row;
     pr.k = cache_k, pr.v = cache_v;
     pr.npages = (int)npages;

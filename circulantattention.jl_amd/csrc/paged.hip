@@ -229,7 +229,7 @@ __device__ __forceinline__ void finish_rows(const PagedProblem &pr, const PagedG
         const int j = __builtin_ctzll(again);
         const int tj = __builtin_amdgcn_readlane(rs.tok, j), gj = __builtin_amdgcn_readlane(rs.g, j);
         forward_row(static_cast<const T *>(pr.q) + (w.q0 + tj) * pr.q_row + (head * pr.G + (int64_t)gj * pr.D),
-                    y + ((int64_t)tj * pr.H + gj) * pr.D, (float *)nullptr, kv, __builtin_amdgcn_readlane(rs.at, j), pr.W, pr.S,
+                    y + ((int64_t)tj * pr.H + gj) * pr.D, (T *)nullptr, kv, __builtin_amdgcn_readlane(rs.at, j), pr.W, pr.S,
                     pr.D, pr.scale * kLog2e);
     }
 }
@@ -504,7 +504,7 @@ __global__ __launch_bounds__(256) void paged_join(PagedProblem pr, PagedGrid gr)
             const int64_t held = (int64_t)pr.maxp << pr.page_log2;
             const int pos = w.first + tj;
             forward_row(static_cast<const T *>(pr.q) + (w.q0 + tj) * pr.q_row + (head * pr.G + (int64_t)gj * pr.D),
-                        static_cast<T *>(pr.y) + (w.q0 + tj) * pr.H * pr.D + head * pr.G + (int64_t)gj * pr.D, (float *)nullptr,
+                        static_cast<T *>(pr.y) + (w.q0 + tj) * pr.H * pr.D + head * pr.G + (int64_t)gj * pr.D, (T *)nullptr,
                         paged_rows_of<T>(pr, w.b, head), pos >= held ? -1 : pos, pr.W, pr.S, pr.D, pr.scale * kLog2e);
         }
     }

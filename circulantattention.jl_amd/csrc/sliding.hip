@@ -84,6 +84,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
     const int rows = n * pr.G, r0 = w.block * 128, all_rows = pr.L * pr.G;
     const int r = r0 + 32 * wave + (lane & 31);
     T *y = static_cast<T *>(pr.y) + (int64_t)b * pr.L * pr.H * pr.D + (int64_t)hk * pr.G * pr.D;
+    T *rest = pr.y_rest == nullptr ? nullptr : static_cast<T *>(pr.y_rest) + (y - static_cast<T *>(pr.y));
     const int64_t stat = ((int64_t)b * pr.Hk + hk) * all_rows;
     // the wavefront's rows, those past the end doubling the last one
     const int rr = r < rows ? r : rows - 1, at = rows > 0 ? rr / pr.G : -1, g = rows > 0 ? rr - at * pr.G : 0;
@@ -173,6 +174,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             bool bad = false;
             if (r < rows) {
                 bad = store_channels(x.o, y + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv);
+                if (rest != nullptr) store_rests(x.o, rest + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv);
                 if (pr.lse != nullptr && lane < 32)
                     pr.lse[stat + r] = l == 0.f ? INFINITY : x.m + __builtin_amdgcn_logf(l);
             }
@@ -186,8 +188,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             for (; again; again &= again - 1) {
                 const int j = __builtin_ctzll(again);
                 const int aj = __builtin_amdgcn_readlane(at, j), gj = __builtin_amdgcn_readlane(g, j);
-                forward_row(qh + aj * pr.q_row + (int64_t)gj * pr.D, y + ((int64_t)aj * pr.H + gj) * pr.D,
-                            (float *)nullptr, kv, aj, pr.W, pr.S, pr.D, c);
+                const int64_t out = ((int64_t)aj * pr.H + gj) * pr.D;
+                forward_row(qh + aj * pr.q_row + (int64_t)gj * pr.D, y + out, rest == nullptr ? rest : rest + out, kv, aj, pr.W, pr.S, pr.D, c);
             }
         }
     }
@@ -204,10 +206,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
 // of its 32 rows as second operands; for 32 keys at a time it forms S' = K Q'
 // and dP' = V dY', from them dS' = P' (dP' - d) in the layout of a second
 // operand, and dQ' += K' dS' with K' by the transposing reads.  dS is rounded to
-// the element type there, as P is in the forward, and d is formed from the
-// rounded y: each term is off by up to half a step of itself, and with small
-// windows, where few terms average out, the error of dq has been up to 1.8 times
-// that of a form that rounds only its results.  2 x 4096 tokens, 16 heads of 128
+// the element type there, as P is in the forward.  d = <dy, y> takes y with what
+// its rounding took (y_rest): where few keys carry a row, the score gradients
+// cancel most, and with the rounded y alone the error of dq was up to 3 times that
+// of a form that rounds only its results, now 1.6.  2 x 4096 tokens, 16 heads of 128
 // over 4, window 512, bf16: 80 us, 610 TFLOP/s of the pairs that are seen.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void sliding_dq(SlidingProblem pr, int blocks) {
@@ -235,6 +237,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
         const T *qh = static_cast<const T *>(pr.q) + b * pr.q_batch + (int64_t)hk * pr.G * pr.D;
         const T *gh = static_cast<const T *>(pr.dy) + b * pr.dy_batch + (int64_t)hk * pr.G * pr.D;
         const T *yh = static_cast<const T *>(pr.y) + head;
+        const T *eh = pr.y_rest == nullptr ? nullptr : static_cast<const T *>(pr.y_rest) + head;
         const Sight see{pr.W, pr.S};
         const TileList<KT> tiles(r0 / pr.G, last / pr.G, pr.W, pr.S);
         const float c = pr.scale * kLog2e;
@@ -254,8 +257,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
             q[k] = load8(qh + at * pr.q_row + (int64_t)g * pr.D, ch, pr.D);
             dy[k] = load8(gh + at * pr.dy_row + (int64_t)g * pr.D, ch, pr.D);
             const V8<T> y = load8(yh + out, ch, pr.D);
+            const V8<T> e = eh == nullptr ? V8<T>{} : load8(eh + out, ch, pr.D);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) d = fmaf((float)y[j], (float)dy[k][j], d);
+            for (int j = 0; j < 8; ++j) d = fmaf((float)y[j] + (float)e[j], (float)dy[k][j], d);
         }
         d += __shfl_xor(d, 32, 64);
         const float lse = pr.lse[stat + rr];
@@ -298,8 +302,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
                                        [&](int i, V8<T> a) { o[i >> 1] = mma(a, ds[i & 1], o[i >> 1]); });
             }
         }
-        // <dy, y> of the exact y is sum_j p_j <dy, v_j>: d, from the rounded y, and what
-        // the score gradients, whose sum is zero, left of it
+        // <dy, y> of the exact y is sum_j p_j <dy, v_j>: d and what the score gradients,
+        // whose sum is zero, left of it (P's rounding in y)
         rest += other_half(rest);
         if (r < rows && lane < 32) pr.work[stat + r] = d + rest;
         if (live) {
@@ -312,7 +316,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
                 const int j = __builtin_ctzll(again);
                 const int aj = __builtin_amdgcn_readlane(at, j), gj = __builtin_amdgcn_readlane(g, j);
                 const int64_t oj = ((int64_t)aj * pr.H + gj) * pr.D, sj = stat + (int64_t)aj * pr.G + gj;
-                dq_row(qh + aj * pr.q_row + (int64_t)gj * pr.D, yh + oj, gh + aj * pr.dy_row + (int64_t)gj * pr.D, dq + oj,
+                dq_row(qh + aj * pr.q_row + (int64_t)gj * pr.D, yh + oj, eh == nullptr ? eh : eh + oj, gh + aj * pr.dy_row + (int64_t)gj * pr.D, dq + oj,
                        pr.lse[sj], pr.work + sj, kv, aj, pr.W, pr.S, pr.D, c, pr.scale);
             }
         }

@@ -36,6 +36,12 @@ __device__ __forceinline__ void store_row(T *p, int lane, int D, Pair v) {
     if (lane < D) p[lane] = (T)v.a;
     if (lane + 64 < D) p[lane + 64] = (T)v.b;
 }
+// x minus x rounded to T, 0 where that is not finite.
+template <typename T>
+__device__ __forceinline__ T rounding_rest(float x) {
+    const float e = x - (float)(T)x;
+    return fabsf(e) < INFINITY ? (T)e : (T)0.f;
+}
 __device__ __forceinline__ float wave_sum(float x) {
     for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m, 64);
     return x;
@@ -44,8 +50,9 @@ __device__ __forceinline__ float dot(Pair x, Pair y) { return wave_sum(x.a * y.a
 
 // y = sum_j softmax_j(c q.k_j) v_j in base 2 over [0, min(S, lo)) and [lo, pos],
 // lo = max(0, pos - W + 1).  kv.row(j): whether key j is there, and its rows.
+// rest: what y's rounding took, or NULL.
 template <typename T, typename KV>
-__device__ void forward_row(const T *q, T *y, float *lse, const KV &kv, int pos, int W, int S, int D,
+__device__ void forward_row(const T *q, T *y, T *rest, const KV &kv, int pos, int W, int S, int D,
                             float c) {
     const int lane = threadIdx.x & 63;
     const Pair qr = load_row(q, lane, D);
@@ -67,18 +74,25 @@ __device__ void forward_row(const T *q, T *y, float *lse, const KV &kv, int pos,
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     store_row(y, lane, D, Pair{o.a * inv, o.b * inv});
-    if (lse != nullptr && lane == 0)
-        *lse = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    if (rest != nullptr)
+        store_row(rest, lane, D, Pair{(float)rounding_rest<T>(o.a * inv), (float)rounding_rest<T>(o.b * inv)});
 }
 
 // The gradient of row i's query: dq = scale sum_j p_j (<dy, v_j> - d) k_j with
-// p_j = exp2(c q.k_j - lse) and d = <dy, y>, which is stored too.
+// p_j = exp2(c q.k_j - lse) and d = <dy, y + rest> (rest may be NULL), which is
+// stored too.
 template <typename T, typename KV>
-__device__ void dq_row(const T *q, const T *y, const T *dy, T *dq, float lse, float *dsum, const KV &kv,
+__device__ void dq_row(const T *q, const T *y, const T *rest, const T *dy, T *dq, float lse, float *dsum, const KV &kv,
                        int pos, int W, int S, int D, float c, float scale) {
     const int lane = threadIdx.x & 63;
     const Pair qr = load_row(q, lane, D), gr = load_row(dy, lane, D);
-    const float d = dot(gr, load_row(y, lane, D));
+    Pair yr = load_row(y, lane, D);
+    if (rest != nullptr) {
+        const Pair e = load_row(rest, lane, D);
+        yr.a += e.a;
+        yr.b += e.b;
+    }
+    const float d = dot(gr, yr);
     if (lane == 0) *dsum = d;
     const int lo = pos - W + 1 > 0 ? pos - W + 1 : 0;
     Pair o{0.f, 0.f};

@@ -404,6 +404,20 @@ __device__ __forceinline__ bool store_channels(const f16v (&o)[OT], T *y, int D,
         }
     return bad;
 }
+// What the rounding of such a row took (0 where it is not finite).
+template <typename T, int OT>
+__device__ __forceinline__ void store_rests(const f16v (&o)[OT], T *rest, int D, int lane, float f) {
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = 32 * t + 2 * i + 4 * (lane >> 5);
+            V4<T> v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = rounding_rest<T>(o[t][i + j] * f);
+            if (d < D) *reinterpret_cast<V4<T> *>(rest + d) = v;
+        }
+}
 template <typename T>
 __device__ __forceinline__ void zero_channels(T *y, int D, int lane) {
     for (int d = 4 * (lane >> 5); d < D; d += 8) *reinterpret_cast<V4<T> *>(y + d) = V4<T>{};

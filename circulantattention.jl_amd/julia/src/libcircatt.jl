@@ -158,13 +158,13 @@ circatt_count_unequal(kind, n, a, b, count, stream) =
           kind, n, a, b, count, stream)
 
 circatt_sliding_fwd(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, q_batch, k,
-                    k_row, k_batch, v, v_row, v_batch, lengths, y, lse, stream) =
+                    k_row, k_batch, v, v_row, v_batch, lengths, y, y_rest, lse, stream) =
     ccall((:circatt_sliding_fwd, libcircatt), Cint,
           (Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Cfloat, Ptr{Cvoid},
            Int64, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Int32},
-           Ptr{Cvoid}, Ptr{Cfloat}, Ptr{Cvoid}),
+           Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cfloat}, Ptr{Cvoid}),
           dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, q_batch, k,
-          k_row, k_batch, v, v_row, v_batch, lengths, y, lse, stream)
+          k_row, k_batch, v, v_row, v_batch, lengths, y, y_rest, lse, stream)
 
 circatt_sliding_bwd_workspace_bytes(dtype, L, B, nheads, kv_heads, dh, window, sinks) =
     ccall((:circatt_sliding_bwd_workspace_bytes, libcircatt), Int64,
@@ -172,15 +172,15 @@ circatt_sliding_bwd_workspace_bytes(dtype, L, B, nheads, kv_heads, dh, window, s
           dtype, L, B, nheads, kv_heads, dh, window, sinks)
 
 circatt_sliding_bwd(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, q_batch, k,
-                    k_row, k_batch, v, v_row, v_batch, lengths, y, lse, dy, dy_row, dy_batch, dq,
+                    k_row, k_batch, v, v_row, v_batch, lengths, y, y_rest, lse, dy, dy_row, dy_batch, dq,
                     dk, dv, workspace, workspace_bytes, stream) =
     ccall((:circatt_sliding_bwd, libcircatt), Cint,
           (Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Cfloat, Ptr{Cvoid},
            Int64, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Int32},
-           Ptr{Cvoid}, Ptr{Cfloat}, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid},
+           Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cfloat}, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid},
            Ptr{Cvoid}, Ptr{Cvoid}, Int64, Ptr{Cvoid}),
           dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, q_batch, k,
-          k_row, k_batch, v, v_row, v_batch, lengths, y, lse, dy, dy_row, dy_batch, dq,
+          k_row, k_batch, v, v_row, v_batch, lengths, y, y_rest, lse, dy, dy_row, dy_batch, dq,
           dk, dv, workspace, workspace_bytes, stream)
 
 circatt_paged_workspace_bytes(dtype, T, B, nheads, kv_heads, dh, window, sinks, page_size,

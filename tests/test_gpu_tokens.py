@@ -752,3 +752,25 @@ def test_refusals_on_device_tensors(ca):
     for kind, text, call in cases:
         with pytest.raises(kind, match=text):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("W,sharp", [(2, 1.0), (512, 4.0), (512, 8.0)])
+def test_query_gradient_of_few_effective_keys(ca, dtype, W, sharp):
+    """dq where few keys carry a row (a short window, or a softmax with sharp
+    peaks) and the score gradients cancel most.  Three roundings of at most u =
+    eps/2 enter, of dS, of P by way of y, and of the result, with mean squares of
+    at most u^2/3 each (uniform in a step): together ||error|| <= u ||dq||.  A d =
+    <dy, y> of the rounded y exceeds it: 1.3 u at the sharpest."""
+    B, n, D = 1, 512, 64
+    q, k, v, g = (randn(731 + i, B, n, D, dtype=dtype) * (sharp if i == 0 else 1) for i in range(4))
+    x = [t.cuda().requires_grad_() for t in (q, k, v)]
+    y = ca.sliding_mh_attention(*x, W, 1)
+    (dq,) = torch.autograd.grad(y, x[:1], g.cuda())
+    q, k, v, g = (t[0].double() for t in (q, k, v, g))
+    i, j = torch.arange(n)[:, None], torch.arange(n)[None]
+    p = (q @ k.T * D ** -0.5).masked_fill((j > i) | (j <= i - W), -math.inf).softmax(-1)
+    dp = g @ v.T
+    want = p * (dp - (p * dp).sum(-1, keepdim=True)) @ k * D ** -0.5
+    u = torch.finfo(dtype).eps / 2
+    assert (dq[0].cpu().double() - want).norm() <= u * want.norm(), (dq[0].cpu().double() - want).norm() / want.norm() / u

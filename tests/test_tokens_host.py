@@ -24,9 +24,9 @@ def expect(L, rc, code, fragment):
 
 
 def fwd(L, dtype=3, n=64, B=2, H=4, Hk=2, dh=64, W=16, S=0, scale=0.125, q=P, q_row=256, q_batch=0, k=P, k_row=128,
-        k_batch=0, v=P, v_row=128, v_batch=0, lengths=None, y=P, lse=None):
+        k_batch=0, v=P, v_row=128, v_batch=0, lengths=None, y=P, rest=None, lse=None):
     return L.lib.circatt_sliding_fwd(dtype, n, B, H, Hk, dh, W, S, scale, q, q_row, q_batch, k, k_row, k_batch, v, v_row,
-                                     v_batch, lengths, y, lse, None)
+                                     v_batch, lengths, y, rest, lse, None)
 
 
 @pytest.mark.parametrize("args,code,fragment", [
@@ -49,8 +49,8 @@ def test_sliding_nothing_to_do(L):
     assert fwd(L, B=0, q=None) == 0
 
 
-def bwd(L, work=P, wbytes=1 << 40, dk=P, dv=P, lse=P, dy=P, dy_row=256, dq=P):
-    return L.lib.circatt_sliding_bwd(3, 64, 2, 4, 2, 64, 16, 0, 0.125, P, 256, 0, P, 128, 0, P, 128, 0, None, P, lse, dy,
+def bwd(L, work=P, wbytes=1 << 40, dk=P, dv=P, lse=P, dy=P, dy_row=256, dq=P, rest=None):
+    return L.lib.circatt_sliding_bwd(3, 64, 2, 4, 2, 64, 16, 0, 0.125, P, 256, 0, P, 128, 0, P, 128, 0, None, P, rest, lse, dy,
                                      dy_row, 0, dq, dk, dv, work, wbytes, None)
 
 
@@ -173,3 +173,23 @@ def test_the_restatement_gives_softmax_attention_and_its_gradients():
     got = M.sliding(*(t.detach() for t in (q, k, v)), W, H, Hk, S, 0.3, None, torch.float32, dy)
     for (x, bound), w in zip(got, want):
         assert torch.allclose(x, w, rtol=1e-10, atol=1e-12) and (bound >= 0).all()
+
+
+@pytest.mark.parametrize("args,fragment", [
+    (dict(rest=ODD), "16-byte"), (dict(rest=P), "must not overlap y"), (dict(dtype=0, rest=P), "16-bit types"),
+])
+def test_rounding_rest_refusals(L, args, fragment):
+    expect(L, fwd(L, **args), -1, fragment)
+    if "dtype" not in args:
+        expect(L, bwd(L, **args), -1, fragment)
+
+
+@pytest.mark.parametrize("at", [
+    dict(q=0x10000), dict(q=0x10000 + 4 * 512 - 16), dict(q=0x10000 - 3 * 512 - 512 + 16),
+    dict(ck=0x10000 - 32), dict(cv=0x10000 - 40944),
+])
+def test_paged_result_over_its_inputs(L, at):
+    """y is 4 rows of 512 bytes at 0x10000, q the same, a cache 10 pages of 4096 (40960 bytes)."""
+    far = dict(q=0x100000, ck=0x200000, cv=0x300000)
+    args = {n: ctypes.c_void_p(a) for n, a in {**far, **at}.items()}
+    expect(L, paged(L, y=P, **args), -1, "must not overlap")
