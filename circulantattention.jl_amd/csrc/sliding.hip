@@ -31,7 +31,8 @@ __device__ __forceinline__ int signal_length(const SlidingProblem &pr, int b) {
 // (both: 53).  Two rounds in one run (the next tile's scores among this one's exponentials)
 // take 166 us where one after another took 175; explicit orders of the run's
 // instructions, wavefront priorities, operands read earlier and tiles of 32 keys
-// in five places changed nothing or lost (177 us).
+// in five places changed nothing or lost (177 us).  For training it also stores what
+// y's rounding took: 2 x 4096 tokens, 16 heads of 128, 63 us without, 73 with.
 //
 // Backward, queries: the same blocks with tiles in two buffers.
 template <typename T, int DP>
@@ -210,7 +211,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
 // its rounding took (y_rest): where few keys carry a row, the score gradients
 // cancel most, and with the rounded y alone the error of dq was up to 3 times that
 // of a form that rounds only its results, now 1.6.  2 x 4096 tokens, 16 heads of 128
-// over 4, window 512, bf16: 80 us, 610 TFLOP/s of the pairs that are seen.
+// over 4, window 512, bf16: 88 us, 550 TFLOP/s of the pairs that are seen.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void sliding_dq(SlidingProblem pr, int blocks) {
     typedef DqShape<T, DP> Sh;
