@@ -202,9 +202,9 @@ circatt_paged_attention(dtype, T, B, nheads, kv_heads, dh, window, sinks, scale,
           cache_v, npages, page_size, page_stride, row_stride, pages, pages_row,
           max_pages, lengths, offsets, y, zero_tail, workspace, workspace_bytes, stream)
 
-circatt_paged_append(dtype, T, B, channels, k, k_row, v, v_row, cache_k, cache_v, npages, page_size,
-                     page_stride, row_stride, pages, pages_row, max_pages, lengths, offsets, stream)
-                     =
+circatt_paged_append(dtype, T, B, channels, k, k_row, v, v_row, cache_k, cache_v, npages,
+                     page_size, page_stride, row_stride, pages, pages_row, max_pages, lengths,
+                     offsets, stream) =
     ccall((:circatt_paged_append, libcircatt), Cint,
           (Cint, Int64, Int64, Int64, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Int64, Ptr{Cvoid},
            Ptr{Cvoid}, Int64, Int64, Int64, Int64, Ptr{Int32}, Int64, Int64, Ptr{Int32},
