@@ -301,6 +301,7 @@ __device__ __forceinline__ void few_rows(const PagedProblem &pr, const PagedGrid
     // join the wavefronts' sums in LDS: each one's maximum and sum, then the outputs,
     // 32 channels at a time, in the order of the wavefronts
     float m = x.m, l = x.total();
+    static_assert(NW * (64 + 16 * 64) * 4 <= Sh::LDS, "");
     __syncthreads();
     float *ml = reinterpret_cast<float *>(lds_mem), *buf = ml + NW * 64;
     if (lane < 32) {
@@ -417,6 +418,7 @@ __device__ __forceinline__ void chunk_rows(const PagedProblem &pr, const PagedGr
     float m = x.m, l = x.total();
     if (NG == 2) {
         // the second group's sums through LDS
+        static_assert(NG == 1 || 4 * (16 * OT + 2) * 64 * 4 <= Sh::LDS, "");
         CIRCATT_LDS float *buf = (CIRCATT_LDS float *)lds_mem + wave * (16 * OT + 2) * 64;
         __syncthreads();
         if (group == 1) {

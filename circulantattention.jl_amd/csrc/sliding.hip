@@ -674,19 +674,26 @@ void sliding_dkdv(SlidingProblem pr, WalkSplit sp) {
     const int lane_e = lane_again(), j_e = j0 + (lane_e & 31);
     CIRCATT_LDS float *buf = (CIRCATT_LDS float *)lds_mem;
     if (NG == 2) {
+        static_assert(NG == 1 || 4 * 4 * Sh::FAR_PART <= (int)sizeof(lds_mem), "four wavefronts' sums");
         __syncthreads();
         if (group == 1) x.put(buf + wave * 64 * DP, lane_e);
         __syncthreads();
         if (group == 0) x.take(buf + wave * 64 * DP, lane_e);
     }
     if (sp.parts == 1 && kb * 4 < sp.far) {
-        // the far sums of the block's keys, by everybody
+        // the far sums of the block's keys, by everybody, as many groups of 32 keys at a
+        // time as the tiles' memory holds: all four, but two of Float32 heads wider than 32
+        constexpr int FIT = (int)sizeof(lds_mem) / (4 * Sh::FAR_PART), AT_ONCE = FIT < 4 ? FIT : 4;
+        static_assert(FIT >= 1, "");
         const int groups = sp.far - kb * 4 < 4 ? sp.far - kb * 4 : 4;
-        __syncthreads();
-        sum_far<T, DP, 256 * NG>(pr.work + sp.far_at + (unit * sp.far + kb * 4) * sp.far_parts * Sh::FAR_PART, groups,
-                                 sp.far_parts, buf);
-        __syncthreads();
-        if (group == 0 && wave < groups) x.take(buf + wave * 64 * DP, lane_e);
+        const float *from = pr.work + sp.far_at + (unit * sp.far + kb * 4) * sp.far_parts * Sh::FAR_PART;
+        for (int g = 0; g < groups; g += AT_ONCE) {
+            const int now = groups - g < AT_ONCE ? groups - g : AT_ONCE;
+            __syncthreads();
+            sum_far<T, DP, 256 * NG>(from + (int64_t)g * sp.far_parts * Sh::FAR_PART, now, sp.far_parts, buf);
+            __syncthreads();
+            if (group == 0 && wave >= g && wave < g + now) x.take(buf + (wave - g) * 64 * DP, lane_e);
+        }
     }
     if (group == 1) return;
     if (sp.parts > 1) {
