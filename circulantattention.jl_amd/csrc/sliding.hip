@@ -736,7 +736,15 @@ __global__ __launch_bounds__(256) void sliding_dkdv_join(SlidingProblem pr, Walk
     for (int x = threadIdx.x >> 6; x < 32; x += 4) {
         const int j = group * 32 + x;
         if (j >= pr.L) return;
+        const int64_t out = ((int64_t)hg.b * pr.L + j) * pr.Hk * pr.D + (int64_t)hg.hk * pr.D;
         Pair k{0.f, 0.f}, v{0.f, 0.f};
+        if (j >= hg.n) {
+            // behind the signal's length: zeros, though a row that is not finite makes
+            // its zero weights' sums NaN
+            store_row(static_cast<T *>(pr.dk) + out, lane, pr.D, k);
+            store_row(static_cast<T *>(pr.dv) + out, lane, pr.D, v);
+            continue;
+        }
         if (group < sp.far) {
             // channel d of the key, as a wavefront's registers hold it
             auto place = [&](int d) { return (16 * (d >> 5) + 4 * ((d >> 3) & 3) + (d & 3)) * 64 + x + 8 * (d & 4); };
@@ -751,13 +759,12 @@ __global__ __launch_bounds__(256) void sliding_dkdv_join(SlidingProblem pr, Walk
             v.a += c.a;
             v.b += c.b;
         }
-        const int64_t out = ((int64_t)hg.b * pr.L + j) * pr.Hk * pr.D + (int64_t)hg.hk * pr.D;
         k.a *= pr.scale;
         k.b *= pr.scale;
         store_row(static_cast<T *>(pr.dk) + out, lane, pr.D, k);
         store_row(static_cast<T *>(pr.dv) + out, lane, pr.D, v);
         // as in sliding_dkdv
-        if (__any(!(fabsf(k.a) + fabsf(k.b) + fabsf(v.a) + fabsf(v.b) < INFINITY)) && j < hg.n) {
+        if (__any(!(fabsf(k.a) + fabsf(k.b) + fabsf(v.a) + fabsf(v.b) < INFINITY))) {
             const Pair key = load_row(hg.k + j * pr.k_row, lane, pr.D);
             if (!__any(key.a != key.a || key.b != key.b)) hg.again(pr, j);
         }

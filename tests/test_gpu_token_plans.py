@@ -51,3 +51,25 @@ def test_far_sinks_without_a_join(ca, shape, dtype):
     want = M.sliding(*(t.double() for t in (q, k, v)), W, H, Hk, S, 1 / math.sqrt(D), None, dt, dy.double())
     for got, (x, bx), name in zip((y, *grads), want, ("y", "dq", "dk", "dv")):
         M.check(got, x, bx, name)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+@pytest.mark.parametrize("shape", [(2, 200, 4, 2, 64, 30, 3), (8, 512, 8, 8, 64, 64, 40)], ids=str)
+def test_padding_gets_no_gradient_from_a_bad_row(ca, shape, value, dtype):
+    """A row of q, dy, k or v that is not finite, in the last token of a signal:
+    gradients behind the signal's length are zeros all the same."""
+    B, L, H, Hk, D, W, S = shape
+    dt = DT[dtype]
+    assert (walk_split(*shape, dt)[0] == 1) == (B == 8)
+    lens = torch.tensor([L - 37 - b for b in range(B)], dtype=torch.int32)
+    base = [randn(17 + i, B, L, h * D, dtype=dt) for i, h in enumerate((H, Hk, Hk, H))]
+    for which in range(4):
+        t = [x.clone() for x in base]
+        for b in range(B):
+            t[which][b, int(lens[b]) - 1, ::3] = value
+        leaves = [x.cuda().requires_grad_(True) for x in t[:3]]
+        y = ca.sliding_mh_attention(*leaves, W, H, kv_heads=Hk, sinks=S, lengths=lens.cuda())
+        for x in (y, *torch.autograd.grad(y, leaves, t[3].cuda())):
+            for b in range(B):
+                assert (x[b, int(lens[b]):] == 0).all(), which
