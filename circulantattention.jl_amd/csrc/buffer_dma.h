@@ -18,9 +18,13 @@ __device__ __forceinline__ i4v dma_rsrc(const float *p, int bytes) {
 }
 // 16-byte LDS-DMA load: each active lane's four floats from byte voff + soff of
 // the buffer to LDS byte m0 + 16 lane.  The caller waits (vmcnt(0) and a
-// barrier).
+// barrier).  A scalar that a vector instruction has written must not be read by a
+// load for five states, and the compiler, which puts waits there for its own loads,
+// knows of none in here: where it restores a spilled descriptor (v_readlane) right
+// before, only the s_nop keeps the load off another's memory.
+#define CIRCATT_SCALARS_READY "s_nop 4\n\t"
 __device__ __forceinline__ void dma16(i4v rs, unsigned m0, int voff, int soff) {
-    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+    asm volatile(CIRCATT_SCALARS_READY "buffer_load_dwordx4 %0, %1, %2 offen lds"
                  :
                  : "v"(voff), "s"(rs), "s"(soff), "{m0}"(m0)
                  : "memory");

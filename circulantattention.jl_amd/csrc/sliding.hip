@@ -403,7 +403,10 @@ __device__ __forceinline__ void fetch_stats(const float *p, int r0, int rows, un
     const dma::i4v rs = dma::dma_rsrc(p + r0, rows > r0 ? (rows - r0 < COUNT ? rows - r0 : COUNT) * 4 : 0);
     const int lane = threadIdx.x & 63;
     if (lane < COUNT)
-        asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" : : "v"(lane * 4), "s"(rs), "{m0}"(to) : "memory");
+        asm volatile(CIRCATT_SCALARS_READY "buffer_load_dword %0, %1, 0 offen lds"
+                     :
+                     : "v"(lane * 4), "s"(rs), "{m0}"(to)
+                     : "memory");
 }
 
 // One wavefront's 32 keys: operands, sums, and 32 query rows' share of them.
