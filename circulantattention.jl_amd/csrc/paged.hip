@@ -205,9 +205,17 @@ __device__ __forceinline__ void zero_rows(const PagedProblem &pr, int blocks) {
         static_cast<u4 *>(pr.y)[i] = u4{};
 }
 
+// Whether one of the values that a block's tiles hold but hide from one of its rows,
+// before its window or behind it, is not finite.
+template <typename T>
+__device__ __forceinline__ bool hidden_values(const PagedProblem &pr, const PagedKV<T> &kv, const RowSight &rs) {
+    const int low = rs.blo - pr.W + 1;
+    return bad_values(kv, low > 0 ? low : 0, rs.bhi - pr.W + 1, pr.D) || bad_values(kv, rs.blo + 1, rs.bhi + 1, pr.D);
+}
+
 // A wavefront's 32 rows (lane: row r of the block's sequence): their outputs, or
-// their partial sums.  Outputs that a value which is not finite reached are formed
-// again from the keys that the row sees alone.
+// their partial sums.  Outputs that are not finite are formed again from the keys that
+// the row sees alone, if a value that is not finite lies where they do not see it.
 template <typename T, int DP, int R>
 __device__ __forceinline__ void finish_rows(const PagedProblem &pr, const PagedGrid &gr, int id, const Block &w,
                                             const RowSight &rs, int r, int lane, const f16v (&o)[DP / 32], float m, float l) {
@@ -222,11 +230,15 @@ __device__ __forceinline__ void finish_rows(const PagedProblem &pr, const PagedG
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T *y = static_cast<T *>(pr.y) + w.q0 * pr.H * pr.D + head * pr.G;
     const bool bad = r < w.rows && store_channels(o, y + ((int64_t)rs.tok * pr.H + rs.g) * pr.D, pr.D, lane, inv);
-    uint64_t again = __ballot(bad && l == l);  // NaN weights: the row is NaN, whatever it sees
-    again = (again | again >> 32) & 0xffffffffu;
+    const uint32_t empty = rows_of(__ballot(bad && l == 0.f));
+    uint32_t again = rows_of(__ballot(bad && l == l));  // NaN weights: the row is NaN, whatever it sees
     const PagedKV<T> kv = paged_rows_of<T>(pr, w.b, head);
+    if (again != 0) {
+        __threadfence_block();  // other lanes' stores
+        if (again != empty && !hidden_values(pr, kv, rs)) again = empty;
+    }
     for (; again; again &= again - 1) {
-        const int j = __builtin_ctzll(again);
+        const int j = __builtin_ctz(again);
         const int tj = __builtin_amdgcn_readlane(rs.tok, j), gj = __builtin_amdgcn_readlane(rs.g, j);
         forward_row(static_cast<const T *>(pr.q) + (w.q0 + tj) * pr.q_row + (head * pr.G + (int64_t)gj * pr.D),
                     y + ((int64_t)tj * pr.H + gj) * pr.D, (T *)nullptr, kv, __builtin_amdgcn_readlane(rs.at, j), pr.W, pr.S,
@@ -475,6 +487,7 @@ __global__ __launch_bounds__(256) void paged_join(PagedProblem pr, PagedGrid gr)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hk = blockIdx.y, d = 4 * (lane & 31);
     const int64_t slot = ((int64_t)blockIdx.x * pr.Hk + hk) * gr.splits * R, head = (int64_t)hk * pr.D;
     const int rows = w.rows - w.r0 < R ? w.rows - w.r0 : R;
+    int hidden = -1;  // hidden_values of the block, once asked for
     for (int i0 = 2 * wave; i0 < rows; i0 += 8) {
         const int i = i0 + (lane >> 5), ii = i < rows ? i : rows - 1;
         float m = -INFINITY, l = 0.f;
@@ -499,7 +512,15 @@ __global__ __launch_bounds__(256) void paged_join(PagedProblem pr, PagedGrid gr)
             bad |= !(fabsf(o[e] * inv) < INFINITY);
         }
         if (i < rows && d < pr.D) *reinterpret_cast<V4<T> *>(y + d) = v;
-        const uint64_t again = __ballot(bad && l == l && i < rows && d < pr.D);
+        const bool in = i < rows && d < pr.D;
+        const uint64_t empty = __ballot(bad && l == 0.f && in);
+        uint64_t again = __ballot(bad && l == l && in);
+        const PagedKV<T> kv = paged_rows_of<T>(pr, w.b, head);
+        if (again != 0) {
+            __threadfence_block();  // other lanes' stores
+            if (again != empty && hidden < 0) hidden = hidden_values(pr, kv, RowSight::of<R>(pr, w, w.r0));
+            if (!hidden) again = empty;
+        }
         for (int h = 0; h < 2; ++h) {
             if (!(uint32_t)(again >> (32 * h))) continue;
             const int rj = w.r0 + i0 + h, tj = rj / pr.G, gj = rj - tj * pr.G;
@@ -507,7 +528,7 @@ __global__ __launch_bounds__(256) void paged_join(PagedProblem pr, PagedGrid gr)
             const int pos = w.first + tj;
             forward_row(static_cast<const T *>(pr.q) + (w.q0 + tj) * pr.q_row + (head * pr.G + (int64_t)gj * pr.D),
                         static_cast<T *>(pr.y) + (w.q0 + tj) * pr.H * pr.D + head * pr.G + (int64_t)gj * pr.D, (T *)nullptr,
-                        paged_rows_of<T>(pr, w.b, head), pos >= held ? -1 : pos, pr.W, pr.S, pr.D, pr.scale * kLog2e);
+                        kv, pos >= held ? -1 : pos, pr.W, pr.S, pr.D, pr.scale * kLog2e);
         }
     }
 }

@@ -84,8 +84,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int rows = n * pr.G, r0 = w.block * 128, all_rows = pr.L * pr.G;
     const int r = r0 + 32 * wave + (lane & 31);
-    T *y = static_cast<T *>(pr.y) + (int64_t)b * pr.L * pr.H * pr.D + (int64_t)hk * pr.G * pr.D;
-    T *rest = pr.y_rest == nullptr ? nullptr : static_cast<T *>(pr.y_rest) + (y - static_cast<T *>(pr.y));
     const int64_t stat = ((int64_t)b * pr.Hk + hk) * all_rows;
     // the wavefront's rows, those past the end doubling the last one
     const int rr = r < rows ? r : rows - 1, at = rows > 0 ? rr / pr.G : -1, g = rows > 0 ? rr - at * pr.G : 0;
@@ -143,60 +141,75 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             next();
             look(t, i + 1);
         };
-        f16v a[NB], b[NB];
+        f16v sa[NB], sb[NB];
         int i = -1;
         for (; i < (live ? first - 1 : count); ++i, next()) round(i);
         if (live) {
             round(i);
-            x.scores(row_at + kp * Rg::TILE, a);
-            look(a, first);
+            x.scores(row_at + kp * Rg::TILE, sa);
+            look(sa, first);
             next();
             ++i;
             for (; i + 1 < end; i += 2) {
-                step(a, b, i);
-                step(b, a, i + 1);
+                step(sa, sb, i);
+                step(sb, sa, i + 1);
             }
             if (i < end) {
-                step(a, b, i);
+                step(sa, sb, i);
 #pragma unroll
-                for (int m = 0; m < NB; ++m) a[m] = b[m];
+                for (int m = 0; m < NB; ++m) sa[m] = sb[m];
                 ++i;
             }
             round(i);
             V8<T> p[2 * NB];
             x.raise(mx);
-            x.weigh(a, p, c);
+            x.weigh(sa, p, c);
             x.template add<NB>(col_at + vp * Rg::TILE, p);
             next();
             for (++i; i < count; ++i, next()) round(i);
         }
+        const SlidingProblem pe = argument_again<SlidingProblem>();
+        const int64_t ky = (int64_t)hk * pe.D, qy = ky * pe.G, yb = (int64_t)b * pe.L * pe.H * pe.D + qy;
+        const SignalKV<T> kv{static_cast<const T *>(pe.k) + b * pe.k_batch + ky,
+                             static_cast<const T *>(pe.v) + b * pe.v_batch + ky, pe.k_row, pe.v_row};
+        T *y = static_cast<T *>(pe.y) + yb, *rest = pe.y_rest == nullptr ? nullptr : static_cast<T *>(pe.y_rest) + yb;
+        uint32_t again = 0;
         if (live) {
             const float l = x.total(), inv = l == 0.f ? 0.f : 1.f / l;
             bool bad = false;
             if (r < rows) {
-                bad = store_channels(x.o, y + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv);
-                if (rest != nullptr) store_rests(x.o, rest + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv);
-                if (pr.lse != nullptr && lane < 32)
-                    pr.lse[stat + r] = l == 0.f ? INFINITY : x.m + __builtin_amdgcn_logf(l);
+                bad = store_channels(x.o, y + ((int64_t)at * pe.H + g) * pe.D, pe.D, lane, inv);
+                if (rest != nullptr) store_rests(x.o, rest + ((int64_t)at * pe.H + g) * pe.D, pe.D, lane, inv);
+                if (pe.lse != nullptr && lane < 32)
+                    pe.lse[stat + r] = l == 0.f ? INFINITY : x.m + __builtin_amdgcn_logf(l);
             }
             // A value that is not finite reaches, as 0 times itself, every row of
-            // a wavefront whose tile holds it: such rows are formed again from
-            // the keys that they see alone.  (Not where the sum of the weights is
-            // NaN: then the row is, whatever it sees.)
-            uint64_t again = __ballot(bad && l == l);
-            again = (again | again >> 32) & 0xffffffffu;
-            const SignalKV<T> kv{kh, vh, pr.k_row, pr.v_row};
-            for (; again; again &= again - 1) {
-                const int j = __builtin_ctzll(again);
-                const int aj = __builtin_amdgcn_readlane(at, j), gj = __builtin_amdgcn_readlane(g, j);
-                const int64_t out = ((int64_t)aj * pr.H + gj) * pr.D;
-                forward_row(qh + aj * pr.q_row + (int64_t)gj * pr.D, y + out, rest == nullptr ? rest : rest + out, kv, aj, pr.W, pr.S, pr.D, c);
+            // a wavefront whose tile holds it: where such a value is among the keys
+            // that the tiles hide from some row (before the rows' windows, behind the
+            // first row, and behind the sinks), rows that are not finite are formed
+            // again from the keys that they see alone.  (Not where the sum of the
+            // weights is NaN: then the row is, whatever it sees.)
+            again = rows_of(__ballot(bad && l == l));
+            if (again != 0) {
+                auto tile_end = [&](int j) { return (int)((int64_t)j + KT - j % KT < n ? j + KT - j % KT : n); };
+                const int window = r0 / pe.G - pe.W + 1;
+                if (!bad_values(kv, window > 0 ? window / KT * KT : 0, hi - pe.W + 1, pe.D) &&
+                    !bad_values(kv, lo + 1, tile_end(hi), pe.D) &&
+                    !(pe.S % KT != 0 && bad_values(kv, pe.S, tile_end(pe.S), pe.D)))
+                    again = 0;
             }
         }
+        share_repairs<4>((CIRCATT_LDS uint32_t *)lds, wave, wave, again, 0, [&](int i, bool, bool) {
+            const int aj = (r0 + i) / pe.G, gj = r0 + i - aj * pe.G;
+            const int64_t out = ((int64_t)aj * pe.H + gj) * pe.D;
+            forward_row(static_cast<const T *>(pe.q) + b * pe.q_batch + qy + aj * pe.q_row + (int64_t)gj * pe.D, y + out,
+                        rest == nullptr ? rest : rest + out, kv, aj, pe.W, pe.S, pe.D, pe.scale * kLog2e);
+        });
     }
     // rows behind the signal's length
     if (r >= rows && r < all_rows) {
         const int t = r / pr.G, gt = r - t * pr.G;
+        T *y = static_cast<T *>(pr.y) + (int64_t)b * pr.L * pr.H * pr.D + (int64_t)hk * pr.G * pr.D;
         zero_channels(y + ((int64_t)t * pr.H + gt) * pr.D, pr.D, lane);
         if (pr.lse != nullptr && lane < 32) pr.lse[stat + r] = INFINITY;
     }
@@ -308,17 +321,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
         rest += other_half(rest);
         if (r < rows && lane < 32) pr.work[stat + r] = d + rest;
         if (live) {
-            // formed again as in the forward; a row whose statistics are NaN is NaN
+            // formed again as in the forward, and where Float16 could not hold a score
+            // gradient; a row whose statistics are not finite is not, whatever it sees
             const bool bad = r < rows && store_channels(o, dq + out, pr.D, lane, pr.scale);
-            uint64_t again = __ballot(bad && lse == lse && d == d);
-            again = (again | again >> 32) & 0xffffffffu;
+            uint32_t again = rows_of(__ballot(bad && is_finite(lse) && is_finite(d)));
             const SignalKV<T> kv{kh, vh, pr.k_row, pr.v_row};
+            if (again != 0) __threadfence_block();  // other lanes' stores
             for (; again; again &= again - 1) {
-                const int j = __builtin_ctzll(again);
+                const int j = __builtin_ctz(again);
                 const int aj = __builtin_amdgcn_readlane(at, j), gj = __builtin_amdgcn_readlane(g, j);
                 const int64_t oj = ((int64_t)aj * pr.H + gj) * pr.D, sj = stat + (int64_t)aj * pr.G + gj;
-                dq_row(qh + aj * pr.q_row + (int64_t)gj * pr.D, yh + oj, eh == nullptr ? eh : eh + oj, gh + aj * pr.dy_row + (int64_t)gj * pr.D, dq + oj,
-                       pr.lse[sj], pr.work + sj, kv, aj, pr.W, pr.S, pr.D, c, pr.scale);
+                dq_row(qh + aj * pr.q_row + (int64_t)gj * pr.D, yh + oj, eh == nullptr ? eh : eh + oj,
+                       gh + aj * pr.dy_row + (int64_t)gj * pr.D, dq + oj, pr.lse[sj], pr.work + sj, kv, aj, pr.W, pr.S, pr.D,
+                       c, pr.scale);
             }
         }
     }
@@ -513,10 +528,12 @@ struct HeadGroup {
     int b, hk, n, rows;
     const T *k, *v, *q, *dy;
     const float *lse, *dsum;
-    __device__ HeadGroup(const SlidingProblem &pr, int64_t unit) {
+    __device__ HeadGroup(const SlidingProblem &pr, int64_t unit)
+        : HeadGroup(pr, unit, uniform(signal_length(pr, (int)(unit / pr.Hk)))) {}
+    __device__ HeadGroup(const SlidingProblem &pr, int64_t unit, int length) {
         b = (int)(unit / pr.Hk);
         hk = (int)(unit - (int64_t)b * pr.Hk);
-        n = uniform(signal_length(pr, b));
+        n = length;
         rows = n * pr.G;
         const int64_t head = (int64_t)hk * pr.D;
         k = static_cast<const T *>(pr.k) + b * pr.k_batch + head;
@@ -527,11 +544,30 @@ struct HeadGroup {
         lse = pr.lse + stat;
         dsum = pr.work + stat;
     }
-    // dk, dv of key j from its rows alone
-    __device__ void again(const SlidingProblem &pr, int j) const {
+    // whether the statistics of one of the packed rows [r0, r1) are not finite
+    __device__ bool bad_rows(int r0, int r1) const {
+        bool bad = false;
+#pragma unroll 4
+        for (int r = r0 + lane_again(); r < r1; r += 64) bad |= !is_finite(lse[r]) || !is_finite(dsum[r]);
+        return __any(bad);
+    }
+    // The gradients of key j, one of the 32 from j0 on, of which dk (bad_k) or dv
+    // (bad_v) are not finite.  A row whose statistics are not finite makes all of
+    // dk that of every key that it sees, and a row of dy that is not finite has such
+    // statistics.  So dk is formed again if no row that sees the key is one, and
+    // dv if a row that the products hid from the key is one: zero times its dy is
+    // NaN.  Those lie before the key, behind its window in the last block of 32 rows,
+    // and, of a group with the last sinks, anywhere behind.
+    __device__ void again(const SlidingProblem &pr, int j, int j0, bool bad_k, bool bad_v) const {
+        const int end = j < pr.S || n - j < pr.W ? n : j + pr.W;
+        const int64_t last = (int64_t)j0 + 31 + pr.W + (30 + pr.G) / pr.G;
+        const bool fix_k = bad_k && !bad_rows(j * pr.G, end * pr.G);
+        const bool fix_v = bad_v && (bad_rows(j0 * pr.G, j * pr.G) ||
+                                     bad_rows(end * pr.G, (j0 < pr.S || last > n ? n : (int)last) * pr.G));
+        if (!fix_k && !fix_v) return;
         const int64_t out = ((int64_t)b * pr.L + j) * pr.Hk * pr.D + (int64_t)hk * pr.D;
         dkdv_row(k + j * pr.k_row, v + j * pr.v_row, q, pr.q_row, dy, pr.dy_row, lse, dsum, static_cast<T *>(pr.dk) + out,
-                 static_cast<T *>(pr.dv) + out, j, n, pr.W, pr.S, pr.G, pr.D, pr.scale * kLog2e, pr.scale);
+                 static_cast<T *>(pr.dv) + out, fix_k, fix_v, j, n, pr.W, pr.S, pr.G, pr.D, pr.scale * kLog2e, pr.scale);
     }
 };
 
@@ -698,27 +734,30 @@ void sliding_dkdv(SlidingProblem pr, WalkSplit sp) {
             if (group == 0 && wave >= g && wave < g + now) x.take(buf + (wave - g) * 64 * DP, lane_e);
         }
     }
-    if (group == 1) return;
     if (sp.parts > 1) {
-        x.write(pr.work + sp.part_at + (unit * sp.blocks * sp.parts + in) * Sh::PART + (32 * wave + (lane_e & 31)) * DP,
-                128 * DP, lane_e);
+        if (group == 0)
+            x.write(pr.work + sp.part_at + (unit * sp.blocks * sp.parts + in) * Sh::PART + (32 * wave + (lane_e & 31)) * DP,
+                    128 * DP, lane_e);
         return;
     }
-    const int64_t out = ((int64_t)hg.b * pr.L + j_e) * pr.Hk * pr.D + (int64_t)hg.hk * pr.D;
-    T *kd = static_cast<T *>(pr.dk) + out, *vd = static_cast<T *>(pr.dv) + out;
-    bool bad = false;
-    if (j_e < n) {
-        bad = store_channels(x.dk, kd, pr.D, lane_e, pr.scale);
-        bad |= store_channels(x.dv, vd, pr.D, lane_e, 1.f);
-    } else if (j_e < pr.L) {
-        zero_channels(kd, pr.D, lane_e);
-        zero_channels(vd, pr.D, lane_e);
+    const SlidingProblem pe = argument_again<SlidingProblem>();
+    const HeadGroup<T> he(pe, unit, n);
+    bool bad_k = false, bad_v = false;
+    if (group == 0) {
+        const int64_t out = ((int64_t)he.b * pe.L + j_e) * pe.Hk * pe.D + (int64_t)he.hk * pe.D;
+        T *kd = static_cast<T *>(pe.dk) + out, *vd = static_cast<T *>(pe.dv) + out;
+        if (j_e < he.n) {
+            bad_k = store_channels(x.dk, kd, pe.D, lane_e, pe.scale);
+            bad_v = store_channels(x.dv, vd, pe.D, lane_e, 1.f);
+        } else if (j_e < pe.L) {
+            zero_channels(kd, pe.D, lane_e);
+            zero_channels(vd, pe.D, lane_e);
+        }
     }
-    // formed again as in the forward; a key that holds NaN has NaN gradients
-    if (bad) bad = !any_nan(hg.k + j_e * pr.k_row, pr.D);
-    uint64_t again = __ballot(bad);
-    again = (again | again >> 32) & 0xffffffffu;
-    for (; again; again &= again - 1) hg.again(pr, j0 + __builtin_ctzll(again));
+    share_repairs<4 * NG>((CIRCATT_LDS uint32_t *)lds_mem, group == 0 ? wave : -1, 4 * group + wave,
+                          rows_of(__ballot(bad_k)), rows_of(__ballot(bad_v)), [&](int i, bool fix_k, bool fix_v) {
+                              he.again(pe, k0 + i, k0 + (i & ~31), fix_k, fix_v);
+                          });
 }
 
 // The partial sums of 32 keys, the far ones first, in the order of their parts: a
@@ -766,10 +805,10 @@ __global__ __launch_bounds__(256) void sliding_dkdv_join(SlidingProblem pr, Walk
         k.b *= pr.scale;
         store_row(static_cast<T *>(pr.dk) + out, lane, pr.D, k);
         store_row(static_cast<T *>(pr.dv) + out, lane, pr.D, v);
-        // as in sliding_dkdv
-        if (__any(!(fabsf(k.a) + fabsf(k.b) + fabsf(v.a) + fabsf(v.b) < INFINITY))) {
-            const Pair key = load_row(hg.k + j * pr.k_row, lane, pr.D);
-            if (!__any(key.a != key.a || key.b != key.b)) hg.again(pr, j);
+        const bool bad_k = __any(!is_finite(k.a) || !is_finite(k.b)), bad_v = __any(!is_finite(v.a) || !is_finite(v.b));
+        if (bad_k || bad_v) {
+            __threadfence_block();  // other lanes' stores
+            hg.again(pr, j, group * 32, bad_k, bad_v);
         }
     }
 }

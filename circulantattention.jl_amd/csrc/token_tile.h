@@ -27,10 +27,7 @@ namespace circatt {
 namespace tok {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
-typedef float f4v __attribute__((ext_vector_type(4)));
 typedef short s4v __attribute__((ext_vector_type(4)));
-template <typename T>
-using V8 = T __attribute__((ext_vector_type(8)));
 template <typename T>
 using V4 = T __attribute__((ext_vector_type(4)));
 #define CIRCATT_LDS __attribute__((address_space(3)))
@@ -134,29 +131,6 @@ __device__ __forceinline__ float other_half(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x),
                                                     false, false);
     return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
-}
-
-// The lane's number formed anew, for what follows a loop whose registers are full: no
-// address that hangs on it is kept through the loop.
-__device__ __forceinline__ int lane_again() {
-    int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
-    asm volatile("" : "+v"(lane));
-    return lane;
-}
-
-// Eight channels from global memory, zero from channel D on (D a multiple of 8).
-template <typename T>
-__device__ __forceinline__ V8<T> load8(const T *p, int d, int D) {
-    V8<T> v{};
-    if (d < D) {
-        if constexpr (sizeof(T) == 2) {
-            v = *reinterpret_cast<const V8<T> *>(p + d);
-        } else {
-            const f4v a = *reinterpret_cast<const f4v *>(p + d), b = *reinterpret_cast<const f4v *>(p + d + 4);
-            v = V8<T>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-        }
-    }
-    return v;
 }
 
 // N products whose first operands are read from LDS, read(i) AHEAD products before
@@ -375,12 +349,48 @@ struct Rows {
     __device__ __forceinline__ float total() const { return l + __shfl_xor(l, 32, 64); }
 };
 
-// Whether a row holds NaN.
-template <typename T>
-__device__ __forceinline__ bool any_nan(const T *p, int D) {
-    bool nan = false;
-    for (int d = 0; d < D; ++d) nan |= (float)p[d] != (float)p[d];
-    return nan;
+// The rows of a wavefront (bits: lanes, a row's two halves) as bits 0 .. 31.
+__device__ __forceinline__ uint32_t rows_of(uint64_t bits) { return (uint32_t)(bits | bits >> 32); }
+
+// A kernel's first argument read anew, for what follows a loop: its fields hold no
+// scalar registers through the loop.
+template <typename P>
+__device__ __forceinline__ P argument_again() {
+    typedef const __attribute__((address_space(4))) uint32_t *Words;
+    Words p = (Words)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    struct {
+        uint32_t w[sizeof(P) / 4];
+    } c;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(P) / 4; ++i) c.w[i] = p[i];
+    return __builtin_bit_cast(P, c);
+}
+
+// Rows that a workgroup forms again, by all of its WAVES wavefronts in turn, as they
+// tend to lie together: `from`, which of four wavefronts with 32 rows each this one
+// is (or -1), with its rows of two kinds, a bit each; `wave`, this one's turn.
+// repair(row of the 128, first kind, second kind) is called by whole wavefronts.
+// The list is LDS that nothing is read from any more once all are here.
+template <int WAVES, typename Repair>
+__device__ __forceinline__ void share_repairs(CIRCATT_LDS uint32_t *list, int from, int wave, uint32_t one, uint32_t two,
+                                              Repair repair) {
+    if ((one | two) != 0) __threadfence_block();  // other wavefronts read the rows
+    __syncthreads();
+    if (from >= 0 && lane_again() == 0) {
+        list[from] = one;
+        list[4 + from] = two;
+    }
+    __syncthreads();
+    int turn = 0;
+#pragma unroll 1  // repair is long
+    for (int w = 0; w < 4; ++w) {
+        const uint32_t o = uniform(list[w]), t = uniform(list[4 + w]);
+        for (uint32_t left = o | t; left; left &= left - 1, turn = turn + 1 == WAVES ? 0 : turn + 1) {
+            const int i = __builtin_ctz(left);
+            if (turn == wave) repair(32 * w + i, o >> i & 1, t >> i & 1);
+        }
+    }
 }
 
 // Writes a row's channels (one lane and its other half), times f; whether one of
