@@ -213,6 +213,10 @@ __device__ __forceinline__ bool hidden_values(const PagedProblem &pr, const Page
     return bad_values(kv, low > 0 ? low : 0, rs.bhi - pr.W + 1, pr.D) || bad_values(kv, rs.blo + 1, rs.bhi + 1, pr.D);
 }
 
+// A row whose weights sum to zero is zero where it sees nothing; where all that it sees
+// has the score -inf, its softmax is NaN.
+__device__ __forceinline__ float without_weights(bool sees) { return sees ? NAN : 0.f; }
+
 // A wavefront's 32 rows (lane: row r of the block's sequence): their outputs, or
 // their partial sums.  Outputs that are not finite are formed again from the keys that
 // the row sees alone, if a value that is not finite lies where they do not see it.
@@ -230,12 +234,20 @@ __device__ __forceinline__ void finish_rows(const PagedProblem &pr, const PagedG
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T *y = static_cast<T *>(pr.y) + w.q0 * pr.H * pr.D + head * pr.G;
     const bool bad = r < w.rows && store_channels(o, y + ((int64_t)rs.tok * pr.H + rs.g) * pr.D, pr.D, lane, inv);
-    const uint32_t empty = rows_of(__ballot(bad && l == 0.f));
-    uint32_t again = rows_of(__ballot(bad && l == l));  // NaN weights: the row is NaN, whatever it sees
+    // NaN weights: the row is NaN, whatever it sees
+    uint32_t again = rows_of(__ballot(bad && l > 0.f)), empty = rows_of(__ballot(r < w.rows && l == 0.f));
     const PagedKV<T> kv = paged_rows_of<T>(pr, w.b, head);
-    if (again != 0) {
-        __threadfence_block();  // other lanes' stores
-        if (again != empty && !hidden_values(pr, kv, rs)) again = empty;
+    if ((again | empty) != 0) __threadfence_block();  // other lanes' stores
+    if (again != 0 && !hidden_values(pr, kv, rs)) again = 0;
+    int asked = -1;
+    bool sees = false;
+    for (; empty; empty &= empty - 1) {
+        const int j = __builtin_ctz(empty), at = __builtin_amdgcn_readlane(rs.at, j);
+        if (at != asked) sees = sees_any(kv, at, pr.W, pr.S);  // heads of one token lie together
+        asked = at;
+        const float v = without_weights(sees);
+        store_row(y + ((int64_t)__builtin_amdgcn_readlane(rs.tok, j) * pr.H + __builtin_amdgcn_readlane(rs.g, j)) * pr.D, lane,
+                  pr.D, Pair{v, v});
     }
     for (; again; again &= again - 1) {
         const int j = __builtin_ctz(again);
@@ -513,22 +525,28 @@ __global__ __launch_bounds__(256) void paged_join(PagedProblem pr, PagedGrid gr)
         }
         if (i < rows && d < pr.D) *reinterpret_cast<V4<T> *>(y + d) = v;
         const bool in = i < rows && d < pr.D;
-        const uint64_t empty = __ballot(bad && l == 0.f && in);
-        uint64_t again = __ballot(bad && l == l && in);
+        const uint64_t empty = __ballot(l == 0.f && in);
+        uint64_t again = __ballot(bad && l > 0.f && in);
         const PagedKV<T> kv = paged_rows_of<T>(pr, w.b, head);
+        if ((again | empty) != 0) __threadfence_block();  // other lanes' stores
         if (again != 0) {
-            __threadfence_block();  // other lanes' stores
-            if (again != empty && hidden < 0) hidden = hidden_values(pr, kv, RowSight::of<R>(pr, w, w.r0));
-            if (!hidden) again = empty;
+            if (hidden < 0) hidden = hidden_values(pr, kv, RowSight::of<R>(pr, w, w.r0));
+            if (!hidden) again = 0;
         }
         for (int h = 0; h < 2; ++h) {
-            if (!(uint32_t)(again >> (32 * h))) continue;
+            const bool form = (uint32_t)(again >> (32 * h)) != 0, none = (uint32_t)(empty >> (32 * h)) != 0;
+            if (!form && !none) continue;
             const int rj = w.r0 + i0 + h, tj = rj / pr.G, gj = rj - tj * pr.G;
             const int64_t held = (int64_t)pr.maxp << pr.page_log2;
-            const int pos = w.first + tj;
-            forward_row(static_cast<const T *>(pr.q) + (w.q0 + tj) * pr.q_row + (head * pr.G + (int64_t)gj * pr.D),
-                        static_cast<T *>(pr.y) + (w.q0 + tj) * pr.H * pr.D + head * pr.G + (int64_t)gj * pr.D, (T *)nullptr,
-                        kv, pos >= held ? -1 : pos, pr.W, pr.S, pr.D, pr.scale * kLog2e);
+            const int pos = w.first + tj, at = pos >= held ? -1 : pos;
+            T *yj = static_cast<T *>(pr.y) + (w.q0 + tj) * pr.H * pr.D + head * pr.G + (int64_t)gj * pr.D;
+            if (form) {
+                forward_row(static_cast<const T *>(pr.q) + (w.q0 + tj) * pr.q_row + (head * pr.G + (int64_t)gj * pr.D), yj,
+                            (T *)nullptr, kv, at, pr.W, pr.S, pr.D, pr.scale * kLog2e);
+            } else {
+                const float v = without_weights(sees_any(kv, at, pr.W, pr.S));
+                store_row(yj, lane, pr.D, Pair{v, v});
+            }
         }
     }
 }

@@ -175,21 +175,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
         T *y = static_cast<T *>(pe.y) + yb, *rest = pe.y_rest == nullptr ? nullptr : static_cast<T *>(pe.y_rest) + yb;
         uint32_t again = 0;
         if (live) {
-            const float l = x.total(), inv = l == 0.f ? 0.f : 1.f / l;
+            // a row sees its own token at least: without a sum of weights all that it sees
+            // has the score -inf, and its softmax is NaN
+            const float l = x.total(), inv = 1.f / l;
             bool bad = false;
             if (r < rows) {
                 bad = store_channels(x.o, y + ((int64_t)at * pe.H + g) * pe.D, pe.D, lane, inv);
                 if (rest != nullptr) store_rests(x.o, rest + ((int64_t)at * pe.H + g) * pe.D, pe.D, lane, inv);
                 if (pe.lse != nullptr && lane < 32)
-                    pe.lse[stat + r] = l == 0.f ? INFINITY : x.m + __builtin_amdgcn_logf(l);
+                    pe.lse[stat + r] = x.m + __builtin_amdgcn_logf(l);
             }
             // A value that is not finite reaches, as 0 times itself, every row of
             // a wavefront whose tile holds it: where such a value is among the keys
             // that the tiles hide from some row (before the rows' windows, behind the
             // first row, and behind the sinks), rows that are not finite are formed
             // again from the keys that they see alone.  (Not where the sum of the
-            // weights is NaN: then the row is, whatever it sees.)
-            again = rows_of(__ballot(bad && l == l));
+            // weights is NaN or 0: then the row is, whatever it sees.)
+            again = rows_of(__ballot(bad && l > 0.f));
             if (again != 0) {
                 auto tile_end = [&](int j) { return (int)((int64_t)j + KT - j % KT < n ? j + KT - j % KT : n); };
                 const int window = r0 / pe.G - pe.W + 1;

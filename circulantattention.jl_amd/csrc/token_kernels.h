@@ -20,8 +20,8 @@ struct SlidingProblem {
     const int32_t *lengths;  // (B) or NULL: all L
     void *y;                 // (B, L, H*D)
     void *y_rest;            // what y's rounding took, laid out as y, or NULL
-    // log2 of a row's sum of exp2(scale log2(e) q.k), +inf for a row that sees
-    // nothing: (B, Hk, L*G), row i*G + g
+    // log2 of a row's sum of exp2(scale log2(e) q.k), +inf for a row behind the
+    // signal's length: (B, Hk, L*G), row i*G + g
     float *lse;
     // backward
     const void *dy;

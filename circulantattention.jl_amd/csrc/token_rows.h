@@ -174,6 +174,19 @@ __device__ __forceinline__ bool bad_values(const KV &kv, int j0, int j1, int D) 
     return __any(bad);
 }
 
+// Whether a row at pos sees one of the keys that kv has.
+template <typename KV>
+__device__ __forceinline__ bool sees_any(const KV &kv, int pos, int W, int S) {
+    const int lo = pos - W + 1 > 0 ? pos - W + 1 : 0;
+    for (int j0 = 0; j0 <= pos; j0 += 64) {
+        if (j0 >= S && j0 < lo) j0 = lo;
+        const int j = j0 + lane_again();
+        typename KV::Ptr kp, vp;
+        if (__any(j <= pos && (j < S || j >= lo) && kv.row(j, kp, vp))) return true;
+    }
+    return false;
+}
+
 // y = sum_j softmax_j(c q.k_j) v_j in base 2 over [0, min(S, lo)) and [lo, pos],
 // lo = max(0, pos - W + 1).  kv.row(j): whether key j is there, and its rows.
 // rest: what y's rounding took, or NULL.
@@ -202,7 +215,7 @@ __device__ void forward_row(const T *q, T *y, T *rest, const KV &kv, int pos, in
         add_rows(o, vp, p, lane, D);
         if (!__any(lacks.open(o))) break;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = 1.f / l;
     lacks.store(y, lane, Pair{o.a * inv, o.b * inv});
     if (rest != nullptr)
         lacks.store(rest, lane, Pair{(float)rounding_rest<T>(o.a * inv), (float)rounding_rest<T>(o.b * inv)});

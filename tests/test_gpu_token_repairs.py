@@ -160,3 +160,45 @@ def test_what_single_numbers_do_not_reach_is_right(ca, shape, dtype):
     for got, (w, b), hit, name in zip((dq, dk, dv), want, (hq, hk, hv), ("dq", "dk", "dv")):
         assert torch.equal(~torch.isfinite(got), hit), name
         M.check(got[~hit], w[~hit], b[~hit], name)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("W,S", [(None, 0), (20, 3)])
+def test_scores_of_minus_infinity_alone_give_nan(ca, dtype, W, S):
+    """A row whose every visible score is -inf has no softmax: it is NaN, and so are
+    the gradients of what it sees.  Over a cache as well, where a row that sees no
+    token is zero."""
+    L, H, Hk, D, page, t = 90, 4, 2, 32, 8, 60
+    dt = DT[dtype]
+    q, k, v, dy = (randn(53 + i, 1, L, h * D, dtype=dt) for i, h in enumerate((H, Hk, Hk, H)))
+    k[..., ::D] = k[..., ::D].abs() + 1
+    good = M.sliding(*(x.double() for x in (q, k, v)), W or L, H, Hk, S, 1 / math.sqrt(D), None, dt, dy.double())
+    q[0, t] = 0
+    q[0, t, ::D] = torch.tensor([1, -math.inf, 1, 1]).to(dt)
+    leaves = [x.cuda().requires_grad_(True) for x in (q, k, v)]
+    y = ca.sliding_mh_attention(*leaves, W, H, kv_heads=Hk, sinks=S)
+    _, dk, dv = (x.cpu()[0] for x in torch.autograd.grad(y, leaves, dy.cuda()))
+    bad = torch.zeros(1, L, H * D, dtype=torch.bool)
+    bad[0, t, D:2 * D] = True
+    assert torch.equal(torch.isnan(y).cpu(), bad)
+    other = torch.ones(L, dtype=torch.bool)
+    other[t] = False
+    M.check(y[:, other], good[0][0][:, other], good[0][1][:, other], "y")
+    seen = M.visible(torch.arange(L), L, W or L, S)[t]
+    for x in (dk, dv):
+        assert torch.equal(torch.isnan(x).reshape(L, Hk, D)[..., 1:].all(-1)[:, 0], seen)
+        assert torch.isfinite(x.reshape(L, Hk, D)[:, 1]).all() and torch.isfinite(x[~seen]).all()
+    # the same tokens over a cache, where a second sequence's pages are not there and a
+    # third one has no token
+    caches = [torch.cat([x[0], torch.zeros(96 - L, Hk * D, dtype=dt)]).reshape(12, page, Hk * D).cuda() for x in (k, v)]
+    for new in (40, 1):
+        one = torch.arange(12, dtype=torch.int32)
+        pages = torch.stack([one, torch.full_like(one, -1), one]).cuda()
+        rows = q[0, t + 1 - new:t + 1]
+        lens = torch.tensor([t + 1, t + 1, 0], dtype=torch.int32).cuda()
+        offs = torch.tensor([0, new, 2 * new, 3 * new], dtype=torch.int32).cuda()
+        got = ca.paged_mh_attention(rows.repeat(3, 1).cuda(), *caches, pages, lens, W, H, kv_heads=Hk, sinks=S, offsets=offs)
+        assert (got[new:] == 0).all()
+        assert torch.equal(torch.isnan(got[:new]).cpu(), bad[0, t + 1 - new:t + 1])
+        if new > 1:
+            M.check(got[:new - 1], good[0][0][0, t + 1 - new:t], good[0][1][0, t + 1 - new:t], "paged")
