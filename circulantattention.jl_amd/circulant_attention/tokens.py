@@ -13,6 +13,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -32,6 +33,15 @@ def _call(device, fn, *args):
             rc = fn(*args, stream_ptr(device))
     if rc != L.OK:
         L.check(rc)
+
+
+def _recorded(*tensors):
+    """Whether a call goes through its autograd function: one of the tensors
+    requires gradients, or forward mode is on, which the function refuses for
+    tensors with a tangent."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any([t.requires_grad for t in tensors])
 
 
 def _require(t, name, like=None, dtypes=_CODES):
@@ -160,7 +170,7 @@ def sliding_mh_attention(q, k, v, W, nheads: int, *, kv_heads: int = None, sinks
     if lengths is not None:
         lengths = _index(lengths, "lengths", q, (q.shape[0],))
     args = (q, k, v, W, sinks, nheads, kv_heads, scale, lengths)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _recorded(q, k, v):
         return SlidingAttentionFn.apply(*args)
     return _sliding(False, *args)[0]
 
@@ -348,7 +358,7 @@ def axial_rotary(x, pairs, nheads: int, *, base: float = 10000.0, positions: tor
         shape = x.shape[:-1] if per_image or x.dim() == 2 else x.shape[1:-1]
         positions = _index(positions, "positions", x, (*shape, len(pairs)))
     meta = (grid, pairs, int(nheads), float(base), per_image, bool(interleaved))
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _recorded(x):
         return AxialRotaryFn.apply(x, positions, *meta)
     return _turn(x, 0, *meta, positions)
 
