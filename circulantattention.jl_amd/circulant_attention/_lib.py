@@ -92,6 +92,8 @@ SIGNATURES = {
                                     _i64, _p, _i64, _i64, _p, _p, _p]),
     "circatt_axial_rotary": (_int, [_int, _int, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                     _i32, _i32, _i32, _f32, _p, _i64, _p, _i64, _p, _p]),
+    "circatt_axial_rotary_wide": (_int, [_int, _int, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                         _i32, _i32, _i32, _f32, _f32, _p, _i64, _p, _i64, _p, _p]),
     "circatt_malloc": (_int, [ctypes.POINTER(_p), _i64]),
     "circatt_free": (_int, [_p]),
     "circatt_memcpy": (_int, [_p, _p, _i64, _int]),

@@ -10,6 +10,7 @@ distance apart (the parts of one projection's output are read in place).
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -318,8 +319,8 @@ def _turn(x, inverse, grid, pairs, H, base, per_image, interleaved, positions):
     nb, P = (shape[0], math.prod(shape[1:-1])) if len(shape) > 2 else (1, shape[0])
     n1, n2, n3 = grid
     p1, p2, p3 = (*pairs, 0, 0)[:3]
-    _call(x.device, L.lib.circatt_axial_rotary, _CODES[x.dtype], inverse, 1 if interleaved else 0, len(pairs), n1, n2, n3,
-          P, nb, H, C // H, p1, p2, p3, base, x.data_ptr(), row, ptr(positions),
+    _call(x.device, L.lib.circatt_axial_rotary_wide, _CODES[x.dtype], inverse, 1 if interleaved else 0, len(pairs), n1, n2,
+          n3, P, nb, H, C // H, p1, p2, p3, *base, x.data_ptr(), row, ptr(positions),
           P * len(pairs) if per_image else 0, y.data_ptr())
     return y
 
@@ -357,7 +358,9 @@ def axial_rotary(x, pairs, nheads: int, *, base: float = 10000.0, positions: tor
         per_image = x.dim() > 2 and positions.dim() == x.dim()
         shape = x.shape[:-1] if per_image or x.dim() == 2 else x.shape[1:-1]
         positions = _index(positions, "positions", x, (*shape, len(pairs)))
-    meta = (grid, pairs, int(nheads), float(base), per_image, bool(interleaved))
+    base = float(base)
+    near = ctypes.c_float(base).value
+    meta = (grid, pairs, int(nheads), (near, base - near), per_image, bool(interleaved))
     if _recorded(x):
         return AxialRotaryFn.apply(x, positions, *meta)
     return _turn(x, 0, *meta, positions)

@@ -97,7 +97,7 @@ int check_kind(int kind) {
 
 extern "C" {
 
-int circatt_version(void) { return 10100; }
+int circatt_version(void) { return 10200; }
 
 int circatt_set_math(int mode) {
     if (mode != CIRCATT_MATH_SPLIT_F16 && mode != CIRCATT_MATH_F32)
@@ -891,6 +891,14 @@ int circatt_axial_rotary(int dtype, int inverse, int interleaved, int naxes, int
                          int64_t P, int64_t nb, int64_t nheads, int64_t dh, int32_t p1, int32_t p2, int32_t p3,
                          float base, const void *x, int64_t x_row, const int32_t *positions, int64_t pos_batch,
                          void *y, void *stream) {
+    return circatt_axial_rotary_wide(dtype, inverse, interleaved, naxes, n1, n2, n3, P, nb, nheads, dh, p1, p2, p3, base,
+                                     0.f, x, x_row, positions, pos_batch, y, stream);
+}
+
+int circatt_axial_rotary_wide(int dtype, int inverse, int interleaved, int naxes, int64_t n1, int64_t n2, int64_t n3,
+                              int64_t P, int64_t nb, int64_t nheads, int64_t dh, int32_t p1, int32_t p2, int32_t p3,
+                              float base, float base_rest, const void *x, int64_t x_row, const int32_t *positions,
+                              int64_t pos_batch, void *y, void *stream) {
     CIRCATT_TRY(check_token_dtype(dtype));
     if (naxes < 1 || naxes > 3) return fail(CIRCATT_ERR_INVALID, "naxes=%d must be 1, 2 or 3", naxes);
     if (nheads < 1 || nheads > 65536 || dh < 2 || dh % 2 != 0 || dh > 65536 || nheads * dh > 1 << 24)
@@ -906,7 +914,9 @@ int circatt_axial_rotary(int dtype, int inverse, int interleaved, int naxes, int
         return fail(CIRCATT_ERR_INVALID, "%lld pairs do not fit heads of %lld channels", (long long)total, (long long)dh);
     if (total > kMaxPairs)
         return fail(CIRCATT_ERR_UNSUPPORTED, "%lld pairs: at most %d are supported", (long long)total, kMaxPairs);
-    if (!(base > 0.f) || !std::isfinite(base)) return fail(CIRCATT_ERR_INVALID, "base=%g must be positive and finite", (double)base);
+    const double whole = (double)base + (double)base_rest;
+    if (!(base > 0.f) || !(whole > 0) || !std::isfinite(whole))
+        return fail(CIRCATT_ERR_INVALID, "base=%g must be positive and finite", whole);
     if (P < 0 || nb < 0 || P > INT32_MAX / 2 || nb > INT32_MAX || (nb > 0 && P > (int64_t)INT32_MAX / nb))
         return fail(CIRCATT_ERR_INVALID, "invalid sizes P=%lld, nb=%lld", (long long)P, (long long)nb);
     if (positions == nullptr) {
@@ -948,7 +958,7 @@ int circatt_axial_rotary(int dtype, int inverse, int interleaved, int naxes, int
     for (int a = 0; a < naxes; ++a) {
         pr.pairs[a] = p[a];
         for (int i = 0; i < p[a]; ++i)
-            pr.turns[at++] = std::pow((double)base, -(double)i / p[a]) / 6.283185307179586476925;
+            pr.turns[at++] = std::pow(whole, -(double)i / p[a]) / 6.283185307179586476925;
     }
     return hip_result(launch_rotary(pr, as_stream(stream)), "circatt_axial_rotary");
 }

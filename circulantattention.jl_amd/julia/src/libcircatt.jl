@@ -221,6 +221,15 @@ circatt_axial_rotary(dtype, inverse, interleaved, naxes, n1, n2, n3, P, nb, nhea
           dtype, inverse, interleaved, naxes, n1, n2, n3, P, nb, nheads, dh, p1, p2, p3,
           base, x, x_row, positions, pos_batch, y, stream)
 
+circatt_axial_rotary_wide(dtype, inverse, interleaved, naxes, n1, n2, n3, P, nb, nheads, dh, p1, p2,
+                          p3, base, base_rest, x, x_row, positions, pos_batch, y, stream) =
+    ccall((:circatt_axial_rotary_wide, libcircatt), Cint,
+          (Cint, Cint, Cint, Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Int32,
+           Int32, Int32, Cfloat, Cfloat, Ptr{Cvoid}, Int64, Ptr{Int32}, Int64, Ptr{Cvoid},
+           Ptr{Cvoid}),
+          dtype, inverse, interleaved, naxes, n1, n2, n3, P, nb, nheads, dh, p1, p2, p3,
+          base, base_rest, x, x_row, positions, pos_batch, y, stream)
+
 circatt_malloc(ptr, bytes) =
     ccall((:circatt_malloc, libcircatt), Cint, (Ptr{Ptr{Cvoid}}, Int64), ptr, bytes)
 

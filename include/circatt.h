@@ -384,12 +384,21 @@ int circatt_paged_append(int dtype, int64_t T, int64_t B, int64_t channels, cons
  * position * base^(-i/p); the channels behind stay.  positions (Int32, naxes a
  * token, P tokens; pos_batch apart from signal to signal, 0: shared), or NULL:
  * token i1 + n1*(i2 + n2*i3) has the positions (i1, i2, i3).  inverse: the
- * turn the other way, which is the gradient.
+ * turn the other way, which is the gradient.  The angle is formed in Float64.
+ *
+ * circatt_axial_rotary_wide takes the base as a sum of two Float32 numbers, the
+ * nearest one and what that leaves (48 bits): position * base^(-i/p) of a base that
+ * Float32 does not hold is off by 1e-3 at position 2^20 if it is rounded first.
  */
 int circatt_axial_rotary(int dtype, int inverse, int interleaved, int naxes, int64_t n1, int64_t n2,
                          int64_t n3, int64_t P, int64_t nb, int64_t nheads, int64_t dh, int32_t p1,
                          int32_t p2, int32_t p3, float base, const void *x, int64_t x_row,
                          const int32_t *positions, int64_t pos_batch, void *y, void *stream);
+int circatt_axial_rotary_wide(int dtype, int inverse, int interleaved, int naxes, int64_t n1, int64_t n2,
+                              int64_t n3, int64_t P, int64_t nb, int64_t nheads, int64_t dh, int32_t p1,
+                              int32_t p2, int32_t p3, float base, float base_rest, const void *x,
+                              int64_t x_row, const int32_t *positions, int64_t pos_batch, void *y,
+                              void *stream);
 
 /*
  * Device memory helpers for hosts without a GPU array package (the reference

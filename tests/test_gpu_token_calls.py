@@ -36,3 +36,18 @@ def test_tangents_are_refused_and_not_dropped(ca):
             with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
                 f(dual)
             assert torch.equal(f(q), w)
+
+
+@pytest.mark.parametrize("base", [12345.678, 10000 * 8 ** (64 / 62), 1.0e6 / 3, 2.5e8 + 1 / 3])
+def test_rotary_base_that_float32_does_not_hold(ca, base):
+    """The angle is formed in 64 bits from the base as it is given: within the
+    restatement's bound (2^-21 of the pair's size, and rounding) to far positions,
+    where the base rounded to Float32 is off by 1e-4 to 1e-3."""
+    pos = torch.tensor([[0], [1], [-7], [1000], [100003], [1 << 20], [-(1 << 24) - 1]], dtype=torch.int32)
+    x = randn(83, 7, 2 * 64)
+    for interleaved in (False, True):
+        t = x.cuda().requires_grad_(True)
+        y = ca.axial_rotary(t, (32,), 2, positions=pos.cuda(), base=base, interleaved=interleaved)
+        M.check(y, *M.rotary(x.double(), (32,), 2, base, pos, interleaved, torch.float32), "y")
+        (g,) = torch.autograd.grad(y, t, x.cuda())
+        M.check(g, *M.rotary(x.double(), (32,), 2, base, pos, interleaved, torch.float32, inverse=True), "dx")
