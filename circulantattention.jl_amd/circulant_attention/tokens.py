@@ -16,6 +16,7 @@ import math
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib as L
 from ._functions import ptr, stream_ptr
@@ -250,6 +251,8 @@ def paged_mh_attention(q, cache_k, cache_v, pages, lengths, W, nheads: int, *, k
           cache_k.data_ptr(), cache_v.data_ptr(), npages, page, page_stride, row_stride, pages.data_ptr(),
           pages.stride(0), pages.shape[1], lengths.data_ptr(), ptr(offsets), y.data_ptr(), 1 if out is None else 0,
           ptr(work), wbytes)
+    if out is not None:
+        increment_version(out)
     return y
 
 
@@ -268,6 +271,7 @@ def paged_append_(cache_k, cache_v, k, v, pages, lengths, *, offsets: torch.Tens
     _call(k.device, L.lib.circatt_paged_append, _CODES[k.dtype], k.shape[0], B, C, k.data_ptr(), k.stride(0), v.data_ptr(),
           v.stride(0), cache_k.data_ptr(), cache_v.data_ptr(), npages, page, page_stride, row_stride, pages.data_ptr(),
           pages.stride(0), pages.shape[1], lengths.data_ptr(), ptr(offsets))
+    increment_version((cache_k, cache_v))
 
 
 def _token_stride(x):

@@ -51,3 +51,34 @@ def test_rotary_base_that_float32_does_not_hold(ca, base):
         M.check(y, *M.rotary(x.double(), (32,), 2, base, pos, interleaved, torch.float32), "y")
         (g,) = torch.autograd.grad(y, t, x.cuda())
         M.check(g, *M.rotary(x.double(), (32,), 2, base, pos, interleaved, torch.float32, inverse=True), "dx")
+
+
+def test_autograd_sees_what_is_written_in_place(ca):
+    """A cache, or an `out`, that a graph has saved and a call then changes: the
+    backward of that graph is an error, not a gradient of other values."""
+    page, C, H = 8, 32, 2
+    pages = torch.arange(4, dtype=torch.int32, device="cuda").reshape(2, 2)
+    lens = torch.tensor([3, 9], dtype=torch.int32, device="cuda")
+    new = randn(1, 2, C).cuda()
+    caches = [randn(2 + i, 4, page, C).cuda() for i in range(2)]
+    out = torch.zeros(2, C, device="cuda")
+    before = [t._version for t in (*caches, out)]
+    w = torch.ones(C, device="cuda", requires_grad=True)
+    lost = [(t * w).sum() for t in (*caches, out)]
+    kept = (new * w).sum()
+    ca.paged_append_(*caches, new, new, pages, lens)
+    ca.paged_mh_attention(new, *caches, pages, lens, None, H, out=out)
+    assert all(t._version > n for t, n in zip((*caches, out), before))
+    for loss in lost:
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+    kept.backward()
+    assert torch.equal(w.grad, new.sum(0))
+    # views count with their base; tensors of inference mode have no counter
+    both = torch.zeros(4, page, 2 * C, device="cuda")
+    ca.paged_append_(*both.chunk(2, -1), new, new, pages, lens)
+    assert both._version > 0
+    with torch.inference_mode():
+        frozen = [torch.zeros(4, page, C, device="cuda") for _ in range(2)]
+        ca.paged_append_(*frozen, new, new, pages, lens)
+        ca.paged_mh_attention(new, *frozen, pages, lens, None, H, out=torch.zeros(2, C, device="cuda"))
