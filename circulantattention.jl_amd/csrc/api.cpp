@@ -641,6 +641,13 @@ int check_rows(const char *name, const void *p, int64_t row, int64_t batch, int6
     return CIRCATT_OK;
 }
 
+// A launch holds less than 2^32 threads along an axis.
+int check_threads(int64_t threads) {
+    if (threads > UINT32_MAX)
+        return fail(CIRCATT_ERR_UNSUPPORTED, "a launch of %lld threads, at most 2^32 - 1 are supported", (long long)threads);
+    return CIRCATT_OK;
+}
+
 int sliding_problem(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
                     int64_t sinks, float scale, SlidingProblem &pr) {
     CIRCATT_TRY(check_token_dtype(dtype));
@@ -648,7 +655,6 @@ int sliding_problem(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_
     CIRCATT_TRY(check_window(window, sinks, scale));
     if (L < 0 || B < 0 || L > INT32_MAX / 2 || B > INT32_MAX || L * nheads > INT32_MAX / 2)
         return fail(CIRCATT_ERR_INVALID, "invalid signal size L=%lld, B=%lld", (long long)L, (long long)B);
-    // launch dimensions: at most one workgroup for 4 rows
     if (B > 0 && L * nheads > (int64_t)INT32_MAX / B)
         return fail(CIRCATT_ERR_UNSUPPORTED, "B*L*nheads = %lld * %lld exceeds 2^31", (long long)B, (long long)(L * nheads));
     pr = SlidingProblem{};
@@ -717,7 +723,7 @@ int paged_problem(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_he
     pr.scale = scale;
     pr.page = (int)page_size;
     pr.maxp = (int)maxp;
-    return CIRCATT_OK;
+    return T == 0 ? CIRCATT_OK : check_threads(paged_threads(pr));
 }
 
 bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
@@ -741,6 +747,7 @@ int circatt_sliding_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t
     SlidingProblem pr;
     CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
     if (L == 0 || B == 0) return ok();
+    CIRCATT_TRY(check_threads(sliding_threads(pr, lse != nullptr)));  // lse: a backward will follow
     const int es = esize_of(dtype);
     CIRCATT_TRY(check_rows("q", q, q_row, q_batch, nheads * dh, es));
     CIRCATT_TRY(check_rows("k", k, k_row, k_batch, kv_heads * dh, es));
@@ -761,7 +768,8 @@ int64_t circatt_sliding_bwd_workspace_bytes(int dtype, int64_t L, int64_t B, int
                                             int64_t dh, int64_t window, int64_t sinks) {
     SlidingProblem pr;
     if (sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, 1.f, pr) != CIRCATT_OK) return -1;
-    return L == 0 || B == 0 ? 0 : 4 * sliding_bwd_workspace_floats(pr);
+    if (L == 0 || B == 0) return 0;
+    return check_threads(sliding_threads(pr, true)) == CIRCATT_OK ? 4 * sliding_bwd_workspace_floats(pr) : -1;
 }
 
 int circatt_sliding_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
@@ -773,6 +781,7 @@ int circatt_sliding_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t
     SlidingProblem pr;
     CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
     if (L == 0 || B == 0) return ok();
+    CIRCATT_TRY(check_threads(sliding_threads(pr, true)));
     const int es = esize_of(dtype);
     CIRCATT_TRY(check_rows("q", q, q_row, q_batch, nheads * dh, es));
     CIRCATT_TRY(check_rows("k", k, k_row, k_batch, kv_heads * dh, es));
@@ -884,6 +893,7 @@ int circatt_paged_append(int dtype, int64_t T, int64_t B, int64_t channels, cons
     pr.npages = (int)npages;
     pr.pages = pages, pr.pages_row = pages_row, pr.maxp = (int)max_pages;
     pr.lengths = lengths, pr.offsets = offsets;
+    CIRCATT_TRY(check_threads(append_threads(pr)));
     return hip_result(launch_append(pr, as_stream(stream)), "circatt_paged_append");
 }
 
@@ -960,6 +970,7 @@ int circatt_axial_rotary_wide(int dtype, int inverse, int interleaved, int naxes
         for (int i = 0; i < p[a]; ++i)
             pr.turns[at++] = std::pow(whole, -(double)i / p[a]) / 6.283185307179586476925;
     }
+    CIRCATT_TRY(check_threads(rotary_threads(pr)));
     return hip_result(launch_rotary(pr, as_stream(stream)), "circatt_axial_rotary");
 }
 

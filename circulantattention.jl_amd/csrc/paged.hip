@@ -659,12 +659,20 @@ __global__ __launch_bounds__(256) void append_rows(AppendProblem pr) {
 
 int64_t paged_workspace_floats(const PagedProblem &pr) { return paged_plan(pr).floats; }
 
+int64_t paged_threads(const PagedProblem &pr) {
+    const PagedPlan pl = paged_plan(pr);
+    // and the workgroups for the rows behind the last sequence
+    return 512 * ((int64_t)(pl.chunk ? pl.chunk_grid.blocks : 0) + pl.few_grid.blocks + 8);
+}
+
 hipError_t launch_paged(const PagedProblem &pr, hipStream_t s) {
     if (pr.dtype == CIRCATT_F32) launch<0>(pr, s);
     else if (pr.dtype == CIRCATT_F16) launch<2>(pr, s);
     else launch<3>(pr, s);
     return hipGetLastError();
 }
+
+int64_t append_threads(const AppendProblem &pr) { return (pr.T + 3) / 4 * 256; }
 
 hipError_t launch_append(const AppendProblem &pr, hipStream_t s) {
     const unsigned blocks = (unsigned)((pr.T + 3) / 4);

@@ -164,53 +164,65 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryProblem pr, int TB, F
     }
 }
 
-template <typename T, int V>
-void launch(const RotaryProblem &pr, hipStream_t s) {
-    // about 1024 units, four a thread, and at most 32 KiB of angles
-    const int upt = pr.H * pr.D / V, most = 4096 / pr.npairs;
-    int TB = (1024 + upt - 1) / upt;
-    TB = TB < most ? TB : most;
-    const unsigned blocks = (unsigned)(pr.nb * ((pr.P + TB - 1) / TB));
-    const size_t lds = (size_t)TB * pr.npairs * 8;
-    const FastDiv d1 = make_fastdiv(pr.n1), d2 = make_fastdiv(pr.n2), dt = make_fastdiv(upt), du = make_fastdiv(pr.D / V),
-                  dp = make_fastdiv(pr.npairs);
-    if (pr.interleaved)
-        rotary_kernel<T, V, true><<<blocks, 256, lds, s>>>(pr, TB, d1, d2, dt, du, dp);
-    else
-        rotary_kernel<T, V, false><<<blocks, 256, lds, s>>>(pr, TB, d1, d2, dt, du, dp);
-}
-
-template <typename T>
-bool launch_any(const RotaryProblem &pr, hipStream_t s) {
-    constexpr int V = 16 / sizeof(T);
-    const int row = pr.H * pr.D, units = row / V, most = 4096 / pr.npairs;
-    int TB = (1024 + units - 1) / units;
-    TB = TB < most ? TB : most;
-    const size_t lds = (size_t)TB * (row * sizeof(T) + pr.npairs * 8);
-    if (pr.D / V > 256 || lds > 64 * 1024) return false;
-    rotary_any_kernel<T><<<(unsigned)(pr.nb * ((pr.P + TB - 1) / TB)), 256, lds, s>>>(
-        pr, TB, make_fastdiv(pr.n1), make_fastdiv(pr.n2), make_fastdiv(pr.H), make_fastdiv(pr.npairs));
-    return true;
-}
-
 // Units of 16 bytes where they divide the head, its sections, the token stride
 // and both addresses; by way of LDS where they divide all but the sections; else
 // single pairs (interleaved) or channels.
-template <typename T>
-void route(const RotaryProblem &pr, hipStream_t s) {
-    const int per = pr.interleaved ? 2 : 1;
+enum Route { kUnits, kAny, kPairs, kSingle };
+struct Plan {
+    Route route;
+    int TB;  // tokens a workgroup: about 1024 units, four a thread, and at most 32 KiB of angles
+    int64_t blocks;
+};
+Plan plan_of(const RotaryProblem &pr) {
+    const int per = pr.interleaved ? 2 : 1, W = pr.dtype == CIRCATT_F32 ? 4 : 8, row = pr.H * pr.D;
     int sections = pr.D;
     for (int a = 0; a < pr.naxes; ++a) sections |= pr.pairs[a] * per;
-    constexpr int W = 16 / sizeof(T);
     const uint64_t addr = reinterpret_cast<uint64_t>(pr.x) | reinterpret_cast<uint64_t>(pr.y);
-    const bool rows = pr.D % W == 0 && pr.x_row % W == 0 && addr % 16 == 0;
-    if (rows && sections % W == 0) launch<T, W>(pr, s);
-    else if (rows && launch_any<T>(pr, s)) return;
-    else if (pr.interleaved) launch<T, 2>(pr, s);
-    else launch<T, 1>(pr, s);
+    auto tokens = [&](int units) {
+        const int most = 4096 / pr.npairs, some = (1024 + units - 1) / units;
+        return some < most ? some : most;
+    };
+    Plan pl{pr.interleaved ? kPairs : kSingle, 0, 0};
+    if (pr.D % W == 0 && pr.x_row % W == 0 && addr % 16 == 0) {
+        pl.TB = tokens(row / W);
+        if (sections % W == 0) pl.route = kUnits;
+        else if (pr.D / W <= 256 && (int64_t)pl.TB * (row * (16 / W) + pr.npairs * 8) <= 64 * 1024) pl.route = kAny;
+    }
+    if (pl.route == kPairs || pl.route == kSingle) pl.TB = tokens(row / (pl.route == kPairs ? 2 : 1));
+    pl.blocks = pr.nb * ((pr.P + pl.TB - 1) / pl.TB);
+    return pl;
+}
+
+template <typename T, int V>
+void launch(const RotaryProblem &pr, const Plan &pl, hipStream_t s) {
+    const size_t lds = (size_t)pl.TB * pr.npairs * 8;
+    const FastDiv d1 = make_fastdiv(pr.n1), d2 = make_fastdiv(pr.n2), dt = make_fastdiv(pr.H * pr.D / V),
+                  du = make_fastdiv(pr.D / V), dp = make_fastdiv(pr.npairs);
+    if (pr.interleaved)
+        rotary_kernel<T, V, true><<<(unsigned)pl.blocks, 256, lds, s>>>(pr, pl.TB, d1, d2, dt, du, dp);
+    else
+        rotary_kernel<T, V, false><<<(unsigned)pl.blocks, 256, lds, s>>>(pr, pl.TB, d1, d2, dt, du, dp);
+}
+
+template <typename T>
+void route(const RotaryProblem &pr, hipStream_t s) {
+    const Plan pl = plan_of(pr);
+    if (pl.route == kUnits) {
+        launch<T, 16 / sizeof(T)>(pr, pl, s);
+    } else if (pl.route == kAny) {
+        const size_t lds = (size_t)pl.TB * (pr.H * pr.D * sizeof(T) + pr.npairs * 8);
+        rotary_any_kernel<T><<<(unsigned)pl.blocks, 256, lds, s>>>(pr, pl.TB, make_fastdiv(pr.n1), make_fastdiv(pr.n2),
+                                                                   make_fastdiv(pr.H), make_fastdiv(pr.npairs));
+    } else if (pl.route == kPairs) {
+        launch<T, 2>(pr, pl, s);
+    } else {
+        launch<T, 1>(pr, pl, s);
+    }
 }
 
 }  // namespace
+
+int64_t rotary_threads(const RotaryProblem &pr) { return 256 * plan_of(pr).blocks; }
 
 hipError_t launch_rotary(const RotaryProblem &pr, hipStream_t s) {
     if (pr.dtype == CIRCATT_F32) route<float>(pr, s);

@@ -52,7 +52,7 @@ struct BlockOrder {
         if (unit >= n) unit = -1;
     }
 };
-unsigned grid8(int64_t n) { return (unsigned)((n + 7) / 8 * 8); }
+int64_t grid8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // Rows [k0, k0 + KT) of one head from p (row bytes rb apart, n rows of D
 // channels in all) into LDS; rows from n on and units from D on are zeros.
@@ -859,7 +859,7 @@ WalkSplit walk_split(const SlidingProblem &pr) {
 template <typename T, int DP>
 hipError_t forward(const SlidingProblem &pr, hipStream_t s) {
     const int blocks = (pr.L * pr.G + 127) / 128;
-    sliding_fwd<T, DP><<<grid8((int64_t)pr.B * pr.Hk * blocks), 256, 0, s>>>(pr, blocks);
+    sliding_fwd<T, DP><<<(unsigned)grid8((int64_t)pr.B * pr.Hk * blocks), 256, 0, s>>>(pr, blocks);
     return hipGetLastError();
 }
 template <int DT>
@@ -871,12 +871,12 @@ hipError_t forward(const SlidingProblem &pr, hipStream_t s) {
 template <typename T, int DP>
 hipError_t backward(const SlidingProblem &pr, hipStream_t s) {
     const int blocks = (pr.L * pr.G + 127) / 128;
-    sliding_dq<T, DP><<<grid8((int64_t)pr.B * pr.Hk * blocks), 256, 0, s>>>(pr, blocks);
+    sliding_dq<T, DP><<<(unsigned)grid8((int64_t)pr.B * pr.Hk * blocks), 256, 0, s>>>(pr, blocks);
     if (pr.dk != nullptr) {
         const WalkSplit sp = walk_split(pr);
         const int64_t units = (int64_t)pr.B * pr.Hk;
         if (sp.far > 0) sliding_dkdv_far<T, DP><<<(unsigned)(units * sp.far * sp.far_parts), 256, 0, s>>>(pr, sp);
-        sliding_dkdv<T, DP><<<grid8(units * sp.blocks * sp.parts), 256 * BwdShape<T, DP>::NG, 0, s>>>(pr, sp);
+        sliding_dkdv<T, DP><<<(unsigned)grid8(units * sp.blocks * sp.parts), 256 * BwdShape<T, DP>::NG, 0, s>>>(pr, sp);
         if (sp.parts > 1) sliding_dkdv_join<T, DP><<<(unsigned)(units * ((pr.L + 31) / 32)), 256, 0, s>>>(pr, sp);
     }
     return hipGetLastError();
@@ -894,6 +894,18 @@ int64_t sliding_bwd_workspace_floats(const SlidingProblem &pr) {
     const WalkSplit sp = walk_split(pr);
     const int DP = (pr.D + 31) / 32 * 32;
     return sp.part_at + (sp.parts > 1 ? (int64_t)pr.B * pr.Hk * sp.blocks * sp.parts * 128 * DP * 2 : 0);
+}
+
+int64_t sliding_threads(const SlidingProblem &pr, bool backward) {
+    const int64_t units = (int64_t)pr.B * pr.Hk, rows = 256 * grid8(units * (((int64_t)pr.L * pr.G + 127) / 128));
+    if (!backward) return rows;
+    const WalkSplit sp = walk_split(pr);
+    // 512 threads, but 256 for some Float32 heads
+    const int64_t keys = 512 * grid8(units * sp.blocks * sp.parts), far = 256 * units * sp.far * sp.far_parts;
+    const int64_t join = sp.parts > 1 ? 256 * units * ((pr.L + 31) / 32) : 0;
+    int64_t most = rows;
+    for (int64_t n : {keys, far, join}) most = n > most ? n : most;
+    return most;
 }
 
 hipError_t launch_sliding_fwd(const SlidingProblem &pr, hipStream_t s) {

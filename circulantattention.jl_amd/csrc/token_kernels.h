@@ -30,6 +30,9 @@ struct SlidingProblem {
     float *work;         // rowsum(dy * y), laid out as lse, then partial sums
 };
 int64_t sliding_bwd_workspace_floats(const SlidingProblem &pr);
+// Threads of the largest launch of the forward, or of the backward: a launch holds
+// less than 2^32 along an axis.
+int64_t sliding_threads(const SlidingProblem &pr, bool backward);
 hipError_t launch_sliding_fwd(const SlidingProblem &pr, hipStream_t s);
 hipError_t launch_sliding_bwd(const SlidingProblem &pr, hipStream_t s);
 
@@ -55,6 +58,7 @@ struct PagedProblem {
     float *work;
 };
 int64_t paged_workspace_floats(const PagedProblem &pr);
+int64_t paged_threads(const PagedProblem &pr);  // along the longest axis
 hipError_t launch_paged(const PagedProblem &pr, hipStream_t s);
 
 struct AppendProblem {
@@ -72,6 +76,7 @@ struct AppendProblem {
     int maxp;
     const int32_t *lengths, *offsets;
 };
+int64_t append_threads(const AppendProblem &pr);
 hipError_t launch_append(const AppendProblem &pr, hipStream_t s);
 
 constexpr int kMaxPairs = 128;
@@ -88,6 +93,7 @@ struct RotaryProblem {
     void *y;
     double turns[kMaxPairs];   // turns for one step of a pair's axis
 };
+int64_t rotary_threads(const RotaryProblem &pr);
 hipError_t launch_rotary(const RotaryProblem &pr, hipStream_t s);
 
 }  // namespace circatt

@@ -30,3 +30,43 @@ def rotary(L, base=1e4, rest=0.0, n=(8, 8, 1), tokens=64, nb=2, H=4, dh=64, p=(1
                                   dict(rest=math.nan), dict(rest=math.inf), dict(base=1.0, rest=-1.0)])
 def test_rotary_bases(L, args):
     expect(L, rotary(L, **args), -1, "base")
+
+
+def fwd(L, dtype=3, n=64, B=2, H=4, Hk=2, dh=64, W=16, S=0, lse=None):
+    return L.lib.circatt_sliding_fwd(dtype, n, B, H, Hk, dh, W, S, 0.125, P, H * dh, 0, P, Hk * dh, 0, P, Hk * dh, 0, None, FAR,
+                                     None, lse, None)
+
+
+def bwd(L, dtype=3, n=64, B=2, H=4, Hk=2, dh=64, W=16, S=0):
+    return L.lib.circatt_sliding_bwd(dtype, n, B, H, Hk, dh, W, S, 0.125, P, H * dh, 0, P, Hk * dh, 0, P, Hk * dh, 0, None, P,
+                                     None, P, P, H * dh, 0, FAR, FAR, FAR, P, 1 << 60, None)
+
+
+def test_launches_of_too_many_threads_are_refused(L):
+    """2^24 workgroups of 256 threads, or 2^23 of 512, and a workgroup at least for
+    each signal and head of keys."""
+    many = dict(n=1, H=1, Hk=1, dh=8)
+    expect(L, fwd(L, B=1 << 24, **many), -2, "threads")
+    expect(L, fwd(L, B=(1 << 24) - 7, **many), -2, "threads")  # a multiple of 8 is launched
+    # what the forward could do and the backward could not: refused before training
+    expect(L, fwd(L, B=1 << 23, lse=P, **many), -2, "threads")
+    expect(L, bwd(L, B=1 << 23, **many), -2, "threads")
+    size = L.lib.circatt_sliding_bwd_workspace_bytes
+    assert size(3, 1, 1 << 23, 1, 1, 8, 16, 0) == -1
+    assert size(3, 1, (1 << 23) - 8, 1, 1, 8, 16, 0) > 0
+    assert size(3, 300, 50000, 4, 2, 64, 3, 40) > 0
+    # long ones: the keys' partial sums would not be the largest launch
+    assert size(3, 1 << 20, 64, 1, 1, 8, 16, 100) > 0
+
+
+def test_paged_append_and_rotary_launches_are_refused(L):
+    rc = L.lib.circatt_paged_attention(3, 1 << 30, 1, 1, 1, 8, 16, 0, 0.125, P, 8, P, P, 10, 16, 128, 8, P, 8, 8, P, P, FAR, 1,
+                                       P, 1 << 60, None)
+    expect(L, rc, -1, "sizes")
+    rc = L.lib.circatt_paged_attention(3, (1 << 30) - 1, 65535, 1, 1, 8, 16, 0, 0.125, P, 8, P, P, 10, 16, 128, 8, P, 8, 8, P, P,
+                                       FAR, 1, P, 1 << 60, None)
+    expect(L, rc, -2, "threads")
+    rc = L.lib.circatt_paged_append(3, 1 << 26, 1, 8, P, 8, P, 8, P, P, 10, 16, 128, 8, P, 8, 8, P, P, None)
+    expect(L, rc, -2, "threads")
+    expect(L, rotary(L, n=(1, 1, 1), tokens=1, nb=1 << 24, H=1, dh=64, x_row=64), -2, "threads")
+    expect(L, rotary(L, n=(1, 1, 1), tokens=1, nb=1 << 24, H=1, dh=66, x_row=66), -2, "threads")
