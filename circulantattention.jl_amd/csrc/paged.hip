@@ -95,7 +95,8 @@ __device__ __forceinline__ Block find_block(const PagedProblem &pr, int which, i
     x.len = uniform(pr.lengths[x.b]);
     x.len = x.len > 0 ? x.len : 0;
     x.first = x.len - x.rows / pr.G;
-    if (x.r0 >= x.rows) x.b = -1;
+    // (before its first row: offsets that do not ascend)
+    if (x.r0 < 0 || x.r0 >= x.rows) x.b = -1;
     return x;
 }
 

@@ -82,3 +82,26 @@ def test_autograd_sees_what_is_written_in_place(ca):
         frozen = [torch.zeros(4, page, C, device="cuda") for _ in range(2)]
         ca.paged_append_(*frozen, new, new, pages, lens)
         ca.paged_mh_attention(new, *frozen, pages, lens, None, H, out=torch.zeros(2, C, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offsets", [(0, 100, 5, 50), (0, 130, 2, 2), (0, 0, 150, 10), (90, 10, 0, 150), (0, -3, 70, 150),
+                                     (0, 50, 1000, 1001), (5, 1 << 30, 7, 150), (-5, 3, 2, 1), (150, 0, 0, 0)])
+def test_offsets_that_do_not_ascend_stay_inside(ca, dtype, offsets):
+    """Offsets are documented to ascend from 0.  Others give unspecified rows, but
+    nothing outside of the arrays is written, whatever they hold."""
+    T, H, Hk, D, page, guard = 150, 4, 1, 32, 8, 300
+    q = randn(1, T, H * D, dtype=dtype).cuda()
+    caches = [randn(2 + i, 60, page, Hk * D, dtype=dtype).cuda() for i in range(2)]
+    pages = torch.arange(60, dtype=torch.int32).reshape(3, 20).cuda()
+    lens = torch.tensor([150, 140, 130], dtype=torch.int32).cuda()
+    offs = torch.tensor(offsets, dtype=torch.int32).cuda()
+    whole = torch.full((T + 2 * guard, H * D), 7.0, dtype=dtype, device="cuda")
+    for W in (None, 9):
+        ca.paged_mh_attention(q, *caches, pages, lens, W, H, kv_heads=Hk, sinks=2, offsets=offs, out=whole[guard:guard + T])
+        ca.paged_mh_attention(q, *caches, pages, lens, W, H, kv_heads=Hk, sinks=2, offsets=offs)
+        assert (whole[:guard] == 7).all() and (whole[guard + T:] == 7).all()
+    kv = torch.full((62, page, Hk * D), 7.0, dtype=dtype, device="cuda")
+    new = randn(4, T, Hk * D, dtype=dtype).cuda()
+    ca.paged_append_(kv[1:61], kv[1:61].clone(), new, new, pages, lens, offsets=offs)
+    assert (kv[0] == 7).all() and (kv[61] == 7).all()
