@@ -140,7 +140,8 @@ def _window(W, sinks, scale, dh):
         raise AssertionError(f"window W={W} must be >= 1")
     if int(sinks) < 0:
         raise AssertionError(f"sinks={sinks} must be >= 0")
-    return W, int(sinks), 1.0 / math.sqrt(dh) if scale is None else float(scale)
+    # what holds every token; larger numbers would lose their high bits on the way to C
+    return min(W, _EVERY), min(int(sinks), _EVERY), 1.0 / math.sqrt(dh) if scale is None else float(scale)
 
 
 def sliding_mh_attention(q, k, v, W, nheads: int, *, kv_heads: int = None, sinks: int = 0, scale: float = None,
@@ -346,7 +347,7 @@ def axial_rotary(x, pairs, nheads: int, *, base: float = 10000.0, positions: tor
     _require(x, "x")
     if x.dim() < 2:
         raise AssertionError("x is (B, *spatial, C) or (T, C)")
-    pairs = tuple(int(p) for p in pairs)
+    pairs = tuple(min(max(int(p), 0), _EVERY) for p in pairs)  # (refused by C as they are)
     if not 1 <= len(pairs) <= 3:
         raise AssertionError(f"{len(pairs)} axes; 1 to 3 are supported")
     _head_count(x.shape[-1], int(nheads), "x's")

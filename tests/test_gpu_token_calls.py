@@ -105,3 +105,16 @@ def test_offsets_that_do_not_ascend_stay_inside(ca, dtype, offsets):
     new = randn(4, T, Hk * D, dtype=dtype).cuda()
     ca.paged_append_(kv[1:61], kv[1:61].clone(), new, new, pages, lens, offsets=offs)
     assert (kv[0] == 7).all() and (kv[61] == 7).all()
+
+
+def test_numbers_beyond_the_c_types(ca):
+    """Windows and sinks of more than 64 bits hold every token; numbers of pairs of
+    more than 32 are refused: none loses its high bits."""
+    q = randn(1, 1, 40, 64).cuda()
+    want = ca.sliding_mh_attention(q, q, q, None, 2)
+    for big in ((1 << 64) + 5, (1 << 63) + 5):
+        assert torch.equal(ca.sliding_mh_attention(q, q, q, big, 2), want)
+        assert torch.equal(ca.sliding_mh_attention(q, q, q, 3, 2, sinks=big), want)
+    for p in ((1 << 32) + 4, (1 << 64) + 4, -4, -(1 << 32) + 4):
+        with pytest.raises(AssertionError, match="pairs"):
+            ca.axial_rotary(q, (p,), 2)

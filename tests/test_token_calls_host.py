@@ -70,3 +70,13 @@ def test_paged_append_and_rotary_launches_are_refused(L):
     expect(L, rc, -2, "threads")
     expect(L, rotary(L, n=(1, 1, 1), tokens=1, nb=1 << 24, H=1, dh=64, x_row=64), -2, "threads")
     expect(L, rotary(L, n=(1, 1, 1), tokens=1, nb=1 << 24, H=1, dh=66, x_row=66), -2, "threads")
+
+
+def test_windows_and_sinks_beyond_64_bits_hold_every_token():
+    from circulant_attention import tokens
+    for W in (1 << 31, (1 << 63) + 5, (1 << 64) + 5, 10 ** 30):
+        assert tokens._window(W, W, None, 64) == (1 << 30, 1 << 30, 0.125)
+    assert tokens._window((1 << 30) - 1, 3, 0.5, 64) == ((1 << 30) - 1, 3, 0.5)
+    for W, S in ((-(1 << 64) + 5, 0), (5, -(1 << 64) + 5)):
+        with pytest.raises(AssertionError):
+            tokens._window(W, S, None, 64)
