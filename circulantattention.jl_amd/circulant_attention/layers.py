@@ -72,9 +72,9 @@ class SlidingAttBlock(torch.nn.Module):
                  rotary=None, base: float = 10000.0, bias: bool = True):
         super().__init__()
         kv_heads = nheads if kv_heads is None else kv_heads
-        if channels % nheads != 0:
+        if nheads < 1 or channels % nheads != 0:
             raise AssertionError(f"channels ({channels}) must be divisible by nheads ({nheads})")
-        if nheads % kv_heads != 0:
+        if kv_heads < 1 or nheads % kv_heads != 0:
             raise AssertionError(f"nheads ({nheads}) must be divisible by kv_heads ({kv_heads})")
         self.window, self.sinks, self.nheads, self.kv_heads = window, sinks, nheads, kv_heads
         self.rotary, self.base = None if rotary is None else tuple(rotary), base

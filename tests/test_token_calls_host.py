@@ -80,3 +80,10 @@ def test_windows_and_sinks_beyond_64_bits_hold_every_token():
     for W, S in ((-(1 << 64) + 5, 0), (5, -(1 << 64) + 5)):
         with pytest.raises(AssertionError):
             tokens._window(W, S, None, 64)
+
+
+@pytest.mark.parametrize("heads", [(0, None), (-4, None), (4, 0), (4, -2)])
+def test_block_without_heads(heads):
+    import circulant_attention as ca
+    with pytest.raises(AssertionError, match="divisible"):
+        ca.SlidingAttBlock(32, 8, *heads)
