@@ -9,6 +9,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
@@ -731,6 +732,29 @@ bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
     return x < y ? y - x < (uintptr_t)na : x - y < (uintptr_t)nb;
 }
 
+// Memory of a call, from end to end of its strides (NULL: none).
+struct Span {
+    const char *name;
+    const void *p;
+    int64_t bytes;
+};
+Span span(const char *name, const void *p, int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t width, int esize) {
+    return Span{name, p, ((n1 - 1) * s1 + (n2 - 1) * s2 + width) * esize};
+}
+// Results are written while other workgroups still read the arguments.
+int check_apart(std::initializer_list<Span> results, std::initializer_list<Span> arguments) {
+    for (const Span *r = results.begin(); r != results.end(); ++r) {
+        if (r->p == nullptr) continue;
+        for (const Span &a : arguments)
+            if (a.p != nullptr && overlap(r->p, r->bytes, a.p, a.bytes))
+                return fail(CIRCATT_ERR_INVALID, "%s must not overlap %s", r->name, a.name);
+        for (const Span *o = results.begin(); o != r; ++o)
+            if (o->p != nullptr && overlap(r->p, r->bytes, o->p, o->bytes))
+                return fail(CIRCATT_ERR_INVALID, "%s must not overlap %s", r->name, o->name);
+    }
+    return CIRCATT_OK;
+}
+
 int check_rests(const void *rest, const void *y, int64_t bytes, int dtype) {
     if (dtype == CIRCATT_F32) return fail(CIRCATT_ERR_INVALID, "y_rest belongs to the 16-bit types");
     if (reinterpret_cast<uintptr_t>(rest) % 16 != 0) return fail(CIRCATT_ERR_INVALID, "y_rest must be 16-byte aligned");
@@ -761,6 +785,11 @@ int circatt_sliding_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t
     pr.y = y;
     pr.y_rest = y_rest;
     pr.lse = lse;
+    const int64_t C = nheads * dh, Ck = kv_heads * dh;
+    CIRCATT_TRY(check_apart({span("y", y, B, L * C, L, C, C, es), span("y_rest", y_rest, B, L * C, L, C, C, es),
+                             span("lse", lse, 1, 0, 1, 0, B * L * nheads, 4)},
+                            {span("q", q, B, q_batch, L, q_row, C, es), span("k", k, B, k_batch, L, k_row, Ck, es),
+                             span("v", v, B, v_batch, L, v_row, Ck, es)}));
     return hip_result(launch_sliding_fwd(pr, as_stream(stream)), "circatt_sliding_fwd");
 }
 
@@ -811,6 +840,14 @@ int circatt_sliding_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t
     pr.dy = dy, pr.dy_row = dy_row, pr.dy_batch = dy_batch;
     pr.dq = dq, pr.dk = dk, pr.dv = dv;
     pr.work = static_cast<float *>(workspace);
+    const int64_t C = nheads * dh, Ck = kv_heads * dh;
+    CIRCATT_TRY(check_apart(
+        {span("dq", dq, B, L * C, L, C, C, es), span("dk", dk, B, L * Ck, L, Ck, Ck, es),
+         span("dv", dv, B, L * Ck, L, Ck, Ck, es), span("workspace", workspace, 1, 0, 1, 0, need, 1)},
+        {span("q", q, B, q_batch, L, q_row, C, es), span("k", k, B, k_batch, L, k_row, Ck, es),
+         span("v", v, B, v_batch, L, v_row, Ck, es), span("y", y, B, L * C, L, C, C, es),
+         span("y_rest", y_rest, B, L * C, L, C, C, es), span("lse", lse, 1, 0, 1, 0, B * L * nheads, 4),
+         span("dy", dy, B, dy_batch, L, dy_row, C, es)}));
     return hip_result(launch_sliding_bwd(pr, as_stream(stream)), "circatt_sliding_bwd");
 }
 
@@ -949,7 +986,10 @@ int circatt_axial_rotary_wide(int dtype, int inverse, int interleaved, int naxes
     CIRCATT_NONNULL(y);
     if (x_row < nheads * dh)
         return fail(CIRCATT_ERR_INVALID, "x: token stride %lld below %lld channels", (long long)x_row, (long long)(nheads * dh));
-    if (x == y) return fail(CIRCATT_ERR_INVALID, "y must not alias x");
+    const int es = esize_of(dtype);
+    const int64_t C = nheads * dh;
+    if (x == y || overlap(y, nb * P * C * es, x, ((nb * P - 1) * x_row + C) * es))
+        return fail(CIRCATT_ERR_INVALID, "y must not alias x");
     pr.dtype = dtype;
     pr.inverse = inverse != 0;
     pr.interleaved = interleaved != 0;

@@ -324,8 +324,9 @@ int circatt_count_unequal(int kind, int64_t n, const void *a, const void *b, int
  * circatt_sliding_bwd: dq, dk, dv of the same (dk and dv both NULL: dq alone),
  * from y, y_rest and lse of the forward.  y_rest may be NULL; then <dy, y> is that
  * of the rounded y, which costs dq precision where few keys carry a row (up to 3
- * times the error of a form that rounds its results alone, else 1.6).  No atomics; gradients of a shared head are
- * summed over its queries' heads in a fixed order.
+ * times the error of a form that rounds its results alone, else 1.6).  No
+ * atomics; gradients of a shared head are summed over its queries' heads in a
+ * fixed order.  Results overlap neither the arguments nor one another.
  */
 int circatt_sliding_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
                         int64_t window, int64_t sinks, float scale, const void *q, int64_t q_row,

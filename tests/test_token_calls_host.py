@@ -87,3 +87,44 @@ def test_block_without_heads(heads):
     import circulant_attention as ca
     with pytest.raises(AssertionError, match="divisible"):
         ca.SlidingAttBlock(32, 8, *heads)
+
+
+def at(address):
+    return ctypes.c_void_p(address)
+
+
+# q is 2 signals of 64 rows of 256 channels (65536 bytes), k and v of 128 (32768), lse 2048 bytes
+Q, K, V, Y, REST, LSE, DY, DQ, DK, DV, WORK = (0x100000 * i for i in range(1, 12))
+
+
+def sliding(L, **where):
+    w = dict(q=Q, k=K, v=V, y=Y, rest=REST, lse=LSE)
+    w.update(where)
+    return L.lib.circatt_sliding_fwd(3, 64, 2, 4, 2, 64, 16, 0, 0.125, at(w["q"]), 256, 64 * 256, at(w["k"]), 128, 64 * 128,
+                                     at(w["v"]), 128, 64 * 128, None, at(w["y"]), at(w["rest"]), at(w["lse"]), None)
+
+
+@pytest.mark.parametrize("where", [dict(y=Q), dict(y=Q + 65536 - 16), dict(y=K - 65536 + 16), dict(y=V + 32768 - 16),
+                                   dict(rest=Q + 16), dict(rest=Y + 65536 - 16), dict(lse=Y + 16), dict(lse=V + 32752)])
+def test_forward_results_over_arguments(L, where):
+    expect(L, sliding(L, **where), -1, "must not overlap")
+
+
+def sliding_bwd(L, **where):
+    w = dict(dq=DQ, dk=DK, dv=DV, work=WORK, dy=DY)
+    w.update(where)
+    return L.lib.circatt_sliding_bwd(3, 64, 2, 4, 2, 64, 16, 0, 0.125, at(Q), 256, 64 * 256, at(K), 128, 64 * 128, at(V), 128,
+                                     64 * 128, None, at(Y), at(REST), at(LSE), at(w["dy"]), 256, 64 * 256, at(w["dq"]),
+                                     at(w["dk"]), at(w["dv"]), at(w["work"]), 1 << 40, None)
+
+
+@pytest.mark.parametrize("where", [dict(dq=DY), dict(dq=Q), dict(dq=Y + 65520), dict(dk=K), dict(dv=V + 16), dict(dv=DK),
+                                   dict(dk=DQ + 65520), dict(work=LSE), dict(work=DV + 32752), dict(dq=REST - 65520)])
+def test_backward_results_over_arguments(L, where):
+    expect(L, sliding_bwd(L, **where), -1, "must not overlap")
+
+
+@pytest.mark.parametrize("y", [0x10000, 0x10010, 0x10000 + 128 * 512 - 16, 0x10000 - 128 * 512 + 16])
+def test_rotary_result_over_its_argument(L, y):
+    """2 x 64 tokens of 512 bytes."""
+    expect(L, rotary(L, y=at(y)), -1, "alias")
