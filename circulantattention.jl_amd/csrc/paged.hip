@@ -494,7 +494,7 @@ __global__ __launch_bounds__((256 * ChunkShape<T, DP>::NG), 1) void paged_chunk(
 // Adds up the partial sums of a block's rows in the order of the splits: half a
 // wavefront a row, four channels a lane.
 template <typename T, int R>
-__global__ __launch_bounds__(256) void paged_join(PagedProblem pr, PagedGrid gr) {
+__global__ __launch_bounds__(256, 8) void paged_join(PagedProblem pr, PagedGrid gr) {
     const Block w = find_block<R>(pr, gr.which, blockIdx.x);
     if (w.b < 0) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hk = blockIdx.y, d = 4 * (lane & 31);

@@ -72,6 +72,12 @@ __device__ __forceinline__ void fetch_rows(const T *p, int64_t row, int k0, int 
     }
 }
 
+template <typename T>
+__device__ __forceinline__ SignalKV<T> signal_rows(const SlidingProblem &pr, int b, int hk) {
+    return SignalKV<T>{static_cast<const T *>(pr.k) + b * pr.k_batch + (int64_t)hk * pr.D,
+                       static_cast<const T *>(pr.v) + b * pr.v_batch + (int64_t)hk * pr.D, pr.k_row, pr.v_row};
+}
+
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void sliding_fwd(SlidingProblem pr, int blocks) {
     typedef Ring<T, DP> Rg;
@@ -84,6 +90,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int rows = n * pr.G, r0 = w.block * 128, all_rows = pr.L * pr.G;
     const int r = r0 + 32 * wave + (lane & 31);
+    T *y = static_cast<T *>(pr.y) + (int64_t)b * pr.L * pr.H * pr.D + (int64_t)hk * pr.G * pr.D;
+    T *rest = pr.y_rest == nullptr ? nullptr : static_cast<T *>(pr.y_rest) + (y - static_cast<T *>(pr.y));
     const int64_t stat = ((int64_t)b * pr.Hk + hk) * all_rows;
     // the wavefront's rows, those past the end doubling the last one
     const int rr = r < rows ? r : rows - 1, at = rows > 0 ? rr / pr.G : -1, g = rows > 0 ? rr - at * pr.G : 0;
@@ -168,11 +176,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             next();
             for (++i; i < count; ++i, next()) round(i);
         }
-        const SlidingProblem pe = argument_again<SlidingProblem>();
-        const int64_t ky = (int64_t)hk * pe.D, qy = ky * pe.G, yb = (int64_t)b * pe.L * pe.H * pe.D + qy;
-        const SignalKV<T> kv{static_cast<const T *>(pe.k) + b * pe.k_batch + ky,
-                             static_cast<const T *>(pe.v) + b * pe.v_batch + ky, pe.k_row, pe.v_row};
-        T *y = static_cast<T *>(pe.y) + yb, *rest = pe.y_rest == nullptr ? nullptr : static_cast<T *>(pe.y_rest) + yb;
         uint32_t again = 0;
         if (live) {
             // a row sees its own token at least: without a sum of weights all that it sees
@@ -180,10 +183,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             const float l = x.total(), inv = 1.f / l;
             bool bad = false;
             if (r < rows) {
-                bad = store_channels(x.o, y + ((int64_t)at * pe.H + g) * pe.D, pe.D, lane, inv);
-                if (rest != nullptr) store_rests(x.o, rest + ((int64_t)at * pe.H + g) * pe.D, pe.D, lane, inv);
-                if (pe.lse != nullptr && lane < 32)
-                    pe.lse[stat + r] = x.m + __builtin_amdgcn_logf(l);
+                bad = store_channels(x.o, y + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv);
+                if (rest != nullptr) store_rests(x.o, rest + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv);
+                if (pr.lse != nullptr && lane < 32) pr.lse[stat + r] = x.m + __builtin_amdgcn_logf(l);
             }
             // A value that is not finite reaches, as 0 times itself, every row of
             // a wavefront whose tile holds it: where such a value is among the keys
@@ -193,6 +195,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             // weights is NaN or 0: then the row is, whatever it sees.)
             again = rows_of(__ballot(bad && l > 0.f));
             if (again != 0) {
+                const SlidingProblem pe = argument_again<SlidingProblem>();
+                const SignalKV<T> kv = signal_rows<T>(pe, b, hk);
                 auto tile_end = [&](int j) { return (int)((int64_t)j + KT - j % KT < n ? j + KT - j % KT : n); };
                 const int window = r0 / pe.G - pe.W + 1;
                 if (!bad_values(kv, window > 0 ? window / KT * KT : 0, hi - pe.W + 1, pe.D) &&
@@ -201,17 +205,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
                     again = 0;
             }
         }
-        share_repairs<4>((CIRCATT_LDS uint32_t *)lds, wave, wave, again, 0, [&](int i, bool, bool) {
-            const int aj = (r0 + i) / pe.G, gj = r0 + i - aj * pe.G;
-            const int64_t out = ((int64_t)aj * pe.H + gj) * pe.D;
-            forward_row(static_cast<const T *>(pe.q) + b * pe.q_batch + qy + aj * pe.q_row + (int64_t)gj * pe.D, y + out,
-                        rest == nullptr ? rest : rest + out, kv, aj, pe.W, pe.S, pe.D, pe.scale * kLog2e);
+        // (The list lies in a K tile: the last round, whose barrier is behind all, reads
+        // none.)
+        share_repairs<4, false>((CIRCATT_LDS uint32_t *)lds, wave, wave, again, 0, [&](int i, bool, bool) {
+            const SlidingProblem pe = argument_again<SlidingProblem>();
+            const int aj = (r0 + i) / pe.G, h = hk * pe.G + r0 + i - aj * pe.G;
+            const int64_t out = (((int64_t)b * pe.L + aj) * pe.H + h) * pe.D;
+            forward_row(static_cast<const T *>(pe.q) + b * pe.q_batch + aj * pe.q_row + (int64_t)h * pe.D,
+                        static_cast<T *>(pe.y) + out, pe.y_rest == nullptr ? nullptr : static_cast<T *>(pe.y_rest) + out,
+                        signal_rows<T>(pe, b, hk), aj, pe.W, pe.S, pe.D, pe.scale * kLog2e);
         });
     }
     // rows behind the signal's length
     if (r >= rows && r < all_rows) {
         const int t = r / pr.G, gt = r - t * pr.G;
-        T *y = static_cast<T *>(pr.y) + (int64_t)b * pr.L * pr.H * pr.D + (int64_t)hk * pr.G * pr.D;
         zero_channels(y + ((int64_t)t * pr.H + gt) * pr.D, pr.D, lane);
         if (pr.lse != nullptr && lane < 32) pr.lse[stat + r] = INFINITY;
     }
@@ -742,24 +749,23 @@ void sliding_dkdv(SlidingProblem pr, WalkSplit sp) {
                     128 * DP, lane_e);
         return;
     }
-    const SlidingProblem pe = argument_again<SlidingProblem>();
-    const HeadGroup<T> he(pe, unit, n);
     bool bad_k = false, bad_v = false;
     if (group == 0) {
-        const int64_t out = ((int64_t)he.b * pe.L + j_e) * pe.Hk * pe.D + (int64_t)he.hk * pe.D;
-        T *kd = static_cast<T *>(pe.dk) + out, *vd = static_cast<T *>(pe.dv) + out;
-        if (j_e < he.n) {
-            bad_k = store_channels(x.dk, kd, pe.D, lane_e, pe.scale);
-            bad_v = store_channels(x.dv, vd, pe.D, lane_e, 1.f);
-        } else if (j_e < pe.L) {
-            zero_channels(kd, pe.D, lane_e);
-            zero_channels(vd, pe.D, lane_e);
+        const int64_t out = ((int64_t)hg.b * pr.L + j_e) * pr.Hk * pr.D + (int64_t)hg.hk * pr.D;
+        T *kd = static_cast<T *>(pr.dk) + out, *vd = static_cast<T *>(pr.dv) + out;
+        if (j_e < n) {
+            bad_k = store_channels(x.dk, kd, pr.D, lane_e, pr.scale);
+            bad_v = store_channels(x.dv, vd, pr.D, lane_e, 1.f);
+        } else if (j_e < pr.L) {
+            zero_channels(kd, pr.D, lane_e);
+            zero_channels(vd, pr.D, lane_e);
         }
     }
-    share_repairs<4 * NG>((CIRCATT_LDS uint32_t *)lds_mem, group == 0 ? wave : -1, 4 * group + wave,
-                          rows_of(__ballot(bad_k)), rows_of(__ballot(bad_v)), [&](int i, bool fix_k, bool fix_v) {
-                              he.again(pe, k0 + i, k0 + (i & ~31), fix_k, fix_v);
-                          });
+    share_repairs<4 * NG, true>((CIRCATT_LDS uint32_t *)lds_mem, group == 0 ? wave : -1, 4 * group + wave,
+                                rows_of(__ballot(bad_k)), rows_of(__ballot(bad_v)), [&](int i, bool fix_k, bool fix_v) {
+                                    const SlidingProblem pe = argument_again<SlidingProblem>();
+                                    HeadGroup<T>(pe, unit, n).again(pe, k0 + i, k0 + (i & ~31), fix_k, fix_v);
+                                });
 }
 
 // The partial sums of 32 keys, the far ones first, in the order of their parts: a

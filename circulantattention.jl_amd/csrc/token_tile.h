@@ -371,12 +371,12 @@ __device__ __forceinline__ P argument_again() {
 // tend to lie together: `from`, which of four wavefronts with 32 rows each this one
 // is (or -1), with its rows of two kinds, a bit each; `wave`, this one's turn.
 // repair(row of the 128, first kind, second kind) is called by whole wavefronts.
-// The list is LDS that nothing is read from any more once all are here.
-template <int WAVES, typename Repair>
+// The list is LDS that nothing is read from any more, or with SYNC once all are here.
+template <int WAVES, bool SYNC, typename Repair>
 __device__ __forceinline__ void share_repairs(CIRCATT_LDS uint32_t *list, int from, int wave, uint32_t one, uint32_t two,
                                               Repair repair) {
     if ((one | two) != 0) __threadfence_block();  // other wavefronts read the rows
-    __syncthreads();
+    if (SYNC) __syncthreads();
     if (from >= 0 && lane_again() == 0) {
         list[from] = one;
         list[4 + from] = two;
