@@ -155,7 +155,8 @@ def sliding_mh_attention(q, k, v, W, nheads: int, *, kv_heads: int = None, sinks
     nheads/kv_heads heads of q (kv_heads None: as many as q's).  W None: every
     token up to i.  scale None: 1/sqrt(D).  lengths (int32, (B,)): a padded
     batch; rows from a signal's length on are zero, receive and give no
-    gradient, and what they hold does not matter.  Differentiable in q, k, v."""
+    gradient, and what they hold does not matter.  A row whose visible scores are
+    all -inf is NaN.  Differentiable in q, k, v, once and not in forward mode."""
     _require(q, "q")
     _require(k, "k", q)
     _require(v, "v", q)
@@ -220,9 +221,11 @@ def paged_mh_attention(q, cache_k, cache_v, pages, lengths, W, nheads: int, *, k
     (int32, (B, most)); lengths (int32, (B,)) counts a sequence's tokens with
     the new ones.  The arrays of numbers are read on the device when the kernels
     run: a captured call follows what they hold then.  A page number that is not
-    in the cache hides its tokens; a row that sees nothing is zero.  Rows of q
-    behind the last sequence give zero rows, or leave ``out`` alone where the
-    caller passes it."""
+    in the cache hides its tokens, and a token behind the table's last page sees
+    nothing; a row that sees nothing is zero.  Offsets ascend from 0: others give
+    unspecified rows.  Rows of q behind the last sequence give zero rows, or leave
+    ``out``, which overlaps neither q nor the caches, alone where the caller
+    passes it."""
     _require(q, "q")
     if q.dim() != 2:
         raise AssertionError("q is (T, C): the new tokens of all sequences in order")
@@ -261,7 +264,7 @@ def paged_append_(cache_k, cache_v, k, v, pages, lengths, *, offsets: torch.Tens
     """Writes the new tokens' keys and values, k and v (T, C), into the caches
     (pages, page size, C): the arguments of paged_mh_attention, lengths counting
     the new tokens.  A token whose page number is not in the cache is dropped;
-    no two tokens may share a slot."""
+    no two tokens may share a slot, and k and v hold no slot that is written."""
     _require(k, "k")
     _require(v, "v", k)
     npages, page, C, page_stride, row_stride = _cache(cache_k, cache_v, k)
@@ -342,8 +345,9 @@ def axial_rotary(x, pairs, nheads: int, *, base: float = 10000.0, positions: tor
     x: (B, *reversed(spatial), C) with nheads heads in C, or packed tokens
     (T, C).  positions None: the grid's own, axis 1 the fastest spatial axis, as
     many axes as spatial ones.  Else int32, (*x.shape[:-1], axes), or without
-    the batch dim to share them.  The angle is formed in 64 bits.  Float32,
-    Float16, BFloat16; differentiable in x."""
+    the batch dim to share them.  The angle is formed in 64 bits, from the base as
+    it is given.  Float32, Float16, BFloat16; differentiable in x, once and not in
+    forward mode."""
     _require(x, "x")
     if x.dim() < 2:
         raise AssertionError("x is (B, *spatial, C) or (T, C)")

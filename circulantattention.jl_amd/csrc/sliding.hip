@@ -21,18 +21,22 @@ __device__ __forceinline__ int signal_length(const SlidingProblem &pr, int b) {
 // LDS (Ring).  Workgroups that share a head of keys run on one XCD (ids 8 apart),
 // whose L2 then holds their common tiles.
 //
-// Bound by the products and the softmax between them, not by memory: a wavefront's
-// tile is 32 products of 32 cycles and, by the counters, some 270 other vector
-// instructions with starts and edges, 32 of them exponentials of 8 cycles.  8192 tokens, 32 heads of 128 over 8, window 1024,
-// 4 sinks, bf16: 166 us, 780 TFLOP/s of the pairs that are seen (870 of those
-// formed: edges of tiles); the same without a window 535 us, 1030 TFLOP/s, where a
-// large library product of this card reaches 1190.  Copies of the kernel without
-// its DMA, or with operands from registers instead of LDS, take 21 and 32 us less
-// (both: 53).  Two rounds in one run (the next tile's scores among this one's exponentials)
-// take 166 us where one after another took 175; explicit orders of the run's
-// instructions, wavefront priorities, operands read earlier and tiles of 32 keys
-// in five places changed nothing or lost (177 us).  For training it also stores what
-// y's rounding took: 2 x 4096 tokens, 16 heads of 128, 63 us without, 73 with.
+// Bound by the products and the softmax between them, and by the blocks' starts and
+// ends: a wavefront's tile is 32 products of 32 cycles and, by the counters, some 270
+// other vector instructions with starts and edges, 32 of them exponentials of 8
+// cycles.  8192 tokens, 32 heads of 128 over 8, window 1024, 4 sinks, bf16: 167 to 170
+// us, 770 TFLOP/s of the pairs that are seen (870 of those formed: edges of tiles); the
+// same without a window 540 us, 1020 TFLOP/s, where a large library product of this
+// card reaches 1190.  From windows of 128 (4 tiles a block, 76 us) to none (64 tiles)
+// the time is 45 us and 7.7 for a tile in every block: the 45, some 6 tiles' time, are
+// the cold start and the end of 2048 blocks in four rounds, a quarter of the time at
+// window 1024.  Copies of the kernel without its DMA, or with operands from registers
+// instead of LDS, take 21 and 32 us less (both: 53).  Two rounds in one run (the next
+// tile's scores among this one's exponentials) take 166 us where one after another took
+// 175; explicit orders of the run's instructions, wavefront priorities, operands read
+// earlier and tiles of 32 keys in five places changed nothing or lost (177 us).  For
+// training it also stores what y's rounding took: 2 x 4096 tokens, 16 heads of 128, 63
+// us without, 73 with.
 //
 // Backward, queries: the same blocks with tiles in two buffers.
 template <typename T, int DP>
@@ -366,7 +370,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
 // order.  At the size above 109 us, 600 TFLOP/s; the operands and sums of 32 keys
 // take 192 of a lane's 256 registers, and what is left bounds how far ahead
 // operands can be read.  An earlier form, workgroups of one group whose walks were
-// split in three for a full chip, took 187 us and 23 more to add up; barriers of a group alone, by a count in LDS, changed nothing.
+// split in three for a full chip, took 187 us and 23 more to add up; barriers of a group
+// alone, by a count in LDS, changed nothing.
 //
 // The rows that see a sink from behind its block's window are another walk,
 // sliding_dkdv_far's, for 32 keys and with a wavefront for every tile: a few

@@ -315,11 +315,12 @@ int circatt_count_unequal(int kind, int64_t n, const void *a, const void *b, int
  *
  * circatt_sliding_fwd: token i of signal b, i < lengths[b] (lengths NULL: L),
  * sees key j <= i if j > i - window or j < sinks, and
- *   y = softmax_j(scale * <q_i, k_j>) v.
- * Rows from lengths[b] on are zero and nothing of q, k, v behind lengths[b]
- * has an influence, whatever it holds.  lse (nheads*L*B floats, for the
- * backward) may be NULL.  y_rest (laid out as y, 16-bit types only) receives what
- * the rounding of y took, for the backward, or is NULL.
+ *   y = softmax_j(scale * <q_i, k_j>) v,
+ * which is NaN where all visible scores are -inf.  Rows from lengths[b] on are
+ * zero and nothing of q, k, v behind lengths[b] has an influence, whatever it
+ * holds.  lse (nheads*L*B floats, for the backward) may be NULL.  y_rest (laid out
+ * as y, 16-bit types only) receives what the rounding of y took, for the backward,
+ * or is NULL.
  *
  * circatt_sliding_bwd: dq, dk, dv of the same (dk and dv both NULL: dq alone),
  * from y, y_rest and lse of the forward.  y_rest may be NULL; then <dy, y> is that
@@ -339,8 +340,9 @@ int circatt_sliding_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t
                         int64_t window, int64_t sinks, float scale, const void *q, int64_t q_row,
                         int64_t q_batch, const void *k, int64_t k_row, int64_t k_batch, const void *v,
                         int64_t v_row, int64_t v_batch, const int32_t *lengths, const void *y,
-                        const void *y_rest, const float *lse, const void *dy, int64_t dy_row, int64_t dy_batch, void *dq,
-                        void *dk, void *dv, void *workspace, int64_t workspace_bytes, void *stream);
+                        const void *y_rest, const float *lse, const void *dy, int64_t dy_row,
+                        int64_t dy_batch, void *dq, void *dk, void *dv, void *workspace,
+                        int64_t workspace_bytes, void *stream);
 
 /*
  * The same attention for serving, over a paged cache: a cache holds npages
@@ -352,14 +354,15 @@ int circatt_sliding_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t
  * offsets[b+1] - 1 (offsets: B+1 ascending numbers from 0; NULL: one row for
  * each sequence, T = B).  pages, lengths and offsets are device arrays that
  * are read when the kernel runs, so a captured call follows their contents.
- * A page number outside [0, npages) is never followed: its tokens are hidden,
- * and a row that sees nothing is zero.  Rows of y behind the last sequence are
+ * A page number outside [0, npages) is never followed: its tokens are hidden.
+ * Tokens from max_pages * page_size on see nothing, and a row that sees nothing is
+ * zero.  Offsets that do not ascend leave rows unspecified.  Rows of y behind the last sequence are
  * zero with zero_tail = 1 and left as they were with 0.  y must not overlap q or
  * the caches.  Row strides are at most 2^22 elements, a cache 63 GiB end to end.
  *
  * circatt_paged_append writes the new tokens' k and v, packed the same way,
  * into their pages; a token whose page number is outside the cache is dropped.
- * No two tokens may share a slot.
+ * No two tokens may share a slot, and k and v hold no slot that is written.
  */
 int64_t circatt_paged_workspace_bytes(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads,
                                       int64_t dh, int64_t window, int64_t sinks, int64_t page_size,
