@@ -120,7 +120,8 @@ __device__ __forceinline__ const CIRCATT_GLOBAL T *lane_of(const T *p, int lane)
 // Loads below are under no condition, which would make each wait for itself: what
 // is not there reads something else in its place.
 //
-// <p, x> of every lane's own row p and one row x that the wavefront holds.
+// <p, x> of every lane's own row p and one row x that the wavefront holds.  For whole
+// wavefronts: under a condition, a lane that is left out has no part of x to read.
 template <typename T>
 __device__ __forceinline__ float lane_dot(const T *p, Pair x, int D) {
     constexpr int N = 4;
@@ -205,7 +206,7 @@ __device__ void forward_row(const T *q, T *y, T *rest, const KV &kv, int pos, in
         const T *kp = q, *vp = q;
         const bool sees = j <= pos && (j < S || j >= lo) && kv.row(j, kp, vp);
         if (!sees) kp = q, vp = zero_row<T>();
-        const float t = sees ? c * lane_dot(kp, qr, D) : -INFINITY;
+        const float score = c * lane_dot(kp, qr, D), t = sees ? score : -INFINITY;
         const float mn = fmaxf(m, wave_max(t)), mu = mn == -INFINITY ? 0.f : mn;
         const float r = __builtin_amdgcn_exp2f(m - mu), p = sees ? __builtin_amdgcn_exp2f(t - mu) : 0.f;
         l = l * r + wave_sum(p);
