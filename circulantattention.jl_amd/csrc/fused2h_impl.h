@@ -152,14 +152,15 @@ __device__ __forceinline__ h4 ldtr(const char *p) {
 // cannot tell the DMA rows from the slots the walk reads, which would expose
 // the whole prefetch at the start of each walk.  The callers wait for the rows
 // (vmcnt(0) and a barrier) before reading them.  (The compiler writes M0 for
-// the asm; one wait state then separates that write from the load.)
+// the asm, and may restore a spilled descriptor by a vector instruction right
+// before it, which the load must not read for five wait states.)
 typedef int i4v __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ i4v dma_rsrc(const float *p, int bytes) {
     const uint64_t b = reinterpret_cast<uint64_t>(p);
     return i4v{(int)(uint32_t)b, (int)((b >> 32) & 0xffffu), bytes, (int)f2d::kRsrcWord3};
 }
 __device__ __forceinline__ void dma16(i4v rs, unsigned m0, int voff) {
-    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                  :
                  : "v"(voff), "s"(rs), "{m0}"(m0)
                  : "memory");
