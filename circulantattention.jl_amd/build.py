@@ -27,7 +27,7 @@ SOURCES = ["api.cpp", "unfused.hip", "apply_rb.hip", "apply_mx.hip", "sim_mx.hip
            "fused1h_bwdq.hip", "fused1h_bwdkv.hip", "fused1h2_fwd.hip", "fused1h2_bwdq.hip",
            "fused1h2_bwdkv.hip", "fused_wide.hip",
            *(f"fused_stream{n}_{m}.hip" for n in (1, 2, 3, 4) for m in ("fwd", "bwdq", "bwdkv")),
-           "batch_ops.hip", "sliding.hip", "paged.hip", "rotary.hip"]
+           "batch_ops.hip", "sliding.hip", "shaped.hip", "capped.hip", "paged.hip", "paged_shaped.hip", "pages.hip", "rotary.hip"]
 FLAGS = [
     f"--offload-arch={ARCH}",
     "-O3",

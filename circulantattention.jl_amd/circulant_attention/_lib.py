@@ -90,6 +90,22 @@ SIGNATURES = {
                                        _i64, _p]),
     "circatt_paged_append": (_int, [_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64,
                                     _i64, _p, _i64, _i64, _p, _p, _p]),
+    "circatt_shaped_fwd": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _p, _p, _p, _i64, _p,
+                                  _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p]),
+    "circatt_shaped_bwd_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int]),
+    "circatt_shaped_bwd": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _p, _p, _p, _i64, _p,
+                                  _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _p,
+                                  _p, _p, _p, _i64, _p]),
+    "circatt_shaped_paged": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _p, _p, _p, _i64,
+                                    _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _int, _p, _i64,
+                                    _p]),
+    "circatt_paged_fork": (_int, [_i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _p, _p, _p, _p]),
+    "circatt_paged_resize_workspace_bytes": (_i64, [_i64, _i64]),
+    "circatt_paged_resize": (_int, [_int, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p,
+                                    _p, _p, _p, _p, _i64, _p]),
+    "circatt_paged_compact_workspace_bytes": (_i64, [_i64]),
+    "circatt_paged_compact": (_int, [_int, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p,
+                                     _p, _i64, _p]),
     "circatt_axial_rotary": (_int, [_int, _int, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                     _i32, _i32, _i32, _f32, _p, _i64, _p, _i64, _p, _p]),
     "circatt_axial_rotary_wide": (_int, [_int, _int, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64,

@@ -1,7 +1,9 @@
 """Attention on token signals: the sliding window in its causal form with
 sinks (the first tokens stay visible), for training and over a paged cache for
-serving, and rotary positions on one to three axes.  No counterpart in the
-reference, whose windows are centred and wrap around.
+serving, its scores capped, biased by distance or masked by documents or a prefix
+where that is asked for; the pages of the cache; and rotary positions on one to
+three axes.  No counterpart in the reference, whose windows are centred and wrap
+around.
 
 Signals are channels-last as in `channels_last=True` of the fused attention:
 (B, L, C) with the heads one after another in C.  Float32, Float16 and
@@ -92,7 +94,47 @@ def _head_count(C, nheads, what):
     return C // nheads
 
 
-def _sliding(train, q, k, v, W, S, H, Hk, scale, lengths):
+class _Shape:
+    """How a call's scores are shaped: cap (0: none), and slopes, prefix and places or
+    None each."""
+    __slots__ = ("cap", "arrays", "row")
+
+    def __init__(self, cap, slopes, prefix, places):
+        self.cap, self.arrays = cap, (slopes, prefix, places)
+        self.row = 0 if places is None else places.shape[1]
+
+    def args(self):
+        slopes, prefix, places = self.arrays
+        return self.cap, ptr(slopes), ptr(prefix), ptr(places), self.row
+
+
+def _shape(q, B, nheads, cap, slopes, prefix, places=None):
+    """The call's _Shape, or None where its scores are plain."""
+    cap = 0.0 if cap is None else float(cap)
+    if cap < 0.0 or not math.isfinite(cap):
+        raise AssertionError(f"cap={cap} must be positive and finite, 0 or None: no cap")
+    if cap == 0.0 and slopes is None and prefix is None and places is None:
+        return None
+    if prefix is not None and places is not None:
+        raise AssertionError("prefix and places do not go together")
+    if slopes is not None:
+        if not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32:
+            raise TypeError("slopes must be a float32 torch.Tensor")
+        if slopes.device != q.device:
+            raise AssertionError("slopes must have the device of the first argument")
+        if tuple(slopes.shape) != (nheads,):
+            raise AssertionError(f"slopes must have shape {(nheads,)}, got {tuple(slopes.shape)}")
+        if slopes.requires_grad and torch.is_grad_enabled():
+            raise AssertionError("slopes must not require gradients: none is formed")
+        slopes = slopes.detach().contiguous()
+    if prefix is not None:
+        prefix = _index(prefix, "prefix", q, (B,))
+    if places is not None:
+        places = _index(places, "places", q, tuple(q.shape[:2]))
+    return _Shape(cap, slopes, prefix, places)
+
+
+def _sliding(train, q, k, v, W, S, H, Hk, scale, lengths, shape=None):
     """y, and with train what the backward takes of the call."""
     (q, qr, qb), (k, kr, kb), (v, vr, vb) = _rows(q), _rows(k), _rows(v)
     B, n, C = q.shape
@@ -100,8 +142,11 @@ def _sliding(train, q, k, v, W, S, H, Hk, scale, lengths):
     lse = torch.empty((B, H * n), dtype=torch.float32, device=q.device) if train else None
     rest = torch.empty_like(y) if train and q.dtype != torch.float32 else None
     code = _CODES[q.dtype]
-    _call(q.device, L.lib.circatt_sliding_fwd, code, n, B, H, Hk, C // H, W, S, scale, q.data_ptr(), qr, qb,
-          k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), ptr(rest), ptr(lse))
+    rows = (q.data_ptr(), qr, qb, k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), ptr(rest), ptr(lse))
+    if shape is None:
+        _call(q.device, L.lib.circatt_sliding_fwd, code, n, B, H, Hk, C // H, W, S, scale, *rows)
+    else:
+        _call(q.device, L.lib.circatt_shaped_fwd, code, n, B, H, Hk, C // H, W, S, scale, *shape.args(), *rows)
     return y, (q, k, v, y, rest, lse, lengths), (code, W, S, H, Hk, scale, qr, qb, kr, kb, vr, vb)
 
 
@@ -117,21 +162,55 @@ class SlidingAttentionFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        q, k, v, y, rest, lse, lengths = ctx.saved_tensors
-        code, W, S, H, Hk, scale, qr, qb, kr, kb, vr, vb = ctx.meta
-        B, n, C = q.shape
-        dy, dr, db = _rows(dy)
-        dq = torch.empty((B, n, C), dtype=q.dtype, device=q.device)
-        dk = dv = None
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            dv = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        wbytes = L.lib.circatt_sliding_bwd_workspace_bytes(code, n, B, H, Hk, C // H, W, S)
-        work = torch.empty((max(wbytes, 4) // 4,), dtype=torch.float32, device=q.device)
-        _call(q.device, L.lib.circatt_sliding_bwd, code, n, B, H, Hk, C // H, W, S, scale, q.data_ptr(), qr, qb,
-              k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), ptr(rest), lse.data_ptr(),
-              dy.data_ptr(), dr, db, dq.data_ptr(), ptr(dk), ptr(dv), work.data_ptr(), wbytes)
-        return dq, dk, dv, None, None, None, None, None, None
+        return (*_sliding_gradients(ctx, dy, ctx.saved_tensors), None, None, None, None, None, None)
+
+
+class ShapedAttentionFn(torch.autograd.Function):
+    """The same with shaped scores (circatt_shaped_fwd / circatt_shaped_bwd).  The
+    shape's arrays are arguments of their own, so that one that is written before
+    the backward is noticed."""
+
+    @staticmethod
+    def forward(ctx, cap, slopes, prefix, places, *args):
+        y, saved, ctx.meta = _sliding(True, *args, _Shape(cap, slopes, prefix, places))
+        ctx.cap = cap
+        ctx.save_for_backward(*saved, slopes, prefix, places)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        *saved, slopes, prefix, places = ctx.saved_tensors
+        grads = _sliding_gradients(ctx, dy, saved, _Shape(ctx.cap, slopes, prefix, places), 4)
+        return (None, None, None, None, *grads, None, None, None, None, None, None)
+
+
+def _sliding_gradients(ctx, dy, saved, shape=None, first=0):
+    """dq, dk, dv of a call; q is its Function's argument number `first`."""
+    q, k, v, y, rest, lse, lengths = saved
+    code, W, S, H, Hk, scale, qr, qb, kr, kb, vr, vb = ctx.meta
+    B, n, C = q.shape
+    dy, dr, db = _rows(dy)
+    dq = torch.empty((B, n, C), dtype=q.dtype, device=q.device)
+    dk = dv = None
+    if ctx.needs_input_grad[first + 1] or ctx.needs_input_grad[first + 2]:
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dv = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    sizes = (code, n, B, H, Hk, C // H, W, S)
+    if shape is None:
+        wbytes = L.lib.circatt_sliding_bwd_workspace_bytes(*sizes)
+    else:
+        slopes, prefix, places = shape.arrays
+        wbytes = L.lib.circatt_shaped_bwd_workspace_bytes(*sizes, slopes is not None,
+                                                          prefix is not None or places is not None)
+    work = torch.empty((max(wbytes, 4) // 4,), dtype=torch.float32, device=q.device)
+    rows = (q.data_ptr(), qr, qb, k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), ptr(rest),
+            lse.data_ptr(), dy.data_ptr(), dr, db, dq.data_ptr(), ptr(dk), ptr(dv), work.data_ptr(), wbytes)
+    if shape is None:
+        _call(q.device, L.lib.circatt_sliding_bwd, *sizes, scale, *rows)
+    else:
+        _call(q.device, L.lib.circatt_shaped_bwd, *sizes, scale, *shape.args(), *rows)
+    return dq, dk, dv
 
 
 def _window(W, sinks, scale, dh):
@@ -145,7 +224,8 @@ def _window(W, sinks, scale, dh):
 
 
 def sliding_mh_attention(q, k, v, W, nheads: int, *, kv_heads: int = None, sinks: int = 0, scale: float = None,
-                         lengths: torch.Tensor = None) -> torch.Tensor:
+                         lengths: torch.Tensor = None, cap: float = None, slopes: torch.Tensor = None,
+                         places: torch.Tensor = None, prefix: torch.Tensor = None) -> torch.Tensor:
     """Causal multi-head attention in a sliding window with sinks: token i of a
     signal sees the W tokens up to itself and the first ``sinks`` ones,
 
@@ -156,7 +236,18 @@ def sliding_mh_attention(q, k, v, W, nheads: int, *, kv_heads: int = None, sinks
     token up to i.  scale None: 1/sqrt(D).  lengths (int32, (B,)): a padded
     batch; rows from a signal's length on are zero, receive and give no
     gradient, and what they hold does not matter.  A row whose visible scores are
-    all -inf is NaN.  Differentiable in q, k, v, once and not in forward mode."""
+    all -inf is NaN.  Differentiable in q, k, v, once and not in forward mode.
+
+    The scores x_ij = scale <q_i, k_j> may be shaped: into
+    ``cap`` tanh(x_ij / cap), and by - ``slopes``[h] |i - j| behind that (float32,
+    (nheads,); not differentiable in them).  And what a token sees:
+    places (int32, (B, L)): signals that hold documents one after another, each token's
+    place in its own, 0, 1, 2, ... (as axial_rotary takes positions).  A token sees
+    its own document alone, whose first tokens are its sinks.  Places that do not
+    count up so give unspecified rows.
+    prefix (int32, (B,)): every token of signal b sees the first prefix[b] ones too, those
+    before them included.  Not together with places.
+    Both are read on the device when the kernels run."""
     _require(q, "q")
     _require(k, "k", q)
     _require(v, "v", q)
@@ -174,9 +265,10 @@ def sliding_mh_attention(q, k, v, W, nheads: int, *, kv_heads: int = None, sinks
     if lengths is not None:
         lengths = _index(lengths, "lengths", q, (q.shape[0],))
     args = (q, k, v, W, sinks, nheads, kv_heads, scale, lengths)
+    shape = _shape(q, q.shape[0], nheads, cap, slopes, prefix, places)
     if _recorded(q, k, v):
-        return SlidingAttentionFn.apply(*args)
-    return _sliding(False, *args)[0]
+        return SlidingAttentionFn.apply(*args) if shape is None else ShapedAttentionFn.apply(shape.cap, *shape.arrays, *args)
+    return _sliding(False, *args, shape)[0]
 
 
 def _cache(cache_k, cache_v, like):
@@ -210,7 +302,8 @@ def _table(pages, lengths, offsets, like):
 
 
 def paged_mh_attention(q, cache_k, cache_v, pages, lengths, W, nheads: int, *, kv_heads: int = None, sinks: int = 0,
-                       scale: float = None, offsets: torch.Tensor = None, out: torch.Tensor = None) -> torch.Tensor:
+                       scale: float = None, offsets: torch.Tensor = None, out: torch.Tensor = None, cap: float = None,
+                       slopes: torch.Tensor = None, prefix: torch.Tensor = None) -> torch.Tensor:
     """sliding_mh_attention of the new tokens of several sequences over a paged
     cache that holds their keys and values (paged_append_), without gradients.
 
@@ -225,7 +318,9 @@ def paged_mh_attention(q, cache_k, cache_v, pages, lengths, W, nheads: int, *, k
     nothing; a row that sees nothing is zero.  Offsets ascend from 0: others give
     unspecified rows.  Rows of q behind the last sequence give zero rows, or leave
     ``out``, which overlaps neither q nor the caches, alone where the caller
-    passes it."""
+    passes it.  cap, slopes and prefix (one number for each sequence) as
+    sliding_mh_attention takes them; of a prefix that is not yet in the cache the new
+    tokens see what is."""
     _require(q, "q")
     if q.dim() != 2:
         raise AssertionError("q is (T, C): the new tokens of all sequences in order")
@@ -248,13 +343,18 @@ def paged_mh_attention(q, cache_k, cache_v, pages, lengths, W, nheads: int, *, k
         _require(y, "out", q)
         if tuple(y.shape) != (T, nheads * dh) or not y.is_contiguous():
             raise AssertionError(f"out must be contiguous {(T, nheads * dh)}")
+    shape = _shape(q, B, nheads, cap, slopes, prefix)
     code = _CODES[q.dtype]
     wbytes = L.lib.circatt_paged_workspace_bytes(code, T, B, nheads, kv_heads, dh, W, sinks, page, pages.shape[1])
     work = torch.empty((wbytes // 4,), dtype=torch.float32, device=q.device) if wbytes > 0 else None
-    _call(q.device, L.lib.circatt_paged_attention, code, T, B, nheads, kv_heads, dh, W, sinks, scale, q.data_ptr(), q_row,
-          cache_k.data_ptr(), cache_v.data_ptr(), npages, page, page_stride, row_stride, pages.data_ptr(),
-          pages.stride(0), pages.shape[1], lengths.data_ptr(), ptr(offsets), y.data_ptr(), 1 if out is None else 0,
-          ptr(work), wbytes)
+    sizes = (code, T, B, nheads, kv_heads, dh, W, sinks, scale)
+    rest = (q.data_ptr(), q_row, cache_k.data_ptr(), cache_v.data_ptr(), npages, page, page_stride, row_stride,
+            pages.data_ptr(), pages.stride(0), pages.shape[1], lengths.data_ptr(), ptr(offsets), y.data_ptr(),
+            1 if out is None else 0, ptr(work), wbytes)
+    if shape is None:
+        _call(q.device, L.lib.circatt_paged_attention, *sizes, *rest)
+    else:
+        _call(q.device, L.lib.circatt_shaped_paged, *sizes, *shape.args()[:3], *rest)
     if out is not None:
         increment_version(out)
     return y
@@ -276,6 +376,92 @@ def paged_append_(cache_k, cache_v, k, v, pages, lengths, *, offsets: torch.Tens
           v.stride(0), cache_k.data_ptr(), cache_v.data_ptr(), npages, page, page_stride, row_stride, pages.data_ptr(),
           pages.stride(0), pages.shape[1], lengths.data_ptr(), ptr(offsets))
     increment_version((cache_k, cache_v))
+
+
+def _held(pages, lengths, counts, like):
+    """The table, lengths and counts of a cache's pages, checked."""
+    if not isinstance(pages, torch.Tensor) or pages.dtype != torch.int32 or pages.dim() != 2:
+        raise TypeError("pages must be an int32 torch.Tensor (sequences, pages of each)")
+    if not pages.is_cuda:
+        raise ValueError("pages must live on a HIP device (libcircatt has no CPU path)")
+    if like is not None and pages.device != like.device:
+        raise AssertionError("pages must have the device of the cache")
+    if pages.shape[0] < 1 or pages.shape[1] < 1:
+        raise AssertionError(f"a page table of {tuple(pages.shape)}")
+    if pages.stride(1) != 1 and pages.shape[1] > 1 or pages.stride(0) < pages.shape[1]:
+        pages = pages.contiguous()
+    if lengths is not None:
+        lengths = _index(lengths, "lengths", pages, (pages.shape[0],))
+    if not isinstance(counts, torch.Tensor) or counts.dim() != 1:
+        raise TypeError("counts must be an int32 torch.Tensor (pages of the cache,)")
+    counts = _index(counts, "counts", pages, tuple(counts.shape) if like is None else (like.shape[0],))
+    return pages, max(pages.stride(0), pages.shape[1]), lengths, counts
+
+
+def paged_fork(pages, lengths, counts, source, page_size: int):
+    """The tables of sequences that go on from others: (pages, lengths, counts) with row n
+    as sequence source[n] had it (int32, (N,); a number outside the old sequences
+    gives an empty one).  The sequences share their pages; no token moves.
+
+    pages (int32, (B, most)) and lengths (int32, (B,)) as paged_mh_attention takes
+    them; counts (int32, (pages of the cache,)) says how often each page is held, 0 for a
+    free one.  Old sequences that nobody goes on from give their pages back.
+    Page numbers outside the cache are kept and not counted."""
+    pages, row, lengths, counts = _held(pages, lengths, counts, None)
+    if not isinstance(source, torch.Tensor) or source.dim() != 1:
+        raise TypeError("source must be an int32 torch.Tensor (sequences,)")
+    source = _index(source, "source", pages, tuple(source.shape))
+    (B, most), N = pages.shape, source.shape[0]
+    new = (torch.empty((N, most), dtype=torch.int32, device=pages.device), torch.empty_like(source), torch.empty_like(counts))
+    _call(pages.device, L.lib.circatt_paged_fork, B, counts.shape[0], int(page_size), pages.data_ptr(), row, most,
+          lengths.data_ptr(), counts.data_ptr(), N, ptr(source), ptr(new[0]), ptr(new[1]), new[2].data_ptr())
+    return new
+
+
+def paged_resize_(cache_k, cache_v, pages, lengths, counts, to):
+    """The tables of sequences that grow, shrink or end: (pages, lengths, counts) with
+    sequence b at to[b] tokens (int32, (B,); no more than its row of the table holds;
+    below 0: as it is), so that paged_append_ finds pages for the new ones.
+
+    Pages behind the new lengths are given back.  Then sequences get what they lack, in
+    their order, the free pages of the lowest numbers first.  A sequence that grows
+    from within a page that is held more than once gets its own copy of that page's
+    tokens, the only ones that move.  From the first sequence on that finds too few free
+    pages, those that need any stay as they are, as the lengths that come back show.
+    Other arguments as paged_fork's."""
+    _require(cache_k, "cache_k")
+    npages, page, C, page_stride, row_stride = _cache(cache_k, cache_v, cache_k)
+    pages, row, lengths, counts = _held(pages, lengths, counts, cache_k)
+    B, most = pages.shape
+    to = _index(to, "to", pages, (B,))
+    new = (torch.empty((B, most), dtype=torch.int32, device=pages.device), torch.empty_like(lengths), torch.empty_like(counts))
+    wbytes = L.lib.circatt_paged_resize_workspace_bytes(B, npages)
+    work = torch.empty((max(wbytes, 4) // 4,), dtype=torch.int32, device=pages.device)
+    _call(pages.device, L.lib.circatt_paged_resize, _CODES[cache_k.dtype], C, cache_k.data_ptr(), cache_v.data_ptr(), npages,
+          page, page_stride, row_stride, B, pages.data_ptr(), row, most, lengths.data_ptr(), counts.data_ptr(), to.data_ptr(),
+          *(t.data_ptr() for t in new), work.data_ptr(), wbytes)
+    increment_version((cache_k, cache_v))
+    return new
+
+
+def paged_compact_(cache_k, cache_v, pages, counts):
+    """The tables of a cache whose held pages have moved to its lowest numbers, with
+    their tokens: (pages, counts).  The held pages from number ``used`` on, as many as
+    there are held ones, take the free numbers below it in order.  Every table that
+    refers to the cache is one: its rows may be those of several, joined.  Other
+    arguments as paged_fork's."""
+    _require(cache_k, "cache_k")
+    npages, page, C, page_stride, row_stride = _cache(cache_k, cache_v, cache_k)
+    pages, row, _, counts = _held(pages, None, counts, cache_k)
+    B, most = pages.shape
+    new = (torch.empty((B, most), dtype=torch.int32, device=pages.device), torch.empty_like(counts))
+    wbytes = L.lib.circatt_paged_compact_workspace_bytes(npages)
+    work = torch.empty((max(wbytes, 4) // 4,), dtype=torch.int32, device=pages.device)
+    _call(pages.device, L.lib.circatt_paged_compact, _CODES[cache_k.dtype], C, cache_k.data_ptr(), cache_v.data_ptr(), npages,
+          page, page_stride, row_stride, B, pages.data_ptr(), row, most, counts.data_ptr(), *(t.data_ptr() for t in new),
+          work.data_ptr(), wbytes)
+    increment_version((cache_k, cache_v))
+    return new
 
 
 def _token_stride(x):
@@ -375,4 +561,5 @@ def axial_rotary(x, pairs, nheads: int, *, base: float = 10000.0, positions: tor
     return _turn(x, 0, *meta, positions)
 
 
-__all__ = ["axial_rotary", "paged_append_", "paged_mh_attention", "sliding_mh_attention"]
+__all__ = ["axial_rotary", "paged_append_", "paged_compact_", "paged_fork", "paged_mh_attention", "paged_resize_",
+           "sliding_mh_attention"]

@@ -764,14 +764,40 @@ int check_rests(const void *rest, const void *y, int64_t bytes, int dtype) {
 
 }  // namespace
 
-int circatt_sliding_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
-                        int64_t sinks, float scale, const void *q, int64_t q_row, int64_t q_batch, const void *k,
-                        int64_t k_row, int64_t k_batch, const void *v, int64_t v_row, int64_t v_batch,
-                        const int32_t *lengths, void *y, void *y_rest, float *lse, void *stream) {
-    SlidingProblem pr;
-    CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
-    if (L == 0 || B == 0) return ok();
-    CIRCATT_TRY(check_threads(sliding_threads(pr, lse != nullptr)));  // lse: a backward will follow
+namespace {
+
+// What scores are shaped by, for signals of up to `tokens` tokens.
+int check_shape(float scale, float cap, const float *slopes, const int32_t *prefix, const int32_t *places, int64_t places_row,
+                int64_t tokens, ScoreShape &sh) {
+    // the kernels form scale / cap and multiples of it and of the cap in Float32
+    if (!(cap >= 0.f) || !(cap <= 1e30f) || (cap > 0.f && (!(scale / cap >= 1e-30f) || !(scale / cap <= 1e30f))))
+        return fail(CIRCATT_ERR_INVALID, "cap=%g must be 0 or positive, and scale / cap within 1e-30 .. 1e30", (double)cap);
+    if (prefix != nullptr && places != nullptr)
+        return fail(CIRCATT_ERR_INVALID, "prefix and places do not go together");
+    if (places != nullptr && places_row < 0) return fail(CIRCATT_ERR_INVALID, "negative stride");
+    if (slopes != nullptr && tokens > (int64_t)1 << 24)
+        return fail(CIRCATT_ERR_UNSUPPORTED, "slopes for %lld tokens, at most 2^24 are supported", (long long)tokens);
+    sh.cap = cap;
+    sh.slopes = slopes;
+    sh.prefix = prefix;
+    sh.places = places;
+    sh.places_row = places_row;
+    return CIRCATT_OK;
+}
+
+// Arrays of a call's shape, which its results must not overlap.
+struct ShapeSpans {
+    Span slopes{"slopes", nullptr, 0}, prefix{"prefix", nullptr, 0}, places{"places", nullptr, 0};
+    ShapeSpans() = default;
+    ShapeSpans(const ScoreShape &sh, int64_t B, int64_t L, int64_t H)
+        : slopes{"slopes", sh.slopes, 4 * H}, prefix{"prefix", sh.prefix, 4 * B},
+          places{"places", sh.places, 4 * ((B - 1) * sh.places_row + L)} {}
+};
+
+int sliding_fwd_arguments(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, const void *q,
+                          int64_t q_row, int64_t q_batch, const void *k, int64_t k_row, int64_t k_batch, const void *v,
+                          int64_t v_row, int64_t v_batch, const int32_t *lengths, void *y, void *y_rest, float *lse,
+                          const ShapeSpans &sh, SlidingProblem &pr) {
     const int es = esize_of(dtype);
     CIRCATT_TRY(check_rows("q", q, q_row, q_batch, nheads * dh, es));
     CIRCATT_TRY(check_rows("k", k, k_row, k_batch, kv_heads * dh, es));
@@ -786,10 +812,67 @@ int circatt_sliding_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t
     pr.y_rest = y_rest;
     pr.lse = lse;
     const int64_t C = nheads * dh, Ck = kv_heads * dh;
-    CIRCATT_TRY(check_apart({span("y", y, B, L * C, L, C, C, es), span("y_rest", y_rest, B, L * C, L, C, C, es),
-                             span("lse", lse, 1, 0, 1, 0, B * L * nheads, 4)},
-                            {span("q", q, B, q_batch, L, q_row, C, es), span("k", k, B, k_batch, L, k_row, Ck, es),
-                             span("v", v, B, v_batch, L, v_row, Ck, es)}));
+    return check_apart({span("y", y, B, L * C, L, C, C, es), span("y_rest", y_rest, B, L * C, L, C, C, es),
+                        span("lse", lse, 1, 0, 1, 0, B * L * nheads, 4)},
+                       {span("q", q, B, q_batch, L, q_row, C, es), span("k", k, B, k_batch, L, k_row, Ck, es),
+                        span("v", v, B, v_batch, L, v_row, Ck, es), sh.slopes, sh.prefix, sh.places});
+}
+
+int sliding_bwd_arguments(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, const void *q,
+                          int64_t q_row, int64_t q_batch, const void *k, int64_t k_row, int64_t k_batch, const void *v,
+                          int64_t v_row, int64_t v_batch, const int32_t *lengths, const void *y, const void *y_rest,
+                          const float *lse, const void *dy, int64_t dy_row, int64_t dy_batch, void *dq, void *dk, void *dv,
+                          void *workspace, int64_t workspace_bytes, int64_t need, const ShapeSpans &sh, SlidingProblem &pr) {
+    const int es = esize_of(dtype);
+    CIRCATT_TRY(check_rows("q", q, q_row, q_batch, nheads * dh, es));
+    CIRCATT_TRY(check_rows("k", k, k_row, k_batch, kv_heads * dh, es));
+    CIRCATT_TRY(check_rows("v", v, v_row, v_batch, kv_heads * dh, es));
+    CIRCATT_TRY(check_rows("y", y, nheads * dh, 0, nheads * dh, es));
+    CIRCATT_TRY(check_rows("dy", dy, dy_row, dy_batch, nheads * dh, es));
+    CIRCATT_TRY(check_rows("dq", dq, nheads * dh, 0, nheads * dh, es));
+    CIRCATT_NONNULL(lse);
+    if ((dk == nullptr) != (dv == nullptr)) return fail(CIRCATT_ERR_INVALID, "dk and dv go together");
+    if (dk != nullptr) {
+        CIRCATT_TRY(check_rows("dk", dk, kv_heads * dh, 0, kv_heads * dh, es));
+        CIRCATT_TRY(check_rows("dv", dv, kv_heads * dh, 0, kv_heads * dh, es));
+    }
+    CIRCATT_NONNULL(workspace);
+    if (workspace_bytes < need)
+        return fail(CIRCATT_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(CIRCATT_ERR_INVALID, "workspace must be 16-byte aligned");
+    pr.q = q, pr.q_row = q_row, pr.q_batch = q_batch;
+    pr.k = k, pr.k_row = k_row, pr.k_batch = k_batch;
+    pr.v = v, pr.v_row = v_row, pr.v_batch = v_batch;
+    pr.lengths = lengths;
+    if (y_rest != nullptr) CIRCATT_TRY(check_rests(y_rest, y, L * B * nheads * dh * es, dtype));
+    pr.y = const_cast<void *>(y);
+    pr.y_rest = const_cast<void *>(y_rest);
+    pr.lse = const_cast<float *>(lse);
+    pr.dy = dy, pr.dy_row = dy_row, pr.dy_batch = dy_batch;
+    pr.dq = dq, pr.dk = dk, pr.dv = dv;
+    pr.work = static_cast<float *>(workspace);
+    const int64_t C = nheads * dh, Ck = kv_heads * dh;
+    return check_apart(
+        {span("dq", dq, B, L * C, L, C, C, es), span("dk", dk, B, L * Ck, L, Ck, Ck, es),
+         span("dv", dv, B, L * Ck, L, Ck, Ck, es), span("workspace", workspace, 1, 0, 1, 0, need, 1)},
+        {span("q", q, B, q_batch, L, q_row, C, es), span("k", k, B, k_batch, L, k_row, Ck, es),
+         span("v", v, B, v_batch, L, v_row, Ck, es), span("y", y, B, L * C, L, C, C, es),
+         span("y_rest", y_rest, B, L * C, L, C, C, es), span("lse", lse, 1, 0, 1, 0, B * L * nheads, 4),
+         span("dy", dy, B, dy_batch, L, dy_row, C, es), sh.slopes, sh.prefix, sh.places});
+}
+
+}  // namespace
+
+int circatt_sliding_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
+                        int64_t sinks, float scale, const void *q, int64_t q_row, int64_t q_batch, const void *k,
+                        int64_t k_row, int64_t k_batch, const void *v, int64_t v_row, int64_t v_batch,
+                        const int32_t *lengths, void *y, void *y_rest, float *lse, void *stream) {
+    SlidingProblem pr;
+    CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
+    if (L == 0 || B == 0) return ok();
+    CIRCATT_TRY(check_threads(sliding_threads(pr, lse != nullptr)));  // lse: a backward will follow
+    CIRCATT_TRY(sliding_fwd_arguments(dtype, L, B, nheads, kv_heads, dh, q, q_row, q_batch, k, k_row, k_batch, v, v_row,
+                                      v_batch, lengths, y, y_rest, lse, ShapeSpans(), pr));
     return hip_result(launch_sliding_fwd(pr, as_stream(stream)), "circatt_sliding_fwd");
 }
 
@@ -811,44 +894,55 @@ int circatt_sliding_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t
     CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
     if (L == 0 || B == 0) return ok();
     CIRCATT_TRY(check_threads(sliding_threads(pr, true)));
-    const int es = esize_of(dtype);
-    CIRCATT_TRY(check_rows("q", q, q_row, q_batch, nheads * dh, es));
-    CIRCATT_TRY(check_rows("k", k, k_row, k_batch, kv_heads * dh, es));
-    CIRCATT_TRY(check_rows("v", v, v_row, v_batch, kv_heads * dh, es));
-    CIRCATT_TRY(check_rows("y", y, nheads * dh, 0, nheads * dh, es));
-    CIRCATT_TRY(check_rows("dy", dy, dy_row, dy_batch, nheads * dh, es));
-    CIRCATT_TRY(check_rows("dq", dq, nheads * dh, 0, nheads * dh, es));
-    CIRCATT_NONNULL(lse);
-    if ((dk == nullptr) != (dv == nullptr)) return fail(CIRCATT_ERR_INVALID, "dk and dv go together");
-    if (dk != nullptr) {
-        CIRCATT_TRY(check_rows("dk", dk, kv_heads * dh, 0, kv_heads * dh, es));
-        CIRCATT_TRY(check_rows("dv", dv, kv_heads * dh, 0, kv_heads * dh, es));
-    }
-    CIRCATT_NONNULL(workspace);
-    const int64_t need = 4 * sliding_bwd_workspace_floats(pr);
-    if (workspace_bytes < need)
-        return fail(CIRCATT_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
-    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(CIRCATT_ERR_INVALID, "workspace must be 16-byte aligned");
-    pr.q = q, pr.q_row = q_row, pr.q_batch = q_batch;
-    pr.k = k, pr.k_row = k_row, pr.k_batch = k_batch;
-    pr.v = v, pr.v_row = v_row, pr.v_batch = v_batch;
-    pr.lengths = lengths;
-    if (y_rest != nullptr) CIRCATT_TRY(check_rests(y_rest, y, L * B * nheads * dh * es, dtype));
-    pr.y = const_cast<void *>(y);
-    pr.y_rest = const_cast<void *>(y_rest);
-    pr.lse = const_cast<float *>(lse);
-    pr.dy = dy, pr.dy_row = dy_row, pr.dy_batch = dy_batch;
-    pr.dq = dq, pr.dk = dk, pr.dv = dv;
-    pr.work = static_cast<float *>(workspace);
-    const int64_t C = nheads * dh, Ck = kv_heads * dh;
-    CIRCATT_TRY(check_apart(
-        {span("dq", dq, B, L * C, L, C, C, es), span("dk", dk, B, L * Ck, L, Ck, Ck, es),
-         span("dv", dv, B, L * Ck, L, Ck, Ck, es), span("workspace", workspace, 1, 0, 1, 0, need, 1)},
-        {span("q", q, B, q_batch, L, q_row, C, es), span("k", k, B, k_batch, L, k_row, Ck, es),
-         span("v", v, B, v_batch, L, v_row, Ck, es), span("y", y, B, L * C, L, C, C, es),
-         span("y_rest", y_rest, B, L * C, L, C, C, es), span("lse", lse, 1, 0, 1, 0, B * L * nheads, 4),
-         span("dy", dy, B, dy_batch, L, dy_row, C, es)}));
+    CIRCATT_TRY(sliding_bwd_arguments(dtype, L, B, nheads, kv_heads, dh, q, q_row, q_batch, k, k_row, k_batch, v, v_row,
+                                      v_batch, lengths, y, y_rest, lse, dy, dy_row, dy_batch, dq, dk, dv, workspace,
+                                      workspace_bytes, 4 * sliding_bwd_workspace_floats(pr), ShapeSpans(), pr));
     return hip_result(launch_sliding_bwd(pr, as_stream(stream)), "circatt_sliding_bwd");
+}
+
+int circatt_shaped_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
+                       int64_t sinks, float scale, float cap, const float *slopes, const int32_t *prefix,
+                       const int32_t *places, int64_t places_row, const void *q, int64_t q_row, int64_t q_batch,
+                       const void *k, int64_t k_row, int64_t k_batch, const void *v, int64_t v_row, int64_t v_batch,
+                       const int32_t *lengths, void *y, void *y_rest, float *lse, void *stream) {
+    ShapedSlidingProblem pr{};
+    CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
+    CIRCATT_TRY(check_shape(scale, cap, slopes, prefix, places, places_row, L, pr.shape));
+    if (L == 0 || B == 0) return ok();
+    CIRCATT_TRY(check_threads(shaped_sliding_threads(pr, prefix != nullptr || places != nullptr, lse != nullptr)));
+    CIRCATT_TRY(sliding_fwd_arguments(dtype, L, B, nheads, kv_heads, dh, q, q_row, q_batch, k, k_row, k_batch, v, v_row,
+                                      v_batch, lengths, y, y_rest, lse, ShapeSpans(pr.shape, B, L, nheads), pr));
+    return hip_result(launch_shaped_fwd(pr, as_stream(stream)), "circatt_shaped_fwd");
+}
+
+int64_t circatt_shaped_bwd_workspace_bytes(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
+                                           int64_t window, int64_t sinks, int biased, int masked) {
+    SlidingProblem pr;
+    if (sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, 1.f, pr) != CIRCATT_OK) return -1;
+    if (L == 0 || B == 0) return 0;
+    return check_threads(shaped_sliding_threads(pr, masked != 0, true)) == CIRCATT_OK
+               ? 4 * shaped_bwd_workspace_floats(pr, biased != 0, masked != 0)
+               : -1;
+}
+
+int circatt_shaped_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
+                       int64_t sinks, float scale, float cap, const float *slopes, const int32_t *prefix,
+                       const int32_t *places, int64_t places_row, const void *q, int64_t q_row, int64_t q_batch,
+                       const void *k, int64_t k_row, int64_t k_batch, const void *v, int64_t v_row, int64_t v_batch,
+                       const int32_t *lengths, const void *y, const void *y_rest, const float *lse, const void *dy,
+                       int64_t dy_row, int64_t dy_batch, void *dq, void *dk, void *dv, void *workspace,
+                       int64_t workspace_bytes, void *stream) {
+    ShapedSlidingProblem pr{};
+    CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
+    CIRCATT_TRY(check_shape(scale, cap, slopes, prefix, places, places_row, L, pr.shape));
+    if (L == 0 || B == 0) return ok();
+    const bool masked = prefix != nullptr || places != nullptr;
+    CIRCATT_TRY(check_threads(shaped_sliding_threads(pr, masked, true)));
+    CIRCATT_TRY(sliding_bwd_arguments(dtype, L, B, nheads, kv_heads, dh, q, q_row, q_batch, k, k_row, k_batch, v, v_row,
+                                      v_batch, lengths, y, y_rest, lse, dy, dy_row, dy_batch, dq, dk, dv, workspace,
+                                      workspace_bytes, 4 * shaped_bwd_workspace_floats(pr, slopes != nullptr, masked),
+                                      ShapeSpans(pr.shape, B, L, nheads), pr));
+    return hip_result(launch_shaped_bwd(pr, as_stream(stream)), "circatt_shaped_bwd");
 }
 
 int64_t circatt_paged_workspace_bytes(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
@@ -859,13 +953,14 @@ int64_t circatt_paged_workspace_bytes(int dtype, int64_t T, int64_t B, int64_t n
     return T == 0 ? 0 : 4 * paged_workspace_floats(pr);
 }
 
-int circatt_paged_attention(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
-                            int64_t window, int64_t sinks, float scale, const void *q, int64_t q_row,
-                            const void *cache_k, const void *cache_v, int64_t npages, int64_t page_size,
-                            int64_t page_stride, int64_t row_stride, const int32_t *pages, int64_t pages_row,
-                            int64_t max_pages, const int32_t *lengths, const int32_t *offsets, void *y, int zero_tail,
-                            void *workspace, int64_t workspace_bytes, void *stream) {
-    PagedProblem pr;
+namespace {
+
+// Everything of a call over a paged cache but the kinds of its scores and the launch; done: nothing to launch.
+int paged_arguments(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
+                    int64_t sinks, float scale, const void *q, int64_t q_row, const void *cache_k, const void *cache_v,
+                    int64_t npages, int64_t page_size, int64_t page_stride, int64_t row_stride, const int32_t *pages,
+                    int64_t pages_row, int64_t max_pages, const int32_t *lengths, const int32_t *offsets, void *y,
+                    int zero_tail, void *workspace, int64_t workspace_bytes, PagedProblem &pr) {
     CIRCATT_TRY(paged_problem(dtype, T, B, nheads, kv_heads, dh, window, sinks, scale, page_size, max_pages, pr));
     const int es = esize_of(dtype);
     CIRCATT_TRY(paged_table(B, npages, page_size, page_stride, row_stride, kv_heads * dh, pages, pages_row, max_pages,
@@ -873,7 +968,7 @@ int circatt_paged_attention(int dtype, int64_t T, int64_t B, int64_t nheads, int
     if (offsets == nullptr && T != B)
         return fail(CIRCATT_ERR_INVALID, "without offsets q has one row for each sequence: %lld rows, %lld sequences",
                     (long long)T, (long long)B);
-    if (T == 0) return ok();
+    if (T == 0) return CIRCATT_OK;
     CIRCATT_TRY(check_rows("q", q, q_row, 0, nheads * dh, es));
     CIRCATT_TRY(check_rows("y", y, nheads * dh, 0, nheads * dh, es));
     const int64_t need = 4 * paged_workspace_floats(pr);
@@ -900,7 +995,40 @@ int circatt_paged_attention(int dtype, int64_t T, int64_t B, int64_t nheads, int
     pr.y = y;
     pr.zero_tail = zero_tail != 0;
     pr.work = static_cast<float *>(workspace);
+    return CIRCATT_OK;
+}
+
+}  // namespace
+
+int circatt_paged_attention(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
+                            int64_t window, int64_t sinks, float scale, const void *q, int64_t q_row,
+                            const void *cache_k, const void *cache_v, int64_t npages, int64_t page_size,
+                            int64_t page_stride, int64_t row_stride, const int32_t *pages, int64_t pages_row,
+                            int64_t max_pages, const int32_t *lengths, const int32_t *offsets, void *y, int zero_tail,
+                            void *workspace, int64_t workspace_bytes, void *stream) {
+    PagedProblem pr;
+    CIRCATT_TRY(paged_arguments(dtype, T, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, cache_k, cache_v, npages,
+                                page_size, page_stride, row_stride, pages, pages_row, max_pages, lengths, offsets, y,
+                                zero_tail, workspace, workspace_bytes, pr));
+    if (T == 0) return ok();
     return hip_result(launch_paged(pr, as_stream(stream)), "circatt_paged_attention");
+}
+
+int circatt_shaped_paged(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh, int64_t window,
+                         int64_t sinks, float scale, float cap, const float *slopes, const int32_t *prefix, const void *q,
+                         int64_t q_row, const void *cache_k, const void *cache_v, int64_t npages, int64_t page_size,
+                         int64_t page_stride, int64_t row_stride, const int32_t *pages, int64_t pages_row,
+                         int64_t max_pages, const int32_t *lengths, const int32_t *offsets, void *y, int zero_tail,
+                         void *workspace, int64_t workspace_bytes, void *stream) {
+    ShapedPagedProblem pr{};
+    CIRCATT_TRY(paged_arguments(dtype, T, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, cache_k, cache_v, npages,
+                                page_size, page_stride, row_stride, pages, pages_row, max_pages, lengths, offsets, y,
+                                zero_tail, workspace, workspace_bytes, pr));
+    CIRCATT_TRY(check_shape(scale, cap, slopes, prefix, nullptr, 0, max_pages * page_size, pr.shape));
+    if (T == 0) return ok();
+    const ShapeSpans sh(pr.shape, B, 0, nheads);
+    CIRCATT_TRY(check_apart({span("y", y, 1, 0, T, nheads * dh, nheads * dh, esize_of(dtype))}, {sh.slopes, sh.prefix}));
+    return hip_result(launch_shaped_paged(pr, as_stream(stream)), "circatt_shaped_paged");
 }
 
 int circatt_paged_append(int dtype, int64_t T, int64_t B, int64_t channels, const void *k, int64_t k_row, const void *v,
@@ -932,6 +1060,140 @@ int circatt_paged_append(int dtype, int64_t T, int64_t B, int64_t channels, cons
     pr.lengths = lengths, pr.offsets = offsets;
     CIRCATT_TRY(check_threads(append_threads(pr)));
     return hip_result(launch_append(pr, as_stream(stream)), "circatt_paged_append");
+}
+
+namespace {
+
+// The sequences of a cache and what they hold; outputs are contiguous and apart from
+// everything that is read.
+int page_table(int64_t B, int64_t maxp, int64_t npages, int64_t page_size, const int32_t *pages, int64_t pages_row,
+               PageTable &pr) {
+    if (B < 1 || B > 65535) return fail(CIRCATT_ERR_INVALID, "invalid sequence count %lld", (long long)B);
+    if (page_size < 1 || page_size > 65536 || (page_size & (page_size - 1)) != 0)
+        return fail(CIRCATT_ERR_UNSUPPORTED, "page size %lld must be a power of two up to 65536", (long long)page_size);
+    if (npages < 1 || npages > INT32_MAX / page_size)
+        return fail(CIRCATT_ERR_INVALID, "a cache of %lld pages of %lld tokens", (long long)npages, (long long)page_size);
+    for (pr.page_log2 = 0; (1 << pr.page_log2) < page_size;) ++pr.page_log2;
+    if (maxp < 1 || pages_row < maxp || maxp > (int64_t)1 << (30 - pr.page_log2))
+        return fail(CIRCATT_ERR_INVALID, "a page table of %lld pages, rows of %lld", (long long)maxp, (long long)pages_row);
+    CIRCATT_NONNULL(pages);
+    pr.B = (int)B;
+    pr.maxp = (int)maxp;
+    pr.npages = (int)npages;
+    pr.pages = pages, pr.pages_row = pages_row;
+    return CIRCATT_OK;
+}
+Span ints(const char *name, const void *p, int64_t n) { return Span{name, p, 4 * n}; }
+
+int page_shape(int dtype, int64_t channels, int64_t B, int64_t npages, int64_t page_size, int64_t page_stride,
+               int64_t row_stride, const int32_t *pages, int64_t pages_row, int64_t maxp, const int32_t *lengths,
+               void *cache_k, void *cache_v, PageShape &sh) {
+    CIRCATT_TRY(check_token_dtype(dtype));
+    if (channels < 1 || channels > 1 << 24) return fail(CIRCATT_ERR_INVALID, "invalid channel count %lld", (long long)channels);
+    int log2;
+    CIRCATT_TRY(paged_table(B, npages, page_size, page_stride, row_stride, channels, pages, pages_row, maxp, lengths,
+                            cache_k, cache_v, esize_of(dtype), log2));
+    if (page_size * channels > INT32_MAX)
+        return fail(CIRCATT_ERR_UNSUPPORTED, "a page of %lld values", (long long)(page_size * channels));
+    // tokens move: rows that lie in one another would be written twice
+    if ((page_size > 1 && row_stride < channels) || (npages > 1 && page_stride < (page_size - 1) * row_stride + channels))
+        return fail(CIRCATT_ERR_INVALID, "the cache's pages must not overlap");
+    sh.esize = esize_of(dtype);
+    sh.C = channels;
+    sh.cache_k = cache_k, sh.cache_v = cache_v;
+    sh.page_stride = page_stride, sh.row_stride = row_stride;
+    return CIRCATT_OK;
+}
+int check_page_workspace(const void *workspace, int64_t bytes, int64_t need) {
+    CIRCATT_NONNULL(workspace);
+    if (bytes < need)
+        return fail(CIRCATT_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)bytes, (long long)need);
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(CIRCATT_ERR_INVALID, "workspace must be 16-byte aligned");
+    return CIRCATT_OK;
+}
+
+}  // namespace
+
+int circatt_paged_fork(int64_t B, int64_t npages, int64_t page_size, const int32_t *pages, int64_t pages_row,
+                       int64_t max_pages, const int32_t *lengths, const int32_t *counts, int64_t N, const int32_t *source,
+                       int32_t *out_pages, int32_t *out_lengths, int32_t *out_counts, void *stream) {
+    ForkProblem pr{};
+    CIRCATT_TRY(page_table(B, max_pages, npages, page_size, pages, pages_row, pr));
+    if (N < 0 || N > 65535) return fail(CIRCATT_ERR_INVALID, "invalid sequence count %lld", (long long)N);
+    CIRCATT_NONNULL(lengths);
+    CIRCATT_NONNULL(counts);
+    CIRCATT_NONNULL(out_counts);
+    if (N > 0) {
+        CIRCATT_NONNULL(source);
+        CIRCATT_NONNULL(out_pages);
+        CIRCATT_NONNULL(out_lengths);
+    }
+    CIRCATT_TRY(check_apart({ints("out_pages", out_pages, N * max_pages), ints("out_lengths", out_lengths, N),
+                             ints("out_counts", out_counts, npages)},
+                            {ints("pages", pages, (B - 1) * pages_row + max_pages), ints("lengths", lengths, B),
+                             ints("counts", counts, npages), ints("source", source, N)}));
+    pr.lengths = lengths, pr.counts = counts;
+    pr.N = (int)N;
+    pr.source = source;
+    pr.out_pages = out_pages, pr.out_lengths = out_lengths, pr.out_counts = out_counts;
+    return hip_result(launch_fork(pr, as_stream(stream)), "circatt_paged_fork");
+}
+
+int64_t circatt_paged_resize_workspace_bytes(int64_t B, int64_t npages) {
+    if (B < 1 || B > 65535 || npages < 1 || npages > INT32_MAX) return -1;
+    return 4 * resize_workspace_ints(B, npages);
+}
+
+int circatt_paged_resize(int dtype, int64_t channels, void *cache_k, void *cache_v, int64_t npages, int64_t page_size,
+                         int64_t page_stride, int64_t row_stride, int64_t B, const int32_t *pages, int64_t pages_row,
+                         int64_t max_pages, const int32_t *lengths, const int32_t *counts, const int32_t *to,
+                         int32_t *out_pages, int32_t *out_lengths, int32_t *out_counts, void *workspace,
+                         int64_t workspace_bytes, void *stream) {
+    ResizeProblem pr{};
+    CIRCATT_TRY(page_table(B, max_pages, npages, page_size, pages, pages_row, pr));
+    CIRCATT_NONNULL(lengths);
+    CIRCATT_TRY(page_shape(dtype, channels, B, npages, page_size, page_stride, row_stride, pages, pages_row, max_pages,
+                           lengths, cache_k, cache_v, pr.shape));
+    CIRCATT_NONNULL(counts);
+    CIRCATT_NONNULL(to);
+    CIRCATT_NONNULL(out_pages);
+    CIRCATT_NONNULL(out_lengths);
+    CIRCATT_NONNULL(out_counts);
+    const int64_t need = 4 * resize_workspace_ints(B, npages);
+    CIRCATT_TRY(check_page_workspace(workspace, workspace_bytes, need));
+    CIRCATT_TRY(check_apart({ints("out_pages", out_pages, B * max_pages), ints("out_lengths", out_lengths, B),
+                             ints("out_counts", out_counts, npages), Span{"workspace", workspace, need}},
+                            {ints("pages", pages, (B - 1) * pages_row + max_pages), ints("lengths", lengths, B),
+                             ints("counts", counts, npages), ints("to", to, B)}));
+    pr.lengths = lengths, pr.counts = counts;
+    pr.to = to;
+    pr.out_pages = out_pages, pr.out_lengths = out_lengths, pr.out_counts = out_counts;
+    return hip_result(launch_resize(pr, static_cast<int32_t *>(workspace), as_stream(stream)), "circatt_paged_resize");
+}
+
+int64_t circatt_paged_compact_workspace_bytes(int64_t npages) {
+    return npages < 1 || npages > INT32_MAX ? -1 : 4 * compact_workspace_ints(npages);
+}
+
+int circatt_paged_compact(int dtype, int64_t channels, void *cache_k, void *cache_v, int64_t npages, int64_t page_size,
+                          int64_t page_stride, int64_t row_stride, int64_t B, const int32_t *pages, int64_t pages_row,
+                          int64_t max_pages, const int32_t *counts, int32_t *out_pages, int32_t *out_counts,
+                          void *workspace, int64_t workspace_bytes, void *stream) {
+    CompactProblem pr{};
+    CIRCATT_TRY(page_table(B, max_pages, npages, page_size, pages, pages_row, pr));
+    CIRCATT_TRY(page_shape(dtype, channels, B, npages, page_size, page_stride, row_stride, pages, pages_row, max_pages,
+                           pages, cache_k, cache_v, pr.shape));
+    CIRCATT_NONNULL(counts);
+    CIRCATT_NONNULL(out_pages);
+    CIRCATT_NONNULL(out_counts);
+    const int64_t need = 4 * compact_workspace_ints(npages);
+    CIRCATT_TRY(check_page_workspace(workspace, workspace_bytes, need));
+    CIRCATT_TRY(check_apart({ints("out_pages", out_pages, B * max_pages), ints("out_counts", out_counts, npages),
+                             Span{"workspace", workspace, need}},
+                            {ints("pages", pages, (B - 1) * pages_row + max_pages), ints("counts", counts, npages)}));
+    pr.counts = counts;
+    pr.out_pages = out_pages, pr.out_counts = out_counts;
+    return hip_result(launch_compact(pr, static_cast<int32_t *>(workspace), as_stream(stream)), "circatt_paged_compact");
 }
 
 int circatt_axial_rotary(int dtype, int inverse, int interleaved, int naxes, int64_t n1, int64_t n2, int64_t n3,

@@ -1,0 +1,75 @@
+// Token attention whose scores are biased by distance, or masked by documents or a
+// prefix (sliding_impl.h); those that are capped as well are capped.hip's.
+#include "sliding_impl.h"
+
+namespace circatt {
+
+hipError_t launch_capped_fwd(const ShapedSlidingProblem &pr, hipStream_t s);
+hipError_t launch_capped_bwd(const ShapedSlidingProblem &pr, hipStream_t s);
+
+namespace {
+
+// What the keys' pass reads of every packed row and token: slopes times log2(e) and
+// tokens as Float32 (exact up to 2^24 of them), and where a token's document ends: at
+// the first later token whose own begins behind it.  (Starts ascend; whatever the
+// places hold, an end lies behind its token and not behind the signal.)
+__global__ __launch_bounds__(256) void shape_rows(ShapedSlidingProblem pr) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t rows = (int64_t)pr.L * pr.G;
+    if (pr.shape.slopes != nullptr) {
+        if (i < rows) pr.row_tokens[i] = (float)(int)(i / pr.G);
+        if (i < rows * pr.Hk) pr.row_slopes[i] = pr.shape.slopes[(int)(i / rows) * pr.G + (int)(i % pr.G)] * kLog2e;
+    }
+    if (pr.shape.places != nullptr && i < (int64_t)pr.B * pr.L) {
+        const int b = (int)(i / pr.L), j = (int)(i - (int64_t)b * pr.L);
+        const int32_t *places = pr.shape.places + b * pr.shape.places_row;
+        int lo = j + 1, hi = pr.L;  // the first t of (j, L) that begins behind j
+        while (lo < hi) {
+            const int t = (lo + hi) >> 1;
+            if (document_start(places, t) > j) hi = t;
+            else lo = t + 1;
+        }
+        pr.ends[i] = lo;
+    }
+}
+
+struct ShapedRegions {
+    int64_t slopes, tokens, ends, floats;
+    ShapedRegions(const SlidingProblem &pr, const WalkSplit &sp, bool biased, bool documents) {
+        auto up = [](int64_t n) { return (n + 3) & ~(int64_t)3; };
+        const int64_t rows = (int64_t)pr.L * pr.G;
+        slopes = up(bwd_floats(pr, sp));
+        tokens = slopes + (biased ? up(rows * pr.Hk) : 0);
+        ends = tokens + (biased ? up(rows) : 0);
+        floats = ends + (documents ? up((int64_t)pr.B * pr.L) : 0);
+    }
+};
+
+}  // namespace
+
+// (masked: room for the documents' ends, with a prefix as well)
+int64_t shaped_bwd_workspace_floats(const SlidingProblem &pr, bool biased, bool masked) {
+    return ShapedRegions(pr, walk_split(pr, masked), biased, masked).floats;
+}
+int64_t shaped_sliding_threads(const SlidingProblem &pr, bool masked, bool backward) {
+    const int64_t n = threads_of(pr, walk_split(pr, masked), backward), rows = (int64_t)pr.L * pr.H + 256;
+    return n > rows ? n : rows;
+}
+hipError_t launch_shaped_fwd(const ShapedSlidingProblem &pr, hipStream_t s) {
+    return pr.shape.cap > 0.f ? launch_capped_fwd(pr, s) : forward_of<Shaped<false>>(pr, s);
+}
+hipError_t launch_shaped_bwd(ShapedSlidingProblem pr, hipStream_t s) {
+    const bool biased = pr.shape.slopes != nullptr, masked = pr.shape.places != nullptr || pr.shape.prefix != nullptr;
+    const WalkSplit sp = walk_split(pr, masked);
+    const ShapedRegions at(pr, sp, biased, masked);
+    pr.row_slopes = pr.work + at.slopes;
+    pr.row_tokens = pr.work + at.tokens;
+    pr.ends = reinterpret_cast<int32_t *>(pr.work + at.ends);
+    if (pr.dk != nullptr && (biased || pr.shape.places != nullptr)) {
+        const int64_t rows = (int64_t)pr.L * pr.H, tokens = (int64_t)pr.B * pr.L, n = rows > tokens ? rows : tokens;
+        shape_rows<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(pr);
+    }
+    return pr.shape.cap > 0.f ? launch_capped_bwd(pr, s) : backward_of<Shaped<false>>(pr, sp, s);
+}
+
+}  // namespace circatt

@@ -29,12 +29,34 @@ struct SlidingProblem {
     void *dq, *dk, *dv;  // contiguous; dk and dv may be NULL (both)
     float *work;         // rowsum(dy * y), laid out as lse, then partial sums
 };
+// How scores follow from products, and what else a row sees (or does not).
+struct ScoreShape {
+    float cap;               // 0: none
+    const float *slopes;     // (H) or NULL
+    const int32_t *prefix;   // (B) or NULL: tokens that all rows see
+    const int32_t *places;   // each token's place in its document, or NULL
+    int64_t places_row;      // from signal to signal
+};
+struct ShapedSlidingProblem : SlidingProblem {
+    ScoreShape shape;
+    // of the backward, in its workspace: slope times log2(e), and token, of every
+    // packed row of a head of keys ((Hk, L*G) and (L*G); with slopes), and the end of
+    // every token's document ((B, L); with places)
+    float *row_slopes, *row_tokens;
+    int32_t *ends;
+};
 int64_t sliding_bwd_workspace_floats(const SlidingProblem &pr);
 // Threads of the largest launch of the forward, or of the backward: a launch holds
 // less than 2^32 along an axis.
 int64_t sliding_threads(const SlidingProblem &pr, bool backward);
 hipError_t launch_sliding_fwd(const SlidingProblem &pr, hipStream_t s);
 hipError_t launch_sliding_bwd(const SlidingProblem &pr, hipStream_t s);
+// The same with shaped scores.  biased, masked: whether slopes, and places or a
+// prefix, are there (the workspace is asked for without them).
+int64_t shaped_bwd_workspace_floats(const SlidingProblem &pr, bool biased, bool masked);
+int64_t shaped_sliding_threads(const SlidingProblem &pr, bool masked, bool backward);
+hipError_t launch_shaped_fwd(const ShapedSlidingProblem &pr, hipStream_t s);
+hipError_t launch_shaped_bwd(ShapedSlidingProblem pr, hipStream_t s);
 
 // The T rows of q are the new tokens of B sequences in order: sequence b has
 // rows offsets[b] .. offsets[b+1] (offsets NULL: row b alone), the last tokens
@@ -57,9 +79,13 @@ struct PagedProblem {
     int zero_tail;  // rows behind the last sequence: 1 zeros, 0 left alone
     float *work;
 };
+struct ShapedPagedProblem : PagedProblem {
+    ScoreShape shape;  // without places
+};
 int64_t paged_workspace_floats(const PagedProblem &pr);
 int64_t paged_threads(const PagedProblem &pr);  // along the longest axis
 hipError_t launch_paged(const PagedProblem &pr, hipStream_t s);
+hipError_t launch_shaped_paged(const ShapedPagedProblem &pr, hipStream_t s);
 
 struct AppendProblem {
     int esize;  // bytes of an element
@@ -78,6 +104,43 @@ struct AppendProblem {
 };
 int64_t append_threads(const AppendProblem &pr);
 hipError_t launch_append(const AppendProblem &pr, hipStream_t s);
+
+// Sequences of a cache and the pages that they hold: row b of pages (pages_row apart)
+// has a page for every 1 << page_log2 of sequence b's tokens, counts the holders of
+// every page.
+struct PageTable {
+    int B, maxp, npages, page_log2;
+    const int32_t *pages;
+    int64_t pages_row;
+    const int32_t *lengths, *counts;
+    int32_t *out_pages, *out_lengths, *out_counts;  // rows of maxp
+};
+struct ForkProblem : PageTable {
+    int N;  // sequences after the fork
+    const int32_t *source;
+};
+hipError_t launch_fork(const ForkProblem &pr, hipStream_t s);
+
+struct PageShape {
+    int esize;
+    int64_t C;  // channels of a token
+    void *cache_k, *cache_v;
+    int64_t page_stride, row_stride;
+};
+struct ResizeProblem : PageTable {
+    PageShape shape;
+    const int32_t *to;
+    int32_t *ranks, *needs, *free_list;
+};
+int64_t resize_workspace_ints(int64_t B, int64_t npages);
+hipError_t launch_resize(ResizeProblem pr, int32_t *work, hipStream_t s);
+
+struct CompactProblem : PageTable {
+    PageShape shape;
+    int32_t *sizes, *holes, *movers, *rank;
+};
+int64_t compact_workspace_ints(int64_t npages);
+hipError_t launch_compact(CompactProblem pr, int32_t *work, hipStream_t s);
 
 constexpr int kMaxPairs = 128;
 struct RotaryProblem {

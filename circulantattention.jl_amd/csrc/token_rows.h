@@ -175,38 +175,36 @@ __device__ __forceinline__ bool bad_values(const KV &kv, int j0, int j1, int D) 
     return __any(bad);
 }
 
-// Whether a row at pos sees one of the keys that kv has.
-template <typename KV>
-__device__ __forceinline__ bool sees_any(const KV &kv, int pos, int W, int S) {
-    const int lo = pos - W + 1 > 0 ? pos - W + 1 : 0;
-    for (int j0 = 0; j0 <= pos; j0 += 64) {
-        if (j0 >= S && j0 < lo) j0 = lo;
+// Whether a row sees one of the keys that kv has.  (see, here and below: which keys the
+// row sees, and their scores from the products: PlainView or ShapedView.)
+template <typename KV, typename V>
+__device__ __forceinline__ bool sees_any(const KV &kv, const V &see) {
+    for (int j0 = see.begin; j0 < see.end; j0 += 64) {
+        if (j0 >= see.head && j0 < see.lo) j0 = see.lo;
         const int j = j0 + lane_again();
         typename KV::Ptr kp, vp;
-        if (__any(j <= pos && (j < S || j >= lo) && kv.row(j, kp, vp))) return true;
+        if (__any(see.sees(j) && kv.row(j, kp, vp))) return true;
     }
     return false;
 }
 
-// y = sum_j softmax_j(c q.k_j) v_j in base 2 over [0, min(S, lo)) and [lo, pos],
-// lo = max(0, pos - W + 1).  kv.row(j): whether key j is there, and its rows.
+// y = sum_j softmax_j(score_j) v_j in base 2 over the keys that the row sees.
+// kv.row(j): whether key j is there, and its rows.
 // rest: what y's rounding took, or NULL.
-template <typename T, typename KV>
-__device__ void forward_row(const T *q, T *y, T *rest, const KV &kv, int pos, int W, int S, int D,
-                            float c) {
+template <typename T, typename KV, typename V>
+__device__ void forward_row(const T *q, T *y, T *rest, const KV &kv, const V &see, int D) {
     const int lane = lane_again();
     const Pair qr = load_row(q, lane, D);
     const Lacks lacks(y, lane, D);
-    const int lo = pos - W + 1 > 0 ? pos - W + 1 : 0;
     float m = -INFINITY, l = 0.f;
     Pair o{0.f, 0.f};
-    for (int j0 = 0; j0 <= pos; j0 += 64) {
-        if (j0 >= S && j0 < lo) j0 = lo;
+    for (int j0 = see.begin; j0 < see.end; j0 += 64) {
+        if (j0 >= see.head && j0 < see.lo) j0 = see.lo;
         const int j = j0 + lane;
         const T *kp = q, *vp = q;
-        const bool sees = j <= pos && (j < S || j >= lo) && kv.row(j, kp, vp);
+        const bool sees = see.sees(j) && kv.row(j, kp, vp);
         if (!sees) kp = q, vp = zero_row<T>();
-        const float score = c * lane_dot(kp, qr, D), t = sees ? score : -INFINITY;
+        const float score = see.score(lane_dot(kp, qr, D), j), t = sees ? score : -INFINITY;
         const float mn = fmaxf(m, wave_max(t)), mu = mn == -INFINITY ? 0.f : mn;
         const float r = __builtin_amdgcn_exp2f(m - mu), p = sees ? __builtin_amdgcn_exp2f(t - mu) : 0.f;
         l = l * r + wave_sum(p);
@@ -223,11 +221,11 @@ __device__ void forward_row(const T *q, T *y, T *rest, const KV &kv, int pos, in
 }
 
 // The gradient of row i's query: dq = scale sum_j p_j (<dy, v_j> - d) k_j with
-// p_j = exp2(c q.k_j - lse) and d = <dy, y + rest> (rest may be NULL), which is
-// stored too.
-template <typename T, typename KV>
+// p_j = exp2(score_j - lse) and d = <dy, y + rest> (rest may be NULL), which is
+// stored too; capped scores bring their derivative.
+template <typename T, typename KV, typename V>
 __device__ void dq_row(const T *q, const T *y, const T *rest, const T *dy, T *dq, float lse, float *dsum, const KV &kv,
-                       int pos, int W, int S, int D, float c, float scale) {
+                       const V &see, int D, float scale) {
     const int lane = lane_again();
     const Pair qr = load_row(q, lane, D), gr = load_row(dy, lane, D);
     const Lacks lacks(dq, lane, D);
@@ -239,42 +237,40 @@ __device__ void dq_row(const T *q, const T *y, const T *rest, const T *dy, T *dq
     }
     const float d = dot(gr, yr);
     if (lane == 0) *dsum = d;
-    const int lo = pos - W + 1 > 0 ? pos - W + 1 : 0;
     Pair o{0.f, 0.f};
-    for (int j0 = 0; j0 <= pos; j0 += 64) {
-        if (j0 >= S && j0 < lo) j0 = lo;
+    for (int j0 = see.begin; j0 < see.end; j0 += 64) {
+        if (j0 >= see.head && j0 < see.lo) j0 = see.lo;
         const int j = j0 + lane;
         const T *kp = q, *vp = q;
-        const bool sees = j <= pos && (j < S || j >= lo) && kv.row(j, kp, vp);
+        const bool sees = see.sees(j) && kv.row(j, kp, vp);
         if (!sees) kp = vp = zero_row<T>();
-        const float p = __builtin_amdgcn_exp2f(c * lane_dot(kp, qr, D) - lse);
-        const float ds = p * (lane_dot(vp, gr, D) - d);
+        const float x = lane_dot(kp, qr, D), p = __builtin_amdgcn_exp2f(see.score(x, j) - lse);
+        const float ds = p * (lane_dot(vp, gr, D) - d) * see.bend(x);
         add_rows(o, kp, sees ? ds : 0.f, lane, D);
         if (!__any(lacks.open(o))) break;
     }
     lacks.store(dq, lane, Pair{o.a * scale, o.b * scale});
 }
 
-// The gradients of key j and value j (fix_k, fix_v: which) over the queries i of
-// [j, j + W) (j < S: all from j on) below n, and the G heads of each: q and dy point
-// at head 0 of query 0 of the group, lse and dsum at its row 0.
-template <typename T>
+// The gradients of key j and value j (fix_k, fix_v: which) over the packed rows
+// [first, end), G heads a token: q and dy point at head 0 of token 0 of the group, lse
+// and dsum at its row 0.  see.score and see.bend as above, by row.
+template <typename T, typename V>
 __device__ void dkdv_row(const T *k, const T *v, const T *q, int64_t q_row, const T *dy, int64_t dy_row,
-                         const float *lse, const float *dsum, T *dk, T *dv, bool fix_k, bool fix_v, int j, int n, int W,
-                         int S, int G, int D, float c, float scale) {
+                         const float *lse, const float *dsum, T *dk, T *dv, bool fix_k, bool fix_v, int first, int end,
+                         int G, int D, const V &see, float scale) {
     const int lane = lane_again();
     const Pair kr = load_row(k, lane, D), vr = load_row(v, lane, D);
     Lacks lk(dk, lane, D), lv(dv, lane, D);
     lk.a &= fix_k, lk.b &= fix_k;
     lv.a &= fix_v, lv.b &= fix_v;
-    const int end = (j < S || n - j < W ? n : j + W) * G;
     Pair ok{0.f, 0.f}, ov{0.f, 0.f};
-    for (int r0 = j * G; r0 < end; r0 += 64) {
+    for (int r0 = first; r0 < end; r0 += 64) {
         const bool in = r0 + lane < end;
         const int r = in ? r0 + lane : end - 1, i = r / G, g = r - i * G;
         const T *qp = q + i * q_row + g * D, *gp = dy + i * dy_row + g * D;
-        const float p = __builtin_amdgcn_exp2f(c * lane_dot(qp, kr, D) - lse[r]);
-        const float ds = p * (lane_dot(gp, vr, D) - dsum[r]);
+        const float x = lane_dot(qp, kr, D), p = __builtin_amdgcn_exp2f(see.score(x, i, g) - lse[r]);
+        const float ds = p * (lane_dot(gp, vr, D) - dsum[r]) * see.bend(x);
         if (fix_v) add_rows(ov, in ? gp : zero_row<T>(), in ? p : 0.f, lane, D);
         if (fix_k) add_rows(ok, in ? qp : zero_row<T>(), in ? ds : 0.f, lane, D);
         if (!__any(lk.open(ok) || lv.open(ov))) break;

@@ -1,0 +1,242 @@
+// What a row of token attention sees, and how a score follows from a product
+// <q, k>.  Two kinds: plain (a causal window with sinks, scores proportional to the
+// products), and shaped, which adds
+//   a cap:       x -> cap tanh(x / cap), x = scale <q, k>
+//   slopes:      - slope_h |i - j| for the query at i and the key at j, behind the cap
+//   documents:   row i sees nothing before the first token of its document, whose
+//                sinks are the first tokens of it
+//   a prefix:    the first tokens of a signal are seen by all of its rows
+// Kernels take the kind as a template argument; the plain one adds nothing to them.
+//
+// Scores count in powers of two (log2(e) times as much), as the exponentials do.
+#pragma once
+
+#include "token_tile.h"
+
+namespace circatt {
+namespace tok {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The capped score from a product.  With E = exp(2 x / cap) and r = 1 / (1 + E) the
+// tangent is 1 - 2 r, off by some 2^-23 throughout: one exponential, one reciprocal
+// and three other instructions.  Where that error, times the cap, would be seen in
+// the result (`fine`: Float32, or a cap above 256), arguments below 0.35 take the
+// odd series up to the eleventh power instead, whose next term is 2^-26 of it.
+struct Curve {
+    float u, x, C;  // 2 log2(e) scale / cap, scale / cap, log2(e) cap
+    __device__ __forceinline__ Curve(float cap, float scale) : u(0.f), x(0.f), C(0.f) {
+        if (cap > 0.f) {
+            x = scale / cap;
+            u = 2.f * kLog2e * x;
+            C = kLog2e * cap;
+        }
+    }
+    static constexpr float kFineCap = 256.f;
+    __device__ __forceinline__ float rest(float dot) const {
+        return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * u) + 1.f);
+    }
+    __device__ __forceinline__ float fine(float dot) const {  // the tangent
+        const float a = dot * x, b = a * a;
+        float p = -1382.f / 155925.f;
+        p = fmaf(p, b, 62.f / 2835.f);
+        p = fmaf(p, b, -17.f / 315.f);
+        p = fmaf(p, b, 2.f / 15.f);
+        p = fmaf(p, b, -1.f / 3.f);
+        const float small = fmaf(a * b, p, a);
+        return fabsf(a) < 0.35f ? small : fmaf(-2.f, rest(dot), 1.f);
+    }
+};
+
+// ---------------------------------------------------------------------------
+// One row, and the rows of one key, for the row by row forms.
+struct PlainView {
+    int begin, head, lo, end;  // keys [begin, head) and [lo, end) are looked at
+    float c;
+    __device__ __forceinline__ PlainView(int pos, int W, int S, float c)
+        : begin(0), head(S), lo(pos - W + 1 > 0 ? pos - W + 1 : 0), end(pos + 1), c(c) {}
+    __device__ __forceinline__ bool sees(int j) const { return j < end && (j < head || j >= lo); }
+    __device__ __forceinline__ float score(float dot, int) const { return c * dot; }
+    __device__ __forceinline__ float bend(float) const { return 1.f; }
+};
+
+// A product's score at a distance, and its derivative by the uncapped one.
+struct ShapedScore {
+    Curve curve;
+    float c, slope;  // slope: of the head, times log2(e)
+    bool cap;
+    __device__ __forceinline__ float at(float dot, int back) const {
+        const float s = cap ? curve.C * curve.fine(dot) : c * dot;
+        return fmaf(-slope, fabsf((float)back), s);
+    }
+    __device__ __forceinline__ float bend(float dot) const {
+        const float t = cap ? curve.fine(dot) : 0.f;
+        return fmaf(-t, t, 1.f);
+    }
+};
+struct ShapedView {
+    int pos, start, begin, head, lo, end, S, P;
+    ShapedScore s;
+    __device__ __forceinline__ ShapedView(int pos, int start, int W, int S, int P, const ShapedScore &s)
+        : pos(pos), start(start), begin(P > 0 ? 0 : start), S(S), P(P), s(s) {
+        head = start + S > P ? start + S : P;
+        lo = pos - W + 1 > start ? pos - W + 1 : start;
+        end = pos + 1 > P ? pos + 1 : P;
+    }
+    __device__ __forceinline__ bool sees(int j) const {
+        return j < P || (j <= pos && j >= start && (j < start + S || j >= lo));
+    }
+    __device__ __forceinline__ float score(float dot, int j) const { return s.at(dot, pos - j); }
+    __device__ __forceinline__ float bend(float dot) const { return s.bend(dot); }
+};
+
+// ---------------------------------------------------------------------------
+// What rows see, by tiles of keys.  Rows of documents have their own first key
+// (start; slo and shi: the first and the last row's, which ascend).
+struct ShapedSight {
+    int W, S, P, start, slo, shi;
+    // of the keys k0 .. k0 + 31, a bit each
+    __device__ __forceinline__ uint32_t bits(int at, int k0) const {
+        const int end = at + 1 - k0, first = start - k0;
+        const int low = end - W > first ? end - W : first, sinks = first + S;
+        return bits_between(low, end) | bits_between(first, end < sinks ? end : sinks) |
+               (at >= 0 ? bits_between(0, P - k0) : 0u);
+    }
+    // (The sinks of documents that begin among the rows lie in their windows' tiles.)
+    __device__ __forceinline__ bool none(int lo, int hi, int k0, int n) const {
+        return k0 >= P && (k0 > hi || k0 + n <= slo || (k0 + n - 1 <= lo - W && k0 >= slo + S));
+    }
+    __device__ __forceinline__ bool all(int lo, int hi, int k0, int n) const {
+        return k0 + n <= P || (k0 + n - 1 <= lo && k0 >= shi && (k0 > hi - W || k0 + n <= slo + S));
+    }
+};
+
+// The tiles of KT keys that rows at [lo, hi] see, in order: those of the prefix or
+// of the sinks of the first row's document, which begins at s0, then the window's.
+template <int KT>
+struct ShapedTiles {
+    int from, sinks, first, count;
+    __device__ ShapedTiles(int lo, int hi, int W, int S, int P, int s0) {
+        const int low = lo - W + 1 > s0 ? lo - W + 1 : s0, top = s0 + S > P ? s0 + S : P;
+        const int w = low > 0 ? low / KT : 0, e = (hi + 1 > P ? hi + 1 : P) - 1;
+        from = P > 0 ? 0 : s0 / KT;
+        const int s = S > 0 || P > 0 ? (top + KT - 1) / KT : 0, to = s < w ? s : w;
+        sinks = to > from ? to - from : 0;
+        first = w;
+        count = hi < 0 ? 0 : sinks + e / KT + 1 - w;
+    }
+    __device__ __forceinline__ int key(int i) const { return (i < sinks ? from + i : first + i - sinks) * KT; }
+};
+
+// ---------------------------------------------------------------------------
+// Scores of 32 rows, one a lane, over blocks of 32 keys: registers hold the
+// products and then the scores.
+struct PlainScorer {
+    float c;
+    __device__ __forceinline__ float factor() const { return c; }
+    template <int NB>
+    __device__ __forceinline__ void shape(f16v (&)[NB], int, int, int, int) const {}
+};
+template <bool CAP, bool FINE>
+struct ShapedScorer {
+    Curve curve;
+    float c, slope;
+    bool biased, fine;
+    __device__ __forceinline__ ShapedScorer(float scale, float cap, float slope, bool biased)
+        : curve(CAP ? cap : 0.f, scale), c(scale * kLog2e), slope(slope), biased(biased),
+          fine(FINE || (CAP && cap > Curve::kFineCap)) {}
+    // of the scores in the registers
+    __device__ __forceinline__ float factor() const { return CAP || biased ? 1.f : c; }
+    // Register i of block n is key k0 + 32 n + 8 (i / 4) + 4 half + i % 4; lo: the
+    // first row's position, behind which a key's distance may count the other way.
+    template <int NB>
+    __device__ __forceinline__ void shape(f16v (&s)[NB], int k0, int at, int lo, int lane) const {
+        if constexpr (CAP) {
+            if (fine) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[n][i] = curve.C * curve.fine(s[n][i]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[n][i] = fmaf(-2.f * curve.C, curve.rest(s[n][i]), curve.C);
+            }
+        }
+        if (biased) bias(s, k0 + 4 * (lane >> 5) - at, k0 + 32 * NB - 1 <= lo);
+    }
+    template <int NB>
+    __device__ __forceinline__ void bias(f16v (&s)[NB], int ahead, bool before) const {
+        const float f = CAP ? 1.f : c;
+        if (before) {  // distances as they are: keys do not lie behind their rows
+            const float b = slope * (float)ahead;
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[n][i] = fmaf(s[n][i], f, fmaf(slope, (float)(32 * n + 8 * (i >> 2) + (i & 3)), b));
+        } else {
+            const float d = (float)ahead;
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[n][i] = fmaf(-slope, fabsf(d + (float)(32 * n + 8 * (i >> 2) + (i & 3))), s[n][i] * f);
+        }
+    }
+    // The same of one key's products with 32 rows, a row a register, whose slopes and
+    // tokens lie at LDS byte st and st + stride.
+    __device__ __forceinline__ void shape_rows(f16v &s, unsigned st, int stride, float token) const {
+        if constexpr (CAP) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                s[i] = fine ? curve.C * curve.fine(s[i]) : fmaf(-2.f * curve.C, curve.rest(s[i]), curve.C);
+        }
+        if (!biased) return;
+        const float f = CAP ? 1.f : c;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const f4v sl = *(const CIRCATT_LDS f4v *)(st + 8 * i), at = *(const CIRCATT_LDS f4v *)(st + stride + 8 * i);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) s[i + y] = fmaf(-sl[y], fabsf(at[y] - token), s[i + y] * f);
+        }
+    }
+    // The derivatives of the capped scores by the uncapped ones, from the products.
+    __device__ __forceinline__ float bend(float dot) const {
+        if (fine) {
+            const float t = curve.fine(dot);
+            return fmaf(-t, t, 1.f);
+        }
+        const float r = 4.f * curve.rest(dot);
+        return fmaf(-0.25f * r, r, r);
+    }
+};
+
+// ---------------------------------------------------------------------------
+// The kinds.
+struct Plain {
+    typedef SlidingProblem Sliding;
+    typedef PagedProblem Paged;
+    static constexpr bool kShaped = false, kCap = false;
+};
+template <bool CAP>
+struct Shaped {
+    typedef ShapedSlidingProblem Sliding;
+    typedef ShapedPagedProblem Paged;
+    static constexpr bool kShaped = true, kCap = CAP;
+};
+
+__device__ __forceinline__ int clamp_prefix(const int32_t *prefix, int b, int n) {
+    const int p = prefix == nullptr ? 0 : prefix[b];
+    return p < 0 ? 0 : p < n ? p : n;
+}
+// The first token of token t's document, from its place in it.
+__device__ __forceinline__ int document_start(const int32_t *places, int t) {
+    if (places == nullptr) return 0;
+    const int p = places[t];
+    return p <= 0 ? t : p < t ? t - p : 0;
+}
+
+}  // namespace tok
+}  // namespace circatt

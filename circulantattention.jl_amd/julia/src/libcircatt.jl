@@ -212,6 +212,89 @@ circatt_paged_append(dtype, T, B, channels, k, k_row, v, v_row, cache_k, cache_v
           dtype, T, B, channels, k, k_row, v, v_row, cache_k, cache_v, npages, page_size,
           page_stride, row_stride, pages, pages_row, max_pages, lengths, offsets, stream)
 
+circatt_shaped_fwd(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, cap, slopes, prefix,
+                   places, places_row, q, q_row, q_batch, k, k_row, k_batch, v, v_row, v_batch,
+                   lengths, y, y_rest, lse, stream) =
+    ccall((:circatt_shaped_fwd, libcircatt), Cint,
+          (Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Cfloat, Cfloat, Ptr{Cfloat},
+           Ptr{Int32}, Ptr{Int32}, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Int64, Int64,
+           Ptr{Cvoid}, Int64, Int64, Ptr{Int32}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cfloat},
+           Ptr{Cvoid}),
+          dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, cap, slopes, prefix, places,
+          places_row, q, q_row, q_batch, k, k_row, k_batch, v, v_row, v_batch, lengths, y,
+          y_rest, lse, stream)
+
+circatt_shaped_bwd_workspace_bytes(dtype, L, B, nheads, kv_heads, dh, window, sinks, biased,
+                                   masked) =
+    ccall((:circatt_shaped_bwd_workspace_bytes, libcircatt), Int64,
+          (Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Cint, Cint),
+          dtype, L, B, nheads, kv_heads, dh, window, sinks, biased, masked)
+
+circatt_shaped_bwd(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, cap, slopes, prefix,
+                   places, places_row, q, q_row, q_batch, k, k_row, k_batch, v, v_row, v_batch,
+                   lengths, y, y_rest, lse, dy, dy_row, dy_batch, dq, dk, dv, workspace,
+                   workspace_bytes, stream) =
+    ccall((:circatt_shaped_bwd, libcircatt), Cint,
+          (Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Cfloat, Cfloat, Ptr{Cfloat},
+           Ptr{Int32}, Ptr{Int32}, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Int64, Int64,
+           Ptr{Cvoid}, Int64, Int64, Ptr{Int32}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cfloat}, Ptr{Cvoid},
+           Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Ptr{Cvoid}),
+          dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, cap, slopes, prefix, places,
+          places_row, q, q_row, q_batch, k, k_row, k_batch, v, v_row, v_batch, lengths, y,
+          y_rest, lse, dy, dy_row, dy_batch, dq, dk, dv, workspace, workspace_bytes, stream)
+
+circatt_shaped_paged(dtype, T, B, nheads, kv_heads, dh, window, sinks, scale, cap, slopes, prefix,
+                     q, q_row, cache_k, cache_v, npages, page_size, page_stride, row_stride,
+                     pages, pages_row, max_pages, lengths, offsets, y, zero_tail, workspace,
+                     workspace_bytes, stream) =
+    ccall((:circatt_shaped_paged, libcircatt), Cint,
+          (Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Cfloat, Cfloat, Ptr{Cfloat},
+           Ptr{Int32}, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Int64,
+           Ptr{Int32}, Int64, Int64, Ptr{Int32}, Ptr{Int32}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Int64,
+           Ptr{Cvoid}),
+          dtype, T, B, nheads, kv_heads, dh, window, sinks, scale, cap, slopes, prefix, q,
+          q_row, cache_k, cache_v, npages, page_size, page_stride, row_stride, pages, pages_row,
+          max_pages, lengths, offsets, y, zero_tail, workspace, workspace_bytes, stream)
+
+circatt_paged_fork(B, npages, page_size, pages, pages_row, max_pages, lengths, counts, N, source,
+                   out_pages, out_lengths, out_counts, stream) =
+    ccall((:circatt_paged_fork, libcircatt), Cint,
+          (Int64, Int64, Int64, Ptr{Int32}, Int64, Int64, Ptr{Int32}, Ptr{Int32}, Int64,
+           Ptr{Int32}, Ptr{Int32}, Ptr{Int32}, Ptr{Int32}, Ptr{Cvoid}),
+          B, npages, page_size, pages, pages_row, max_pages, lengths, counts, N, source,
+          out_pages, out_lengths, out_counts, stream)
+
+circatt_paged_resize_workspace_bytes(B, npages) =
+    ccall((:circatt_paged_resize_workspace_bytes, libcircatt), Int64,
+          (Int64, Int64),
+          B, npages)
+
+circatt_paged_resize(dtype, channels, cache_k, cache_v, npages, page_size, page_stride,
+                     row_stride, B, pages, pages_row, max_pages, lengths, counts, to, out_pages,
+                     out_lengths, out_counts, workspace, workspace_bytes, stream) =
+    ccall((:circatt_paged_resize, libcircatt), Cint,
+          (Cint, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Int64, Int64, Ptr{Int32},
+           Int64, Int64, Ptr{Int32}, Ptr{Int32}, Ptr{Int32}, Ptr{Int32}, Ptr{Int32}, Ptr{Int32},
+           Ptr{Cvoid}, Int64, Ptr{Cvoid}),
+          dtype, channels, cache_k, cache_v, npages, page_size, page_stride, row_stride, B,
+          pages, pages_row, max_pages, lengths, counts, to, out_pages, out_lengths, out_counts,
+          workspace, workspace_bytes, stream)
+
+circatt_paged_compact_workspace_bytes(npages) =
+    ccall((:circatt_paged_compact_workspace_bytes, libcircatt), Int64,
+          (Int64,),
+          npages)
+
+circatt_paged_compact(dtype, channels, cache_k, cache_v, npages, page_size, page_stride,
+                      row_stride, B, pages, pages_row, max_pages, counts, out_pages, out_counts,
+                      workspace, workspace_bytes, stream) =
+    ccall((:circatt_paged_compact, libcircatt), Cint,
+          (Cint, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Int64, Int64, Ptr{Int32},
+           Int64, Int64, Ptr{Int32}, Ptr{Int32}, Ptr{Int32}, Ptr{Cvoid}, Int64, Ptr{Cvoid}),
+          dtype, channels, cache_k, cache_v, npages, page_size, page_stride, row_stride, B,
+          pages, pages_row, max_pages, counts, out_pages, out_counts, workspace,
+          workspace_bytes, stream)
+
 circatt_axial_rotary(dtype, inverse, interleaved, naxes, n1, n2, n3, P, nb, nheads, dh, p1, p2, p3,
                      base, x, x_row, positions, pos_batch, y, stream) =
     ccall((:circatt_axial_rotary, libcircatt), Cint,

@@ -381,6 +381,89 @@ int circatt_paged_append(int dtype, int64_t T, int64_t B, int64_t channels, cons
                          const int32_t *lengths, const int32_t *offsets, void *stream);
 
 /*
+ * The same attention with shaped scores.  With x = scale * <q_i, k_j>,
+ *   s_ij = cap * tanh(x / cap) - slopes[h] * |i - j|
+ * takes the place of x: cap 0 leaves x as it is, slopes (nheads Float32 numbers on the
+ * device) may be NULL.  With prefix (B numbers) every token of signal b also sees the
+ * first prefix[b] tokens, those before them included.  With places ((B, L) numbers,
+ * places_row apart from signal to signal) a signal holds documents one after another:
+ * token i's begins at i - places[i], and tokens before that are not seen; sinks are a
+ * document's first tokens.  Places of a document count up from 0, others give
+ * unspecified rows.  Prefix and places do not go together.  slopes need L (or max_pages *
+ * page_size) of at most 2^24.  No gradient of the slopes is formed.
+ *
+ * biased, masked: whether slopes, and whether prefix or places, will be given.
+ */
+int circatt_shaped_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
+                       int64_t window, int64_t sinks, float scale, float cap, const float *slopes,
+                       const int32_t *prefix, const int32_t *places, int64_t places_row, const void *q,
+                       int64_t q_row, int64_t q_batch, const void *k, int64_t k_row, int64_t k_batch,
+                       const void *v, int64_t v_row, int64_t v_batch, const int32_t *lengths, void *y,
+                       void *y_rest, float *lse, void *stream);
+int64_t circatt_shaped_bwd_workspace_bytes(int dtype, int64_t L, int64_t B, int64_t nheads,
+                                           int64_t kv_heads, int64_t dh, int64_t window, int64_t sinks,
+                                           int biased, int masked);
+int circatt_shaped_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
+                       int64_t window, int64_t sinks, float scale, float cap, const float *slopes,
+                       const int32_t *prefix, const int32_t *places, int64_t places_row, const void *q,
+                       int64_t q_row, int64_t q_batch, const void *k, int64_t k_row, int64_t k_batch,
+                       const void *v, int64_t v_row, int64_t v_batch, const int32_t *lengths, const void *y,
+                       const void *y_rest, const float *lse, const void *dy, int64_t dy_row,
+                       int64_t dy_batch, void *dq, void *dk, void *dv, void *workspace,
+                       int64_t workspace_bytes, void *stream);
+/* circatt_paged_attention likewise; its workspace is circatt_paged_workspace_bytes'. */
+int circatt_shaped_paged(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
+                         int64_t window, int64_t sinks, float scale, float cap, const float *slopes,
+                         const int32_t *prefix, const void *q, int64_t q_row, const void *cache_k,
+                         const void *cache_v, int64_t npages, int64_t page_size, int64_t page_stride,
+                         int64_t row_stride, const int32_t *pages, int64_t pages_row, int64_t max_pages,
+                         const int32_t *lengths, const int32_t *offsets, void *y, int zero_tail,
+                         void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * The pages of a paged cache.  A sequence of n tokens holds the first n / page_size
+ * (rounded up) pages of its row of the table, and counts[p] (npages numbers) says how
+ * often page p is held, 0: it is free.  Tables, lengths and counts are read on the device
+ * and written to new arrays (rows of max_pages, -1 behind a sequence's pages), which
+ * overlap nothing that is read; numbers outside the cache are kept and not counted.
+ *
+ * circatt_paged_fork: new sequence n of N goes on from sequence source[n], with which it
+ * shares all pages; a number outside [0, B) gives an empty one.  Old sequences that
+ * nobody goes on from give their pages back.
+ *
+ * circatt_paged_resize: sequence b comes to to[b] tokens, no more than its row of the
+ * table holds (below 0: it stays as it is).  First pages behind the new lengths are given
+ * back.  Then sequences get the pages that they lack, in their order, the free pages
+ * of the lowest numbers first.  A sequence that grows and whose last page is
+ * partly filled and held more than once gets one for it too, and the part's tokens are
+ * copied there, in both caches.  From the first sequence on that finds too few free
+ * pages, those that need any stay as they are, which their new lengths show.
+ *
+ * circatt_paged_compact: the held pages from number `used` on, `used` being how many are
+ * held, move in order to the free numbers below it, in both caches, and table and counts
+ * follow.  What the pages from `used` on hold stays there.
+ *
+ * The pages of a cache do not overlap one another, B and N are at most 65535.
+ */
+int circatt_paged_fork(int64_t B, int64_t npages, int64_t page_size, const int32_t *pages,
+                       int64_t pages_row, int64_t max_pages, const int32_t *lengths,
+                       const int32_t *counts, int64_t N, const int32_t *source, int32_t *out_pages,
+                       int32_t *out_lengths, int32_t *out_counts, void *stream);
+int64_t circatt_paged_resize_workspace_bytes(int64_t B, int64_t npages);
+int circatt_paged_resize(int dtype, int64_t channels, void *cache_k, void *cache_v, int64_t npages,
+                         int64_t page_size, int64_t page_stride, int64_t row_stride, int64_t B,
+                         const int32_t *pages, int64_t pages_row, int64_t max_pages,
+                         const int32_t *lengths, const int32_t *counts, const int32_t *to,
+                         int32_t *out_pages, int32_t *out_lengths, int32_t *out_counts, void *workspace,
+                         int64_t workspace_bytes, void *stream);
+int64_t circatt_paged_compact_workspace_bytes(int64_t npages);
+int circatt_paged_compact(int dtype, int64_t channels, void *cache_k, void *cache_v, int64_t npages,
+                          int64_t page_size, int64_t page_stride, int64_t row_stride, int64_t B,
+                          const int32_t *pages, int64_t pages_row, int64_t max_pages,
+                          const int32_t *counts, int32_t *out_pages, int32_t *out_counts,
+                          void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
  * Rotary positions with naxes (1 to 3) axes on P tokens of each of nb signals
  * (rows x_row elements apart): the first 2*p1 channels of a head belong to
  * axis 1, the next 2*p2 to axis 2, then 2*p3; pair i of an axis (channels i
