@@ -61,7 +61,8 @@ class SlidingAttBlock(torch.nn.Module):
     channels): causal attention in a sliding window with sinks
     (sliding_mh_attention), nheads heads of queries over kv_heads of keys and
     values, and rotary positions with `rotary` = (pairs, ...) pairs for each axis
-    (None: no positions).
+    (None: no positions).  `cap` bounds the scores, and with `distance` they fall by
+    2^(-8 (h + 1) / nheads) a token of distance in head h (`slopes`, a buffer).
 
     `forward` is for training and whole prompts; `step` takes the new tokens of
     several sequences, appends their keys and values to a paged cache and
@@ -69,7 +70,7 @@ class SlidingAttBlock(torch.nn.Module):
     `forward` gives for the whole."""
 
     def __init__(self, channels: int, window: int, nheads: int = 1, kv_heads: int = None, sinks: int = 0,
-                 rotary=None, base: float = 10000.0, bias: bool = True):
+                 rotary=None, base: float = 10000.0, bias: bool = True, cap: float = None, distance: bool = False):
         super().__init__()
         kv_heads = nheads if kv_heads is None else kv_heads
         if nheads < 1 or channels % nheads != 0:
@@ -78,10 +79,23 @@ class SlidingAttBlock(torch.nn.Module):
             raise AssertionError(f"nheads ({nheads}) must be divisible by kv_heads ({kv_heads})")
         self.window, self.sinks, self.nheads, self.kv_heads = window, sinks, nheads, kv_heads
         self.rotary, self.base = None if rotary is None else tuple(rotary), base
+        self.cap = cap
+        self.register_buffer("slopes", self._slopes() if distance else None, persistent=False)
         self.parts = [channels, channels // nheads * kv_heads, channels // nheads * kv_heads]
         # one projection: the attention reads its three parts in place
         self.qkv = torch.nn.Linear(channels, sum(self.parts), bias=bias)
         self.o = torch.nn.Linear(channels, channels, bias=bias)
+
+    def _slopes(self):
+        h = torch.arange(1, self.nheads + 1, dtype=torch.float64, device="cpu")
+        return torch.exp2(-8.0 * h / self.nheads).float()
+
+    def _apply(self, fn, *args, **kwargs):
+        # the slopes stay Float32 in a block of another type
+        out = super()._apply(fn, *args, **kwargs)
+        if self.slopes is not None:
+            self.slopes = self._slopes().to(self.slopes.device)
+        return out
 
     def _project(self, x, positions):
         q, k, v = self.qkv(x).split(self.parts, dim=-1)
@@ -90,17 +104,22 @@ class SlidingAttBlock(torch.nn.Module):
             k = axial_rotary(k, self.rotary, self.kv_heads, base=self.base, positions=positions)
         return q, k, v
 
-    def forward(self, x: torch.Tensor, lengths: torch.Tensor = None, positions: torch.Tensor = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, lengths: torch.Tensor = None, positions: torch.Tensor = None,
+                places: torch.Tensor = None, prefix: torch.Tensor = None) -> torch.Tensor:
         """positions (int32, (L, axes) or (B, L, axes)): None for one axis that
-        counts the tokens."""
+        counts the tokens, of their document where places are given.  places, prefix:
+        as sliding_mh_attention takes them."""
+        if places is not None and positions is None and self.rotary is not None and len(self.rotary) == 1:
+            positions = places[..., None]
         q, k, v = self._project(x, positions)
         y = sliding_mh_attention(q, k, v, self.window, self.nheads, kv_heads=self.kv_heads, sinks=self.sinks,
-                                 lengths=lengths)
+                                 lengths=lengths, cap=self.cap, slopes=self.slopes, places=places, prefix=prefix)
         return x + self.o(y)
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, pages: torch.Tensor,
-             lengths: torch.Tensor, offsets: torch.Tensor = None, positions: torch.Tensor = None) -> torch.Tensor:
+             lengths: torch.Tensor, offsets: torch.Tensor = None, positions: torch.Tensor = None,
+             prefix: torch.Tensor = None) -> torch.Tensor:
         """x: (T, channels), the new tokens; the other arguments as
         paged_mh_attention takes them.  positions (int32, (T, axes)): None, with
         one new token a sequence and one axis, for each token's place."""
@@ -111,7 +130,7 @@ class SlidingAttBlock(torch.nn.Module):
         q, k, v = self._project(x, positions)
         paged_append_(cache_k, cache_v, k, v, pages, lengths, offsets=offsets)
         y = paged_mh_attention(q, cache_k, cache_v, pages, lengths, self.window, self.nheads, kv_heads=self.kv_heads,
-                               sinks=self.sinks, offsets=offsets)
+                               sinks=self.sinks, offsets=offsets, cap=self.cap, slopes=self.slopes, prefix=prefix)
         return x + self.o(y)
 
 

@@ -109,12 +109,10 @@ class _Shape:
 
 
 def _shape(q, B, nheads, cap, slopes, prefix, places=None):
-    """The call's _Shape, or None where its scores are plain."""
-    cap = 0.0 if cap is None else float(cap)
-    if cap < 0.0 or not math.isfinite(cap):
+    """The call's _Shape."""
+    cap = float(cap or 0.0)
+    if not 0.0 <= cap < math.inf:
         raise AssertionError(f"cap={cap} must be positive and finite, 0 or None: no cap")
-    if cap == 0.0 and slopes is None and prefix is None and places is None:
-        return None
     if prefix is not None and places is not None:
         raise AssertionError("prefix and places do not go together")
     if slopes is not None:
@@ -265,7 +263,8 @@ def sliding_mh_attention(q, k, v, W, nheads: int, *, kv_heads: int = None, sinks
     if lengths is not None:
         lengths = _index(lengths, "lengths", q, (q.shape[0],))
     args = (q, k, v, W, sinks, nheads, kv_heads, scale, lengths)
-    shape = _shape(q, q.shape[0], nheads, cap, slopes, prefix, places)
+    plain = not cap and slopes is None and prefix is None and places is None
+    shape = None if plain else _shape(q, q.shape[0], nheads, cap, slopes, prefix, places)
     if _recorded(q, k, v):
         return SlidingAttentionFn.apply(*args) if shape is None else ShapedAttentionFn.apply(shape.cap, *shape.arrays, *args)
     return _sliding(False, *args, shape)[0]
@@ -343,7 +342,7 @@ def paged_mh_attention(q, cache_k, cache_v, pages, lengths, W, nheads: int, *, k
         _require(y, "out", q)
         if tuple(y.shape) != (T, nheads * dh) or not y.is_contiguous():
             raise AssertionError(f"out must be contiguous {(T, nheads * dh)}")
-    shape = _shape(q, B, nheads, cap, slopes, prefix)
+    shape = None if not cap and slopes is None and prefix is None else _shape(q, B, nheads, cap, slopes, prefix)
     code = _CODES[q.dtype]
     wbytes = L.lib.circatt_paged_workspace_bytes(code, T, B, nheads, kv_heads, dh, W, sinks, page, pages.shape[1])
     work = torch.empty((wbytes // 4,), dtype=torch.float32, device=q.device) if wbytes > 0 else None
