@@ -182,8 +182,9 @@ def test_python_layer():
     from circulant_attention import tokens as T
     q = torch.zeros(2, 9, 32)
     ok = torch.zeros(4)
-    assert T._shape(q, 2, 4, 5, None, None).args() == (5.0, None, None, None, 0)
-    assert T._shape(q, 2, 4, None, ok, None).args()[:2] == (0.0, ok.data_ptr())
+    cap, *arrays, row = T._shape(q, 2, 4, 5, None, None).args()
+    assert cap == 5.0 and row == 0 and all(a.value is None for a in arrays)
+    assert T._shape(q, 2, 4, None, ok, None).args()[1].value == ok.data_ptr()
     for cap in (-1.0, math.nan, math.inf):
         with pytest.raises(AssertionError, match="cap"):
             T._shape(q, 2, 4, cap, None, None)
