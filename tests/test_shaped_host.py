@@ -183,7 +183,7 @@ def test_python_layer():
     q = torch.zeros(2, 9, 32)
     ok = torch.zeros(4)
     cap, *arrays, row = T._shape(q, 2, 4, 5, None, None).args()
-    assert cap == 5.0 and row == 0 and all(a.value is None for a in arrays)
+    assert cap == 5.0 and row == 0 and not any(arrays)
     assert T._shape(q, 2, 4, None, ok, None).args()[1].value == ok.data_ptr()
     for cap in (-1.0, math.nan, math.inf):
         with pytest.raises(AssertionError, match="cap"):
