@@ -767,7 +767,7 @@ int check_rests(const void *rest, const void *y, int64_t bytes, int dtype) {
 namespace {
 
 // What scores are shaped by, for signals of up to `tokens` tokens.
-int check_shape(float scale, float cap, const float *slopes, const int32_t *prefix, const int32_t *places, int64_t places_row,
+int check_shape(int dtype, float scale, float cap, const float *slopes, const int32_t *prefix, const int32_t *places, int64_t places_row,
                 int64_t tokens, ScoreShape &sh) {
     // the kernels form scale / cap and multiples of it and of the cap in Float32
     if (!(cap >= 0.f) || !(cap <= 1e30f) || (cap > 0.f && (!(scale / cap >= 1e-30f) || !(scale / cap <= 1e30f))))
@@ -778,6 +778,7 @@ int check_shape(float scale, float cap, const float *slopes, const int32_t *pref
     if (slopes != nullptr && tokens > (int64_t)1 << 24)
         return fail(CIRCATT_ERR_UNSUPPORTED, "slopes for %lld tokens, at most 2^24 are supported", (long long)tokens);
     sh.cap = cap;
+    sh.curve = make_curve(cap, scale, dtype);
     sh.slopes = slopes;
     sh.prefix = prefix;
     sh.places = places;
@@ -907,7 +908,7 @@ int circatt_shaped_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t 
                        const int32_t *lengths, void *y, void *y_rest, float *lse, void *stream) {
     ShapedSlidingProblem pr{};
     CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
-    CIRCATT_TRY(check_shape(scale, cap, slopes, prefix, places, places_row, L, pr.shape));
+    CIRCATT_TRY(check_shape(dtype, scale, cap, slopes, prefix, places, places_row, L, pr.shape));
     if (L == 0 || B == 0) return ok();
     CIRCATT_TRY(check_threads(shaped_sliding_threads(pr, prefix != nullptr || places != nullptr, lse != nullptr)));
     CIRCATT_TRY(sliding_fwd_arguments(dtype, L, B, nheads, kv_heads, dh, q, q_row, q_batch, k, k_row, k_batch, v, v_row,
@@ -934,7 +935,7 @@ int circatt_shaped_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t 
                        int64_t workspace_bytes, void *stream) {
     ShapedSlidingProblem pr{};
     CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
-    CIRCATT_TRY(check_shape(scale, cap, slopes, prefix, places, places_row, L, pr.shape));
+    CIRCATT_TRY(check_shape(dtype, scale, cap, slopes, prefix, places, places_row, L, pr.shape));
     if (L == 0 || B == 0) return ok();
     const bool masked = prefix != nullptr || places != nullptr;
     CIRCATT_TRY(check_threads(shaped_sliding_threads(pr, masked, true)));
@@ -1024,7 +1025,7 @@ int circatt_shaped_paged(int dtype, int64_t T, int64_t B, int64_t nheads, int64_
     CIRCATT_TRY(paged_arguments(dtype, T, B, nheads, kv_heads, dh, window, sinks, scale, q, q_row, cache_k, cache_v, npages,
                                 page_size, page_stride, row_stride, pages, pages_row, max_pages, lengths, offsets, y,
                                 zero_tail, workspace, workspace_bytes, pr));
-    CIRCATT_TRY(check_shape(scale, cap, slopes, prefix, nullptr, 0, max_pages * page_size, pr.shape));
+    CIRCATT_TRY(check_shape(dtype, scale, cap, slopes, prefix, nullptr, 0, max_pages * page_size, pr.shape));
     if (T == 0) return ok();
     const ShapeSpans sh(pr.shape, B, 0, nheads);
     CIRCATT_TRY(check_apart({span("y", y, 1, 0, T, nheads * dh, nheads * dh, esize_of(dtype))}, {sh.slopes, sh.prefix}));

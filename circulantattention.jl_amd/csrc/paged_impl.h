@@ -121,13 +121,13 @@ struct ShapedSequence {
     template <typename T>
     __device__ __forceinline__ ShapedScorer<CAP, CAP && sizeof(T) == 4> scorer(const ShapedPagedProblem &pr, int h) const {
         const bool biased = pr.shape.slopes != nullptr;
-        return ShapedScorer<CAP, CAP && sizeof(T) == 4>(pr.scale, pr.shape.cap, biased ? pr.shape.slopes[h] * kLog2e : 0.f,
-                                                        biased);
+        return ShapedScorer<CAP, CAP && sizeof(T) == 4>(pr.scale, pr.shape.curve, biased ? pr.shape.slopes[h] * kLog2e : 0.f,
+                                                        biased, !__is_same(T, _Float16));
     }
     __device__ __forceinline__ ShapedView view(const ShapedPagedProblem &pr, int pos, int h) const {
         const float slope = pr.shape.slopes == nullptr ? 0.f : pr.shape.slopes[h] * kLog2e;
         return ShapedView(pos, 0, pr.W, pr.S, pos < 0 ? 0 : P,
-                          ShapedScore{Curve(pr.shape.cap, pr.scale), pr.scale * kLog2e, slope, CAP});
+                          ShapedScore{pr.shape.curve, pr.scale * kLog2e, slope, CAP});
     }
 };
 template <typename X>
@@ -360,7 +360,7 @@ __device__ __forceinline__ void few_rows(const typename X::Paged &pr, const Page
                 asm volatile("");
                 hide_keys(s[0], see.bits(rs.at, k0) & there, lane);
             }
-            x.raise(x.largest(s) * score.factor());
+            score.raise(x, score.largest(x, s));
             x.weigh(s, p, score.factor());
             x.template add<1>(col_at + to, p);
         }
@@ -481,7 +481,7 @@ __device__ __forceinline__ void chunk_rows(const typename X::Paged &pr, const Pa
                 for (int m = 0; m < NB; ++m)
                     hide_keys(s[m], see.bits(rs.at, k0 + 32 * m) & (uint32_t)(there >> (32 * m)), lane);
             }
-            x.raise(x.largest(s) * c);
+            score.raise(x, score.largest(x, s));
             x.weigh(s, p, c);
             x.template add<NB>(col_at + to, p);
         }

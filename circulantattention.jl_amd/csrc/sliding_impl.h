@@ -120,13 +120,13 @@ struct ShapedSignal {
     template <typename T>
     __device__ __forceinline__ ShapedScorer<CAP, CAP && sizeof(T) == 4> scorer(const ShapedSlidingProblem &pr, int h) const {
         const bool biased = pr.shape.slopes != nullptr;
-        return ShapedScorer<CAP, CAP && sizeof(T) == 4>(pr.scale, pr.shape.cap, biased ? pr.shape.slopes[h] * kLog2e : 0.f,
-                                                        biased);
+        return ShapedScorer<CAP, CAP && sizeof(T) == 4>(pr.scale, pr.shape.curve, biased ? pr.shape.slopes[h] * kLog2e : 0.f,
+                                                        biased, !__is_same(T, _Float16));
     }
     __device__ __forceinline__ ShapedView view(const ShapedSlidingProblem &pr, int pos, int h) const {
         const float slope = pr.shape.slopes == nullptr ? 0.f : pr.shape.slopes[h] * kLog2e;
         return ShapedView(pos, document_start(places, pos), pr.W, pr.S, P,
-                          ShapedScore{Curve(pr.shape.cap, pr.scale), pr.scale * kLog2e, slope, CAP});
+                          ShapedScore{pr.shape.curve, pr.scale * kLog2e, slope, CAP});
     }
 };
 template <typename X>
@@ -202,12 +202,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
 #pragma unroll
                 for (int m = 0; m < NB; ++m) hide_keys(s[m], see.bits(at, k0 + 32 * m), lane);
             }
-            mx = x.largest(s) * c;
+            mx = score.largest(x, s);
         };
         auto step = [&](const f16v (&s)[NB], f16v (&t)[NB], int i) {
             round(i);
             V8<T> p[2 * NB];
-            x.raise(mx);
+            score.raise(x, mx);
             x.scores(row_at + kp * Rg::TILE, t);
             x.weigh(s, p, c);
             x.template add<NB>(col_at + vp * Rg::TILE, p);
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             }
             round(i);
             V8<T> p[2 * NB];
-            x.raise(mx);
+            score.raise(x, mx);
             x.weigh(sa, p, c);
             x.template add<NB>(col_at + vp * Rg::TILE, p);
             next();
@@ -392,13 +392,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
                                               else s = mma(a, q[i >> 1], s);
                                           });
                 f16v bend = f16v{};
-                if constexpr (X::kCap) {
-#pragma unroll
-                    for (int x = 0; x < 16; ++x) bend[x] = score.bend(s[x]);
-                }
                 if constexpr (X::kShaped) {
                     f16v one[1] = {s};
-                    score.shape(one, k0, at, lo, lane);
+                    score.caps(one);
+                    if constexpr (X::kCap) {
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) bend[x] = score.bend(one[0][x]);
+                    }
+                    score.biases(one, k0, at, lo, lane);
                     s = one[0];
                 }
 #pragma unroll
@@ -634,7 +635,7 @@ struct ShapedRowScore {
     const float *slopes;
     int j;
     __device__ __forceinline__ ShapedRowScore(const ShapedSlidingProblem &pr, int hk, int j)
-        : s{Curve(pr.shape.cap, pr.scale), pr.scale * kLog2e, 0.f, CAP},
+        : s{pr.shape.curve, pr.scale * kLog2e, 0.f, CAP},
           slopes(pr.shape.slopes == nullptr ? nullptr : pr.shape.slopes + (int64_t)hk * pr.G), j(j) {}
     __device__ __forceinline__ float score(float dot, int i, int g) const {
         ShapedScore x = s;
@@ -661,7 +662,7 @@ template <bool CAP, bool FINE>
 struct ShapedKeyScore : ShapedScorer<CAP, FINE> {
     float token;  // of the key
     __device__ __forceinline__ ShapedKeyScore(const ShapedSlidingProblem &pr, int j)
-        : ShapedScorer<CAP, FINE>(pr.scale, pr.shape.cap, 0.f, pr.shape.slopes != nullptr), token((float)j) {}
+        : ShapedScorer<CAP, FINE>(pr.scale, pr.shape.curve, 0.f, pr.shape.slopes != nullptr, false), token((float)j) {}
 };
 template <typename X, typename T>
 struct KeyScoreOf {
@@ -710,15 +711,16 @@ struct KeySums {
                                           else s = mma(a, k[i >> 1], s);
                                       });
         f16v bend = f16v{};
-        if constexpr (X::kCap) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) bend[x] = score.bend(s[x]);
-        }
         float c;
         if constexpr (X::kShaped) {
             f16v one[1] = {s};
-            score.shape_rows(one[0], st + 2 * stride, stride, score.token);
+            score.caps(one);
             s = one[0];
+            if constexpr (X::kCap) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x) bend[x] = score.bend(s[x]);
+            }
+            score.bias_rows(s, st + 2 * stride, stride, score.token);
             c = score.factor();
         } else {
             c = score.c;

@@ -29,9 +29,22 @@ struct SlidingProblem {
     void *dq, *dk, *dv;  // contiguous; dk and dv may be NULL (both)
     float *work;         // rowsum(dy * y), laid out as lse, then partial sums
 };
+// How capped scores follow from products d: C tanh(x d), in powers of two
+// (token_shape.h).
+struct Curve {
+    float x, u, C;  // scale / cap, 2 log2(e) x, log2(e) cap
+    // up to these |d| the tangent is d (few[0] + few[1] d^2 + ...) or d (more[0] + ...);
+    // below 0: never
+    float near, far;
+    float few[3], more[5];
+    int fine;       // whether an error of 2^-22 of the cap would be seen in the result
+};
+Curve make_curve(float cap, float scale, int dtype);
+
 // How scores follow from products, and what else a row sees (or does not).
 struct ScoreShape {
     float cap;               // 0: none
+    Curve curve;
     const float *slopes;     // (H) or NULL
     const int32_t *prefix;   // (B) or NULL: tokens that all rows see
     const int32_t *places;   // each token's place in its document, or NULL

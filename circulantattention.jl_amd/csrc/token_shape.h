@@ -18,35 +18,35 @@ namespace tok {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// The capped score from a product.  With E = exp(2 x / cap) and r = 1 / (1 + E) the
-// tangent is 1 - 2 r, off by some 2^-23 throughout: one exponential, one reciprocal
-// and three other instructions.  Where that error, times the cap, would be seen in
-// the result (`fine`: Float32, or a cap above 256), arguments below 0.35 take the
-// odd series up to the eleventh power instead, whose next term is 2^-26 of it.
-struct Curve {
-    float u, x, C;  // 2 log2(e) scale / cap, scale / cap, log2(e) cap
-    __device__ __forceinline__ Curve(float cap, float scale) : u(0.f), x(0.f), C(0.f) {
-        if (cap > 0.f) {
-            x = scale / cap;
-            u = 2.f * kLog2e * x;
-            C = kLog2e * cap;
-        }
-    }
-    static constexpr float kFineCap = 256.f;
-    __device__ __forceinline__ float rest(float dot) const {
-        return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * u) + 1.f);
-    }
-    __device__ __forceinline__ float fine(float dot) const {  // the tangent
-        const float a = dot * x, b = a * a;
-        float p = -1382.f / 155925.f;
-        p = fmaf(p, b, 62.f / 2835.f);
-        p = fmaf(p, b, -17.f / 315.f);
-        p = fmaf(p, b, 2.f / 15.f);
-        p = fmaf(p, b, -1.f / 3.f);
-        const float small = fmaf(a * b, p, a);
-        return fabsf(a) < 0.35f ? small : fmaf(-2.f, rest(dot), 1.f);
-    }
-};
+// The tangent from a product.  With E = exp(2 x d) and r = 1 / (1 + E) it is 1 - 2 r, off
+// by some 2^-23 of the cap throughout, at one exponential, one reciprocal and three
+// other instructions.  Where no product of a tile passes 0.7 / x, as in a model that
+// keeps its scores well below the cap, a series of five terms with the same error takes
+// six multiplications instead, and where none passes 0.3 / x one of three terms four.
+// Float32, and caps above 256 outside the series' range, ask for more:
+// there arguments below 0.35 take the power series up to the eleventh term, whose next
+// is 2^-26 of it.
+__device__ __forceinline__ float curve_rest(const Curve &c, float dot) {
+    return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * c.u) + 1.f);
+}
+__device__ __forceinline__ float curve_fine(const Curve &c, float dot) {
+    const float a = dot * c.x, b = a * a;
+    float p = -1382.f / 155925.f;
+    p = fmaf(p, b, 62.f / 2835.f);
+    p = fmaf(p, b, -17.f / 315.f);
+    p = fmaf(p, b, 2.f / 15.f);
+    p = fmaf(p, b, -1.f / 3.f);
+    const float small = fmaf(a * b, p, a);
+    return fabsf(a) < 0.35f ? small : fmaf(-2.f, curve_rest(c, dot), 1.f);
+}
+template <int N>
+__device__ __forceinline__ float curve_series(const float (&p)[N], float dot) {
+    const float b = dot * dot;
+    float t = p[N - 1];
+#pragma unroll
+    for (int i = N - 2; i >= 0; --i) t = fmaf(t, b, p[i]);
+    return dot * t;
+}
 
 // ---------------------------------------------------------------------------
 // One row, and the rows of one key, for the row by row forms.
@@ -66,11 +66,11 @@ struct ShapedScore {
     float c, slope;  // slope: of the head, times log2(e)
     bool cap;
     __device__ __forceinline__ float at(float dot, int back) const {
-        const float s = cap ? curve.C * curve.fine(dot) : c * dot;
+        const float s = cap ? curve.C * curve_fine(curve, dot) : c * dot;
         return fmaf(-slope, fabsf((float)back), s);
     }
     __device__ __forceinline__ float bend(float dot) const {
-        const float t = cap ? curve.fine(dot) : 0.f;
+        const float t = cap ? curve_fine(curve, dot) : 0.f;
         return fmaf(-t, t, 1.f);
     }
 };
@@ -134,6 +134,14 @@ struct ShapedTiles {
 struct PlainScorer {
     float c;
     __device__ __forceinline__ float factor() const { return c; }
+    template <int NB, typename R>
+    __device__ __forceinline__ float largest(const R &x, const f16v (&s)[NB]) const {
+        return x.largest(s) * c;
+    }
+    template <typename R>
+    __device__ __forceinline__ void raise(R &x, float most) const {
+        x.raise(most);
+    }
     template <int NB>
     __device__ __forceinline__ void shape(f16v (&)[NB], int, int, int, int) const {}
 };
@@ -141,34 +149,71 @@ template <bool CAP, bool FINE>
 struct ShapedScorer {
     Curve curve;
     float c, slope;
-    bool biased, fine;
-    __device__ __forceinline__ ShapedScorer(float scale, float cap, float slope, bool biased)
-        : curve(CAP ? cap : 0.f, scale), c(scale * kLog2e), slope(slope), biased(biased),
-          fine(FINE || (CAP && cap > Curve::kFineCap)) {}
-    // of the scores in the registers
-    __device__ __forceinline__ float factor() const { return CAP || biased ? 1.f : c; }
+    bool biased;
+    // Scores that no bias takes off lie within the cap: where 2^cap and its reciprocal are
+    // well within the type that probabilities are rounded to, zero is as good a reference
+    // for the softmax as the largest score, and none is looked for.
+    bool bounded;
+    __device__ __forceinline__ ShapedScorer(float scale, const Curve &curve, float slope, bool biased, bool wide)
+        : curve(curve), c(scale * kLog2e), slope(slope), biased(biased), bounded(CAP && wide && !biased && curve.C <= 90.f) {}
+    template <int NB, typename R>
+    __device__ __forceinline__ float largest(const R &x, const f16v (&s)[NB]) const {
+        if (CAP && bounded) return 0.f;
+        return x.largest(s) * factor();
+    }
+    template <typename R>
+    __device__ __forceinline__ void raise(R &x, float most) const {
+        if (CAP && bounded) x.m = 0.f;
+        else x.raise(most);
+    }
+    // What the registers still lack to scores in powers of two: they hold products, or
+    // tangents of capped ones, and where there are slopes the scores themselves.
+    __device__ __forceinline__ float unit() const { return CAP ? curve.C : c; }
+    __device__ __forceinline__ float factor() const { return biased ? 1.f : unit(); }
+    // Tangents in the place of products: all by the series, or all by the exponential.
+    // (The products pass through an empty asm on each side, or the compiler forms all
+    // sides before the branch.)
+    template <int NB, typename F>
+    __device__ __forceinline__ static void each(f16v (&s)[NB], F f) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) asm volatile("" : "+v"(s[n]));
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] = f(s[n][i]);
+    }
+    template <int NB>
+    __device__ __forceinline__ void caps(f16v (&s)[NB]) const {
+        if constexpr (CAP && FINE) {
+            each(s, [&](float d) { return curve_fine(curve, d); });
+        } else if constexpr (CAP) {
+            float most = 0.f;
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(s[n][i]));
+            if (!__any(most > curve.near)) each(s, [&](float d) { return curve_series(curve.few, d); });
+            else if (!__any(most > curve.far)) each(s, [&](float d) { return curve_series(curve.more, d); });
+            else if (curve.fine) each(s, [&](float d) { return curve_fine(curve, d); });
+            else each(s, [&](float d) { return fmaf(-2.f, curve_rest(curve, d), 1.f); });
+        }
+    }
+    // The derivative of a capped score by the uncapped one, from its tangent.
+    __device__ __forceinline__ static float bend(float t) { return fmaf(-t, t, 1.f); }
     // Register i of block n is key k0 + 32 n + 8 (i / 4) + 4 half + i % 4; lo: the
     // first row's position, behind which a key's distance may count the other way.
     template <int NB>
-    __device__ __forceinline__ void shape(f16v (&s)[NB], int k0, int at, int lo, int lane) const {
-        if constexpr (CAP) {
-            if (fine) {
-#pragma unroll
-                for (int n = 0; n < NB; ++n)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[n][i] = curve.C * curve.fine(s[n][i]);
-            } else {
-#pragma unroll
-                for (int n = 0; n < NB; ++n)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[n][i] = fmaf(-2.f * curve.C, curve.rest(s[n][i]), curve.C);
-            }
-        }
+    __device__ __forceinline__ void biases(f16v (&s)[NB], int k0, int at, int lo, int lane) const {
         if (biased) bias(s, k0 + 4 * (lane >> 5) - at, k0 + 32 * NB - 1 <= lo);
     }
     template <int NB>
+    __device__ __forceinline__ void shape(f16v (&s)[NB], int k0, int at, int lo, int lane) const {
+        caps(s);
+        biases(s, k0, at, lo, lane);
+    }
+    template <int NB>
     __device__ __forceinline__ void bias(f16v (&s)[NB], int ahead, bool before) const {
-        const float f = CAP ? 1.f : c;
+        const float f = unit();
         if (before) {  // distances as they are: keys do not lie behind their rows
             const float b = slope * (float)ahead;
 #pragma unroll
@@ -187,29 +232,15 @@ struct ShapedScorer {
     }
     // The same of one key's products with 32 rows, a row a register, whose slopes and
     // tokens lie at LDS byte st and st + stride.
-    __device__ __forceinline__ void shape_rows(f16v &s, unsigned st, int stride, float token) const {
-        if constexpr (CAP) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                s[i] = fine ? curve.C * curve.fine(s[i]) : fmaf(-2.f * curve.C, curve.rest(s[i]), curve.C);
-        }
+    __device__ __forceinline__ void bias_rows(f16v &s, unsigned st, int stride, float token) const {
         if (!biased) return;
-        const float f = CAP ? 1.f : c;
+        const float f = unit();
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             const f4v sl = *(const CIRCATT_LDS f4v *)(st + 8 * i), at = *(const CIRCATT_LDS f4v *)(st + stride + 8 * i);
 #pragma unroll
             for (int y = 0; y < 4; ++y) s[i + y] = fmaf(-sl[y], fabsf(at[y] - token), s[i + y] * f);
         }
-    }
-    // The derivatives of the capped scores by the uncapped ones, from the products.
-    __device__ __forceinline__ float bend(float dot) const {
-        if (fine) {
-            const float t = curve.fine(dot);
-            return fmaf(-t, t, 1.f);
-        }
-        const float r = 4.f * curve.rest(dot);
-        return fmaf(-0.25f * r, r, r);
     }
 };
 
