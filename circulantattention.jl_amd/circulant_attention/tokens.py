@@ -411,7 +411,7 @@ def paged_fork(pages, lengths, counts, source, page_size: int):
         raise TypeError("source must be an int32 torch.Tensor (sequences,)")
     source = _index(source, "source", pages, tuple(source.shape))
     (B, most), N = pages.shape, source.shape[0]
-    new = (torch.empty((N, most), dtype=torch.int32, device=pages.device), torch.empty_like(source), torch.empty_like(counts))
+    new = pages.new_empty((N, most)), torch.empty_like(source), torch.empty_like(counts)
     _call(pages.device, L.lib.circatt_paged_fork, B, counts.shape[0], int(page_size), pages.data_ptr(), row, most,
           lengths.data_ptr(), counts.data_ptr(), N, ptr(source), ptr(new[0]), ptr(new[1]), new[2].data_ptr())
     return new
@@ -428,14 +428,13 @@ def paged_resize_(cache_k, cache_v, pages, lengths, counts, to):
     tokens, the only ones that move.  From the first sequence on that finds too few free
     pages, those that need any stay as they are, as the lengths that come back show.
     Other arguments as paged_fork's."""
-    _require(cache_k, "cache_k")
     npages, page, C, page_stride, row_stride = _cache(cache_k, cache_v, cache_k)
     pages, row, lengths, counts = _held(pages, lengths, counts, cache_k)
     B, most = pages.shape
     to = _index(to, "to", pages, (B,))
-    new = (torch.empty((B, most), dtype=torch.int32, device=pages.device), torch.empty_like(lengths), torch.empty_like(counts))
+    new = pages.new_empty((B, most)), torch.empty_like(lengths), torch.empty_like(counts)
     wbytes = L.lib.circatt_paged_resize_workspace_bytes(B, npages)
-    work = torch.empty((max(wbytes, 4) // 4,), dtype=torch.int32, device=pages.device)
+    work = pages.new_empty(max(wbytes, 4) // 4)
     _call(pages.device, L.lib.circatt_paged_resize, _CODES[cache_k.dtype], C, cache_k.data_ptr(), cache_v.data_ptr(), npages,
           page, page_stride, row_stride, B, pages.data_ptr(), row, most, lengths.data_ptr(), counts.data_ptr(), to.data_ptr(),
           *(t.data_ptr() for t in new), work.data_ptr(), wbytes)
@@ -449,13 +448,12 @@ def paged_compact_(cache_k, cache_v, pages, counts):
     there are held ones, take the free numbers below it in order.  Every table that
     refers to the cache is one: its rows may be those of several, joined.  Other
     arguments as paged_fork's."""
-    _require(cache_k, "cache_k")
     npages, page, C, page_stride, row_stride = _cache(cache_k, cache_v, cache_k)
     pages, row, _, counts = _held(pages, None, counts, cache_k)
     B, most = pages.shape
-    new = (torch.empty((B, most), dtype=torch.int32, device=pages.device), torch.empty_like(counts))
+    new = pages.new_empty((B, most)), torch.empty_like(counts)
     wbytes = L.lib.circatt_paged_compact_workspace_bytes(npages)
-    work = torch.empty((max(wbytes, 4) // 4,), dtype=torch.int32, device=pages.device)
+    work = pages.new_empty(max(wbytes, 4) // 4)
     _call(pages.device, L.lib.circatt_paged_compact, _CODES[cache_k.dtype], C, cache_k.data_ptr(), cache_v.data_ptr(), npages,
           page, page_stride, row_stride, B, pages.data_ptr(), row, most, counts.data_ptr(), *(t.data_ptr() for t in new),
           work.data_ptr(), wbytes)

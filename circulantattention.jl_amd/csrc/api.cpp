@@ -1077,6 +1077,8 @@ int page_table(int64_t B, int64_t maxp, int64_t npages, int64_t page_size, const
     for (pr.page_log2 = 0; (1 << pr.page_log2) < page_size;) ++pr.page_log2;
     if (maxp < 1 || pages_row < maxp || maxp > (int64_t)1 << (30 - pr.page_log2))
         return fail(CIRCATT_ERR_INVALID, "a page table of %lld pages, rows of %lld", (long long)maxp, (long long)pages_row);
+    if (maxp + 1 > INT32_MAX / B)  // pages that all sequences may ask for are counted in 32 bits
+        return fail(CIRCATT_ERR_UNSUPPORTED, "a table of %lld sequences with %lld pages", (long long)B, (long long)maxp);
     CIRCATT_NONNULL(pages);
     pr.B = (int)B;
     pr.maxp = (int)maxp;

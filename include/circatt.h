@@ -443,7 +443,8 @@ int circatt_shaped_paged(int dtype, int64_t T, int64_t B, int64_t nheads, int64_
  * held, move in order to the free numbers below it, in both caches, and table and counts
  * follow.  What the pages from `used` on hold stays there.
  *
- * The pages of a cache do not overlap one another, B and N are at most 65535.
+ * The pages of a cache do not overlap one another, B and N are at most 65535, and
+ * B * (max_pages + 1) is below 2^31.
  */
 int circatt_paged_fork(int64_t B, int64_t npages, int64_t page_size, const int32_t *pages,
                        int64_t pages_row, int64_t max_pages, const int32_t *lengths,

@@ -137,7 +137,7 @@ def compact(L, dtype=3, C=64, k=P, v=P, npages=100, page=16, ps=1024, rs=64, B=4
 TABLES = [
     (dict(B=0), -1, "sequence count"), (dict(B=65536), -1, "sequence count"), (dict(page=24), -2, "power of two"),
     (dict(npages=0), -1, "a cache of"), (dict(npages=1 << 28), -1, "a cache of"), (dict(maxp=0), -1, "page table"),
-    (dict(row=7), -1, "page table"), (dict(maxp=1 << 27, row=1 << 27), -1, "page table"), (dict(pages=None), -1, "pages is NULL"),
+    (dict(B=65535, maxp=1 << 15, row=1 << 15, page=1), -2, "a table of"), (dict(row=7), -1, "page table"), (dict(maxp=1 << 27, row=1 << 27), -1, "page table"), (dict(pages=None), -1, "pages is NULL"),
     (dict(counts=None), -1, "counts is NULL"), (dict(oc=None), -1, "out_counts is NULL"),
     (dict(op=None), -1, "out_pages is NULL"), (dict(op=P), -1, "out_pages must not overlap pages"),
     (dict(oc=ctypes.c_void_p(P.value + 396)), -1, "out_counts must not overlap"), (dict(oc=FAR), -1, "must not overlap"),
