@@ -200,7 +200,7 @@ def _sliding_gradients(ctx, dy, saved, shape=None, first=0):
     else:
         slopes, prefix, places = shape.arrays
         wbytes = L.lib.circatt_shaped_bwd_workspace_bytes(*sizes, slopes is not None,
-                                                          prefix is not None or places is not None)
+                                                          1 if places is not None else 2 if prefix is not None else 0)
     work = torch.empty((max(wbytes, 4) // 4,), dtype=torch.float32, device=q.device)
     rows = (q.data_ptr(), qr, qb, k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, ptr(lengths), y.data_ptr(), ptr(rest),
             lse.data_ptr(), dy.data_ptr(), dr, db, dq.data_ptr(), ptr(dk), ptr(dv), work.data_ptr(), wbytes)

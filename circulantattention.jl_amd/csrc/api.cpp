@@ -910,7 +910,7 @@ int circatt_shaped_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t 
     CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
     CIRCATT_TRY(check_shape(dtype, scale, cap, slopes, prefix, places, places_row, L, pr.shape));
     if (L == 0 || B == 0) return ok();
-    CIRCATT_TRY(check_threads(shaped_sliding_threads(pr, prefix != nullptr || places != nullptr, lse != nullptr)));
+    CIRCATT_TRY(check_threads(shaped_sliding_threads(pr, masked_by(pr.shape), lse != nullptr)));
     CIRCATT_TRY(sliding_fwd_arguments(dtype, L, B, nheads, kv_heads, dh, q, q_row, q_batch, k, k_row, k_batch, v, v_row,
                                       v_batch, lengths, y, y_rest, lse, ShapeSpans(pr.shape, B, L, nheads), pr));
     return hip_result(launch_shaped_fwd(pr, as_stream(stream)), "circatt_shaped_fwd");
@@ -920,9 +920,13 @@ int64_t circatt_shaped_bwd_workspace_bytes(int dtype, int64_t L, int64_t B, int6
                                            int64_t window, int64_t sinks, int biased, int masked) {
     SlidingProblem pr;
     if (sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, 1.f, pr) != CIRCATT_OK) return -1;
+    if (masked < kUnmasked || masked > kPrefix) {
+        fail(CIRCATT_ERR_INVALID, "masked=%d must be 0, 1 or 2", masked);
+        return -1;
+    }
     if (L == 0 || B == 0) return 0;
-    return check_threads(shaped_sliding_threads(pr, masked != 0, true)) == CIRCATT_OK
-               ? 4 * shaped_bwd_workspace_floats(pr, biased != 0, masked != 0)
+    return check_threads(shaped_sliding_threads(pr, masked, true)) == CIRCATT_OK
+               ? 4 * shaped_bwd_workspace_floats(pr, biased != 0, masked)
                : -1;
 }
 
@@ -937,7 +941,7 @@ int circatt_shaped_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t 
     CIRCATT_TRY(sliding_problem(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, pr));
     CIRCATT_TRY(check_shape(dtype, scale, cap, slopes, prefix, places, places_row, L, pr.shape));
     if (L == 0 || B == 0) return ok();
-    const bool masked = prefix != nullptr || places != nullptr;
+    const int masked = masked_by(pr.shape);
     CIRCATT_TRY(check_threads(shaped_sliding_threads(pr, masked, true)));
     CIRCATT_TRY(sliding_bwd_arguments(dtype, L, B, nheads, kv_heads, dh, q, q_row, q_batch, k, k_row, k_batch, v, v_row,
                                       v_batch, lengths, y, y_rest, lse, dy, dy_row, dy_batch, dq, dk, dv, workspace,

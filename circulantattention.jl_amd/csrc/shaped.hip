@@ -76,11 +76,10 @@ Curve make_curve(float cap, float scale, int dtype) {
     return c;
 }
 
-// (masked: room for the documents' ends, with a prefix as well)
-int64_t shaped_bwd_workspace_floats(const SlidingProblem &pr, bool biased, bool masked) {
-    return ShapedRegions(pr, walk_split(pr, masked), biased, masked).floats;
+int64_t shaped_bwd_workspace_floats(const SlidingProblem &pr, bool biased, int masked) {
+    return ShapedRegions(pr, walk_split(pr, masked), biased, masked == kPlaces).floats;
 }
-int64_t shaped_sliding_threads(const SlidingProblem &pr, bool masked, bool backward) {
+int64_t shaped_sliding_threads(const SlidingProblem &pr, int masked, bool backward) {
     const int64_t n = threads_of(pr, walk_split(pr, masked), backward), rows = (int64_t)pr.L * pr.H + 256;
     return n > rows ? n : rows;
 }
@@ -88,9 +87,9 @@ hipError_t launch_shaped_fwd(const ShapedSlidingProblem &pr, hipStream_t s) {
     return pr.shape.cap > 0.f ? launch_capped_fwd(pr, s) : forward_of<Shaped<false>>(pr, s);
 }
 hipError_t launch_shaped_bwd(ShapedSlidingProblem pr, hipStream_t s) {
-    const bool biased = pr.shape.slopes != nullptr, masked = pr.shape.places != nullptr || pr.shape.prefix != nullptr;
-    const WalkSplit sp = walk_split(pr, masked);
-    const ShapedRegions at(pr, sp, biased, masked);
+    const bool biased = pr.shape.slopes != nullptr;
+    const WalkSplit sp = walk_split(pr, masked_by(pr.shape));
+    const ShapedRegions at(pr, sp, biased, pr.shape.places != nullptr);
     pr.row_slopes = pr.work + at.slopes;
     pr.row_tokens = pr.work + at.tokens;
     pr.ends = reinterpret_cast<int32_t *>(pr.work + at.ends);

@@ -659,10 +659,10 @@ struct PlainKeyScore {
     __device__ __forceinline__ PlainKeyScore(const SlidingProblem &pr, int) : c(pr.scale * kLog2e) {}
 };
 template <bool CAP, bool FINE>
-struct ShapedKeyScore : ShapedScorer<CAP, FINE> {
+struct ShapedKeyScore : ShapedScorer<CAP, FINE, ReadCurve<ShapedSlidingProblem>> {
     float token;  // of the key
     __device__ __forceinline__ ShapedKeyScore(const ShapedSlidingProblem &pr, int j)
-        : ShapedScorer<CAP, FINE>(pr.scale, pr.shape.curve, 0.f, pr.shape.slopes != nullptr, false), token((float)j) {}
+        : ShapedScorer<CAP, FINE, ReadCurve<ShapedSlidingProblem>>(pr.scale, pr.shape.curve, 0.f, pr.shape.slopes != nullptr, false), token((float)j) {}
 };
 template <typename X, typename T>
 struct KeyScoreOf {
@@ -1120,8 +1120,12 @@ __global__ __launch_bounds__(256) void sliding_dkdv_join(typename X::Sliding pr,
 // walk, or the longest walk alone, and three tiles' time for a workgroup's start
 // and end, six where it leaves partial sums.  (The lengths of a padded batch are
 // not known here: all signals count as full.)
-// masked: with documents or a prefix, whose blocks' walks leave no rows behind.
-inline WalkSplit walk_split(const SlidingProblem &pr, bool masked = false) {
+// With documents or a prefix walks leave no rows behind, and where there is a prefix
+// the first block's is all rows.  Partial sums count for more where most walks are short:
+// 2 x 4096 tokens, 16 heads of 128 over 4, window 1024, prefixes of 64: a backward of 624
+// us in one part, 413 in two, 349 in three, 411 in six; 3 x 1531 tokens, 16 heads of 64
+// over 8, window 512, prefixes of 576: 103, 129, 132 and 168.
+inline WalkSplit walk_split(const SlidingProblem &pr, int masked = kUnmasked) {
     const bool wide = pr.dtype == CIRCATT_F32;
     const int QT = wide ? 32 : 64, DP = (pr.D + 31) / 32 * 32;
     WalkSplit sp;
@@ -1134,11 +1138,11 @@ inline WalkSplit walk_split(const SlidingProblem &pr, bool masked = false) {
     };
     double all = 0;
     for (int kb = 0; kb < sp.blocks; ++kb) all += walk(kb * 128);
-    const double mean = all / sp.blocks, longest = walk(0);
+    const double mean = all / sp.blocks, longest = masked == kPrefix ? (double)pr.L * pr.G / QT : walk(0);
     double best = 1e300;
     for (int p = 1; p <= 8; ++p) {
         const double rounds = (double)((n * p + 255) / 256), a = rounds * (mean / p), b = longest / p;
-        const double cost = (a > b ? a : b) + rounds * (p > 1 ? 6 : 3);
+        const double cost = (a > b ? a : b) + rounds * (p == 1 ? 3 : masked == kUnmasked ? 6 : 12);
         if (cost < best) best = cost, sp.parts = p;
     }
     // sinks that are seen from behind the window of their block; 4 tiles of 32 rows
@@ -1146,7 +1150,7 @@ inline WalkSplit walk_split(const SlidingProblem &pr, bool masked = false) {
     sp.far = 0;
     sp.far_parts = 1;
     const int64_t behind = (int64_t)pr.L - 127 - pr.W;
-    if (!masked && pr.S > 0 && behind > 0) {
+    if (masked == kUnmasked && pr.S > 0 && behind > 0) {
         const int64_t seen = pr.S < behind + 127 ? pr.S : behind + 127;
         sp.far = (int)((seen + 31) / 32);
         // and no more workgroups than fill the chip four times

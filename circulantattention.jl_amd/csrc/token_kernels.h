@@ -64,10 +64,14 @@ int64_t sliding_bwd_workspace_floats(const SlidingProblem &pr);
 int64_t sliding_threads(const SlidingProblem &pr, bool backward);
 hipError_t launch_sliding_fwd(const SlidingProblem &pr, hipStream_t s);
 hipError_t launch_sliding_bwd(const SlidingProblem &pr, hipStream_t s);
-// The same with shaped scores.  biased, masked: whether slopes, and places or a
-// prefix, are there (the workspace is asked for without them).
-int64_t shaped_bwd_workspace_floats(const SlidingProblem &pr, bool biased, bool masked);
-int64_t shaped_sliding_threads(const SlidingProblem &pr, bool masked, bool backward);
+// The same with shaped scores.  biased: whether slopes are there; masked: what else rows
+// see (the workspace is asked for without the arrays).
+enum Masked { kUnmasked, kPlaces, kPrefix };
+inline int masked_by(const ScoreShape &sh) {
+    return sh.places != nullptr ? kPlaces : sh.prefix != nullptr ? kPrefix : kUnmasked;
+}
+int64_t shaped_bwd_workspace_floats(const SlidingProblem &pr, bool biased, int masked);
+int64_t shaped_sliding_threads(const SlidingProblem &pr, int masked, bool backward);
 hipError_t launch_shaped_fwd(const ShapedSlidingProblem &pr, hipStream_t s);
 hipError_t launch_shaped_bwd(ShapedSlidingProblem pr, hipStream_t s);
 

@@ -145,17 +145,30 @@ struct PlainScorer {
     template <int NB>
     __device__ __forceinline__ void shape(f16v (&)[NB], int, int, int, int) const {}
 };
-template <bool CAP, bool FINE>
+// ANEW: the kernel's first argument, from which the curve is read for every tile where
+// its numbers would take more scalar registers through a loop than there are; or void.
+struct KeptCurve {
+    Curve kept;
+    __device__ __forceinline__ explicit KeptCurve(const Curve &c) : kept(c) {}
+    __device__ __forceinline__ Curve get() const { return kept; }
+};
+template <typename P>
+struct ReadCurve {
+    __device__ __forceinline__ explicit ReadCurve(const Curve &) {}
+    __device__ __forceinline__ Curve get() const { return argument_again<P>().shape.curve; }
+};
+template <bool CAP, bool FINE, typename From = KeptCurve>
 struct ShapedScorer {
-    Curve curve;
-    float c, slope;
+    From from;
+    float c, C, slope;
     bool biased;
     // Scores that no bias takes off lie within the cap: where 2^cap and its reciprocal are
     // well within the type that probabilities are rounded to, zero is as good a reference
     // for the softmax as the largest score, and none is looked for.
     bool bounded;
     __device__ __forceinline__ ShapedScorer(float scale, const Curve &curve, float slope, bool biased, bool wide)
-        : curve(curve), c(scale * kLog2e), slope(slope), biased(biased), bounded(CAP && wide && !biased && curve.C <= 90.f) {}
+        : from(curve), c(scale * kLog2e), C(curve.C), slope(slope), biased(biased),
+          bounded(CAP && wide && !biased && curve.C <= 90.f) {}
     template <int NB, typename R>
     __device__ __forceinline__ float largest(const R &x, const f16v (&s)[NB]) const {
         if (CAP && bounded) return 0.f;
@@ -168,7 +181,7 @@ struct ShapedScorer {
     }
     // What the registers still lack to scores in powers of two: they hold products, or
     // tangents of capped ones, and where there are slopes the scores themselves.
-    __device__ __forceinline__ float unit() const { return CAP ? curve.C : c; }
+    __device__ __forceinline__ float unit() const { return CAP ? C : c; }
     __device__ __forceinline__ float factor() const { return biased ? 1.f : unit(); }
     // Tangents in the place of products: all by the series, or all by the exponential.
     // (The products pass through an empty asm on each side, or the compiler forms all
@@ -184,6 +197,8 @@ struct ShapedScorer {
     }
     template <int NB>
     __device__ __forceinline__ void caps(f16v (&s)[NB]) const {
+        if constexpr (!CAP) return;
+        const Curve curve = from.get();
         if constexpr (CAP && FINE) {
             each(s, [&](float d) { return curve_fine(curve, d); });
         } else if constexpr (CAP) {

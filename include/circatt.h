@@ -392,7 +392,7 @@ int circatt_paged_append(int dtype, int64_t T, int64_t B, int64_t channels, cons
  * unspecified rows.  Prefix and places do not go together.  slopes need L (or max_pages *
  * page_size) of at most 2^24.  No gradient of the slopes is formed.
  *
- * biased, masked: whether slopes, and whether prefix or places, will be given.
+ * biased: whether slopes will be given; masked: 0, 1 with places, 2 with a prefix.
  */
 int circatt_shaped_fwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
                        int64_t window, int64_t sinks, float scale, float cap, const float *slopes,

@@ -95,10 +95,11 @@ def test_workspaces(L):
     args = (3, 500, 2, 4, 2, 64, 16, 0)
     assert size(*args, 0, 0) >= plain(*args)
     assert size(*args, 1, 0) >= size(*args, 0, 0) + 4 * (500 * 4 + 500 * 2)  # slopes and tokens of packed rows
-    assert size(*args, 0, 1) >= plain(*args) + 4 * 500 * 2                   # ends of documents
+    assert size(*args, 0, 1) >= 4 * (500 * 4 * 2 + 500 * 2)                  # sums of the rows, ends of documents
     # sinks behind the window are a walk of their own, but not with documents or a prefix
     far = (3, 4000, 2, 4, 2, 64, 16, 40)
     assert size(*far, 0, 0) > size(*far, 0, 1)
+    assert size(*args, 0, 3) == size(*args, 0, -1) == -1
     assert size(3, 0, 2, 4, 2, 64, 16, 0, 1, 1) == 0 and size(3, 64, 2, 4, 3, 64, 16, 0, 0, 0) == -1
     expect(L, bwd(L, shape(slopes=P), wbytes=100), -1, "workspace of 100")
     expect(L, bwd(L, shape(cap=3.0), work=None), -1, "workspace is NULL")
