@@ -124,7 +124,7 @@ def _shape(q, B, nheads, cap, slopes, prefix, places=None):
             raise AssertionError(f"slopes must have shape {(nheads,)}, got {tuple(slopes.shape)}")
         if slopes.requires_grad and torch.is_grad_enabled():
             raise AssertionError("slopes must not require gradients: none is formed")
-        slopes = slopes.detach().contiguous()
+        slopes = slopes.contiguous()
     if prefix is not None:
         prefix = _index(prefix, "prefix", q, (B,))
     if places is not None:

@@ -95,7 +95,7 @@ struct PlainSequence {
         return TileList<KT>(lo, hi, pr.W, pr.S);
     }
     template <typename T>
-    __device__ __forceinline__ PlainScorer scorer(const PagedProblem &pr, int) const {
+    __device__ __forceinline__ PlainScorer scorer(const PagedProblem &pr, const Block &, int, int, int) const {
         return PlainScorer{pr.scale * kLog2e};
     }
     __device__ __forceinline__ PlainView view(const PagedProblem &pr, int pos, int) const {
@@ -118,11 +118,20 @@ struct ShapedSequence {
     __device__ __forceinline__ ShapedTiles<KT> tiles(const ShapedPagedProblem &pr, int lo, int hi) const {
         return ShapedTiles<KT>(lo, hi, pr.W, pr.S, P, 0);
     }
+    // Whether the pages of the positions [lo, hi] are all in the cache.
+    __device__ __forceinline__ static bool there(const ShapedPagedProblem &pr, const Block &w, int lo, int hi) {
+        bool none = false;
+        for (int e = (lo >> pr.page_log2) + (threadIdx.x & 63); e <= hi >> pr.page_log2; e += 64)
+            none |= (unsigned)pr.pages[w.b * pr.pages_row + e] >= (unsigned)pr.npages;
+        return !__any(none);
+    }
+    // lo, hi: the block's first and last position that see something
     template <typename T>
-    __device__ __forceinline__ ShapedScorer<CAP, CAP && sizeof(T) == 4> scorer(const ShapedPagedProblem &pr, int h) const {
-        const bool biased = pr.shape.slopes != nullptr;
+    __device__ __forceinline__ ShapedScorer<CAP, CAP && sizeof(T) == 4> scorer(const ShapedPagedProblem &pr, const Block &w, int lo,
+                                                                               int hi, int h) const {
+        const bool biased = pr.shape.slopes != nullptr, own = CAP && !__is_same(T, _Float16) && (!biased || there(pr, w, lo, hi));
         return ShapedScorer<CAP, CAP && sizeof(T) == 4>(pr.scale, pr.shape.curve, biased ? pr.shape.slopes[h] * kLog2e : 0.f,
-                                                        biased, !__is_same(T, _Float16));
+                                                        biased, own);
     }
     __device__ __forceinline__ ShapedView view(const ShapedPagedProblem &pr, int pos, int h) const {
         const float slope = pr.shape.slopes == nullptr ? 0.f : pr.shape.slopes[h] * kLog2e;
@@ -260,7 +269,8 @@ __device__ __forceinline__ float without_weights(bool sees) { return sees ? NAN 
 
 // A wavefront's 32 rows (lane: row r of the block's sequence): their outputs, or
 // their partial sums.  Outputs that are not finite are formed again from the keys that
-// the row sees alone, if a value that is not finite lies where they do not see it.
+// the row sees alone, if a value that is not finite lies where they do not see it (those
+// of capped scores always: their reference may be less than the largest).
 template <typename X, typename T, int DP, int R>
 __device__ __forceinline__ void finish_rows(const typename X::Paged &pr, const PagedGrid &gr, int id, const Block &w,
                                             const RowSight &rs, int r, int lane, const f16v (&o)[DP / 32], float m, float l) {
@@ -273,14 +283,14 @@ __device__ __forceinline__ void finish_rows(const typename X::Paged &pr, const P
                           l, pr.D, lane);
         return;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : out_of_reach<X::kCap>(l);
     T *y = static_cast<T *>(pr.y) + w.q0 * pr.H * pr.D + head * pr.G;
     const bool bad = r < w.rows && store_channels(o, y + ((int64_t)rs.tok * pr.H + rs.g) * pr.D, pr.D, lane, inv);
     // NaN weights: the row is NaN, whatever it sees
     uint32_t again = rows_of(__ballot(bad && l > 0.f)), empty = rows_of(__ballot(r < w.rows && l == 0.f));
     const PagedKV<T> kv = paged_rows_of<T>(pr, w.b, head);
     if ((again | empty) != 0) __threadfence_block();  // other lanes' stores
-    if (again != 0 && !hidden_values(pr, kv, rs, sq)) again = 0;
+    if (!X::kCap && again != 0 && !hidden_values(pr, kv, rs, sq)) again = 0;
     int asked = -1;
     bool sees = false;
     for (; empty; empty &= empty - 1) {
@@ -321,7 +331,7 @@ __device__ __forceinline__ void few_rows(const typename X::Paged &pr, const Page
     const typename SequenceOf<X>::type sq(pr, w);
     const auto see = sq.sight(pr);
     const auto tiles = sq.template tiles<32>(pr, rs.blo, rs.bhi);
-    const auto score = sq.template scorer<T>(pr, hk * pr.G + rs.g);
+    const auto score = sq.template scorer<T>(pr, w, rs.blo, rs.bhi, hk * pr.G + rs.g);
     const Pages<T> pg(pr, w, rs, hk, sq.head(pr), sq.keys(rs.bhi));
     const int parts = gr.splits * NW, part = blockIdx.z * NW + wave;
     const int i0 = (int)((int64_t)tiles.count * part / parts), i1 = (int)((int64_t)tiles.count * (part + 1) / parts);
@@ -360,7 +370,7 @@ __device__ __forceinline__ void few_rows(const typename X::Paged &pr, const Page
                 asm volatile("");
                 hide_keys(s[0], see.bits(rs.at, k0) & there, lane);
             }
-            score.raise(x, score.largest(x, s));
+            score.raise(x, score.largest(x, s, i == i0));
             x.weigh(s, p, score.factor());
             x.template add<1>(col_at + to, p);
         }
@@ -426,7 +436,7 @@ __device__ __forceinline__ void chunk_rows(const typename X::Paged &pr, const Pa
     const typename SequenceOf<X>::type sq(pr, w);
     const auto see = sq.sight(pr);
     const auto tiles = sq.template tiles<KT>(pr, rs.blo, rs.bhi);
-    const auto score = sq.template scorer<T>(pr, hk * pr.G + rs.g);
+    const auto score = sq.template scorer<T>(pr, w, rs.blo, rs.bhi, hk * pr.G + rs.g);
     const Pages<T> pg(pr, w, rs, hk, sq.head(pr), sq.keys(rs.bhi));
     const int parts = gr.splits * NG;
     auto bound = [&](int part) { return (int)((int64_t)tiles.count * part / parts); };
@@ -481,7 +491,7 @@ __device__ __forceinline__ void chunk_rows(const typename X::Paged &pr, const Pa
                 for (int m = 0; m < NB; ++m)
                     hide_keys(s[m], see.bits(rs.at, k0 + 32 * m) & (uint32_t)(there >> (32 * m)), lane);
             }
-            score.raise(x, score.largest(x, s));
+            score.raise(x, score.largest(x, s, i == i0));
             x.weigh(s, p, c);
             x.template add<NB>(col_at + to, p);
         }
@@ -562,7 +572,7 @@ __global__ __launch_bounds__(256, 8) void paged_join(typename X::Paged pr, Paged
             l += ls * f;
             if (d < pr.D) o += *reinterpret_cast<const f4v *>(p.o + d) * f;
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = l == 0.f ? 0.f : out_of_reach<X::kCap>(l);
         const int tok = (w.r0 + ii) / pr.G, g = w.r0 + ii - tok * pr.G;
         T *y = static_cast<T *>(pr.y) + (w.q0 + tok) * pr.H * pr.D + head * pr.G + (int64_t)g * pr.D;
         V4<T> v;
@@ -578,7 +588,7 @@ __global__ __launch_bounds__(256, 8) void paged_join(typename X::Paged pr, Paged
         uint64_t again = __ballot(bad && l > 0.f && in);
         const PagedKV<T> kv = paged_rows_of<T>(pr, w.b, head);
         if ((again | empty) != 0) __threadfence_block();  // other lanes' stores
-        if (again != 0) {
+        if (!X::kCap && again != 0) {
             if (hidden < 0) hidden = hidden_values(pr, kv, RowSight::of<R>(pr, w, w.r0), sq);
             if (!hidden) again = 0;
         }

@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
         while (end > first && see.none(lo, hi, tiles.key(end), KT)) --end;
         const unsigned row_at = Tile<T, DP>::row_lane(lane) + ring, col_at = Tile<T, DP>::col_lane(lane) + ring + Rg::V;
         float mx = 0.f;
-        auto look = [&](f16v (&s)[NB], int i) {  // scores of tile i, its keys hidden, and the largest
+        auto look = [&](f16v (&s)[NB], int i, bool first) {  // scores of tile i, its keys hidden, and the largest
             const int k0 = tiles.key(i);
             score.shape(s, k0, at, lo, lane);
             if (!see.all(lo, hi, k0, KT)) {
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
 #pragma unroll
                 for (int m = 0; m < NB; ++m) hide_keys(s[m], see.bits(at, k0 + 32 * m), lane);
             }
-            mx = score.largest(x, s);
+            mx = score.largest(x, s, first);
         };
         auto step = [&](const f16v (&s)[NB], f16v (&t)[NB], int i) {
             round(i);
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             x.weigh(s, p, c);
             x.template add<NB>(col_at + vp * Rg::TILE, p);
             next();
-            look(t, i + 1);
+            look(t, i + 1, false);
         };
         f16v sa[NB], sb[NB];
         int i = -1;
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
         if (live) {
             round(i);
             x.scores(row_at + kp * Rg::TILE, sa);
-            look(sa, first);
+            look(sa, first, true);
             next();
             ++i;
             for (; i + 1 < end; i += 2) {
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
         if (live) {
             // a row sees its own token at least: without a sum of weights all that it sees
             // has the score -inf, and its softmax is NaN
-            const float l = x.total(), inv = 1.f / l;
+            const float l = x.total(), inv = out_of_reach<X::kCap>(l);
             bool bad = false;
             if (r < rows) {
                 bad = store_channels(x.o, y + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv);
@@ -260,10 +260,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             // weights is NaN or 0: then the row is, whatever it sees.)
             again = rows_of(__ballot(bad && l > 0.f));
             if (again != 0) {
+                // (With capped scores they may be for want of a larger reference too.)
                 const Problem pe = argument_again<Problem>();
                 const SignalKV<T> kv = signal_rows<T>(pe, b, hk);
                 auto tile_end = [&](int j) { return (int)((int64_t)j + KT - j % KT < n ? j + KT - j % KT : n); };
-                if constexpr (X::kShaped) {
+                if constexpr (X::kCap) {
+                } else if constexpr (X::kShaped) {
                     // Hidden from a row: what its tiles hold before its document and
                     // its window, the tiles of the first document's sinks or of the
                     // prefix, and what lies behind the first row.

@@ -131,11 +131,21 @@ struct ShapedTiles {
 // ---------------------------------------------------------------------------
 // Scores of 32 rows, one a lane, over blocks of 32 keys: registers hold the
 // products and then the scores.
+// What a row's sum of weighted values is multiplied by, from the sum of the weights: NaN,
+// as rows are marked that are formed again, where values might have been lost under the
+// weights.
+template <bool CAP>
+__device__ __forceinline__ float out_of_reach(float l) {
+    return CAP && l < 0x1p-20f ? NAN : 1.f / l;
+}
+
 struct PlainScorer {
     float c;
     __device__ __forceinline__ float factor() const { return c; }
+    // The rows' largest scores of a tile (first: the first that is looked at), and what
+    // follows of them for the reference of the exponentials.
     template <int NB, typename R>
-    __device__ __forceinline__ float largest(const R &x, const f16v (&s)[NB]) const {
+    __device__ __forceinline__ float largest(R &x, const f16v (&s)[NB], bool) const {
         return x.largest(s) * c;
     }
     template <typename R>
@@ -162,22 +172,27 @@ struct ShapedScorer {
     From from;
     float c, C, slope;
     bool biased;
-    // Scores that no bias takes off lie within the cap: where 2^cap and its reciprocal are
-    // well within the type that probabilities are rounded to, zero is as good a reference
-    // for the softmax as the largest score, and none is looked for.
+    // Scores lie below the cap, and a row's own token's, which no bias takes anything off,
+    // above its negative.  Where probabilities are rounded to a type with Float32's
+    // exponents, the largest score of the first tile alone is the softmax's reference then,
+    // or C - 100 if that is more: weights stay below 2^100, their sum below 2^124, and that
+    // of the row's own token, or of the first tile's best, above 2^(100 - 2 C).  (Rows whose
+    // sums of values pass Float32 so, or whose weights are all below 2^-20, are formed
+    // again: out_of_reach.)  `wide`: such a type, and rows that all see their own token.
     bool bounded;
     __device__ __forceinline__ ShapedScorer(float scale, const Curve &curve, float slope, bool biased, bool wide)
         : from(curve), c(scale * kLog2e), C(curve.C), slope(slope), biased(biased),
-          bounded(CAP && wide && !biased && curve.C <= 90.f) {}
+          bounded(CAP && wide && curve.C <= 90.f && __all(slope >= 0.f)) {}
     template <int NB, typename R>
-    __device__ __forceinline__ float largest(const R &x, const f16v (&s)[NB]) const {
-        if (CAP && bounded) return 0.f;
-        return x.largest(s) * factor();
+    __device__ __forceinline__ float largest(R &x, const f16v (&s)[NB], bool first) const {
+        if (CAP && bounded && !first) return 0.f;
+        const float most = x.largest(s) * factor();
+        if (CAP && bounded) x.m = fmaxf(most, C - 100.f);
+        return most;
     }
     template <typename R>
     __device__ __forceinline__ void raise(R &x, float most) const {
-        if (CAP && bounded) x.m = 0.f;
-        else x.raise(most);
+        if (!(CAP && bounded)) x.raise(most);
     }
     // What the registers still lack to scores in powers of two: they hold products, or
     // tangents of capped ones, and where there are slopes the scores themselves.

@@ -259,6 +259,62 @@ def test_scores_beyond_the_type_are_the_cap(ca, dtype, sign):
     assert (dq == 0).all() and (dk == 0).all() and torch.isfinite(dv).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cap,loud", [(20.0, 0.5), (20.0, 3.0), (20.0, 30.0), (400.0, 2.0), (400.0, 60.0), (400.0, 600.0),
+                                      (1e4, 1.0), (1e6, 1.0), (0.05, 1.0), (1e-4, 1.0)])
+def test_all_reaches_of_the_curve(ca, cap, loud, dtype):
+    """Scores far below the cap, about it and beyond it; caps that leave nothing and that
+    leave everything as it is."""
+    compare(ca, 1, 150, 2, 1, 64, 70, 3, None, DT[dtype], {"cap": cap}, loud=loud)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [1e30, 1e-25])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("biased", [False, True])
+def test_capped_values_of_any_size(ca, biased, sign, size, dtype):
+    """Values near the ends of Float32 under scores near the cap's: the weights' reference
+    must not cost their range.  Prompt, single tokens and chunks; half of the keys at one
+    end of the cap, half at the other, the first tiles at the lower one."""
+    L, H, D, page, dt = 400, 2, 64, 16, DT[dtype]
+    q, k = (randn(5 + i, 1, L, H * D, dtype=dt, scale=0.1) for i in range(2))
+    q.view(1, L, H, D)[..., 0] = 40.0
+    k.view(1, L, H, D)[..., 0] = 40.0 * sign * torch.where(torch.arange(L) < L // 2, -1.0, 1.0)[None, :, None]
+    v = randn(9, 1, L, H * D, dtype=dt, scale=size)
+    sh = {"cap": 60.0, "slopes": torch.tensor([0.01, 0.002]) if biased else None}
+    want = M.sliding(*(t.double() for t in (q, k, v)), L, H, H, 0, 1 / math.sqrt(D), None, dt, **sh)[0]
+    dev = {n: t.cuda() if isinstance(t, torch.Tensor) else t for n, t in sh.items()}
+    with torch.no_grad():
+        y = ca.sliding_mh_attention(q.cuda(), k.cuda(), v.cuda(), None, H, **dev)
+    M.check(y, want[0], want[1], "prompt")
+    pages, ck, cv = (t.cuda() for t in cache_of(5, [L], page, H * D, dt))
+    lengths = torch.tensor([L], dtype=torch.int32, device="cuda")
+    ca.paged_append_(ck, cv, k[0].cuda(), v[0].cuda(), pages, lengths, offsets=torch.tensor([0, L], dtype=torch.int32, device="cuda"))
+    for n in (1, 200):
+        offsets = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        y = ca.paged_mh_attention(q[0, L - n:].cuda(), ck, cv, pages, lengths, None, H, offsets=offsets, **dev)
+        M.check(y, want[0][0, L - n:], want[1][0, L - n:], f"{n} tokens")
+
+
+def test_slopes_with_a_tangent_are_refused(ca):
+    import torch.autograd.forward_ad as fwAD
+    q = torch.zeros(1, 8, 32, device="cuda")
+    with fwAD.dual_level():
+        slopes = fwAD.make_dual(torch.ones(2, device="cuda"), torch.ones(2, device="cuda"))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            ca.sliding_mh_attention(q, q, q, None, 2, slopes=slopes)
+
+
+def test_arrays_written_before_the_backward_are_noticed(ca):
+    q, k, v = (randn(3 + i, 1, 40, 64).cuda().requires_grad_(True) for i in range(3))
+    for name, t in (("slopes", torch.ones(2, device="cuda")), ("prefix", torch.tensor([5], dtype=torch.int32, device="cuda")),
+                    ("places", torch.arange(40, dtype=torch.int32, device="cuda")[None].clone())):
+        y = ca.sliding_mh_attention(q, k, v, 10, 2, **{name: t})
+        t.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
 def test_slopes_far_out(ca):
     """Distances whose bias passes what exponentials hold: the far keys count nothing."""
     L, H, D = 4000, 2, 32
