@@ -486,6 +486,11 @@ struct BwdShape {
 
 struct WalkSplit {
     int blocks, parts;   // of 128 keys; workgroups a block
+    int each;            // with documents or a prefix, tiles a part: short walks have fewer parts
+    __device__ __forceinline__ int of(int tiles) const {
+        const int p = (tiles + each / 2) / each;
+        return p < 1 ? 1 : p < parts ? p : parts;
+    }
     int far, far_parts;  // groups of 32 sinks that rows behind their window see; workgroups each
     FastDiv heads;       // G
     int64_t far_at, part_at;  // floats before the far sums and the parts' in the workspace
@@ -592,14 +597,17 @@ struct ShapedKeys {
         const bool far = j < P || j - document_start(places, j) < pr.S;
         return KeyRows{j < P ? 0 : j, far || most - j < pr.W ? most : j + pr.W};
     }
-    __device__ __forceinline__ KeyRows walk(const ShapedSlidingProblem &pr, int k0, int kn, int n, int lane) const {
-        if (!masked) return KeyRows{k0, n - kn > pr.W ? kn + pr.W : n};
-        int most = 0;
-        for (int j = k0 + lane; j <= kn; j += 64) {
-            const int e = rows(pr, j, n).end;
-            most = e > most ? e : most;
+    // The block's last key is seen furthest, a sink of its document, or of a prefix, to the
+    // document's end.
+    __device__ __forceinline__ KeyRows walk(const ShapedSlidingProblem &pr, int k0, int kn, int n, int) const {
+        int last = n;
+        bool far = k0 < P;
+        if (places != nullptr && k0 < n) {
+            const int e = ends[kn];
+            last = e < n ? e : n;
+            far = pr.S > 0 && k0 - document_start(places, kn) < pr.S;
         }
-        return KeyRows{k0 < P ? 0 : k0, wave_most(most)};
+        return KeyRows{k0 < P ? 0 : k0, far || last - kn < pr.W ? last : kn + pr.W};
     }
     // (keys from `end` on: what the walk's last has)
     __device__ __forceinline__ KeyRows one(const ShapedSlidingProblem &pr, int j0, int end, int lane) const {
@@ -949,10 +957,26 @@ void sliding_dkdv(typename X::Sliding pr, WalkSplit sp) {
     constexpr int QT = Sh::QT, NG = Sh::NG, NS = (X::kShaped ? 16 : 8) * QT;  // bytes of a tile's statistics
     __shared__ __attribute__((aligned(1024))) char lds_mem[NG * (4 * Sh::TILE + 2 * NS)];
     // workgroups of one unit: its blocks, part by part, on one XCD
-    const int64_t id = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-    const int64_t unit = id / (sp.blocks * sp.parts);
-    if (unit >= (int64_t)pr.B * pr.Hk) return;
-    const int in = (int)(id - unit * (sp.blocks * sp.parts)), kb = in / sp.parts, part = in - kb * sp.parts;
+    // (shaped: all blocks' last parts, which long walks alone have, then those before:
+    // the long walks begin first, and no idle workgroups lie at every other place, as
+    // workgroups go to the chip's engines in turn and would leave engines without work)
+    int64_t unit;
+    int kb, part;
+    if constexpr (X::kShaped) {
+        const int per = (gridDim.x >> 3) / sp.parts, at = blockIdx.x >> 3;
+        part = sp.parts - 1 - at / per;
+        const int64_t id = (int64_t)(blockIdx.x & 7) * per + at % per;
+        unit = id / sp.blocks;
+        if (unit >= (int64_t)pr.B * pr.Hk) return;
+        kb = (int)(id - unit * sp.blocks);
+    } else {
+        const int64_t id = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+        unit = id / (sp.blocks * sp.parts);
+        if (unit >= (int64_t)pr.B * pr.Hk) return;
+        const int in = (int)(id - unit * (sp.blocks * sp.parts));
+        kb = in / sp.parts;
+        part = in - kb * sp.parts;
+    }
     const HeadGroup<T> hg(pr, unit);
     const int n = hg.n, lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6) & 3, group = uniform(threadIdx.x >> 8);
     const int tid = threadIdx.x & 255;
@@ -962,7 +986,12 @@ void sliding_dkdv(typename X::Sliding pr, WalkSplit sp) {
     const KeyRows walk = keys.walk(pr, k0, kn, n, lane);
     const int begin = X::kShaped ? uniform(walk.first) : walk.first, end = X::kShaped ? uniform(walk.end) : walk.end;
     const int tiles = k0 < n ? ((end - begin) * pr.G + QT - 1) / QT : 0;
-    const int i0 = (int)((int64_t)tiles * part / sp.parts), i1 = (int)((int64_t)tiles * (part + 1) / sp.parts);
+    int parts = sp.parts;
+    if constexpr (X::kShaped) {
+        if (keys.masked) parts = uniform(sp.of(tiles));
+        if (part >= parts) return;
+    }
+    const int i0 = (int)((int64_t)tiles * part / parts), i1 = (int)((int64_t)tiles * (part + 1) / parts);
     const int j0 = k0 + 32 * wave, j = j0 + (lane & 31), jj = j < n ? j : n - 1;
     const unsigned lds = lds_byte((const CIRCATT_LDS char *)lds_mem) + group * 4 * Sh::TILE;
     const unsigned stats = lds_byte((const CIRCATT_LDS char *)lds_mem) + NG * 4 * Sh::TILE + group * 2 * NS;
@@ -1025,7 +1054,7 @@ void sliding_dkdv(typename X::Sliding pr, WalkSplit sp) {
         __syncthreads();
         if (group == 0) x.take(buf + wave * 64 * DP, lane_e);
     }
-    if (sp.parts == 1 && kb * 4 < sp.far) {
+    if (parts == 1 && kb * 4 < sp.far) {
         // the far sums of the block's keys, by everybody, as many groups of 32 keys at a
         // time as the tiles' memory holds: all four, but two of Float32 heads wider than 32
         constexpr int FIT = (int)sizeof(lds_mem) / (4 * Sh::FAR_PART), AT_ONCE = FIT < 4 ? FIT : 4;
@@ -1040,9 +1069,9 @@ void sliding_dkdv(typename X::Sliding pr, WalkSplit sp) {
             if (group == 0 && wave >= g && wave < g + now) x.take(buf + (wave - g) * 64 * DP, lane_e);
         }
     }
-    if (sp.parts > 1) {
+    if (parts > 1) {
         if (group == 0)
-            x.write(pr.work + sp.part_at + (unit * sp.blocks * sp.parts + in) * Sh::PART + (32 * wave + (lane_e & 31)) * DP,
+            x.write(pr.work + sp.part_at + ((unit * sp.blocks + kb) * sp.parts + part) * Sh::PART + (32 * wave + (lane_e & 31)) * DP,
                     128 * DP, lane_e);
         return;
     }
@@ -1080,6 +1109,16 @@ __global__ __launch_bounds__(256) void sliding_dkdv_join(typename X::Sliding pr,
         __syncthreads();
     }
     const HeadGroup<T> hg(pr, unit);
+    int parts = sp.parts;
+    if constexpr (X::kShaped) {
+        const ShapedKeys keys(pr, hg.b, hg.n);
+        if (keys.masked) {
+            const int k0 = group / 4 * 128, kn = k0 + 127 < hg.n - 1 ? k0 + 127 : hg.n - 1;
+            const KeyRows walk = keys.walk(pr, k0, kn, hg.n, lane);
+            parts = uniform(sp.of(k0 < hg.n ? ((walk.end - walk.first) * pr.G + Sh::QT - 1) / Sh::QT : 0));
+            if (parts == 1) return;  // the block's gradients are written
+        }
+    }
     for (int x = threadIdx.x >> 6; x < 32; x += 4) {
         const int j = group * 32 + x;
         if (j >= pr.L) return;
@@ -1099,7 +1138,7 @@ __global__ __launch_bounds__(256) void sliding_dkdv_join(typename X::Sliding pr,
             if (lane + 64 < DP) k.b = far[place(lane + 64)], v.b = far[Sh::FAR_PART / 2 + place(lane + 64)];
         }
         const float *w = pr.work + sp.part_at + (unit * sp.blocks + (j >> 7)) * sp.parts * Sh::PART + (j & 127) * DP;
-        for (int i = 0; i < sp.parts; ++i, w += Sh::PART) {
+        for (int i = 0; i < parts; ++i, w += Sh::PART) {
             const Pair a = load_row(w, lane, DP), c = load_row(w + Sh::PART / 2, lane, DP);
             k.a += a.a;
             k.b += a.b;
@@ -1123,10 +1162,11 @@ __global__ __launch_bounds__(256) void sliding_dkdv_join(typename X::Sliding pr,
 // and end, six where it leaves partial sums.  (The lengths of a padded batch are
 // not known here: all signals count as full.)
 // With documents or a prefix walks leave no rows behind, and where there is a prefix
-// the first block's is all rows.  Partial sums count for more where most walks are short:
-// 2 x 4096 tokens, 16 heads of 128 over 4, window 1024, prefixes of 64: a backward of 624
-// us in one part, 413 in two, 349 in three, 411 in six; 3 x 1531 tokens, 16 heads of 64
-// over 8, window 512, prefixes of 576: 103, 129, 132 and 168.
+// the first block's is all rows: parts are for those, and the kernels give short walks
+// fewer (of).  2 x 4096 tokens, 16 heads of 128 over 4, window 1024, prefixes of 64: 280
+// us and 22 to add up, in one part 520; all walks in four parts 305 and 28.  2 x 4099
+// tokens in documents of up to 1200, 12 heads of 80 over 4: 105 and 13, all walks in four
+// parts 108 and 22.
 inline WalkSplit walk_split(const SlidingProblem &pr, int masked = kUnmasked) {
     const bool wide = pr.dtype == CIRCATT_F32;
     const int QT = wide ? 32 : 64, DP = (pr.D + 31) / 32 * 32;
@@ -1147,6 +1187,9 @@ inline WalkSplit walk_split(const SlidingProblem &pr, int masked = kUnmasked) {
         const double cost = (a > b ? a : b) + rounds * (p == 1 ? 3 : masked == kUnmasked ? 6 : 12);
         if (cost < best) best = cost, sp.parts = p;
     }
+    // what a part is worth: half of the longest walk's, but 32 tiles
+    sp.each = (int)(longest / (2 * sp.parts));
+    sp.each = sp.each > 32 ? sp.each : 32;
     // sinks that are seen from behind the window of their block; 4 tiles of 32 rows
     // for each of four wavefronts
     sp.far = 0;
@@ -1182,7 +1225,8 @@ hipError_t backward(const typename X::Sliding &pr, const WalkSplit &sp, hipStrea
     if (pr.dk != nullptr) {
         const int64_t units = (int64_t)pr.B * pr.Hk;
         if (sp.far > 0) sliding_dkdv_far<X, T, DP><<<(unsigned)(units * sp.far * sp.far_parts), 256, 0, s>>>(pr, sp);
-        sliding_dkdv<X, T, DP><<<(unsigned)grid8(units * sp.blocks * sp.parts), 256 * BwdShape<T, DP>::NG, 0, s>>>(pr, sp);
+        const int64_t walks = X::kShaped ? grid8(units * sp.blocks) * sp.parts : grid8(units * sp.blocks * sp.parts);
+        sliding_dkdv<X, T, DP><<<(unsigned)walks, 256 * BwdShape<T, DP>::NG, 0, s>>>(pr, sp);
         if (sp.parts > 1) sliding_dkdv_join<X, T, DP><<<(unsigned)(units * ((pr.L + 31) / 32)), 256, 0, s>>>(pr, sp);
     }
     return hipGetLastError();
@@ -1215,7 +1259,7 @@ inline int64_t threads_of(const SlidingProblem &pr, const WalkSplit &sp, bool ba
     const int64_t units = (int64_t)pr.B * pr.Hk, rows = 256 * grid8(units * (((int64_t)pr.L * pr.G + 127) / 128));
     if (!backward) return rows;
     // 512 threads, but 256 for some Float32 heads
-    const int64_t keys = 512 * grid8(units * sp.blocks * sp.parts), far = 256 * units * sp.far * sp.far_parts;
+    const int64_t keys = 512 * grid8(units * sp.blocks) * sp.parts, far = 256 * units * sp.far * sp.far_parts;
     const int64_t join = sp.parts > 1 ? 256 * units * ((pr.L + 31) / 32) : 0;
     int64_t most = rows;
     for (int64_t n : {keys, far, join}) most = n > most ? n : most;
