@@ -138,7 +138,9 @@ struct SignalOf<Plain> {
     typedef PlainSignal type;
 };
 
-template <typename X, typename T, int DP>
+// KEPT: of a training step with shaped scores: y_rest takes y to the output that is
+// divided by the sum of the rounded weights (y itself is a call's without gradients).
+template <typename X, typename T, int DP, bool KEPT>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void sliding_fwd(typename X::Sliding pr, int blocks) {
     typedef typename X::Sliding Problem;
     typedef typename SignalOf<X>::type Signal;
@@ -204,12 +206,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             }
             mx = score.largest(x, s, first);
         };
+        auto weigh = [&](const f16v (&s)[NB], V8<T> (&p)[2 * NB]) {
+            x.template weigh<NB, KEPT>(s, p, c);
+        };
         auto step = [&](const f16v (&s)[NB], f16v (&t)[NB], int i) {
             round(i);
             V8<T> p[2 * NB];
             score.raise(x, mx);
             x.scores(row_at + kp * Rg::TILE, t);
-            x.weigh(s, p, c);
+            weigh(s, p);
             x.template add<NB>(col_at + vp * Rg::TILE, p);
             next();
             look(t, i + 1, false);
@@ -236,7 +241,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             round(i);
             V8<T> p[2 * NB];
             score.raise(x, mx);
-            x.weigh(sa, p, c);
+            weigh(sa, p);
             x.template add<NB>(col_at + vp * Rg::TILE, p);
             next();
             for (++i; i < count; ++i, next()) round(i);
@@ -249,7 +254,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
             bool bad = false;
             if (r < rows) {
                 bad = store_channels(x.o, y + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv);
-                if (rest != nullptr) store_rests(x.o, rest + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv);
+                if (rest != nullptr)
+                    store_rests(x.o, rest + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv,
+                                KEPT ? 1.f / x.total_rounded() : inv);
                 if (pr.lse != nullptr && lane < 32) pr.lse[stat + r] = x.m + __builtin_amdgcn_logf(l);
             }
             // A value that is not finite reaches, as 0 times itself, every row of
@@ -318,12 +325,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
 // cancel most, and with the rounded y alone the error of dq was up to 3 times that
 // of a form that rounds only its results, now 1.6.  2 x 4096 tokens, 16 heads of 128
 // over 4, window 512, bf16: 88 us, 550 TFLOP/s of the pairs that are seen.
+//
+// Of shaped scores dS goes into dQ' as two values of the element type, the second what
+// rounding took from the first: capped scores are large ones, of which few keys carry a
+// row, and dq was up to 2.2 times as far off as where its results alone are rounded;
+// with that and the forward's sum of rounded weights, 1.2 times.  A third more products
+// here: of 2 x 4099 tokens in documents of up to 1200, 12 heads of 80 over 4, f16, 87 us
+// have become 97, of 2 x 4096 with slopes, 16 heads of 128 over 4, window 1024, bf16,
+// 143 have become 165.
 template <typename X, typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void sliding_dq(typename X::Sliding pr, int blocks) {
     typedef typename SignalOf<X>::type Signal;
     typedef DqShape<T, DP> Sh;
     typedef Tile<T, DP> Tl;
     constexpr int KT = Sh::KT, STEPS = DP / 16, OT = DP / 32;
+    constexpr bool kLow = X::kShaped && sizeof(T) == 2;
     __shared__ __attribute__((aligned(1024))) char lds_mem[4 * Sh::TILE];
     const CIRCATT_LDS char *lds = (const CIRCATT_LDS char *)lds_mem;
     const BlockOrder w(pr.B * pr.Hk, blocks);
@@ -416,14 +432,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
                             if constexpr (X::kCap) bend[x] = 0.f;
                         }
                 }
-                V8<T> ds[2];
+                V8<T> ds[2], low[2];
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
                     rest += s[x];  // (of the capped scores: those sum to zero)
-                    ds[x >> 3][x & 7] = (T)(X::kCap ? s[x] * bend[x] : s[x]);
+                    const float e = X::kCap ? s[x] * bend[x] : s[x];
+                    ds[x >> 3][x & 7] = (T)e;
+                    if constexpr (kLow) low[x >> 3][x & 7] = (T)(e - (float)ds[x >> 3][x & 7]);
                 }
                 products<T, 2 * OT, 4>([&](int i) { return Tl::col(kc, 16 * (i & 1), i >> 1); },
-                                       [&](int i, V8<T> a) { o[i >> 1] = mma(a, ds[i & 1], o[i >> 1]); });
+                                       [&](int i, V8<T> a) {
+                                           o[i >> 1] = mma(a, ds[i & 1], o[i >> 1]);
+                                           if constexpr (kLow) o[i >> 1] = mma(a, low[i & 1], o[i >> 1]);
+                                       });
             }
         }
         // <dy, y> of the exact y is sum_j p_j <dy, v_j>: d and what the score gradients,
@@ -1215,7 +1236,13 @@ inline int64_t bwd_floats(const SlidingProblem &pr, const WalkSplit &sp) {
 template <typename X, typename T, int DP>
 hipError_t forward(const typename X::Sliding &pr, hipStream_t s) {
     const int blocks = (pr.L * pr.G + 127) / 128;
-    sliding_fwd<X, T, DP><<<(unsigned)grid8((int64_t)pr.B * pr.Hk * blocks), 256, 0, s>>>(pr, blocks);
+    const unsigned grid = (unsigned)grid8((int64_t)pr.B * pr.Hk * blocks);
+    if constexpr (X::kShaped && sizeof(T) == 2)
+        if (pr.y_rest != nullptr) {
+            sliding_fwd<X, T, DP, true><<<grid, 256, 0, s>>>(pr, blocks);
+            return hipGetLastError();
+        }
+    sliding_fwd<X, T, DP, false><<<grid, 256, 0, s>>>(pr, blocks);
     return hipGetLastError();
 }
 template <typename X, typename T, int DP>

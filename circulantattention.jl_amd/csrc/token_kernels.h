@@ -19,7 +19,7 @@ struct SlidingProblem {
     int64_t q_row, q_batch, k_row, k_batch, v_row, v_batch;
     const int32_t *lengths;  // (B) or NULL: all L
     void *y;                 // (B, L, H*D)
-    void *y_rest;            // what y's rounding took, laid out as y, or NULL
+    void *y_rest;            // what y lacks for its rounding, laid out as y, or NULL
     // log2 of a row's sum of exp2(scale log2(e) q.k), +inf for a row behind the
     // signal's length: (B, Hk, L*G), row i*G + g
     float *lse;

@@ -92,11 +92,16 @@ struct Lacks {
         if (b) p[lane + 64] = (T)v.b;
     }
 };
-// x minus x rounded to T, 0 where that is not finite.
+// What x (to `exact`, a value nearer to the one meant) lacks when rounded to T, 0 where
+// that is not finite.
+template <typename T>
+__device__ __forceinline__ T rounding_rest(float x, float exact) {
+    const float e = exact - (float)(T)x;
+    return fabsf(e) < INFINITY ? (T)e : (T)0.f;
+}
 template <typename T>
 __device__ __forceinline__ T rounding_rest(float x) {
-    const float e = x - (float)(T)x;
-    return fabsf(e) < INFINITY ? (T)e : (T)0.f;
+    return rounding_rest<T>(x, x);
 }
 __device__ __forceinline__ float wave_sum(float x) {
     for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m, 64);

@@ -270,6 +270,16 @@ __device__ __forceinline__ void hide_keys(f16v &s, uint32_t seen, int lane) {
         if (!(half & place_bit(i))) s[i] = -INFINITY;
 }
 
+// c + a + b by one instruction.
+__device__ __forceinline__ float add_pair(__bf16 a, __bf16 b, float c) {
+    typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(Pair{a, b}, Pair{1.f, 1.f}, c, false);
+}
+__device__ __forceinline__ float add_pair(_Float16 a, _Float16 b, float c) {
+    typedef _Float16 Pair __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(Pair{a, b}, Pair{1.f, 1.f}, c, false);
+}
+
 // Running softmax and output of 32 rows (lane l and l + 32: row l % 32).
 // Scores count in units of log2(e) scale; the row's maximum is raised only when
 // a score passes it by more than 2^6 in the exponent, so that most tiles leave
@@ -282,6 +292,7 @@ struct Rows {
     V8<T> q[STEPS];
     f16v o[OT];
     float m, l;  // l: this lane's keys alone
+    float rounded;
 
     __device__ __forceinline__ void start(const T *qrow, int D, int lane) {
 #pragma unroll
@@ -289,7 +300,7 @@ struct Rows {
 #pragma unroll
         for (int t = 0; t < OT; ++t) o[t] = f16v{};
         m = -INFINITY;
-        l = 0.f;
+        l = rounded = 0.f;
     }
 
     // A round of NB blocks of 32 keys, in steps.
@@ -316,6 +327,7 @@ struct Rows {
         if (__any(mx > m + RAISE || (m == -INFINITY && mx > -INFINITY))) {
             const float mn = fmaxf(m, mx), r = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             l *= r;
+            rounded *= r;
 #pragma unroll
             for (int t = 0; t < OT; ++t)
 #pragma unroll
@@ -323,7 +335,9 @@ struct Rows {
             m = mn;
         }
     }
-    template <int NB>
+    // KEPT: `rounded` sums the weights as they are rounded.  Where few keys carry a row,
+    // most of that error cancels from an output divided by this sum.
+    template <int NB, bool KEPT = false>
     __device__ __forceinline__ void weigh(const f16v (&s)[NB], V8<T> (&p)[2 * NB], float c) {
         const float mu = m == -INFINITY ? 0.f : m;
         float sum = 0.f;
@@ -336,6 +350,12 @@ struct Rows {
                 p[2 * n + (i >> 3)][i & 7] = (T)e;
             }
         l += sum;
+        if constexpr (KEPT) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2)
+#pragma unroll
+                for (int n = 0; n < 2 * NB; ++n) rounded = add_pair(p[n][i], p[n][i + 1], rounded);
+        }
     }
     template <int NB>
     __device__ __forceinline__ void add(unsigned vt, const V8<T> (&p)[2 * NB]) {
@@ -345,8 +365,9 @@ struct Rows {
             for (int t = 0; t < OT; ++t) o[t] = mma(Tile<T, DP>::col(vt, 16 * n, t), p[n], o[t]);
     }
 
-    // sum over both halves' keys
+    // sums over both halves' keys
     __device__ __forceinline__ float total() const { return l + __shfl_xor(l, 32, 64); }
+    __device__ __forceinline__ float total_rounded() const { return rounded + __shfl_xor(rounded, 32, 64); }
 };
 
 // The rows of a wavefront (bits: lanes, a row's two halves) as bits 0 .. 31.
@@ -414,9 +435,10 @@ __device__ __forceinline__ bool store_channels(const f16v (&o)[OT], T *y, int D,
         }
     return bad;
 }
-// What the rounding of such a row took (0 where it is not finite).
+// What the rounding of such a row took (0 where it is not finite); e: a factor that is
+// more exact than f, that the rests take their row to, or f.
 template <typename T, int OT>
-__device__ __forceinline__ void store_rests(const f16v (&o)[OT], T *rest, int D, int lane, float f) {
+__device__ __forceinline__ void store_rests(const f16v (&o)[OT], T *rest, int D, int lane, float f, float e) {
 #pragma unroll
     for (int t = 0; t < OT; ++t)
 #pragma unroll
@@ -424,7 +446,7 @@ __device__ __forceinline__ void store_rests(const f16v (&o)[OT], T *rest, int D,
             const int d = 32 * t + 2 * i + 4 * (lane >> 5);
             V4<T> v;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = rounding_rest<T>(o[t][i + j] * f);
+            for (int j = 0; j < 4; ++j) v[j] = rounding_rest<T>(o[t][i + j] * f, o[t][i + j] * e);
             if (d < D) *reinterpret_cast<V4<T> *>(rest + d) = v;
         }
 }

@@ -296,6 +296,26 @@ def test_capped_values_of_any_size(ca, biased, sign, size, dtype):
         M.check(y, want[0][0, L - n:], want[1][0, L - n:], f"{n} tokens")
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("W,docs", [(3, None), (40, None), (None, 30)], ids=str)
+def test_query_gradients_of_few_keys(ca, W, docs, dtype):
+    """Where few keys carry a row its score gradients cancel.  Rounded results alone are
+    off by a number e of the type (2-norm).  On top of those come weights rounded in y,
+    normalised by their own sum: with n keys that carry a row, the part of their
+    errors (e each) along the row's mean falls away, and what is left in <dy, y> is at
+    most e times the spread of <dy, v> over the row, the size of the score gradients
+    themselves.  Both together: sqrt(2) e."""
+    L, H, D = 400, 2, 64
+    q, k, v, dy = (randn(60 + i, 1, L, H * D, dtype=DT[dtype], scale=3.0 if i == 0 else 1.0) for i in range(4))
+    shape = {"cap": 30.0, "places": None if docs is None else places_of([[docs] * (L // docs)], L)}
+    got = run(ca, q, k, v, dy, W, H, H, 0, None, shape)
+    want = M.sliding(*(t.double() for t in (q, k, v)), W or L, H, H, 0, 1 / math.sqrt(D), None, DT[dtype], dy=dy.double(), **shape)
+    exact = want[1][0]
+    e = float((exact.to(DT[dtype]).double() - exact).norm())
+    assert float((got[1].double().cpu() - exact).norm()) <= math.sqrt(2.0) * e
+
+
+
 def test_slopes_with_a_tangent_are_refused(ca):
     import torch.autograd.forward_ad as fwAD
     q = torch.zeros(1, 8, 32, device="cuda")
