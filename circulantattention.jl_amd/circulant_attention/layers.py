@@ -92,9 +92,11 @@ class SlidingAttBlock(torch.nn.Module):
 
     def _apply(self, fn, *args, **kwargs):
         # the slopes stay Float32 in a block of another type
+        slopes = self.slopes
         out = super()._apply(fn, *args, **kwargs)
-        if self.slopes is not None:
-            self.slopes = self._slopes().to(self.slopes.device)
+        if slopes is not None:
+            at = self.slopes.device
+            self.slopes = (self._slopes() if slopes.is_meta and at.type != "meta" else slopes).to(at)
         return out
 
     def _project(self, x, positions):

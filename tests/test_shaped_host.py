@@ -243,3 +243,16 @@ def test_the_model_of_pages_keeps_count():
         rows, counts, moves = PM.compact(rows, counts)
         checked(rows, lengths, counts)
         assert all(c > 0 for c in counts[:sum(x > 0 for x in counts)])
+
+
+def test_a_block_keeps_its_slopes():
+    import circulant_attention as ca
+
+    m = ca.SlidingAttBlock(64, 20, nheads=2, distance=True)
+    assert torch.equal(m.slopes, torch.tensor([2.0 ** -4, 2.0 ** -8]))
+    m.slopes.mul_(3.0)  # others than it was made with
+    m = m.to(torch.bfloat16)
+    assert m.slopes.dtype == torch.float32 and torch.equal(m.slopes, 3.0 * torch.tensor([2.0 ** -4, 2.0 ** -8]))
+    assert next(m.parameters()).dtype == torch.bfloat16
+    m = m.to("meta").to_empty(device="cpu")
+    assert torch.equal(m.slopes, torch.tensor([2.0 ** -4, 2.0 ** -8])) and "slopes" not in m.state_dict()
