@@ -237,12 +237,12 @@ def sliding_mh_attention(q, k, v, W, nheads: int, *, kv_heads: int = None, sinks
     all -inf is NaN.  Differentiable in q, k, v, once and not in forward mode.
 
     The scores x_ij = scale <q_i, k_j> may be shaped: into
-    ``cap`` tanh(x_ij / cap), and by - ``slopes``[h] |i - j| behind that (float32,
-    (nheads,); not differentiable in them).  And what a token sees:
+    ``cap`` tanh(x_ij / cap) (with a scale above 0), and by - ``slopes``[h] |i - j| behind
+    that (float32, (nheads,); not differentiable in them).  And what a token sees:
     places (int32, (B, L)): signals that hold documents one after another, each token's
     place in its own, 0, 1, 2, ... (as axial_rotary takes positions).  A token sees
     its own document alone, whose first tokens are its sinks.  Places that do not
-    count up so give unspecified rows.
+    count up so give unspecified rows; those behind lengths are not looked at.
     prefix (int32, (B,)): every token of signal b sees the first prefix[b] ones too, those
     before them included.  Not together with places.
     Both are read on the device when the kernels run."""

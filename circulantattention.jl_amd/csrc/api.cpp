@@ -767,8 +767,8 @@ int check_rests(const void *rest, const void *y, int64_t bytes, int dtype) {
 namespace {
 
 // What scores are shaped by, for signals of up to `tokens` tokens.
-int check_shape(int dtype, float scale, float cap, const float *slopes, const int32_t *prefix, const int32_t *places, int64_t places_row,
-                int64_t tokens, ScoreShape &sh) {
+int check_shape(int dtype, float scale, float cap, const float *slopes, const int32_t *prefix, const int32_t *places,
+                int64_t places_row, int64_t tokens, ScoreShape &sh) {
     // the kernels form scale / cap and multiples of it and of the cap in Float32
     if (!(cap >= 0.f) || !(cap <= 1e30f) || (cap > 0.f && (!(scale / cap >= 1e-30f) || !(scale / cap <= 1e30f))))
         return fail(CIRCATT_ERR_INVALID, "cap=%g must be 0 or positive, and scale / cap within 1e-30 .. 1e30", (double)cap);

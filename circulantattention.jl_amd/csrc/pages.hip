@@ -408,7 +408,8 @@ __device__ __forceinline__ void compact_pages(const CompactProblem &pr, const in
 }
 __global__ __launch_bounds__(256) void compact_apply(CompactProblem pr) {
     const int used = pr.sizes[0], moved = pr.sizes[1];
-    compact_tables(pr, pr.counts, pr.holes, pr.movers, pr.rank, used, moved, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+    compact_tables(pr, pr.counts, pr.holes, pr.movers, pr.rank, used, moved,
+                   (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
     compact_pages(pr, pr.holes, pr.movers, moved, blockIdx.x, gridDim.x, threadIdx.x, 256);
 }
 

@@ -14,7 +14,8 @@ namespace {
 // What the keys' pass reads of every packed row and token: slopes times log2(e) and
 // tokens as Float32 (exact up to 2^24 of them), and where a token's document ends: at
 // the first later token whose own begins behind it.  (Starts ascend; whatever the
-// places hold, an end lies behind its token and not behind the signal.)
+// places hold, an end lies behind its token and not behind the signal, and those behind
+// its length are not looked at.)
 __global__ __launch_bounds__(256) void shape_rows(ShapedSlidingProblem pr) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t rows = (int64_t)pr.L * pr.G;
@@ -25,7 +26,8 @@ __global__ __launch_bounds__(256) void shape_rows(ShapedSlidingProblem pr) {
     if (pr.shape.places != nullptr && i < (int64_t)pr.B * pr.L) {
         const int b = (int)(i / pr.L), j = (int)(i - (int64_t)b * pr.L);
         const int32_t *places = pr.shape.places + b * pr.shape.places_row;
-        int lo = j + 1, hi = pr.L;  // the first t of (j, L) that begins behind j
+        const int n = signal_length(pr, b);
+        int lo = j + 1, hi = n > j ? n : j + 1;  // the first t of (j, n) that begins behind j
         while (lo < hi) {
             const int t = (lo + hi) >> 1;
             if (document_start(places, t) > j) hi = t;

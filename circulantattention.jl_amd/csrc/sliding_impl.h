@@ -606,7 +606,8 @@ struct ShapedKeys {
     bool masked;
     __device__ __forceinline__ ShapedKeys(const ShapedSlidingProblem &pr, int b, int n)
         : places(pr.shape.places == nullptr ? nullptr : pr.shape.places + b * pr.shape.places_row),
-          ends(pr.shape.places == nullptr ? nullptr : pr.ends + (int64_t)b * pr.L), P(uniform(clamp_prefix(pr.shape.prefix, b, n))),
+          ends(pr.shape.places == nullptr ? nullptr : pr.ends + (int64_t)b * pr.L),
+          P(uniform(clamp_prefix(pr.shape.prefix, b, n))),
           masked(pr.shape.places != nullptr || pr.shape.prefix != nullptr) {}
     // key j < n among rows below `end`, the signal's length or a walk's end
     __device__ __forceinline__ KeyRows rows(const ShapedSlidingProblem &pr, int j, int end) const {
@@ -693,7 +694,9 @@ template <bool CAP, bool FINE>
 struct ShapedKeyScore : ShapedScorer<CAP, FINE, ReadCurve<ShapedSlidingProblem>> {
     float token;  // of the key
     __device__ __forceinline__ ShapedKeyScore(const ShapedSlidingProblem &pr, int j)
-        : ShapedScorer<CAP, FINE, ReadCurve<ShapedSlidingProblem>>(pr.scale, pr.shape.curve, 0.f, pr.shape.slopes != nullptr, false), token((float)j) {}
+        : ShapedScorer<CAP, FINE, ReadCurve<ShapedSlidingProblem>>(pr.scale, pr.shape.curve, 0.f,
+                                                                   pr.shape.slopes != nullptr, false),
+          token((float)j) {}
 };
 template <typename X, typename T>
 struct KeyScoreOf {

@@ -360,6 +360,23 @@ def test_places_that_are_not_ascending_stay_in_bounds(ca):
             assert all((g[1, 77:] == 0).all() for g in got)
 
 
+@pytest.mark.parametrize("D,W", [(64, None), (32, 40)], ids=str)
+def test_places_behind_the_lengths_are_not_looked_at(ca, D, W):
+    L, H, lens = 900, 2, (900, 111, 300)
+    q, k, v, dy = (randn(80 + i, 3, L, H * D, dtype=torch.bfloat16) for i in range(4))
+    places = places_of([[60, 200, 5, 700], [70, 1000], [130, 128, 1000]], L)
+    lengths = torch.tensor(lens, dtype=torch.int32)
+    want = run(ca, q, k, v, dy, W or L, H, H, 3, lengths, {"places": places})
+    g = torch.Generator().manual_seed(1)
+    for low, high in ((-5, 5), (-2 ** 31, 2 ** 31 - 1), (L, 2 * L)):
+        other = places.clone()
+        for b, n in enumerate(lens):
+            other[b, n:] = torch.randint(low, high, (L - n,), generator=g, dtype=torch.int64).int()
+        for a, b in zip(run(ca, q, k, v, dy, W or L, H, H, 3, lengths, {"places": other}), want):
+            assert torch.equal(a, b)
+
+
+
 def test_rows_apart_streams_and_graphs(ca):
     """Parts of one projection read in place, on a stream of their own, and captured with the
     backward: every replay gives the eager results."""
