@@ -326,20 +326,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
 // of a form that rounds only its results, now 1.6.  2 x 4096 tokens, 16 heads of 128
 // over 4, window 512, bf16: 88 us, 550 TFLOP/s of the pairs that are seen.
 //
-// Of shaped scores dS goes into dQ' as two values of the element type, the second what
-// rounding took from the first: capped scores are large ones, of which few keys carry a
-// row, and dq was up to 2.2 times as far off as where its results alone are rounded;
-// with that and the forward's sum of rounded weights, 1.2 times.  A third more products
-// here: of 2 x 4099 tokens in documents of up to 1200, 12 heads of 80 over 4, f16, 87 us
-// have become 97, of 2 x 4096 with slopes, 16 heads of 128 over 4, window 1024, bf16,
-// 143 have become 165.
-template <typename X, typename T, int DP>
+// LOW: dS goes into dQ' as two values of the element type, the second what rounding took
+// from the first.  Capped scores are large ones, of which few keys carry a row, and dq was
+// up to 2.2 times as far off as where its results alone are rounded; with that and the
+// forward's sum of rounded weights, 1.2 times.  It is a third more products: of 2 x 4099
+// tokens in documents of up to 1200, 12 heads of 80 over 4, cap 30, f16, 87 us have become
+// 97.  Scores that are not capped have it (few_keys) where rows see few keys at most: with a
+// window of 3 keys rounded dS gives 1.53 times that error and with 512 1.46, and two
+// values there cost 22 us of 143 (2 x 4096 tokens, 16 heads of 128 over 4, window 1024,
+// slopes, bf16).
+template <typename X, typename T, int DP, bool LOW>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void sliding_dq(typename X::Sliding pr, int blocks) {
     typedef typename SignalOf<X>::type Signal;
     typedef DqShape<T, DP> Sh;
     typedef Tile<T, DP> Tl;
     constexpr int KT = Sh::KT, STEPS = DP / 16, OT = DP / 32;
-    constexpr bool kLow = X::kShaped && sizeof(T) == 2;
     __shared__ __attribute__((aligned(1024))) char lds_mem[4 * Sh::TILE];
     const CIRCATT_LDS char *lds = (const CIRCATT_LDS char *)lds_mem;
     const BlockOrder w(pr.B * pr.Hk, blocks);
@@ -438,12 +439,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
                     rest += s[x];  // (of the capped scores: those sum to zero)
                     const float e = X::kCap ? s[x] * bend[x] : s[x];
                     ds[x >> 3][x & 7] = (T)e;
-                    if constexpr (kLow) low[x >> 3][x & 7] = (T)(e - (float)ds[x >> 3][x & 7]);
+                    if constexpr (LOW) low[x >> 3][x & 7] = (T)(e - (float)ds[x >> 3][x & 7]);
                 }
                 products<T, 2 * OT, 4>([&](int i) { return Tl::col(kc, 16 * (i & 1), i >> 1); },
                                        [&](int i, V8<T> a) {
                                            o[i >> 1] = mma(a, ds[i & 1], o[i >> 1]);
-                                           if constexpr (kLow) o[i >> 1] = mma(a, low[i & 1], o[i >> 1]);
+                                           if constexpr (LOW) o[i >> 1] = mma(a, low[i & 1], o[i >> 1]);
                                        });
             }
         }
@@ -619,11 +620,11 @@ struct ShapedKeys {
         const bool far = j < P || j - document_start(places, j) < pr.S;
         return KeyRows{j < P ? 0 : j, far || most - j < pr.W ? most : j + pr.W};
     }
-    // The block's last key is seen furthest, a sink of its document, or of a prefix, to the
-    // document's end.
+    // The block's last key is seen furthest, a sink of its document to the document's end, or
+    // of a signal that has or might have had a prefix, and the prefix, to the signal's.
     __device__ __forceinline__ KeyRows walk(const ShapedSlidingProblem &pr, int k0, int kn, int n, int) const {
         int last = n;
-        bool far = k0 < P;
+        bool far = k0 < P || (masked && k0 < pr.S);
         if (places != nullptr && k0 < n) {
             const int e = ends[kn];
             last = e < n ? e : n;
@@ -1248,10 +1249,18 @@ hipError_t forward(const typename X::Sliding &pr, hipStream_t s) {
     sliding_fwd<X, T, DP, false><<<grid, 256, 0, s>>>(pr, blocks);
     return hipGetLastError();
 }
+// Whether rows may see few keys: in a narrow window, a short signal, documents of any length.
+inline bool few_keys(const SlidingProblem &pr) { return (pr.W < pr.L ? pr.W : pr.L) < 64; }
+inline bool few_keys(const ShapedSlidingProblem &pr) {
+    return pr.shape.places != nullptr || few_keys(static_cast<const SlidingProblem &>(pr));
+}
 template <typename X, typename T, int DP>
 hipError_t backward(const typename X::Sliding &pr, const WalkSplit &sp, hipStream_t s) {
     const int blocks = (pr.L * pr.G + 127) / 128;
-    sliding_dq<X, T, DP><<<(unsigned)grid8((int64_t)pr.B * pr.Hk * blocks), 256, 0, s>>>(pr, blocks);
+    const unsigned grid = (unsigned)grid8((int64_t)pr.B * pr.Hk * blocks);
+    constexpr bool HALF = X::kShaped && sizeof(T) == 2;
+    if (HALF && (X::kCap || few_keys(pr))) sliding_dq<X, T, DP, HALF><<<grid, 256, 0, s>>>(pr, blocks);
+    else sliding_dq<X, T, DP, HALF && X::kCap><<<grid, 256, 0, s>>>(pr, blocks);
     if (pr.dk != nullptr) {
         const int64_t units = (int64_t)pr.B * pr.Hk;
         if (sp.far > 0) sliding_dkdv_far<X, T, DP><<<(unsigned)(units * sp.far * sp.far_parts), 256, 0, s>>>(pr, sp);

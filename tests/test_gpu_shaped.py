@@ -296,6 +296,16 @@ def test_capped_values_of_any_size(ca, biased, sign, size, dtype):
         M.check(y, want[0][0, L - n:], want[1][0, L - n:], f"{n} tokens")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("S,W", [(1, 1), (4, 30), (130, 2)], ids=str)
+def test_sinks_of_signals_without_their_prefix(ca, S, W, dtype):
+    """A batch whose prefixes are empty but for one: sinks are seen from behind the windows
+    of their keys' blocks all the same."""
+    compare(ca, 3, 420, 2, 1, 32, W, S, (420, 420, 300), DT[dtype],
+            {"cap": 15.0, "prefix": torch.tensor([3, 0, 0], dtype=torch.int32)})
+
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("W,docs", [(3, None), (40, None), (None, 30)], ids=str)
 def test_query_gradients_of_few_keys(ca, W, docs, dtype):
