@@ -129,7 +129,7 @@ struct ShapedSequence {
     template <typename T>
     __device__ __forceinline__ ShapedScorer<CAP, CAP && sizeof(T) == 4> scorer(const ShapedPagedProblem &pr, const Block &w, int lo,
                                                                                int hi, int h) const {
-        const bool biased = pr.shape.slopes != nullptr, own = CAP && !__is_same(T, _Float16) && (!biased || there(pr, w, lo, hi));
+        const bool biased = pr.shape.slopes != nullptr, own = CAP && __is_same(T, __bf16) && (!biased || there(pr, w, lo, hi));
         return ShapedScorer<CAP, CAP && sizeof(T) == 4>(pr.scale, pr.shape.curve, biased ? pr.shape.slopes[h] * kLog2e : 0.f,
                                                         biased, own);
     }

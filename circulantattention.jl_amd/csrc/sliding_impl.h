@@ -121,7 +121,7 @@ struct ShapedSignal {
     __device__ __forceinline__ ShapedScorer<CAP, CAP && sizeof(T) == 4> scorer(const ShapedSlidingProblem &pr, int h) const {
         const bool biased = pr.shape.slopes != nullptr;
         return ShapedScorer<CAP, CAP && sizeof(T) == 4>(pr.scale, pr.shape.curve, biased ? pr.shape.slopes[h] * kLog2e : 0.f,
-                                                        biased, !__is_same(T, _Float16));
+                                                        biased, __is_same(T, __bf16));
     }
     __device__ __forceinline__ ShapedView view(const ShapedSlidingProblem &pr, int pos, int h) const {
         const float slope = pr.shape.slopes == nullptr ? 0.f : pr.shape.slopes[h] * kLog2e;
@@ -709,7 +709,9 @@ struct KeyScoreOf<Plain, T> {
 };
 
 // One wavefront's 32 keys: operands, sums, and 32 query rows' share of them.
-template <typename X, typename T, int DP>
+// LOW: P and dS as two values of the element type each (the second: what rounding took
+// from the first).
+template <typename X, typename T, int DP, bool LOW = false>
 struct KeySums {
     typedef Tile<T, DP> Tl;
     static constexpr int STEPS = DP / 16, OT = DP / 32, AHEAD = 4;
@@ -733,7 +735,7 @@ struct KeySums {
     // of the rows at LDS bytes st and st + stride; half: the rows that see the key, a
     // bit each, unless every one does
     struct Weights {
-        V8<T> p[2], ds[2];
+        V8<T> p[2], ds[2], low_p[2], low_ds[2];
     };
     // (and with slopes the rows' slopes and tokens, 2 and 3 strides on)
     typedef typename KeyScoreOf<X, T>::type Score;
@@ -781,6 +783,10 @@ struct KeySums {
         for (int x = 0; x < 16; ++x) {
             w.p[x >> 3][x & 7] = (T)s[x];
             w.ds[x >> 3][x & 7] = (T)dp[x];
+            if constexpr (LOW) {
+                w.low_p[x >> 3][x & 7] = (T)(s[x] - (float)w.p[x >> 3][x & 7]);
+                w.low_ds[x >> 3][x & 7] = (T)(dp[x] - (float)w.ds[x >> 3][x & 7]);
+            }
         }
     }
     __device__ __forceinline__ void add(unsigned qc, unsigned gc, const Weights &w) {
@@ -788,6 +794,10 @@ struct KeySums {
                                    [&](int i, V8<T> a) {
                                        if (i & 1) dk[i >> 2] = mma(a, w.ds[(i >> 1) & 1], dk[i >> 2]);
                                        else dv[i >> 2] = mma(a, w.p[(i >> 1) & 1], dv[i >> 2]);
+                                       if constexpr (LOW) {
+                                           if (i & 1) dk[i >> 2] = mma(a, w.low_ds[(i >> 1) & 1], dk[i >> 2]);
+                                           else dv[i >> 2] = mma(a, w.low_p[(i >> 1) & 1], dv[i >> 2]);
+                                       }
                                    });
     }
     // through LDS or a workspace, one float for every register and lane
@@ -973,7 +983,7 @@ __device__ __forceinline__ void sum_far(const float *w, int groups, int parts, C
     }
 }
 
-template <typename X, typename T, int DP>
+template <typename X, typename T, int DP, bool LOW>
 __global__ __launch_bounds__((256 * BwdShape<T, DP>::NG), (sizeof(T) == 2 && DP <= 64 ? 2 : 1))
 void sliding_dkdv(typename X::Sliding pr, WalkSplit sp) {
     typedef typename X::Sliding Problem;
@@ -1021,7 +1031,7 @@ void sliding_dkdv(typename X::Sliding pr, WalkSplit sp) {
     const unsigned lds = lds_byte((const CIRCATT_LDS char *)lds_mem) + group * 4 * Sh::TILE;
     const unsigned stats = lds_byte((const CIRCATT_LDS char *)lds_mem) + NG * 4 * Sh::TILE + group * 2 * NS;
     const typename KeyScoreOf<X, T>::type score(pr, j);
-    KeySums<X, T, DP> x;
+    KeySums<X, T, DP, LOW> x;
     if (i0 < i1) {
         // a group's turn i: tile i0 + NG i + group
         const int mine = (i1 - i0 - group + NG - 1) / NG, turns = (i1 - i0 + NG - 1) / NG;
@@ -1061,7 +1071,7 @@ void sliding_dkdv(typename X::Sliding pr, WalkSplit sp) {
                 const int r0 = first_row(i) + m;
                 if (r0 + 32 <= any0 || r0 >= any1) continue;
                 const unsigned to = (i & 1) * 2 * Sh::TILE + m * Tl::ROW;
-                typename KeySums<X, T, DP>::Weights w;
+                typename KeySums<X, T, DP, LOW>::Weights w;
                 x.weigh(row_at + to, row_at + to + Sh::TILE, stats + (i & 1) * NS + m * 4 + 16 * (lane >> 5), 4 * QT,
                         r0 >= all0 && r0 + 32 <= all1, bits_between(see0 - r0, see1 - r0) >> (4 * (lane >> 5)), score, w);
                 x.add(col_at + to, col_at + to + Sh::TILE, w);
@@ -1265,7 +1275,11 @@ hipError_t backward(const typename X::Sliding &pr, const WalkSplit &sp, hipStrea
         const int64_t units = (int64_t)pr.B * pr.Hk;
         if (sp.far > 0) sliding_dkdv_far<X, T, DP><<<(unsigned)(units * sp.far * sp.far_parts), 256, 0, s>>>(pr, sp);
         const int64_t walks = X::kShaped ? grid8(units * sp.blocks) * sp.parts : grid8(units * sp.blocks * sp.parts);
-        sliding_dkdv<X, T, DP><<<(unsigned)walks, 256 * BwdShape<T, DP>::NG, 0, s>>>(pr, sp);
+        // A signal of one block of keys: P and dS in two values (KeySums).  Its gradients are
+        // sums of few terms, and rounded ones gave some a dk 1.8 times as far off as where
+        // results alone are rounded, where longer signals have 1.45; a launch's time hides it.
+        if (HALF && pr.L <= 128) sliding_dkdv<X, T, DP, HALF><<<(unsigned)walks, 256 * BwdShape<T, DP>::NG, 0, s>>>(pr, sp);
+        else sliding_dkdv<X, T, DP, false><<<(unsigned)walks, 256 * BwdShape<T, DP>::NG, 0, s>>>(pr, sp);
         if (sp.parts > 1) sliding_dkdv_join<X, T, DP><<<(unsigned)(units * ((pr.L + 31) / 32)), 256, 0, s>>>(pr, sp);
     }
     return hipGetLastError();

@@ -173,12 +173,13 @@ struct ShapedScorer {
     float c, C, slope;
     bool biased;
     // Scores lie below the cap, and a row's own token's, which no bias takes anything off,
-    // above its negative.  Where probabilities are rounded to a type with Float32's
-    // exponents, the largest score of the first tile alone is the softmax's reference then,
-    // or C - 100 if that is more: weights stay below 2^100, their sum below 2^124, and that
-    // of the row's own token, or of the first tile's best, above 2^(100 - 2 C).  (Rows whose
-    // sums of values pass Float32 so, or whose weights are all below 2^-20, are formed
-    // again: out_of_reach.)  `wide`: such a type, and rows that all see their own token.
+    // above its negative.  Where probabilities are rounded to BFloat16, the largest score of
+    // the first tile alone is the softmax's reference then, or C - 100 if that is more:
+    // weights stay below 2^100, their sum below 2^124, and that of the row's own token, or
+    // of the first tile's best, above 2^(100 - 2 C).  (Rows whose sums of values pass Float32
+    // so, or whose weights are all below 2^-20, are formed again: out_of_reach.  Float16 does
+    // not hold such weights, and exponents of some 100 are off by 2^-18, ten times the rest of
+    // a Float32 signal's error.)  `wide`: that type, and rows that all see their own token.
     bool bounded;
     __device__ __forceinline__ ShapedScorer(float scale, const Curve &curve, float slope, bool biased, bool wide)
         : from(curve), c(scale * kLog2e), C(curve.C), slope(slope), biased(biased),

@@ -296,6 +296,39 @@ def test_capped_values_of_any_size(ca, biased, sign, size, dtype):
         M.check(y, want[0][0, L - n:], want[1][0, L - n:], f"{n} tokens")
 
 
+@pytest.mark.parametrize("shape", [(1, 666, 1, 8, 181, 20.0, 3), (1, 900, 2, 64, None, 7.0, None)], ids=str)
+def test_float32_signals_keep_their_precision(ca, shape):
+    """Gradients of capped scores (2-norm): a product's exponent is rounded by 2^-24 of its
+    size, which is the largest capped score times log2(e), 29, and twice that with the sum
+    of the weights; sums of n terms add sqrt(n) 2^-24.  Results of those are off by less than
+    2^-19 of themselves: (2 * 29 ln 2 + sqrt(900)) 2^-24 = 70 * 2^-24 at most, and a
+    quarter as rounding errors are not all alike."""
+    B, L, H, D, W, cap, docs = shape
+    q, k, v, dy = (randn(90 + i, B, L, H * D, scale=3.0 if i == 0 else 1.0) for i in range(4))
+    kw = {"cap": cap, "places": None if docs is None else places_of([[docs] * (L // docs)], L)}
+    got = run(ca, q, k, v, dy, W or L, H, H, 0, None, kw)
+    want = M.sliding(*(t.double() for t in (q, k, v)), W or L, H, H, 0, 1 / math.sqrt(D), None, torch.float32, dy=dy.double(), **kw)
+    for g, (x, _), name in zip(got, want, ("y", "dq", "dk", "dv")):
+        assert float((g.double().cpu() - x).norm() / x.norm()) <= 70 * 2.0 ** -26, name
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 5, 14, 2, 8), (1, 4, 16, 4, 128), (2, 2, 5, 1, 128), (1, 120, 2, 2, 64)], ids=str)
+def test_gradients_of_short_signals(ca, shape, dtype):
+    """Weights and score gradients go into the keys' gradients in two values, so that these
+    are off by their own rounding e (2-norm) and little more; <dy, y> with the weights'
+    rounding in y, as in test_query_gradients_of_few_keys, adds at most e to dk's."""
+    B, L, H, Hk, D = shape
+    q, k, v, dy = (randn(95 + i, B, L, h * D, dtype=DT[dtype], scale=3.0 if i == 0 else 1.0) for i, h in enumerate((H, Hk, Hk, H)))
+    kw = {"cap": 21.0}
+    got = run(ca, q, k, v, dy, L, H, Hk, 0, None, kw)
+    want = M.sliding(*(t.double() for t in (q, k, v)), L, H, Hk, 0, 1 / math.sqrt(D), None, DT[dtype], dy=dy.double(), **kw)
+    for g, (x, _) in zip(got[1:], want[1:]):
+        e = float((x.to(DT[dtype]).double() - x).norm())
+        assert float((g.double().cpu() - x).norm()) <= math.sqrt(2.0) * e
+
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("S,W", [(1, 1), (4, 30), (130, 2)], ids=str)
 def test_sinks_of_signals_without_their_prefix(ca, S, W, dtype):
