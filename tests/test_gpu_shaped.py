@@ -309,7 +309,7 @@ def test_float32_signals_keep_their_precision(ca, shape):
     got = run(ca, q, k, v, dy, W or L, H, H, 0, None, kw)
     want = M.sliding(*(t.double() for t in (q, k, v)), W or L, H, H, 0, 1 / math.sqrt(D), None, torch.float32, dy=dy.double(), **kw)
     for g, (x, _), name in zip(got, want, ("y", "dq", "dk", "dv")):
-        assert float((g.double().cpu() - x).norm() / x.norm()) <= 70 * 2.0 ** -26, name
+        assert float((g.detach().double().cpu() - x).norm() / x.norm()) <= 70 * 2.0 ** -26, name
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
