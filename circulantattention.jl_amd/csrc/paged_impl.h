@@ -365,13 +365,12 @@ __device__ __forceinline__ void few_rows(const typename X::Paged &pr, const Page
             f16v s[1];
             V8<T> p[2];
             x.scores(row_at + to, s);
-            score.shape(s, k0, rs.at, lo, lane);
+            score.lowered(x, s, k0, rs.at, lo, lane);
             if (there != ~0u || !(plain && see.all(lo, hi, k0, 32))) {
                 asm volatile("");
                 hide_keys(s[0], see.bits(rs.at, k0) & there, lane);
             }
-            score.raise(x, score.largest(x, s, i == i0));
-            x.weigh(s, p, score.factor());
+            score.weigh(x, s, p, i == i0);
             x.template add<1>(col_at + to, p);
         }
     } else {
@@ -446,7 +445,6 @@ __device__ __forceinline__ void chunk_rows(const typename X::Paged &pr, const Pa
         const int n = bound(blockIdx.z * NG + g + 1) - bound(blockIdx.z * NG + g);
         rounds = n > rounds ? n : rounds;
     }
-    const float c = score.factor();
     Rows<T, DP> x;
     const T *qr = static_cast<const T *>(pr.q) + (w.q0 + rs.tok) * pr.q_row + ((int64_t)(hk * pr.G + rs.g) * pr.D);
     x.start(qr, i0 < i1 ? pr.D : 0, lane);
@@ -484,15 +482,14 @@ __device__ __forceinline__ void chunk_rows(const typename X::Paged &pr, const Pa
             if (mine) x.scores(row_at + to, s);
             if (NG == 2) __builtin_amdgcn_s_barrier();
             if (!mine) continue;
-            score.shape(s, k0, rs.at, lo, lane);
+            score.lowered(x, s, k0, rs.at, lo, lane);
             if ((there & kFull) != kFull || !(plain && see.all(lo, hi, k0, KT))) {
                 asm volatile("");
 #pragma unroll
                 for (int m = 0; m < NB; ++m)
                     hide_keys(s[m], see.bits(rs.at, k0 + 32 * m) & (uint32_t)(there >> (32 * m)), lane);
             }
-            score.raise(x, score.largest(x, s, i == i0));
-            x.weigh(s, p, c);
+            score.weigh(x, s, p, i == i0);
             x.template add<NB>(col_at + to, p);
         }
         if (NG == 2 && group == 0) __builtin_amdgcn_s_barrier();

@@ -367,7 +367,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
         const auto see = sg.sight(pr, at, lo, hi);
         const auto tiles = sg.template tiles<KT>(pr, r0 / pr.G, last / pr.G);
         const auto score = sg.template scorer<T>(pr, hk * pr.G + g);
-        const float c = score.factor();
+        const float c = score.unit();
         auto fetch = [&](int i) {
             const int k0 = tiles.key(i);
             fetch_rows<T, DP, KT, 256>(kh, pr.k_row, k0, n, pr.D, lds + (i & 1) * 2 * Sh::TILE);
@@ -418,11 +418,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
 #pragma unroll
                         for (int x = 0; x < 16; ++x) bend[x] = score.bend(one[0][x]);
                     }
-                    score.biases(one, k0, at, lo, lane);
+                    score.exponents(one, k0, at, lo, lane, lse);
                     s = one[0];
                 }
 #pragma unroll
-                for (int x = 0; x < 16; ++x) s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -lse)) * (dp[x] - d);
+                for (int x = 0; x < 16; ++x)
+                    s[x] = __builtin_amdgcn_exp2f(X::kShaped ? s[x] : fmaf(s[x], c, -lse)) * (dp[x] - d);
                 if (!see.all(lo, hi, k0, 32)) {
                     asm volatile("");  // a branch: few tiles need it
                     const uint32_t half = see.bits(at, k0) >> (4 * (lane >> 5));
@@ -690,6 +691,7 @@ struct RowScoreOf<Plain> {
 struct PlainKeyScore {
     float c;
     __device__ __forceinline__ PlainKeyScore(const SlidingProblem &pr, int) : c(pr.scale * kLog2e) {}
+    __device__ __forceinline__ float unit() const { return c; }
 };
 template <bool CAP, bool FINE>
 struct ShapedKeyScore : ShapedScorer<CAP, FINE, ReadCurve<ShapedSlidingProblem>> {
@@ -748,7 +750,6 @@ struct KeySums {
                                           else s = mma(a, k[i >> 1], s);
                                       });
         f16v bend = f16v{};
-        float c;
         if constexpr (X::kShaped) {
             f16v one[1] = {s};
             score.caps(one);
@@ -757,18 +758,15 @@ struct KeySums {
 #pragma unroll
                 for (int x = 0; x < 16; ++x) bend[x] = score.bend(s[x]);
             }
-            score.bias_rows(s, st + 2 * stride, stride, score.token);
-            c = score.factor();
-        } else {
-            c = score.c;
+            score.exponents_of_rows(s, st, stride, score.token);
         }
 #pragma unroll
         for (int x = 0; x < 16; x += 4) {
-            const f4v ls = *(const CIRCATT_LDS f4v *)(st + 8 * x);
+            const f4v ls = X::kShaped ? f4v{} : *(const CIRCATT_LDS f4v *)(st + 8 * x);
             const f4v dd = *(const CIRCATT_LDS f4v *)(st + stride + 8 * x);
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-                s[x + y] = __builtin_amdgcn_exp2f(fmaf(s[x + y], c, -ls[y]));
+                s[x + y] = __builtin_amdgcn_exp2f(X::kShaped ? s[x + y] : fmaf(s[x + y], score.unit(), -ls[y]));
                 dp[x + y] = s[x + y] * (dp[x + y] - dd[y]);
                 if constexpr (X::kCap) dp[x + y] *= bend[x + y];
             }
@@ -1260,9 +1258,10 @@ hipError_t forward(const typename X::Sliding &pr, hipStream_t s) {
     return hipGetLastError();
 }
 // Whether rows may see few keys: in a narrow window, a short signal, documents of any length.
+// (Or heads are narrow, whose score gradients are large beside their sums: 1.58 in places.)
 inline bool few_keys(const SlidingProblem &pr) { return (pr.W < pr.L ? pr.W : pr.L) < 64; }
 inline bool few_keys(const ShapedSlidingProblem &pr) {
-    return pr.shape.places != nullptr || few_keys(static_cast<const SlidingProblem &>(pr));
+    return pr.shape.places != nullptr || pr.D <= 32 || few_keys(static_cast<const SlidingProblem &>(pr));
 }
 template <typename X, typename T, int DP>
 hipError_t backward(const typename X::Sliding &pr, const WalkSplit &sp, hipStream_t s) {

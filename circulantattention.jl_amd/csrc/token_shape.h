@@ -142,6 +142,7 @@ __device__ __forceinline__ float out_of_reach(float l) {
 struct PlainScorer {
     float c;
     __device__ __forceinline__ float factor() const { return c; }
+    __device__ __forceinline__ float unit() const { return c; }
     // The rows' largest scores of a tile (first: the first that is looked at), and what
     // follows of them for the reference of the exponentials.
     template <int NB, typename R>
@@ -154,6 +155,13 @@ struct PlainScorer {
     }
     template <int NB>
     __device__ __forceinline__ void shape(f16v (&)[NB], int, int, int, int) const {}
+    template <int NB, typename R>
+    __device__ __forceinline__ void lowered(const R &, f16v (&)[NB], int, int, int, int) const {}
+    template <int NB, typename R, typename P>
+    __device__ __forceinline__ void weigh(R &x, f16v (&s)[NB], P &p, bool) const {
+        x.raise(x.largest(s) * c);
+        x.weigh(s, p, c);
+    }
 };
 // ANEW: the kernel's first argument, from which the curve is read for every tile where
 // its numbers would take more scalar registers through a loop than there are; or void.
@@ -209,24 +217,24 @@ struct ShapedScorer {
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[n][i] = f(s[n][i]);
+            for (int i = 0; i < 16; ++i) s[n][i] = f(s[n][i], (float)(32 * n + 8 * (i >> 2) + (i & 3)));
     }
     template <int NB>
     __device__ __forceinline__ void caps(f16v (&s)[NB]) const {
         if constexpr (!CAP) return;
         const Curve curve = from.get();
         if constexpr (CAP && FINE) {
-            each(s, [&](float d) { return curve_fine(curve, d); });
+            each(s, [&](float d, float) { return curve_fine(curve, d); });
         } else if constexpr (CAP) {
             float most = 0.f;
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(s[n][i]));
-            if (!__any(most > curve.near)) each(s, [&](float d) { return curve_series(curve.few, d); });
-            else if (!__any(most > curve.far)) each(s, [&](float d) { return curve_series(curve.more, d); });
-            else if (curve.fine) each(s, [&](float d) { return curve_fine(curve, d); });
-            else each(s, [&](float d) { return fmaf(-2.f, curve_rest(curve, d), 1.f); });
+            if (!__any(most > curve.near)) each(s, [&](float d, float) { return curve_series(curve.few, d); });
+            else if (!__any(most > curve.far)) each(s, [&](float d, float) { return curve_series(curve.more, d); });
+            else if (curve.fine) each(s, [&](float d, float) { return curve_fine(curve, d); });
+            else each(s, [&](float d, float) { return fmaf(-2.f, curve_rest(curve, d), 1.f); });
         }
     }
     // The derivative of a capped score by the uncapped one, from its tangent.
@@ -236,11 +244,6 @@ struct ShapedScorer {
     template <int NB>
     __device__ __forceinline__ void biases(f16v (&s)[NB], int k0, int at, int lo, int lane) const {
         if (biased) bias(s, k0 + 4 * (lane >> 5) - at, k0 + 32 * NB - 1 <= lo);
-    }
-    template <int NB>
-    __device__ __forceinline__ void shape(f16v (&s)[NB], int k0, int at, int lo, int lane) const {
-        caps(s);
-        biases(s, k0, at, lo, lane);
     }
     template <int NB>
     __device__ __forceinline__ void bias(f16v (&s)[NB], int ahead, bool before) const {
@@ -261,16 +264,72 @@ struct ShapedScorer {
                     s[n][i] = fmaf(-slope, fabsf(d + (float)(32 * n + 8 * (i >> 2) + (i & 3))), s[n][i] * f);
         }
     }
-    // The same of one key's products with 32 rows, a row a register, whose slopes and
-    // tokens lie at LDS byte st and st + stride.
-    __device__ __forceinline__ void bias_rows(f16v &s, unsigned st, int stride, float token) const {
-        if (!biased) return;
+    template <int NB>
+    __device__ __forceinline__ void shape(f16v (&s)[NB], int k0, int at, int lo, int lane) const {
+        caps(s);
+        biases(s, k0, at, lo, lane);
+    }
+    // Exponents: the scores less `by`, which costs nothing behind a bias.
+    template <int NB>
+    __device__ __forceinline__ void exponents(f16v (&s)[NB], int k0, int at, int lo, int lane, float by) const {
+        const float f = unit(), ahead = (float)(k0 + 4 * (lane >> 5) - at);
+        if (!biased) {
+            each(s, [&](float d, float) { return fmaf(d, f, -by); });
+        } else if (k0 + 32 * NB - 1 <= lo) {
+            const float b = fmaf(slope, ahead, -by);
+            each(s, [&](float d, float k) { return fmaf(d, f, fmaf(slope, k, b)); });
+        } else {
+            each(s, [&](float d, float k) { return fmaf(-slope, fabsf(ahead + k), fmaf(d, f, -by)); });
+        }
+    }
+    // A tile's products to what its weights are formed from, hidden ones -inf by then, and
+    // those to weights; first: of the first tile that is looked at.  Capped scores go by
+    // exponents: chunks with cap, slopes and prefixes 167 us, 146 so.  Others have no
+    // reason to (128 us instead of 124), and in sliding_fwd, which has a tile more in
+    // registers, exponents spill (8192 tokens 563 us instead of 483).
+    template <int NB, typename R>
+    __device__ __forceinline__ void lowered(const R &x, f16v (&s)[NB], int k0, int at, int lo, int lane) const {
+        caps(s);
+        if constexpr (CAP) exponents(s, k0, at, lo, lane, x.reference());
+        else biases(s, k0, at, lo, lane);
+    }
+    template <int NB, typename R>
+    __device__ __forceinline__ float largest_lowered(R &x, f16v (&s)[NB], bool first) const {
+        if (bounded && !first) return 0.f;
+        const float most = x.largest(s);
+        if (bounded) {
+            x.m = fmaxf(most, C - 100.f);
+            x.lower(s, x.m);
+        }
+        return most;
+    }
+    template <int NB, typename R, typename P>
+    __device__ __forceinline__ void weigh(R &x, f16v (&s)[NB], P &p, bool first) const {
+        if constexpr (CAP) {
+            const float most = largest_lowered(x, s, first);
+            if (!bounded) x.raise(s, most);
+            x.weigh(s, p);
+        } else {
+            x.raise(largest(x, s, first));
+            x.weigh(s, p, factor());
+        }
+    }
+    // Exponents of one key's products (or tangents) with 32 rows, a row a register: the rows'
+    // logarithms of sums lie at LDS byte st, their slopes and tokens 2 and 3 strides behind.
+    __device__ __forceinline__ void exponents_of_rows(f16v &s, unsigned st, int stride, float token) const {
         const float f = unit();
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-            const f4v sl = *(const CIRCATT_LDS f4v *)(st + 8 * i), at = *(const CIRCATT_LDS f4v *)(st + stride + 8 * i);
+            const f4v ls = *(const CIRCATT_LDS f4v *)(st + 8 * i);
 #pragma unroll
-            for (int y = 0; y < 4; ++y) s[i + y] = fmaf(-sl[y], fabsf(at[y] - token), s[i + y] * f);
+            for (int y = 0; y < 4; ++y) s[i + y] = fmaf(s[i + y], f, -ls[y]);
+        }
+        if (!biased) return;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const f4v sl = *(const CIRCATT_LDS f4v *)(st + 2 * stride + 8 * i), at = *(const CIRCATT_LDS f4v *)(st + 3 * stride + 8 * i);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) s[i + y] = fmaf(-sl[y], fabsf(at[y] - token), s[i + y]);
         }
     }
 };

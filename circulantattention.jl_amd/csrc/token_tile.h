@@ -357,6 +357,43 @@ struct Rows {
                 for (int n = 0; n < 2 * NB; ++n) rounded = add_pair(p[n][i], p[n][i + 1], rounded);
         }
     }
+    // The same of exponents: scores from which the reference is taken off.
+    template <int NB>
+    __device__ __forceinline__ void weigh(const f16v (&s)[NB], V8<T> (&p)[2 * NB]) {
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(s[n][i]);
+                sum += e;
+                p[2 * n + (i >> 3)][i & 7] = (T)e;
+            }
+        l += sum;
+    }
+    // (of those: `most` is the row's largest, and they are lowered too)
+    template <int NB>
+    __device__ __forceinline__ void raise(f16v (&s)[NB], float most) {
+        if (__any(most > RAISE || (m == -INFINITY && most > -INFINITY))) {
+            const float mu = reference(), mn = fmaxf(m, most + mu), r = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            l *= r;
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] *= r;
+            m = mn;
+            lower(s, reference() - mu);
+        }
+    }
+    // what exponents are lowered by; nothing until a row has seen something
+    __device__ __forceinline__ float reference() const { return m == -INFINITY ? 0.f : m; }
+    template <int NB>
+    __device__ __forceinline__ static void lower(f16v (&s)[NB], float by) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] -= by;
+    }
     template <int NB>
     __device__ __forceinline__ void add(unsigned vt, const V8<T> (&p)[2 * NB]) {
 #pragma unroll
