@@ -14,7 +14,11 @@
 // the chain from load to load.  A call is two launches, a plan by one workgroup, whose
 // barriers stand between its steps, and the work of it by many; or one, where the plan's
 // workgroup does a small call's work as well (kSmall; a launch is some 3 us to the host
-// and 3 to the GPU).
+// and 3 to the GPU).  Kernels, us: fork to 128 of 64 sequences of 4096 2.8 + 2.7, resize of
+// those by a token 6.4 + 5.0; of 256 sequences of up to 2048, most by 512, 17.8 + 4.0; with
+// the plan's counts in memory instead of LDS that call took 31.5 in all, now 20.3.
+// Compaction of 64 sequences of up to 2048 tokens, 1024 channels, half of them gone, 7.3 +
+// 28.8, 5.9 TB/s of the move.
 #include "token_kernels.h"
 
 namespace circatt {
