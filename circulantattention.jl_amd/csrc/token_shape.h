@@ -327,7 +327,8 @@ struct ShapedScorer {
         if (!biased) return;
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-            const f4v sl = *(const CIRCATT_LDS f4v *)(st + 2 * stride + 8 * i), at = *(const CIRCATT_LDS f4v *)(st + 3 * stride + 8 * i);
+            const f4v sl = *(const CIRCATT_LDS f4v *)(st + 2 * stride + 8 * i);
+            const f4v at = *(const CIRCATT_LDS f4v *)(st + 3 * stride + 8 * i);
 #pragma unroll
             for (int y = 0; y < 4; ++y) s[i + y] = fmaf(-sl[y], fabsf(at[y] - token), s[i + y]);
         }
