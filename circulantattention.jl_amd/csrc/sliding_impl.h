@@ -418,12 +418,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
                                           });
                 f16v bend = f16v{};
                 if constexpr (X::kShaped) {
+                    if constexpr (X::kCap) score.caps(s, bend);
                     f16v one[1] = {s};
-                    score.caps(one);
-                    if constexpr (X::kCap) {
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) bend[x] = score.bend(one[0][x]);
-                    }
                     score.exponents(one, k0, at, lo, lane, lse);
                     s = one[0];
                 }
@@ -762,13 +758,7 @@ struct KeySums {
                                       });
         f16v bend = f16v{};
         if constexpr (X::kShaped) {
-            f16v one[1] = {s};
-            score.caps(one);
-            s = one[0];
-            if constexpr (X::kCap) {
-#pragma unroll
-                for (int x = 0; x < 16; ++x) bend[x] = score.bend(s[x]);
-            }
+            if constexpr (X::kCap) score.caps(s, bend);
             score.exponents_of_rows(s, st, stride, score.token);
         }
 #pragma unroll

@@ -29,15 +29,33 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float curve_rest(const Curve &c, float dot) {
     return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * c.u) + 1.f);
 }
-__device__ __forceinline__ float curve_fine(const Curve &c, float dot) {
-    const float a = dot * c.x, b = a * a;
+__device__ __forceinline__ float curve_power(float a) {
+    const float b = a * a;
     float p = -1382.f / 155925.f;
     p = fmaf(p, b, 62.f / 2835.f);
     p = fmaf(p, b, -17.f / 315.f);
     p = fmaf(p, b, 2.f / 15.f);
     p = fmaf(p, b, -1.f / 3.f);
-    const float small = fmaf(a * b, p, a);
+    return fmaf(a * b, p, a);
+}
+__device__ __forceinline__ float curve_fine(const Curve &c, float dot) {
+    const float a = dot * c.x, small = curve_power(a);
     return fabsf(a) < 0.35f ? small : fmaf(-2.f, curve_rest(c, dot), 1.f);
+}
+// A tangent with its derivative 1 - t^2 by the argument.  Formed of t that would be what
+// t's rounding left (off by a third of a per cent at 7, by all of it at 9); with r of |d|
+// it is 4 r (1 - r), as exact as r wherever t lies.
+struct Bent {
+    float t, bend;
+};
+__device__ __forceinline__ Bent curve_bent(const Curve &c, float dot) {
+    const float twice = 2.f * curve_rest(c, fabsf(dot)), t = 1.f - twice;
+    return Bent{copysignf(t, dot), fmaf(twice, t, twice)};
+}
+__device__ __forceinline__ Bent curve_fine_bent(const Curve &c, float dot) {
+    const float a = dot * c.x, small = curve_power(a);
+    const Bent far = curve_bent(c, dot);
+    return Bent{fabsf(a) < 0.35f ? small : far.t, far.bend};
 }
 template <int N>
 __device__ __forceinline__ float curve_series(const float (&p)[N], float dot) {
@@ -69,10 +87,7 @@ struct ShapedScore {
         const float s = cap ? curve.C * curve_fine(curve, dot) : c * dot;
         return fmaf(-slope, fabsf((float)back), s);
     }
-    __device__ __forceinline__ float bend(float dot) const {
-        const float t = cap ? curve_fine(curve, dot) : 0.f;
-        return fmaf(-t, t, 1.f);
-    }
+    __device__ __forceinline__ float bend(float dot) const { return cap ? curve_bent(curve, dot).bend : 1.f; }
 };
 struct ShapedView {
     int pos, start, begin, head, lo, end, S, P;
@@ -237,8 +252,36 @@ struct ShapedScorer {
             else each(s, [&](float d, float) { return fmaf(-2.f, curve_rest(curve, d), 1.f); });
         }
     }
-    // The derivative of a capped score by the uncapped one, from its tangent.
-    __device__ __forceinline__ static float bend(float t) { return fmaf(-t, t, 1.f); }
+    // The same, with the tangents' derivatives by their arguments.
+    template <typename F>
+    __device__ __forceinline__ static void each_bent(f16v &s, f16v &bend, F f) {
+        asm volatile("" : "+v"(s));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const Bent b = f(s[i]);
+            s[i] = b.t;
+            bend[i] = b.bend;
+        }
+    }
+    template <int N>
+    __device__ __forceinline__ static Bent series_bent(const float (&p)[N], float d) {
+        const float t = curve_series(p, d);
+        return Bent{t, fmaf(-t, t, 1.f)};
+    }
+    __device__ __forceinline__ void caps(f16v &s, f16v &bend) const {
+        const Curve curve = from.get();
+        if constexpr (FINE) {
+            each_bent(s, bend, [&](float d) { return curve_fine_bent(curve, d); });
+        } else {
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(s[i]));
+            if (!__any(most > curve.near)) each_bent(s, bend, [&](float d) { return series_bent(curve.few, d); });
+            else if (!__any(most > curve.far)) each_bent(s, bend, [&](float d) { return series_bent(curve.more, d); });
+            else if (curve.fine) each_bent(s, bend, [&](float d) { return curve_fine_bent(curve, d); });
+            else each_bent(s, bend, [&](float d) { return curve_bent(curve, d); });
+        }
+    }
     // Register i of block n is key k0 + 32 n + 8 (i / 4) + 4 half + i % 4; lo: the
     // first row's position, behind which a key's distance may count the other way.
     template <int NB>
