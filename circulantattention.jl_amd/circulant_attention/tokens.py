@@ -113,6 +113,8 @@ def _shape(q, B, nheads, cap, slopes, prefix, places=None):
     cap = float(cap or 0.0)
     if not 0.0 <= cap < math.inf:
         raise AssertionError(f"cap={cap} must be positive and finite, 0 or None: no cap")
+    if cap > 0.0 and ctypes.c_float(cap).value == 0.0:
+        raise AssertionError(f"cap={cap} is 0 in Float32, in which the kernels take it")
     if prefix is not None and places is not None:
         raise AssertionError("prefix and places do not go together")
     if slopes is not None:
