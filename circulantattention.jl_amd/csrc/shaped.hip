@@ -55,7 +55,8 @@ struct ShapedRegions {
 // [0, 0.3] and [0, 0.7] are least, 1.2e-6 and 3.0e-7 (found by linear programming over
 // 4000 places): 3.4e-7 and 1.8e-7 of the cap.  x is worked into their coefficients; where
 // Float32 does not hold one of those (scale / cap below some 1e-4 or above 1e4) they are
-// not taken.
+// not taken.  An error of 9e-5 of a score, 3.4e-7 of a cap of 256, is what 16-bit weights do
+// not show; under larger caps the series end at scores that have it.
 Curve make_curve(float cap, float scale, int dtype) {
     Curve c{};
     c.near = c.far = -1.f;
@@ -74,7 +75,8 @@ Curve make_curve(float cap, float scale, int dtype) {
         c.more[i] = (float)(kMore[i] * power);
         if (i < 3) c.few[i] = (float)(kFew[i] * power);
     }
-    if (held) c.near = (float)(0.3 / x), c.far = (float)(0.7 / x);
+    const double within = cap > 256.f ? 256.0 / cap : 1.0;
+    if (held) c.near = (float)(0.3 * within / x), c.far = (float)(0.7 * within / x);
     return c;
 }
 

@@ -23,6 +23,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // other instructions.  Where no product of a tile passes 0.7 / x, as in a model that
 // keeps its scores well below the cap, a series of five terms with the same error takes
 // six multiplications instead, and where none passes 0.3 / x one of three terms four.
+// Of caps above 256 the series are for scores of the size that those arguments have under
+// 256: a series then puts a score off by 1e-4 at most.
 // Float32, and caps above 256 outside the series' range, ask for more:
 // there arguments below 0.35 take the power series up to the eleventh term, whose next
 // is 2^-26 of it.
