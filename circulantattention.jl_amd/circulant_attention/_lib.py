@@ -96,6 +96,7 @@ SIGNATURES = {
     "circatt_shaped_bwd": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _p, _p, _p, _i64, _p,
                                   _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _p,
                                   _p, _p, _p, _i64, _p]),
+    "circatt_shaped_paged_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int]),
     "circatt_shaped_paged": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _p, _p, _p, _i64,
                                     _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _int, _p, _i64,
                                     _p]),

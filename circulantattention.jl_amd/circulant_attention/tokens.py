@@ -346,7 +346,9 @@ def paged_mh_attention(q, cache_k, cache_v, pages, lengths, W, nheads: int, *, k
             raise AssertionError(f"out must be contiguous {(T, nheads * dh)}")
     shape = None if not cap and slopes is None and prefix is None else _shape(q, B, nheads, cap, slopes, prefix)
     code = _CODES[q.dtype]
-    wbytes = L.lib.circatt_paged_workspace_bytes(code, T, B, nheads, kv_heads, dh, W, sinks, page, pages.shape[1])
+    room = (code, T, B, nheads, kv_heads, dh, W, sinks, page, pages.shape[1])
+    wbytes = (L.lib.circatt_paged_workspace_bytes(*room) if prefix is None
+              else L.lib.circatt_shaped_paged_workspace_bytes(*room, 1))
     work = torch.empty((wbytes // 4,), dtype=torch.float32, device=q.device) if wbytes > 0 else None
     sizes = (code, T, B, nheads, kv_heads, dh, W, sinks, scale)
     rest = (q.data_ptr(), q_row, cache_k.data_ptr(), cache_v.data_ptr(), npages, page, page_stride, row_stride,

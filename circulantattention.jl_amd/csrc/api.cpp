@@ -958,6 +958,15 @@ int64_t circatt_paged_workspace_bytes(int dtype, int64_t T, int64_t B, int64_t n
     return T == 0 ? 0 : 4 * paged_workspace_floats(pr);
 }
 
+int64_t circatt_shaped_paged_workspace_bytes(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
+                                             int64_t window, int64_t sinks, int64_t page_size, int64_t max_pages,
+                                             int prefixed) {
+    PagedProblem pr;
+    if (paged_problem(dtype, T, B, nheads, kv_heads, dh, window, sinks, 1.f, page_size, max_pages, pr) != CIRCATT_OK)
+        return -1;
+    return T == 0 ? 0 : 4 * paged_workspace_floats(pr, prefixed != 0);
+}
+
 namespace {
 
 // Everything of a call over a paged cache but the kinds of its scores and the launch; done: nothing to launch.
@@ -1033,7 +1042,11 @@ int circatt_shaped_paged(int dtype, int64_t T, int64_t B, int64_t nheads, int64_
     if (T == 0) return ok();
     const ShapeSpans sh(pr.shape, B, 0, nheads);
     CIRCATT_TRY(check_apart({span("y", y, 1, 0, T, nheads * dh, nheads * dh, esize_of(dtype))}, {sh.slopes, sh.prefix}));
-    return hip_result(launch_shaped_paged(pr, as_stream(stream)), "circatt_shaped_paged");
+    // the plan for prefixes where the workspace holds what it leaves, which may be more than
+    // was asked for above
+    const bool whole = prefix != nullptr && (workspace != nullptr ? workspace_bytes : 0) >= 4 * paged_workspace_floats(pr, true) &&
+                       reinterpret_cast<uintptr_t>(workspace) % 16 == 0;
+    return hip_result(launch_shaped_paged(pr, whole, as_stream(stream)), "circatt_shaped_paged");
 }
 
 int circatt_paged_append(int dtype, int64_t T, int64_t B, int64_t channels, const void *k, int64_t k_row, const void *v,

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) void append_rows(AppendProblem pr) {
 
 }  // namespace
 
-int64_t paged_workspace_floats(const PagedProblem &pr) { return paged_plan(pr).floats; }
+int64_t paged_workspace_floats(const PagedProblem &pr, bool whole) { return paged_plan(pr, whole).floats; }
 
 int64_t paged_threads(const PagedProblem &pr) {
     const PagedPlan pl = paged_plan(pr);
@@ -59,7 +59,7 @@ int64_t paged_threads(const PagedProblem &pr) {
     return 512 * ((int64_t)(pl.chunk ? pl.chunk_grid.blocks : 0) + pl.few_grid.blocks + 8);
 }
 
-hipError_t launch_paged(const PagedProblem &pr, hipStream_t s) { return launch_of<Plain>(pr, s); }
+hipError_t launch_paged(const PagedProblem &pr, hipStream_t s) { return launch_of<Plain>(pr, paged_plan(pr), s); }
 
 int64_t append_threads(const AppendProblem &pr) { return (pr.T + 3) / 4 * 256; }
 

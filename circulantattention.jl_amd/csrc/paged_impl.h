@@ -174,6 +174,19 @@ struct RowSight {
     }
 };
 
+// Of the parts that blocks of 32 rows have at most, those that a block with `tiles` tiles
+// has behind a prefix, by `waves` wavefronts each: of four rounds at least, which adding up
+// is worth.
+template <typename X>
+__device__ __forceinline__ int parts_of(const typename X::Paged &pr, int splits, int tiles, int waves) {
+    if constexpr (X::kShaped)
+        if (pr.shape.prefix != nullptr) {
+            const int p = uniform(tiles / (4 * waves));
+            return p < 1 ? 1 : p < splits ? p : splits;
+        }
+    return splits;
+}
+
 // What a block's rows may read of the cache: keys [0, S) (S: of sinks or a prefix) and
 // [low, len).
 template <typename T>
@@ -271,16 +284,16 @@ __device__ __forceinline__ bool hidden_values(const PagedProblem &pr, const Page
 __device__ __forceinline__ float without_weights(bool sees) { return sees ? NAN : 0.f; }
 
 // A wavefront's 32 rows (lane: row r of the block's sequence): their outputs, or
-// their partial sums.  Outputs that are not finite are formed again from the keys that
+// their partial sums (splits: the block's parts).  Outputs that are not finite are formed again from the keys that
 // the row sees alone, if a value that is not finite lies where they do not see it (those
 // of capped scores always: their reference may be less than the largest).
 template <typename X, typename T, int DP, int R>
-__device__ __forceinline__ void finish_rows(const typename X::Paged &pr, const PagedGrid &gr, int id, const Block &w,
+__device__ __forceinline__ void finish_rows(const typename X::Paged &pr, const PagedGrid &gr, int splits, int id, const Block &w,
                                             const RowSight &rs, int r, int lane, const f16v (&o)[DP / 32], float m, float l) {
     const typename SequenceOf<X>::type sq(pr, w);
     const int hk = blockIdx.y;
     const int64_t head = (int64_t)hk * pr.D;
-    if (gr.splits > 1) {
+    if (splits > 1) {
         if (r < w.rows)
             store_partial(o, Partial(pr, gr, (((int64_t)id * pr.Hk + hk) * gr.splits + blockIdx.z) * R + r - w.r0), m,
                           l, pr.D, lane);
@@ -313,9 +326,11 @@ __device__ __forceinline__ void finish_rows(const typename X::Paged &pr, const P
     }
 }
 
+// Wavefronts of a block of 32 rows: the tiles of wide Float32 heads fill LDS with two.
+__host__ __device__ constexpr int few_waves(int esize, int D) { return esize == 4 && D > 64 ? 2 : 4; }
 template <typename T, int DP>
 struct FewShape {
-    static constexpr int NW = sizeof(T) == 4 && DP > 64 ? 2 : 4, TILE = 32 * Tile<T, DP>::ROW, LDS = NW * 4 * TILE;
+    static constexpr int NW = few_waves(sizeof(T), DP), TILE = 32 * Tile<T, DP>::ROW, LDS = NW * 4 * TILE;
 };
 
 // Block number id, by the first NW wavefronts of a workgroup.
@@ -334,9 +349,11 @@ __device__ __forceinline__ void few_rows(const typename X::Paged &pr, const Page
     const typename SequenceOf<X>::type sq(pr, w);
     const auto see = sq.sight(pr);
     const auto tiles = sq.template tiles<32>(pr, rs.blo, rs.bhi);
+    const int splits = parts_of<X>(pr, gr.splits, tiles.count, NW);
+    if (X::kShaped && (int)blockIdx.z >= splits) return;
     const auto score = sq.template scorer<T>(pr, w, rs.blo, rs.bhi, hk * pr.G + rs.g);
     const Pages<T> pg(pr, w, rs, hk, sq.head(pr), sq.keys(rs.bhi));
-    const int parts = gr.splits * NW, part = blockIdx.z * NW + wave;
+    const int parts = splits * NW, part = blockIdx.z * NW + wave;
     const int i0 = (int)((int64_t)tiles.count * part / parts), i1 = (int)((int64_t)tiles.count * (part + 1) / parts);
     Rows<T, DP> x;
     const T *qr = static_cast<const T *>(pr.q) + (w.q0 + rs.tok) * pr.q_row + ((int64_t)(hk * pr.G + rs.g) * pr.D);
@@ -411,7 +428,7 @@ __device__ __forceinline__ void few_rows(const typename X::Paged &pr, const Page
             }
         __syncthreads();
     }
-    if (wave == 0) finish_rows<X, T, DP, 32>(pr, gr, id, w, rs, r, lane, x.o, mm, ll);
+    if (wave == 0) finish_rows<X, T, DP, 32>(pr, gr, splits, id, w, rs, r, lane, x.o, mm, ll);
 }
 
 template <typename T, int DP>
@@ -523,7 +540,7 @@ __device__ __forceinline__ void chunk_rows(const typename X::Paged &pr, const Pa
 #pragma unroll
             for (int i = 0; i < 16; ++i) x.o[t][i] = x.o[t][i] * f0 + buf[(16 * t + i) * 64 + lane] * f1;
     }
-    if (live) finish_rows<X, T, DP, 128>(pr, gr, id, w, rs, r, lane, x.o, m, l);
+    if (live) finish_rows<X, T, DP, 128>(pr, gr, gr.splits, id, w, rs, r, lane, x.o, m, l);
 }
 
 // A call's blocks: those of 128 rows (which take longest) first, those of 32 behind
@@ -556,15 +573,21 @@ __global__ __launch_bounds__(256, 8) void paged_join(typename X::Paged pr, Paged
     if (w.b < 0) return;
     const typename SequenceOf<X>::type sq(pr, w);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hk = blockIdx.y, d = 4 * (lane & 31);
+    int splits = gr.splits;
+    if constexpr (X::kShaped && R == 32) {
+        const RowSight rs = RowSight::of<R>(pr, w, w.r0);
+        splits = parts_of<X>(pr, splits, sq.template tiles<32>(pr, rs.blo, rs.bhi).count, few_waves(sizeof(T), pr.D));
+        if (splits == 1) return;  // the block's rows are written
+    }
     const int64_t slot = ((int64_t)blockIdx.x * pr.Hk + hk) * gr.splits * R, head = (int64_t)hk * pr.D;
     const int rows = w.rows - w.r0 < R ? w.rows - w.r0 : R;
     int hidden = -1;  // hidden_values of the block, once asked for
     for (int i0 = 2 * wave; i0 < rows; i0 += 8) {
         const int i = i0 + (lane >> 5), ii = i < rows ? i : rows - 1;
         float m = -INFINITY, l = 0.f;
-        for (int s = 0; s < gr.splits; ++s) m = fmaxf(m, Partial(pr, gr, slot + s * R + ii).ml[0]);
+        for (int s = 0; s < splits; ++s) m = fmaxf(m, Partial(pr, gr, slot + s * R + ii).ml[0]);
         f4v o = f4v{};
-        for (int s = 0; s < gr.splits; ++s) {
+        for (int s = 0; s < splits; ++s) {
             const Partial p(pr, gr, slot + s * R + ii);
             const float ls = p.ml[1];
             if (ls == 0.f) continue;  // saw nothing, and wrote no outputs
@@ -633,24 +656,38 @@ inline int count_splits(double blocks, double tiles) {
     return best;
 }
 
-inline PagedPlan paged_plan(const PagedProblem &pr) {
+// whole: rows see a prefix, whose length the device alone knows.  Blocks of 32 rows may walk
+// all that the table holds then, and have room for the parts of that as far as the chip is
+// half empty without; how many of them each has is parts_of's.  A token of one sequence of
+// 16384, window 32, 8 heads of 128 keys, bf16, behind prefixes of 100, 700, 4096, 16000: 10.8, 16.9, 18.2, 37
+// us on the GPU, with parts for window and sinks alone 9.1, 14.7, 49, 167.  (Not blocks of 128 rows:
+// some 40 workgroups, 128 new tokens behind 8000, took 17 -> 43 us behind short prefixes and
+// 133 -> 101 behind all.)
+inline PagedPlan paged_plan(const PagedProblem &pr, bool whole = false) {
     PagedPlan pl;
     const int64_t rows = pr.T * pr.G;
     pl.chunk = pr.T != pr.B && rows > (int64_t)pr.B * 32;
     pl.few = !pl.chunk || pr.B > 1;
     const bool wide = pr.dtype == CIRCATT_F32;
     const int64_t held = (int64_t)pr.maxp * pr.page, window = (int64_t)pr.W + pr.S;
+    const int64_t walks = pl.chunk ? 0 : (rows / 32 + pr.B) * pr.Hk;  // workgroups of one part each
+    const int room = !whole || walks == 0 ? 0 : walks < 32 ? 8 : (int)(256 / walks);
     auto grid = [&](int R, int KT, int waves, int which) {
         PagedGrid gr;
         gr.which = which;
         gr.blocks = which == kShort ? pr.B : (int)(rows / R) + pr.B;
         const int64_t seen = window + R / pr.G < held ? window + R / pr.G : held;
         const double blocks = which == kLong ? (double)rows / R + 1 : gr.blocks;
-        gr.splits = count_splits(blocks * pr.Hk, (double)((seen + KT - 1) / KT) / waves);
+        auto splits = [&](int64_t keys) { return count_splits(blocks * pr.Hk, (double)((keys + KT - 1) / KT) / waves); };
+        gr.splits = splits(seen);
+        if (gr.splits < room) {
+            const int most = splits(held);
+            gr.splits = most < gr.splits ? gr.splits : most < room ? most : room;
+        }
         gr.rows = gr.splits > 1 ? (int64_t)gr.blocks * pr.Hk * gr.splits * R : 0;
         return gr;
     };
-    pl.few_grid = grid(32, 32, wide && pr.D > 64 ? 2 : 4, pl.chunk ? kShort : kAll);
+    pl.few_grid = grid(32, 32, few_waves(wide ? 4 : 2, pr.D), pl.chunk ? kShort : kAll);
     pl.chunk_grid = grid(128, wide ? 32 : 64, wide && pr.D > 64 ? 1 : 2, pl.few ? kLong : kAll);
     pl.few_grid.at = 0;
     pl.chunk_grid.at = pl.few ? (pl.few_grid.rows * (pr.D + 2) + 3) & ~(int64_t)3 : 0;
@@ -659,8 +696,7 @@ inline PagedPlan paged_plan(const PagedProblem &pr) {
 }
 
 template <typename X, typename T, int DP>
-void launch(const typename X::Paged &pr, hipStream_t s) {
-    const PagedPlan pl = paged_plan(pr);
+void launch(const typename X::Paged &pr, const PagedPlan &pl, hipStream_t s) {
     const int tail = pr.zero_tail && pr.offsets != nullptr ? 8 : 0;
     if (pl.chunk) {
         PagedGrid few = pl.few_grid;
@@ -680,18 +716,18 @@ void launch(const typename X::Paged &pr, hipStream_t s) {
     }
 }
 template <typename X, int DT>
-void launch_type(const typename X::Paged &pr, hipStream_t s) {
+void launch_type(const typename X::Paged &pr, const PagedPlan &pl, hipStream_t s) {
     typedef typename Elem<DT>::T T;
-    if (pr.D <= 32) launch<X, T, 32>(pr, s);
-    else if (pr.D <= 64) launch<X, T, 64>(pr, s);
-    else if (pr.D <= 96) launch<X, T, 96>(pr, s);
-    else launch<X, T, 128>(pr, s);
+    if (pr.D <= 32) launch<X, T, 32>(pr, pl, s);
+    else if (pr.D <= 64) launch<X, T, 64>(pr, pl, s);
+    else if (pr.D <= 96) launch<X, T, 96>(pr, pl, s);
+    else launch<X, T, 128>(pr, pl, s);
 }
 template <typename X>
-hipError_t launch_of(const typename X::Paged &pr, hipStream_t s) {
-    if (pr.dtype == CIRCATT_F32) launch_type<X, 0>(pr, s);
-    else if (pr.dtype == CIRCATT_F16) launch_type<X, 2>(pr, s);
-    else launch_type<X, 3>(pr, s);
+hipError_t launch_of(const typename X::Paged &pr, const PagedPlan &pl, hipStream_t s) {
+    if (pr.dtype == CIRCATT_F32) launch_type<X, 0>(pr, pl, s);
+    else if (pr.dtype == CIRCATT_F16) launch_type<X, 2>(pr, pl, s);
+    else launch_type<X, 3>(pr, pl, s);
     return hipGetLastError();
 }
 

@@ -99,10 +99,11 @@ struct PagedProblem {
 struct ShapedPagedProblem : PagedProblem {
     ScoreShape shape;  // without places
 };
-int64_t paged_workspace_floats(const PagedProblem &pr);
+// whole: of a plan for rows that may see all that the table holds, behind a prefix
+int64_t paged_workspace_floats(const PagedProblem &pr, bool whole = false);
 int64_t paged_threads(const PagedProblem &pr);  // along the longest axis
 hipError_t launch_paged(const PagedProblem &pr, hipStream_t s);
-hipError_t launch_shaped_paged(const ShapedPagedProblem &pr, hipStream_t s);
+hipError_t launch_shaped_paged(const ShapedPagedProblem &pr, bool whole, hipStream_t s);
 
 struct AppendProblem {
     int esize;  // bytes of an element

@@ -243,6 +243,12 @@ circatt_shaped_bwd(dtype, L, B, nheads, kv_heads, dh, window, sinks, scale, cap,
           places_row, q, q_row, q_batch, k, k_row, k_batch, v, v_row, v_batch, lengths, y,
           y_rest, lse, dy, dy_row, dy_batch, dq, dk, dv, workspace, workspace_bytes, stream)
 
+circatt_shaped_paged_workspace_bytes(dtype, T, B, nheads, kv_heads, dh, window, sinks, page_size,
+                                     max_pages, prefixed) =
+    ccall((:circatt_shaped_paged_workspace_bytes, libcircatt), Int64,
+          (Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Cint),
+          dtype, T, B, nheads, kv_heads, dh, window, sinks, page_size, max_pages, prefixed)
+
 circatt_shaped_paged(dtype, T, B, nheads, kv_heads, dh, window, sinks, scale, cap, slopes, prefix,
                      q, q_row, cache_k, cache_v, npages, page_size, page_stride, row_stride,
                      pages, pages_row, max_pages, lengths, offsets, y, zero_tail, workspace,

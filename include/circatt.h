@@ -411,7 +411,12 @@ int circatt_shaped_bwd(int dtype, int64_t L, int64_t B, int64_t nheads, int64_t 
                        const void *y_rest, const float *lse, const void *dy, int64_t dy_row,
                        int64_t dy_batch, void *dq, void *dk, void *dv, void *workspace,
                        int64_t workspace_bytes, void *stream);
-/* circatt_paged_attention likewise; its workspace is circatt_paged_workspace_bytes'. */
+/* circatt_paged_attention likewise.  Its workspace is circatt_shaped_paged_workspace_bytes';
+ * prefixed: whether a prefix will be given.  (circatt_paged_workspace_bytes' is enough, but
+ * leaves the walk of a long prefix to few workgroups.) */
+int64_t circatt_shaped_paged_workspace_bytes(int dtype, int64_t T, int64_t B, int64_t nheads,
+                                             int64_t kv_heads, int64_t dh, int64_t window, int64_t sinks,
+                                             int64_t page_size, int64_t max_pages, int prefixed);
 int circatt_shaped_paged(int dtype, int64_t T, int64_t B, int64_t nheads, int64_t kv_heads, int64_t dh,
                          int64_t window, int64_t sinks, float scale, float cap, const float *slopes,
                          const int32_t *prefix, const void *q, int64_t q_row, const void *cache_k,
