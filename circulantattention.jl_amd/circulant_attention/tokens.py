@@ -429,7 +429,10 @@ def paged_resize_(cache_k, cache_v, pages, lengths, counts, to):
     Pages behind the new lengths are given back.  Then sequences get what they lack, in
     their order, the free pages of the lowest numbers first.  A sequence that grows
     from within a page that is held more than once gets its own copy of that page's
-    tokens, the only ones that move.  From the first sequence on that finds too few free
+    tokens, the only ones that move; of several that do so in one call each gets one.  One that
+    shrinks gets none: a step that takes tokens off a sequence and brings it new ones
+    resizes it twice, to what stays of it and then to that with the new ones (an append
+    behind one resize to fewer tokens may write into a page that others hold).  From the first sequence on that finds too few free
     pages, those that need any stay as they are, as the lengths that come back show.
     Other arguments as paged_fork's."""
     npages, page, C, page_stride, row_stride = _cache(cache_k, cache_v, cache_k)

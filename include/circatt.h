@@ -441,7 +441,9 @@ int circatt_shaped_paged(int dtype, int64_t T, int64_t B, int64_t nheads, int64_
  * back.  Then sequences get the pages that they lack, in their order, the free pages
  * of the lowest numbers first.  A sequence that grows and whose last page is
  * partly filled and held more than once gets one for it too, and the part's tokens are
- * copied there, in both caches.  From the first sequence on that finds too few free
+ * copied there, in both caches; of several that do so in one call each gets one.  A
+ * sequence that shrinks gets none: where tokens are taken off a sequence and new ones
+ * appended, it is resized to what stays of it, and then to that with the new ones.  From the first sequence on that finds too few free
  * pages, those that need any stay as they are, which their new lengths show.
  *
  * circatt_paged_compact: the held pages from number `used` on, `used` being how many are
