@@ -498,7 +498,11 @@ __global__ __launch_bounds__(kPlan) void compact_small(CompactProblem pr) {
     compact_pages(pr, holes, movers, s.all >> 16, tid >> 6, kPlan / 64, tid & 63, 64);
 }
 
-// What one workgroup copies in about the time of another launch.
+// What one workgroup copies while the host brings the next call, where another launch would
+// take the host longer.  Calls from Python one after another, us, 256 KiB copied by one
+// workgroup and by a second launch: resize 16 and 18.6, compact 13.5 and 16; 512 KiB: 16 to 28 and
+// 18.7, 17 to 22 and 16; 1 MiB: 27 to 51 and 18.7, 28 to 39 and 16.  (The kernels alone, as
+// in a captured graph: 11 to 16 and 7, 11 to 14 and 10; 64 KiB 7 and 7, 7 to 10 and 9.)
 constexpr int64_t kSmallBytes = 256 * 1024;
 int64_t page_bytes(const PageShape &sh, int page_log2) { return (sh.C * sh.esize << page_log2) * 2; }
 
@@ -545,8 +549,8 @@ hipError_t launch_compact(CompactProblem pr, int32_t *work, hipStream_t s) {
     pr.movers = pr.holes + pr.npages;
     pr.rank = pr.movers + pr.npages;
     const int64_t items = (int64_t)pr.B * pr.maxp, bytes = pr.npages * page_bytes(pr.shape, pr.page_log2);
-    // half of the pages move at most, and an eighth in earnest
-    if (items + pr.npages <= kSmall && bytes <= 8 * kSmallBytes) {
+    // half of the pages move at most, and a quarter where half of the sequences ended
+    if (items + pr.npages <= kSmall && bytes <= 4 * kSmallBytes) {
         compact_small<<<1, kPlan, 0, s>>>(pr);
     } else {
         compact_plan<<<1, kPlan, 0, s>>>(pr);
