@@ -22,8 +22,8 @@ using namespace tok;
 //   512 tokens behind up to 12000, window 4096, 32 heads of 128 over 8: 86 us, 650
 //   TFLOP/s.
 // Shaped: the first case with cap 50 186 us, 5.1 TB/s still; four chunks of 512 behind up
-// to 6000, window 2048, prefixes to 700, cap and slopes 146 us, 440 TFLOP/s, without cap and
-// slopes 118.
+// to 6000, window 2048, prefixes to 700, cap and slopes 143 us, 450 TFLOP/s, without cap and
+// slopes 115.
 // Where blocks are few, each is split along its tiles over `splits` workgroups,
 // whose partial sums paged_join adds up.  A mixed batch has both kinds in one launch
 // (33 sequences, some of one token, some of up to 128: 59 us; in two launches 104).

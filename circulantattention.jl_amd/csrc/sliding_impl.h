@@ -29,7 +29,7 @@ __device__ __forceinline__ int signal_length(const SlidingProblem &pr, int b) {
 // cycles.  8192 tokens, 32 heads of 128 over 8, window 1024, 4 sinks, bf16: 167 to 170
 // us, 770 TFLOP/s of the pairs that are seen (870 of those formed: edges of tiles); the
 // same without a window 540 us, 1020 TFLOP/s, where a large library product of this
-// card reaches 1190.  From windows of 128 (4 tiles a block, 76 us) to none (64 tiles)
+// card reaches 1390 (1610 with its second operand transposed).  From windows of 128 (4 tiles a block, 76 us) to none (64 tiles)
 // the time is 45 us and 7.7 for a tile in every block: the 45, some 6 tiles' time, are
 // the cold start and the end of 2048 blocks in four rounds, a quarter of the time at
 // window 1024.  Copies of the kernel without its DMA, or with operands from registers
@@ -337,10 +337,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
 // up to 2.2 times as far off as where its results alone are rounded; with that and the
 // forward's sum of rounded weights, 1.2 times.  It is a third more products: of 2 x 4099
 // tokens in documents of up to 1200, 12 heads of 80 over 4, cap 30, f16, 87 us have become
-// 97.  Scores that are not capped have it (few_keys) where rows see few keys at most: with a
-// window of 3 keys rounded dS gives 1.53 times that error and with 512 1.46, and two
-// values there cost 22 us of 143 (2 x 4096 tokens, 16 heads of 128 over 4, window 1024,
-// slopes, bf16).
+// 97.  Scores that are not capped have it where walks are short or that may be (few_keys).
 template <typename X, typename T, int DP, bool LOW>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void sliding_dq(typename X::Sliding pr, int blocks) {
     typedef typename SignalOf<X>::type Signal;
@@ -499,8 +496,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) void slidin
 // sliding_dkdv_far's, for 32 keys and with a wavefront for every tile: a few
 // sinks would leave most of a workgroup of 128 keys idle (18 us at the size above).
 //
-// Shaped: 2 x 4096 tokens, 16 heads of 128 over 4, window 1024, slopes, bf16: 205 us,
-// waiting 0.54 of the cycles; 2 x 4099 in documents of up to 1200, 12 heads of 80 over 4,
+// Shaped: 2 x 4096 tokens, 16 heads of 128 over 4, window 1024, slopes, bf16: 200 us,
+// waiting 0.50 of the cycles, capped at 50 instead 255 and 0.61; 2 x 4099 in documents of up to 1200, 12 heads of 80 over 4,
 // cap 30, f16: 100 us and 13 to add up, walks of some 20 tiles, whose starts and ends are
 // most of it.
 template <typename T, int DP>
@@ -1258,8 +1255,14 @@ hipError_t forward(const typename X::Sliding &pr, hipStream_t s) {
     sliding_fwd<X, T, DP, false><<<grid, 256, 0, s>>>(pr, blocks);
     return hipGetLastError();
 }
-// Whether rows may see few keys: in a narrow window, a short signal, documents of any length.
-// (Or heads are narrow, whose score gradients are large beside their sums: 1.58 in places.)
+// Whether dS of scores that are not capped goes into dq as two values.  Errors of dq as
+// multiples of rounded results', one value and two, by the window of 1280 tokens: 2 keys 1.51 and
+// 1.12, 8 1.47 and 1.06, 16 and more 1.45 and 1.04; heads of 8 channels 1.55 and 1.06 at any
+// window.  Cost of two, 2 x 4096 tokens, 16 heads over 4, bf16: up to windows of 128 keys none that
+// shows in a call (60 us from Python), 10% of the pass at 512, 16% at 1024 (128 channels), 7% at 1024
+// (32).  So windows below 64 keys and heads of up to 32 channels have them.  Documents have them for the short ones that
+// may be among them, whose lengths the device alone knows (of 4 tokens 1.50 and 1.10; of 600
+// 1.45 and 1.03, at 12%).
 inline bool few_keys(const SlidingProblem &pr) { return (pr.W < pr.L ? pr.W : pr.L) < 64; }
 inline bool few_keys(const ShapedSlidingProblem &pr) {
     return pr.shape.places != nullptr || pr.D <= 32 || few_keys(static_cast<const SlidingProblem &>(pr));
