@@ -299,9 +299,10 @@ __device__ __forceinline__ void finish_rows(const typename X::Paged &pr, const P
                           l, pr.D, lane);
         return;
     }
-    const float inv = l == 0.f ? 0.f : out_of_reach<X::kCap>(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     T *y = static_cast<T *>(pr.y) + w.q0 * pr.H * pr.D + head * pr.G;
-    const bool bad = r < w.rows && store_channels(o, y + ((int64_t)rs.tok * pr.H + rs.g) * pr.D, pr.D, lane, inv);
+    const bool bad = r < w.rows && store_channels(o, y + ((int64_t)rs.tok * pr.H + rs.g) * pr.D, pr.D, lane, inv,
+                                                  out_of_reach<X::kCap>(l));
     // NaN weights: the row is NaN, whatever it sees
     uint32_t again = rows_of(__ballot(bad && l > 0.f)), empty = rows_of(__ballot(r < w.rows && l == 0.f));
     const PagedKV<T> kv = paged_rows_of<T>(pr, w.b, head);
@@ -595,15 +596,16 @@ __global__ __launch_bounds__(256, 8) void paged_join(typename X::Paged pr, Paged
             l += ls * f;
             if (d < pr.D) o += *reinterpret_cast<const f4v *>(p.o + d) * f;
         }
-        const float inv = l == 0.f ? 0.f : out_of_reach<X::kCap>(l);
+        const float inv = l == 0.f ? 0.f : 1.f / l, least = out_of_reach<X::kCap>(l);
         const int tok = (w.r0 + ii) / pr.G, g = w.r0 + ii - tok * pr.G;
         T *y = static_cast<T *>(pr.y) + (w.q0 + tok) * pr.H * pr.D + head * pr.G + (int64_t)g * pr.D;
         V4<T> v;
         bool bad = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            v[e] = (T)(o[e] * inv);
-            bad |= !(fabsf(o[e] * inv) < INFINITY);
+            const float x = fabsf(o[e]) < least ? NAN : o[e] * inv;
+            v[e] = (T)x;
+            bad |= !(fabsf(x) < INFINITY);
         }
         if (i < rows && d < pr.D) *reinterpret_cast<V4<T> *>(y + d) = v;
         const bool in = i < rows && d < pr.D;

@@ -256,10 +256,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void slidin
         if (live) {
             // a row sees its own token at least: without a sum of weights all that it sees
             // has the score -inf, and its softmax is NaN
-            const float l = x.total(), inv = out_of_reach<X::kCap>(l);
+            const float l = x.total(), inv = 1.f / l;
             bool bad = false;
             if (r < rows) {
-                bad = store_channels(x.o, y + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv);
+                bad = store_channels(x.o, y + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv, out_of_reach<X::kCap>(l));
                 if (rest != nullptr)
                     store_rests(x.o, rest + ((int64_t)at * pr.H + g) * pr.D, pr.D, lane, inv,
                                 KEPT ? 1.f / x.total_rounded() : inv);

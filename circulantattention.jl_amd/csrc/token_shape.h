@@ -148,12 +148,14 @@ struct ShapedTiles {
 // ---------------------------------------------------------------------------
 // Scores of 32 rows, one a lane, over blocks of 32 keys: registers hold the
 // products and then the scores.
-// What a row's sum of weighted values is multiplied by, from the sum of the weights: NaN,
-// as rows are marked that are formed again, where values might have been lost under the
-// weights.
+// Where the sum l of a row's weights is small, as it may be under a fixed reference
+// (ShapedScorer), weighted values below 2^-126 are lost, n 2^-126 of n keys' sum at most.
+// Channels whose sum is below this become NaN, as those are marked that are formed again:
+// 2^-13 of one could be lost of 8192 keys.  (All such rows formed again: 2048 tokens, 32 heads of
+// 128 over 8, cap 60 and scores about -40, 5.9 ms instead of 0.08.)
 template <bool CAP>
 __device__ __forceinline__ float out_of_reach(float l) {
-    return CAP && l < 0x1p-20f ? NAN : 1.f / l;
+    return CAP && l < 0x1p-20f ? 0x1p-100f : 0.f;
 }
 
 struct PlainScorer {
@@ -202,7 +204,7 @@ struct ShapedScorer {
     // the first tile alone is the softmax's reference then, or C - 100 if that is more:
     // weights stay below 2^100, their sum below 2^124, and that of the row's own token, or
     // of the first tile's best, above 2^(100 - 2 C).  (Rows whose sums of values pass Float32
-    // so, or whose weights are all below 2^-20, are formed again: out_of_reach.  Float16 does
+    // so, or of values too small for their weights, are formed again: out_of_reach.  Float16 does
     // not hold such weights, and exponents of some 100 are off by 2^-18, ten times the rest of
     // a Float32 signal's error.)  `wide`: that type, and rows that all see their own token.
     bool bounded;

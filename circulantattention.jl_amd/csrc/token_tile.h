@@ -451,10 +451,11 @@ __device__ __forceinline__ void share_repairs(CIRCATT_LDS uint32_t *list, int fr
     }
 }
 
-// Writes a row's channels (one lane and its other half), times f; whether one of
-// them is not finite (as Float32: one that the row's type cannot hold is itself).
+// Writes a row's channels (one lane and its other half), times f, NaN for those below
+// `least`; whether one of them is not finite (as Float32: one that the row's type cannot
+// hold is itself).
 template <typename T, int OT>
-__device__ __forceinline__ bool store_channels(const f16v (&o)[OT], T *y, int D, int lane, float f) {
+__device__ __forceinline__ bool store_channels(const f16v (&o)[OT], T *y, int D, int lane, float f, float least = 0.f) {
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < OT; ++t)
@@ -464,7 +465,7 @@ __device__ __forceinline__ bool store_channels(const f16v (&o)[OT], T *y, int D,
             V4<T> v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float x = o[t][i + j] * f;
+                const float x = fabsf(o[t][i + j]) < least ? NAN : o[t][i + j] * f;
                 bad |= !(fabsf(x) < INFINITY) && d < D;
                 v[j] = (T)x;
             }
